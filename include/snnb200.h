@@ -516,6 +516,50 @@ int64_t snnb_first_conv_tc_weight_k(int64_t Cin);
 int snnb_split_bf16_terms(const float* x, int64_t rows, int64_t C, int64_t Cp, void* out,
                           snnb_stream_t stream);
 
+/* microscaled formats: blocks of 32 values along the last axis share a power-of-two scale */
+#define SNNB_MXFP4  0   /* E2M1 elements, 4 bits, magnitudes 0 .5 1 1.5 2 3 4 6 */
+#define SNNB_MXFP8  1   /* E4M3 elements, 8 bits, magnitudes up to 448 */
+
+/*
+ * Microscaled tensors [rows, K] (no counterpart in the reference; for the low-bit linear
+ * layers next to spikes, which E2M1 holds exactly).  nb = ceil(K / 32) blocks a row.
+ *   data    [rows, 16 * nb] bytes (SNNB_MXFP4, the even element in the low four bits) or
+ *           [rows, 32 * nb] (SNNB_MXFP8); elements past K are zero
+ *   scales  ceil(rows / 128) * ceil(nb / 4) groups of 512 bytes: the scale byte b of row r,
+ *           block j (value 2^(b - 127), 255 = NaN) is byte
+ *           (r % 32) * 16 + (r % 128 / 32) * 4 + j % 4 of group (r / 128) * ceil(nb / 4) + j / 4;
+ *           bytes that no block owns are zero
+ * Both 16-byte aligned.
+ *
+ * snnb_mx_quantize: x [rows, K] (row stride ldx elements, unit column stride) of x_dtype.  A
+ * block's scale is 2^(floor(log2(largest magnitude)) - 2), - 8 for SNNB_MXFP8, and at least
+ * 2^-127; its elements are rounded to the nearest, ties to even, magnitudes above the largest
+ * element clamped to it.  A block with an infinity or a NaN gets the NaN scale.
+ * snnb_mx_dequantize: the values, rounded once to out_dtype; out [rows, K] contiguous.
+ */
+int snnb_mx_quantize(const void* x, int x_dtype, int64_t rows, int64_t K, int64_t ldx, int fmt,
+                     void* data, void* scales, snnb_stream_t stream);
+int snnb_mx_dequantize(const void* data, const void* scales, int fmt, int64_t rows, int64_t K,
+                       void* out, int out_dtype, snnb_stream_t stream);
+
+/*
+ * out [rows, N] = a [rows, K] * w [N, K]^T + bias: a of a_fmt, w of SNNB_MXFP4, both as above;
+ * bias [N] float32 or NULL; float32 sums, rounded once to out_dtype (F32 / F16 / BF16).
+ */
+int snnb_mx_linear(const void* a, const void* a_scales, int a_fmt, int64_t rows, int64_t K,
+                   const void* w, const void* w_scales, int64_t N, const float* bias, void* out,
+                   int out_dtype, snnb_stream_t stream);
+
+/*
+ * h = x + residual (float32; h = x when residual is NULL), stored to h_out in x_dtype unless
+ * NULL; y = (h / sqrt(mean(h^2) + eps)) * weight in float32, written as codes and scales of
+ * `fmt` (snnb_mx_quantize).  x and residual [rows, K] with row strides ldx, ldr; weight [K] of
+ * x_dtype or float32; h_out [rows, K] contiguous, overlapping neither x nor residual.
+ */
+int snnb_rms_norm_mx(const void* x, int64_t ldx, const void* residual, int64_t ldr, int x_dtype,
+                     const void* weight, int weight_dtype, float eps, int64_t rows, int64_t K,
+                     int fmt, void* data, void* scales, void* h_out, snnb_stream_t stream);
+
 /*
  * Reads and clears the device status word that kernels with bounded waits write
  * (SNNB_ERR_TIMEOUT after a wait gave up).  Synchronises `stream`.

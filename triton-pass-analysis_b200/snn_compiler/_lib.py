@@ -65,6 +65,10 @@ SIGNATURES = {
     "snnb_linear_f32": [P, I64, I64, I64, P, P, I64, P, P],
     "snnb_spike_attention_core": [P, P, P, I64, I64, I64, I64, P, P, P, I64, I64, I64, I64,
                                   I64, I64, I64, I64, I64, F, F, F, F, F, I32, P],
+    "snnb_mx_quantize": [P, I32, I64, I64, I64, I32, P, P, P],
+    "snnb_mx_dequantize": [P, P, I32, I64, I64, P, I32, P],
+    "snnb_mx_linear": [P, P, I32, I64, I64, P, P, I64, P, P, I32, P],
+    "snnb_rms_norm_mx": [P, I64, P, I64, I32, P, I32, F, I64, I64, I32, P, P, P, P],
     "snnb_conv3x3_lif_static_scratch": [P, I64, I64, I64, I64, I64, P, P, I64, F, F, F, F, I32,
                                         I32, I32, I32, P, P],
 }
