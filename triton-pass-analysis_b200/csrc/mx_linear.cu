@@ -26,12 +26,13 @@ namespace {
 
 struct MxParams {
     int rows, N, groups;             // tokens, features, 128-wide groups of K
-    int tiles_w, tiles;              // feature tiles, tiles in all
+    int tiles_w, tiles;              // feature tiles (of 128, or 256 a pair), tiles in all
     int64_t w_row_bytes;
-    const uint8_t *w, *w_scales, *a_scales;
+    const uint8_t* w;
     const float* bias;
     void* out;
     int out_dtype;
+    int pairs;                       // 16-bit outputs may be stored two features at a time
     int* status;
 };
 
@@ -45,38 +46,85 @@ __host__ __device__ constexpr uint32_t idesc_mx(int a_type, int b_type, int M, i
 __device__ __forceinline__ uint32_t idesc_scale_byte(uint32_t byte) {
     return (byte << 4) | (byte << 29);
 }
-template <int FMT>
+// PAIR: M = 256 over the two CTAs of a cluster, issued by one thread of the even CTA.
+#define SNNB_MX_MMA(group, kind, vec)                                                        \
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"                           \
+                 "tcgen05.mma.cta_group::" group ".kind::" kind ".block_scale.scale_vec::" vec \
+                 " [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),                        \
+                 "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)       \
+                 : "memory")
+template <int FMT, bool PAIR>
 __device__ __forceinline__ void umma_mx(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                         uint32_t sa, uint32_t sb, uint32_t accumulate) {
-    if constexpr (FMT == SNNB_MXFP4)
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X"
-            " [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
-            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
-            : "memory");
-    else
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X"
-            " [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
-            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
-            : "memory");
+    if constexpr (FMT == SNNB_MXFP4 && PAIR) SNNB_MX_MMA("2", "mxf4", "2X");
+    else if constexpr (FMT == SNNB_MXFP4) SNNB_MX_MMA("1", "mxf4", "2X");
+    else if constexpr (PAIR) SNNB_MX_MMA("2", "mxf8f6f4", "1X");
+    else SNNB_MX_MMA("1", "mxf8f6f4", "1X");
 }
+#undef SNNB_MX_MMA
 // One 512-byte scale group (32 rows of 16 bytes, unswizzled) to 4 TMEM columns, the same 32
-// lanes in each of the four lane quarters.
+// lanes in each of the four lane quarters.  PAIR: in both CTAs, each from its own memory.
+template <bool PAIR>
 __device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t saddr) {
     uint64_t d = (uint64_t)((saddr & 0x3FFFFu) >> 4);
     d |= (uint64_t)(128 >> 4) << 32;                 // 8 rows to the next 8: 128 bytes
     d |= (uint64_t)1 << 46;
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(d) : "memory");
+    if constexpr (PAIR)
+        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(d)
+                     : "memory");
+    else
+        asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(d)
+                     : "memory");
 }
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
-                                          uint32_t bar) {
+// Tiled loads completing on `bar`; PAIR: a barrier of the even CTA (a shared::cluster address).
+template <bool PAIR>
+__device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int c0,
+                                        int c1) {
+    if constexpr (PAIR)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+            "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(c0), "r"(c1)
+            : "memory");
+    else
+        tc::tma_load_2d(dst, tm, bar, c0, c1);
+}
+template <bool PAIR>
+__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int c0,
+                                        int c1, int c2) {
+    if constexpr (PAIR) tc::tma_load_3d_pair(dst, tm, bar, c0, c1, c2);
+    else tc::tma_load_3d(dst, tm, bar, c0, c1, c2);
+}
+// tc::mbar_wait_lane with cluster-scope acquire: threads of the pair's other CTA arrive on the
+// barrier too.
+__device__ __forceinline__ uint32_t mbar_wait_lane_cluster(uint32_t bar, uint32_t parity,
+                                                           uint32_t skip) {
+    uint32_t ok;
     asm volatile(
-        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
+        "{\n\t.reg .pred p, q;\n\t.reg .u64 t0, t1, lim;\n\t"
+        "setp.ne.u32 q, %3, 0;\n\t"
+        "@q bra LFAIL_%=;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "@p bra LOK_%=;\n\t"
+        "ld.volatile.u64 lim, [%4];\n\t"
+        "mov.u64 t0, %%clock64;\n\t"
+        "LLOOP_%=:\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "@p bra LOK_%=;\n\t"
+        "mov.u64 t1, %%clock64;\n\t"
+        "sub.u64 t1, t1, t0;\n\t"
+        "setp.lt.u64 q, t1, lim;\n\t"
+        "@q bra LLOOP_%=;\n\t"
+        "LFAIL_%=:\n\t"
+        "mov.u32 %0, 0;\n\t"
+        "bra.uni LEND_%=;\n\t"
+        "LOK_%=:\n\t"
+        "mov.u32 %0, 1;\n\t"
+        "LEND_%=:\n\t}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(skip), "l"(&tc::g_wait_limit)
         : "memory");
+    return ok;
 }
 template <int N>
 __device__ __forceinline__ void cp_async_wait_group() {
@@ -87,12 +135,13 @@ __device__ __forceinline__ void cp_async_commit() {
 }
 
 // ---- shared memory -----------------------------------------------------------------------
-template <int FMT, int BN, int STAGES>
+template <int FMT, int BN, int STAGES, bool PAIR>
 struct MxSmem {
     static constexpr int GROUPS = FMT == SNNB_MXFP4 ? 2 : 1;     // 128-wide groups of K a stage
-    static constexpr int TOKEN_TILES = (BN + 127) / 128;
+    static constexpr int TOKEN_TILES = (BN + 127) / 128;         // scale tiles of the tokens
+    static constexpr int A_ROWS = PAIR ? BN / 2 : BN;            // a pair: half the tokens a CTA
     static constexpr int W_TILE = 128 * 128;
-    static constexpr int A_TILE = BN * 128;
+    static constexpr int A_TILE = A_ROWS * 128;
     static constexpr int W_SCALES = GROUPS * mx::GROUP_BYTES;
     static constexpr int A_SCALES = TOKEN_TILES * GROUPS * mx::GROUP_BYTES;
     static constexpr int STAGE = W_TILE + A_TILE;                // operand tiles, 1024-aligned
@@ -112,25 +161,69 @@ struct MxSmem {
     static_assert(DYN <= 227 * 1024, "shared memory");
 };
 
-template <int FMT> constexpr int mx_threads() { return FMT == SNNB_MXFP4 ? 192 : 320; }
-
-__device__ __forceinline__ void store_out(const MxParams& p, int64_t i, float v) {
-    if (!SNNB_IN_BOUNDS(i, (int64_t)p.rows * p.N, p.status)) return;
-    if (p.out_dtype == SNNB_F32)
-        static_cast<float*>(p.out)[i] = v;
-    else if (p.out_dtype == SNNB_F16)
-        static_cast<__half*>(p.out)[i] = __float2half_rn(v);
-    else
-        static_cast<__nv_bfloat16*>(p.out)[i] = __float2bfloat16_rn(v);
+// Warps: the producers (one kind of load each), the MMA issuer, 4 epilogue warps, and for E4M3
+// tokens 4 that place the weight pieces.
+template <int FMT> constexpr int mx_producers() { return FMT == SNNB_MXFP4 ? 4 : 3; }
+template <int FMT> constexpr int mx_threads() {
+    return 32 * (mx_producers<FMT>() + 1 + 4 + (FMT == SNNB_MXFP4 ? 0 : 4));
 }
 
-// SPLIT: the K range of one tile over a cluster of CTAs, their float32 partial sums joined in
-// rank order through distributed shared memory; otherwise a CTA walks whole tiles.
-template <int FMT, int BN, int STAGES, bool SPLIT>
+// STEP accumulator columns (tokens r0 .., the first `cols` of them inside) of this lane's
+// feature n.  16-bit outputs go out in pairs of features: neighbouring lanes swap a value, so
+// that the even lane stores both features of one token and the odd lane of the next.
+template <typename O, int STEP>
+__device__ __forceinline__ void store_cols16(const MxParams& p, const float (&r)[STEP], float bias,
+                                             int n, int64_t r0, int cols) {
+    O* out = static_cast<O*>(p.out);
+    const int odd = threadIdx.x & 1;
+    if (p.pairs) {
+        O* o = out + (r0 + odd) * p.N + (n & ~1);
+#pragma unroll
+        for (int i = 0; i < STEP; i += 2) {
+            const float a = r[i] + bias, b = r[i + 1] + bias;
+            const float other = __shfl_xor_sync(0xffffffffu, odd ? a : b, 1);
+            const uint32_t v = odd ? mx::round_pair(other, b, out) : mx::round_pair(a, other, out);
+            if (n < p.N && i + odd < cols &&
+                SNNB_IN_BOUNDS((r0 + odd + i) * p.N + n, (int64_t)p.rows * p.N, p.status))
+                *reinterpret_cast<uint32_t*>(o + (int64_t)i * p.N) = v;
+        }
+    } else {
+        O* o = out + r0 * p.N + n;
+#pragma unroll
+        for (int i = 0; i < STEP; ++i)
+            if (n < p.N && i < cols &&
+                SNNB_IN_BOUNDS((r0 + i) * p.N + n, (int64_t)p.rows * p.N, p.status))
+                mx::round_to(r[i] + bias, o + (int64_t)i * p.N);
+    }
+}
+template <int STEP>
+__device__ __forceinline__ void store_cols(const MxParams& p, const float (&r)[STEP], float bias,
+                                           int n, int64_t r0, int cols) {
+    if (p.out_dtype == SNNB_F32) {
+        float* o = static_cast<float*>(p.out) + r0 * p.N + n;
+#pragma unroll
+        for (int i = 0; i < STEP; ++i)
+            if (n < p.N && i < cols &&
+                SNNB_IN_BOUNDS((r0 + i) * p.N + n, (int64_t)p.rows * p.N, p.status))
+                o[(int64_t)i * p.N] = r[i] + bias;
+    } else if (p.out_dtype == SNNB_F16) {
+        store_cols16<__half, STEP>(p, r, bias, n, r0, cols);
+    } else {
+        store_cols16<__nv_bfloat16, STEP>(p, r, bias, n, r0, cols);
+    }
+}
+
+// PAIR: two CTAs share a 256-feature x BN-token tile (each stages its own 128 features and half
+// of the tokens) and walk whole tiles.  Otherwise: one tile, its K range split over the CTAs of
+// a cluster, their float32 partial sums joined in rank order through distributed shared memory.
+template <int FMT, int BN, int STAGES, bool PAIR>
 __global__ void __launch_bounds__(mx_threads<FMT>(), 1)
 mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmA,
+                 const __grid_constant__ CUtensorMap tmWS, const __grid_constant__ CUtensorMap tmAS,
                  const MxParams p) {
-    using S = MxSmem<FMT, BN, STAGES>;
+    using S = MxSmem<FMT, BN, STAGES, PAIR>;
+    constexpr int NP = mx_producers<FMT>();
+    constexpr int CTAS = PAIR ? 2 : 1;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -146,70 +239,79 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
     auto scales_at = [&](int s) { return sbase + (uint32_t)(S::SCALES_OFF + s * S::SCALES); };
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + S::TMEM_OFF);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int crank = PAIR ? (int)tc::cluster_rank() : 0;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
-            tc::mbar_init(full_bar(s), FMT == SNNB_MXFP4 ? 1 : 5);
+            tc::mbar_init(full_bar(s), NP + (FMT == SNNB_MXFP4 ? 0 : 4 * CTAS));
             tc::mbar_init(empty_bar(s), 1);
         }
         for (int b = 0; b < S::ACCS; ++b) {
             tc::mbar_init(accf_bar(b), 1);
-            tc::mbar_init(acce_bar(b), 4);
+            tc::mbar_init(acce_bar(b), 4 * CTAS);
         }
         tc::mbar_init(done_bar, 1);
         tc::fence_mbar_init();
         tc::prefetch_tmap(&tmW);
         tc::prefetch_tmap(&tmA);
+        tc::prefetch_tmap(&tmWS);
+        tc::prefetch_tmap(&tmAS);
     }
-    if (warp == 1) {
-        tc::tmem_alloc(sbase + S::TMEM_OFF, S::COLS);
-        tc::tmem_relinquish();
+    if (warp == NP) {
+        if constexpr (PAIR) {
+            tc::tmem_alloc_pair(sbase + S::TMEM_OFF, S::COLS);
+            tc::tmem_relinquish_pair();
+        } else {
+            tc::tmem_alloc(sbase + S::TMEM_OFF, S::COLS);
+            tc::tmem_relinquish();
+        }
     }
     tc::tc_fence_before();
     __syncthreads();
+    if constexpr (PAIR) tc::cluster_sync();          // the even CTA's barriers are initialised
     tc::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     pdl_trigger();
     pdl_wait();
 
     // this CTA's tiles and, within a tile, its stages of K
-    const int splits = SPLIT ? (int)gridDim.x / p.tiles : 1;
-    const int rank = SPLIT ? (int)blockIdx.x % splits : 0;
-    const int tile0 = SPLIT ? (int)blockIdx.x / splits : (int)blockIdx.x;
-    const int tile_step = SPLIT ? p.tiles : (int)gridDim.x;
+    const int splits = PAIR ? 1 : (int)gridDim.x / p.tiles;
+    const int rank = PAIR ? 0 : (int)blockIdx.x % splits;
+    const int tile0 = PAIR ? (int)blockIdx.x / 2 : (int)blockIdx.x / splits;
+    const int tile_step = PAIR ? (int)gridDim.x / 2 : p.tiles;
     const int nstages = (p.groups + S::GROUPS - 1) / S::GROUPS;
     const int k0 = (int)((int64_t)nstages * rank / splits);
     const int k1 = (int)((int64_t)nstages * (rank + 1) / splits);
     uint32_t failed = 0;
 
-    if (warp == 0) {
+    if (warp < NP) {
         // ------------------------------------------------------------- copies
+        // Issuing a tiled copy holds its thread for ~250 cycles, so each kind has a warp of its
+        // own: 0 tokens, 1 token scales, 2 weight scales, 3 weights (E2M1 tokens).  All bytes of
+        // a stage, a pair's both halves, complete the (even CTA's) full barrier.
+        constexpr uint32_t BYTES[4] = {S::A_TILE, S::A_SCALES, S::W_SCALES, S::W_TILE};
+        const uint32_t mine = (warp == 0 ? BYTES[0] : warp == 1 ? BYTES[1] : warp == 2 ? BYTES[2]
+                                                                                      : BYTES[3]) *
+                              (uint32_t)CTAS;
         uint32_t it = 0, issued = 0;
         for (int tile = tile0; tile < p.tiles; tile += tile_step) {
-            const int tw = tile % p.tiles_w, tt = tile / p.tiles_w;
+            const int tw = (tile % p.tiles_w) * CTAS + crank, tt = tile / p.tiles_w;
             for (int ks = k0; ks < k1; ++ks, ++it) {
                 const int s = (int)(it % STAGES);
                 failed |= 1u - tc::mbar_wait_warp(empty_bar(s), ((it / STAGES) & 1u) ^ 1u, failed);
                 if (failed) break;
                 if (tc::elect_one()) {
-                    const int g0 = ks * S::GROUPS;
-                    const uint32_t gb = (uint32_t)(min(S::GROUPS, p.groups - g0) * mx::GROUP_BYTES);
-                    // token tiles of 128 rows that exist (the others' scales are not read)
-                    const int tiles128 = min(S::TOKEN_TILES, (p.rows + 127) / 128 - tt * S::TOKEN_TILES);
-                    const uint32_t bytes = (uint32_t)S::A_TILE + gb * (uint32_t)(1 + tiles128) +
-                                           (FMT == SNNB_MXFP4 ? (uint32_t)S::W_TILE : 0u);
-                    tc::mbar_expect_tx(full_bar(s), bytes);
-                    if (FMT == SNNB_MXFP4)
-                        tc::tma_load_2d(w_tile(s), &tmW, full_bar(s), ks * 128, tw * 128);
-                    tc::tma_load_2d(a_tile(s), &tmA, full_bar(s), ks * 128, tt * BN);
-                    const uint32_t sc = scales_at(s);
-                    bulk_load(sc, p.w_scales + ((int64_t)tw * p.groups + g0) * mx::GROUP_BYTES, gb,
-                              full_bar(s));
-                    for (int h = 0; h < tiles128; ++h)
-                        bulk_load(sc + S::W_SCALES + h * S::GROUPS * mx::GROUP_BYTES,
-                                  p.a_scales + ((int64_t)(tt * S::TOKEN_TILES + h) * p.groups + g0) *
-                                                   mx::GROUP_BYTES,
-                                  gb, full_bar(s));
+                    if (crank == 0) tc::mbar_expect_tx(full_bar(s), mine);
+                    const uint32_t fb = PAIR ? tc::map_to_rank(full_bar(s), 0) : full_bar(s);
+                    if (warp == 0)
+                        load_2d<PAIR>(a_tile(s), &tmA, fb, ks * 128, tt * BN + crank * S::A_ROWS);
+                    else if (warp == 1)
+                        load_3d<PAIR>(scales_at(s) + S::W_SCALES, &tmAS, fb, 0, ks * S::GROUPS,
+                                      tt * S::TOKEN_TILES);
+                    else if (warp == 2)
+                        load_3d<PAIR>(scales_at(s), &tmWS, fb, 0, ks * S::GROUPS, tw);
+                    else
+                        load_2d<PAIR>(w_tile(s), &tmW, fb, ks * 128, tw * 128);
                 }
                 __syncwarp();
                 ++issued;
@@ -217,75 +319,96 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
             if (failed) break;
         }
         if (failed) {
-            // copies still in flight land before the CTA may exit
+            // copies still in flight land before the CTA may exit: on the full barrier, or for
+            // the odd CTA of a pair (whose copies complete the even CTA's) on the stage's release
             for (uint32_t k = 0; k < issued && k < (uint32_t)STAGES; ++k) {
                 const uint32_t g = issued - 1 - k;
-                tc::mbar_wait_warp<true>(full_bar((int)(g % STAGES)), (g / STAGES) & 1u, 0);
+                tc::mbar_wait_warp<true>(crank ? empty_bar((int)(g % STAGES)) : full_bar((int)(g % STAGES)),
+                                         (g / STAGES) & 1u, 0);
             }
         }
-    } else if (warp == 1) {
+    } else if (warp == NP) {
         // ------------------------------------------------------------- MMA issuer
-        constexpr uint32_t IDESC = FMT == SNNB_MXFP4 ? idesc_mx(1, 1, 128, BN)
-                                                     : idesc_mx(5, 0, 128, BN);
-        if (tc::elect_one()) {
-            uint32_t it = 0, local = 0;
-            for (int tile = tile0; tile < p.tiles; tile += tile_step, ++local) {
-                const int b = (int)(local % S::ACCS);
-                failed |= 1u - tc::mbar_wait_lane(acce_bar(b), ((local / S::ACCS) & 1u) ^ 1u, failed);
-                tc::tc_fence_after();
-                const uint32_t d = tmem + (uint32_t)(b * BN);
-                for (int ks = k0; ks < k1; ++ks, ++it) {
-                    const int s = (int)(it % STAGES);
-                    failed |= 1u - tc::mbar_wait_lane(full_bar(s), (it / STAGES) & 1u, failed);
+        constexpr uint32_t IDESC = FMT == SNNB_MXFP4 ? idesc_mx(1, 1, 128 * CTAS, BN)
+                                                     : idesc_mx(5, 0, 128 * CTAS, BN);
+        auto commit = [&](uint32_t bar) {
+            if constexpr (PAIR) tc::umma_commit_pair(bar, 3);
+            else tc::umma_commit(bar);
+        };
+        auto wait_full = [&](uint32_t it) {
+            const uint32_t bar = full_bar((int)(it % STAGES)), ph = (it / STAGES) & 1u;
+            if constexpr (PAIR && FMT != SNNB_MXFP4)
+                failed |= 1u - mbar_wait_lane_cluster(bar, ph, failed);
+            else
+                failed |= 1u - tc::mbar_wait_lane(bar, ph, failed);
+            tc::tc_fence_after();
+        };
+        if (crank == 0) {
+            if (tc::elect_one()) {
+                uint32_t it = 0, local = 0;
+                for (int tile = tile0; tile < p.tiles; tile += tile_step, ++local) {
+                    const int b = (int)(local % S::ACCS);
+                    failed |= 1u - tc::mbar_wait_lane(acce_bar(b), ((local / S::ACCS) & 1u) ^ 1u, failed);
                     tc::tc_fence_after();
-                    if (!failed) {
-                        const uint32_t sw = tmem + (uint32_t)(S::ACCS * BN + s * S::SCALE_COLS);
-                        const uint32_t sa = sw + 4 * S::GROUPS;
-                        const uint32_t sc = scales_at(s);
-                        const int ng = min(S::GROUPS, p.groups - ks * S::GROUPS);
-                        for (int g = 0; g < ng; ++g) {
-                            copy_scales(sw + 4 * g, sc + g * mx::GROUP_BYTES);
+                    wait_full(it);
+                    const uint32_t d = tmem + (uint32_t)(b * BN);
+                    for (int ks = k0; ks < k1; ++ks, ++it) {
+                        const int s = (int)(it % STAGES);
+                        if (!failed) {
+                            const uint32_t sw = tmem + (uint32_t)(S::ACCS * BN + s * S::SCALE_COLS);
+                            const uint32_t sa = sw + 4 * S::GROUPS;
+                            const uint32_t sc = scales_at(s);
+                            const uint64_t dw = tc::sdesc_k_sw128(w_tile(s));
+                            const uint64_t da = tc::sdesc_k_sw128(a_tile(s));
+                            constexpr int PER_GROUP = 4 / S::GROUPS;     // MMAs per 128 of K
 #pragma unroll
-                            for (int h = 0; h < S::TOKEN_TILES; ++h)
-                                copy_scales(sa + 4 * (g * S::TOKEN_TILES + h),
-                                            sc + S::W_SCALES + (h * S::GROUPS + g) * mx::GROUP_BYTES);
-                        }
-                        const uint64_t dw = tc::sdesc_k_sw128(w_tile(s));
-                        const uint64_t da = tc::sdesc_k_sw128(a_tile(s));
-                        constexpr int PER_GROUP = 4 / S::GROUPS;     // MMAs per 128 of K
-                        for (int g = 0; g < ng; ++g) {
+                            for (int g = 0; g < S::GROUPS; ++g) {
+                                if (g > 0 && ks * S::GROUPS + g >= p.groups) break;
+                                copy_scales<PAIR>(sw + 4 * g, sc + g * mx::GROUP_BYTES);
 #pragma unroll
-                            for (int m = 0; m < PER_GROUP; ++m) {
-                                const int k = g * PER_GROUP + m;
-                                umma_mx<FMT>(d, dw + 2 * k, da + 2 * k,
-                                             IDESC | idesc_scale_byte(m * S::GROUPS), sw + 4 * g,
-                                             sa + 4 * g * S::TOKEN_TILES, (ks != k0) || (k != 0));
+                                for (int h = 0; h < S::TOKEN_TILES; ++h)
+                                    copy_scales<PAIR>(sa + 4 * (g * S::TOKEN_TILES + h),
+                                                      sc + S::W_SCALES +
+                                                          (h * S::GROUPS + g) * mx::GROUP_BYTES);
+#pragma unroll
+                                for (int m = 0; m < PER_GROUP; ++m) {
+                                    const int k = g * PER_GROUP + m;
+                                    umma_mx<FMT, PAIR>(d, dw + 2 * k, da + 2 * k,
+                                                       IDESC | idesc_scale_byte(m * S::GROUPS),
+                                                       sw + 4 * g, sa + 4 * g * S::TOKEN_TILES,
+                                                       (ks != k0) || (k != 0));
+                                }
                             }
                         }
+                        // the next stage before this one's commit: a wait behind a commit
+                        // returns only once the tensor pipe has drained
+                        if (ks + 1 < k1) wait_full(it + 1);
+                        commit(empty_bar(s));
                     }
-                    tc::umma_commit(empty_bar(s));
+                    commit(accf_bar(b));
                 }
-                tc::umma_commit(accf_bar(b));
+                commit(done_bar);
             }
-            tc::umma_commit(done_bar);
+            __syncwarp();
+            failed = __shfl_sync(0xffffffffu, failed, 0);
         }
-        __syncwarp();
-        failed = __shfl_sync(0xffffffffu, failed, 0);
+        // every MMA of this CTA's (or its pair's) has completed
         failed |= 1u - tc::mbar_wait_warp<true>(done_bar, 0, 0);
-    } else if (warp < 6) {
+    } else if (warp < NP + 5) {
         // ------------------------------------------------------------- epilogue
         const int q = warp & 3;
         uint32_t local = 0;
         for (int tile = tile0; tile < p.tiles; tile += tile_step, ++local) {
-            const int tw = tile % p.tiles_w, tt = tile / p.tiles_w;
+            const int tw = (tile % p.tiles_w) * CTAS + crank, tt = tile / p.tiles_w;
             const int b = (int)(local % S::ACCS);
+            const int n = tw * 128 + 32 * q + lane;
+            const float bias = p.bias && n < p.N ? __ldg(p.bias + n) : 0.0f;
             failed |= 1u - tc::mbar_wait_warp(accf_bar(b), (local / S::ACCS) & 1u, failed);
             tc::tc_fence_after();
             if (failed) break;
             const uint32_t t = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(b * BN);
-            const int n = tw * 128 + 32 * q + lane;
             constexpr int STEP = BN < 32 ? 16 : 32;
-            if (SPLIT && splits > 1) {
+            if (!PAIR && splits > 1) {
                 // partial sums [column][lane] in the drained ring
                 float* part = reinterpret_cast<float*>(smem) + 32 * q + lane;
 #pragma unroll 1
@@ -297,36 +420,39 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
                     for (int i = 0; i < 16; ++i) part[(c + i) * 128] = r[i];
                 }
             } else {
-                const float bias = p.bias && n < p.N ? __ldg(p.bias + n) : 0.0f;
                 const int64_t left = (int64_t)p.rows - (int64_t)tt * BN;
                 const int cols = (int)(left < BN ? left : BN);
-                int64_t o = (int64_t)tt * BN * p.N + n;
 #pragma unroll 1
                 for (int c = 0; c < cols; c += STEP) {
                     float r[STEP];
                     if constexpr (STEP == 32) tc::tmem_ld32(t + c, r);
                     else tc::tmem_ld16(t + c, r);
                     tc::tmem_wait_ld();
-                    if (n < p.N) {
-#pragma unroll
-                        for (int i = 0; i < STEP; ++i)
-                            if (c + i < cols) store_out(p, o + (int64_t)(c + i) * p.N, r[i] + bias);
-                    }
+                    store_cols<STEP>(p, r, bias, n, (int64_t)tt * BN + c, cols - c);
                 }
             }
             tc::tc_fence_before();
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(acce_bar(b));
+            if (lane == 0) {
+                if constexpr (PAIR) tc::mbar_arrive_cluster(tc::map_to_rank(acce_bar(b), 0));
+                else tc::mbar_arrive(acce_bar(b));
+            }
         }
     } else {
         // ------------------------------------------------------------- weight pieces (E4M3)
         // 16 codes (8 bytes) to the low half of a 16-byte slot; slot c of row r at c ^ (r % 8)
         constexpr int AHEAD = STAGES - 2;
-        const int i = (warp - 6) * 32 + lane;
+        auto publish = [&](uint32_t g) {
+            if (lane != 0) return;
+            const uint32_t bar = full_bar((int)(g % STAGES));
+            if constexpr (PAIR) tc::mbar_arrive_cluster(tc::map_to_rank(bar, 0));
+            else tc::mbar_arrive(bar);
+        };
+        const int i = (warp - NP - 5) * 32 + lane;
         const int c = i & 7;
         uint32_t it = 0;
         for (int tile = tile0; tile < p.tiles; tile += tile_step) {
-            const int64_t n0 = (int64_t)(tile % p.tiles_w) * 128;
+            const int64_t n0 = (int64_t)((tile % p.tiles_w) * CTAS + crank) * 128;
             for (int ks = k0; ks < k1; ++ks, ++it) {
                 const int s = (int)(it % STAGES);
                 failed |= 1u - tc::mbar_wait_warp(empty_bar(s), ((it / STAGES) & 1u) ^ 1u, failed);
@@ -345,7 +471,7 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
                     cp_async_wait_group<AHEAD>();
                     tc::fence_proxy_async_smem();
                     __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(full_bar((int)((it - AHEAD) % STAGES)));
+                    publish(it - AHEAD);
                 }
             }
             if (failed) break;
@@ -353,14 +479,13 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
         tc::cp_async_wait_all();
         tc::fence_proxy_async_smem();
         __syncwarp();
-        if (!failed && lane == 0)
-            for (uint32_t g = it > (uint32_t)AHEAD ? it - AHEAD : 0; g < it; ++g)
-                tc::mbar_arrive(full_bar((int)(g % STAGES)));
+        if (!failed)
+            for (uint32_t g = it > (uint32_t)AHEAD ? it - AHEAD : 0; g < it; ++g) publish(g);
     }
     if (failed && lane == 0) atomicExch(p.status, SNNB_ERR_TIMEOUT);
-    if (SPLIT && splits > 1) {
+    if (!PAIR && splits > 1) {
         tc::cluster_sync();                          // every CTA's partial sums are in place
-        if (warp >= 2 && warp < 6) {
+        if (warp > NP && warp < NP + 5) {
             const int q = warp & 3;
             const int tw = tile0 % p.tiles_w, tt = tile0 / p.tiles_w;
             const int n = tw * 128 + 32 * q + lane;
@@ -369,79 +494,114 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
             const int cols = (int)(left < BN ? left : BN);
             const uint32_t mine = sbase + (uint32_t)(32 * q + lane) * 4u;
             for (int c = rank; c < cols; c += splits) {
-                float v = 0.0f;
-                for (int r = 0; r < splits; ++r) {
-                    float x;
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];"
-                                 : "=f"(x)
-                                 : "r"(tc::map_to_rank(mine + (uint32_t)c * 512u, (uint32_t)r)));
-                    v += x;
+                float x[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    x[r] = 0.0f;
+                    if (r < splits)
+                        asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                                     : "=f"(x[r])
+                                     : "r"(tc::map_to_rank(mine + (uint32_t)c * 512u, (uint32_t)r)));
                 }
-                if (n < p.N) store_out(p, ((int64_t)tt * BN + c) * p.N + n, v + bias);
+                float v[1] = {x[0]};
+#pragma unroll
+                for (int r = 1; r < 8; ++r) v[0] += x[r];
+                const int64_t o = ((int64_t)tt * BN + c) * p.N + n;
+                if (n < p.N && SNNB_IN_BOUNDS(o, (int64_t)p.rows * p.N, p.status)) {
+                    if (p.out_dtype == SNNB_F32)
+                        static_cast<float*>(p.out)[o] = v[0] + bias;
+                    else if (p.out_dtype == SNNB_F16)
+                        static_cast<__half*>(p.out)[o] = __float2half_rn(v[0] + bias);
+                    else
+                        static_cast<__nv_bfloat16*>(p.out)[o] = __float2bfloat16_rn(v[0] + bias);
+                }
             }
         }
-        tc::cluster_sync();                          // nobody reads this CTA's memory any more
     }
     tc::tc_fence_before();
     __syncthreads();
-    if (warp == 1) {
+    // neither CTA of a pair leaves while the other may signal its barriers or have its memory
+    // read by the tensor pipe; nor one of a split cluster while its partial sums are read
+    if (PAIR || splits > 1) tc::cluster_sync();
+    if (warp == NP) {
         tc::tc_fence_after();
-        tc::tmem_dealloc(tmem, S::COLS);
+        if constexpr (PAIR) tc::tmem_dealloc_pair(tmem, S::COLS);
+        else tc::tmem_dealloc(tmem, S::COLS);
     }
 }
 
-template <int FMT, int BN, int STAGES, bool SPLIT>
-int launch_mx(const CUtensorMap& tw, const CUtensorMap& ta, const MxParams& p, int splits,
+struct MxMaps {
+    CUtensorMap w, a, ws, as;
+};
+
+template <int FMT, int BN, int STAGES, bool PAIR>
+int launch_mx(const void* a, const void* as, const void* w, const void* ws, int64_t K, MxParams p,
               cudaStream_t s) {
-    using S = MxSmem<FMT, BN, STAGES>;
-    auto k = mx_linear_kernel<FMT, BN, STAGES, SPLIT>;
+    using S = MxSmem<FMT, BN, STAGES, PAIR>;
+    const uint64_t nb = (uint64_t)mx::blocks_of(K), groups = (uint64_t)p.groups;
+    MxMaps m;
+    const uint64_t wrow = nb * 16, arow = nb * mx::Fmt<FMT>::BLOCK_BYTES;
+    const uint64_t wdims[2] = {wrow, (uint64_t)p.N}, adims[2] = {arow, (uint64_t)p.rows};
+    const uint32_t wbox[2] = {128, 128}, abox[2] = {128, (uint32_t)S::A_ROWS};
+    int rc = encode_tmap(&m.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, a, adims, &arow, abox,
+                         CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc != SNNB_OK) return rc;
+    rc = encode_tmap(&m.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, w, wdims, &wrow, wbox,
+                     CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc != SNNB_OK) return rc;
+    // scale groups as [row tile][group][128 words]
+    const uint64_t str[2] = {512, groups * 512};
+    const uint64_t asdims[3] = {128, groups, (uint64_t)(p.rows + 127) / 128};
+    const uint64_t wsdims[3] = {128, groups, (uint64_t)(p.N + 127) / 128};
+    const uint32_t asbox[3] = {128, S::GROUPS, S::TOKEN_TILES}, wsbox[3] = {128, S::GROUPS, 1};
+    rc = encode_tmap(&m.as, CU_TENSOR_MAP_DATA_TYPE_INT32, 3, as, asdims, str, asbox,
+                     CU_TENSOR_MAP_SWIZZLE_NONE);
+    if (rc != SNNB_OK) return rc;
+    rc = encode_tmap(&m.ws, CU_TENSOR_MAP_DATA_TYPE_INT32, 3, ws, wsdims, str, wsbox,
+                     CU_TENSOR_MAP_SWIZZLE_NONE);
+    if (rc != SNNB_OK) return rc;
+    const int64_t width = PAIR ? 256 : 128;
+    p.tiles_w = (int)((p.N + width - 1) / width);
+    const int64_t tiles = p.tiles_w * (((int64_t)p.rows + BN - 1) / BN);
+    if (tiles > 0x7fffffff / 8) return SNNB_ERR_ARG;
+    p.tiles = (int)tiles;
+    auto k = mx_linear_kernel<FMT, BN, STAGES, PAIR>;
     const cudaError_t e =
         cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::DYN);
     if (e != cudaSuccess) return record_cuda_error(e);
-    if (SPLIT)
-        return launch_kc(k, dim3((unsigned)(p.tiles * splits)), dim3(mx_threads<FMT>()), S::DYN, s,
-                         (unsigned)splits, tw, ta, p);
-    const int grid = p.tiles < 148 ? p.tiles : 148;
-    return launch_k(k, dim3((unsigned)grid), dim3(mx_threads<FMT>()), S::DYN, s, tw, ta, p);
+    unsigned grid, cluster;
+    if (PAIR) {
+        grid = 2 * (unsigned)(tiles < 74 ? tiles : 74);
+        cluster = 2;
+    } else {
+        const int nstages = (p.groups + S::GROUPS - 1) / S::GROUPS;
+        int splits = 1;
+        while (splits < 8 && tiles * splits * 2 <= 296 && splits * 2 <= nstages) splits *= 2;
+        grid = (unsigned)(tiles * splits);
+        cluster = (unsigned)splits;
+    }
+    return launch_kc(k, dim3(grid), dim3(mx_threads<FMT>()), S::DYN, s, cluster, m.w, m.a, m.ws,
+                     m.as, p);
 }
 
 template <int FMT>
 int run_mx(const void* a, const void* as, int64_t rows, int64_t K, const void* w, const void* ws,
            int64_t N, const float* bias, void* out, int out_dtype, cudaStream_t s) {
-    int* status = device_status_ptr();
-    if (!status) return SNNB_ERR_CUDA;
-    const int64_t nb = mx::blocks_of(K);
-    const int BN = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
-    CUtensorMap tw = {}, ta = {};
-    const uint64_t wrow = (uint64_t)nb * 16, arow = (uint64_t)nb * mx::Fmt<FMT>::BLOCK_BYTES;
-    const uint64_t wdims[2] = {wrow, (uint64_t)N}, adims[2] = {arow, (uint64_t)rows};
-    const uint32_t wbox[2] = {128, 128}, abox[2] = {128, (uint32_t)BN};
-    int rc = encode_tmap(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, a, adims, &arow, abox,
-                         CU_TENSOR_MAP_SWIZZLE_128B);
-    if (rc != SNNB_OK) return rc;
-    rc = encode_tmap(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, w, wdims, &wrow, wbox,
-                     CU_TENSOR_MAP_SWIZZLE_128B);
-    if (rc != SNNB_OK) return rc;
     MxParams p = {};
+    p.status = device_status_ptr();
+    if (!p.status) return SNNB_ERR_CUDA;
     p.rows = (int)rows; p.N = (int)N; p.groups = (int)mx::groups_of(K);
-    p.tiles_w = (int)((N + 127) / 128);
-    const int64_t tiles = p.tiles_w * ((rows + BN - 1) / BN);
-    if (tiles > 0x7fffffff / 8) return SNNB_ERR_ARG;
-    p.tiles = (int)tiles;
-    p.w_row_bytes = (int64_t)wrow;
+    p.w_row_bytes = mx::blocks_of(K) * 16;
     p.w = static_cast<const uint8_t*>(w);
-    p.w_scales = static_cast<const uint8_t*>(ws);
-    p.a_scales = static_cast<const uint8_t*>(as);
-    p.bias = bias; p.out = out; p.out_dtype = out_dtype; p.status = status;
-    const int per = FMT == SNNB_MXFP4 ? 2 : 1;
-    const int nstages = (p.groups + per - 1) / per;
-    int splits = 1;
-    while (splits < 8 && tiles * splits * 2 <= 296 && splits * 2 <= nstages) splits *= 2;
-    if (BN == 16) return launch_mx<FMT, 16, 5, true>(tw, ta, p, splits, s);
-    if (BN == 32) return launch_mx<FMT, 32, 4, true>(tw, ta, p, splits, s);
-    if (BN == 64) return launch_mx<FMT, 64, 4, true>(tw, ta, p, splits, s);
-    if (BN == 128) return launch_mx<FMT, 128, 5, true>(tw, ta, p, splits, s);
-    return launch_mx<FMT, 256, 4, false>(tw, ta, p, 1, s);
+    p.bias = bias; p.out = out; p.out_dtype = out_dtype;
+    p.pairs = N % 2 == 0 && reinterpret_cast<uintptr_t>(out) % 4 == 0;
+    const int64_t tiles128 = ((N + 127) / 128) * ((rows + 127) / 128);
+    if (rows <= 16) return launch_mx<FMT, 16, 5, false>(a, as, w, ws, K, p, s);
+    if (rows <= 32) return launch_mx<FMT, 32, 4, false>(a, as, w, ws, K, p, s);
+    if (rows <= 64) return launch_mx<FMT, 64, 4, false>(a, as, w, ws, K, p, s);
+    if (rows <= 128 || tiles128 <= 74) return launch_mx<FMT, 128, 6, false>(a, as, w, ws, K, p, s);
+    if (K <= 1024) return launch_mx<FMT, 128, 7, true>(a, as, w, ws, K, p, s);
+    return launch_mx<FMT, 256, 6, true>(a, as, w, ws, K, p, s);
 }
 
 }  // namespace
