@@ -11,13 +11,16 @@
 //   a in E2M1: both operands by TMA as packed 4-bit codes, K = 256 a stage, kind::mxf4 (K = 64
 //              an MMA, two scales a row each)
 //   a in E4M3: the tokens by TMA, K = 128 a stage, kind::mxf8f6f4 (K = 32 an MMA, one scale a
-//              row), which wants 16 4-bit codes as 8 bytes in a 16-byte slot: four warps copy the
-//              weights' 8-byte pieces there with cp.async
-//   scales     512-byte groups (128 rows x 4 blocks) as they lie in memory, by bulk copies; the
-//              MMA thread copies them on to TMEM (tcgen05.cp), a slot per ring stage
+//              row), which wants 16 4-bit codes as 8 bytes in a 16-byte slot: the packed weight
+//              rows come by TMA into a second ring, and four warps, a stage each in turn, move
+//              their 8-byte pieces into the slots
+//   scales     512-byte groups (128 rows x 4 blocks) as they lie in memory; the MMA thread
+//              copies them on to TMEM (tcgen05.cp), a slot per ring stage
 //
-//   warp 0     TMA and bulk copies        warps 2-5  epilogue, thread = TMEM lane = feature
-//   warp 1     MMA issuer                 warps 6-9  (E4M3 only) weight pieces
+//   warps 0-3  one kind of load each: tokens, their scales, the weights' scales, weights
+//   warp 4     MMA issuer
+//   warps 5-   epilogue (4, or 8 for 128 tokens and more, half of the columns each), thread =
+//              TMEM lane = feature; then, for E4M3, the 4 warps that place the weight pieces
 #include "mx.cuh"
 #include "tc_common.cuh"
 
@@ -27,8 +30,6 @@ namespace {
 struct MxParams {
     int rows, N, groups;             // tokens, features, 128-wide groups of K
     int tiles_w, tiles;              // feature tiles (of 128, or 256 a pair), tiles in all
-    int64_t w_row_bytes;
-    const uint8_t* w;
     const float* bias;
     void* out;
     int out_dtype;
@@ -126,14 +127,6 @@ __device__ __forceinline__ uint32_t mbar_wait_lane_cluster(uint32_t bar, uint32_
         : "memory");
     return ok;
 }
-template <int N>
-__device__ __forceinline__ void cp_async_wait_group() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() {
-    asm volatile("cp.async.commit_group;" ::: "memory");
-}
-
 // ---- shared memory -----------------------------------------------------------------------
 template <int FMT, int BN, int STAGES, bool PAIR>
 struct MxSmem {
@@ -147,9 +140,11 @@ struct MxSmem {
     static constexpr int STAGE = W_TILE + A_TILE;                // operand tiles, 1024-aligned
     static constexpr int SCALES_OFF = STAGES * STAGE;
     static constexpr int SCALES = W_SCALES + A_SCALES;           // per stage
-    static constexpr int BAR_OFF = SCALES_OFF + STAGES * SCALES;
+    static constexpr int PACKED = FMT == SNNB_MXFP4 ? 0 : 128 * 64;  // packed weights, per stage
+    static constexpr int PACKED_OFF = SCALES_OFF + STAGES * SCALES;
+    static constexpr int BAR_OFF = PACKED_OFF + STAGES * PACKED;
     static constexpr int ACCS = BN <= 128 ? 2 : 1;               // accumulators in TMEM
-    static constexpr int NBARS = 2 * STAGES + 2 * ACCS + 1;
+    static constexpr int NBARS = (PACKED ? 4 : 2) * STAGES + 2 * ACCS + 1;
     static constexpr int TMEM_OFF = BAR_OFF + NBARS * 8;
     static constexpr int TOTAL = TMEM_OFF + 8;
     static constexpr int DYN = TOTAL + 1024;
@@ -161,55 +156,78 @@ struct MxSmem {
     static_assert(DYN <= 227 * 1024, "shared memory");
 };
 
-// Warps: the producers (one kind of load each), the MMA issuer, 4 epilogue warps, and for E4M3
-// tokens 4 that place the weight pieces.
-template <int FMT> constexpr int mx_producers() { return FMT == SNNB_MXFP4 ? 4 : 3; }
-template <int FMT> constexpr int mx_threads() {
-    return 32 * (mx_producers<FMT>() + 1 + 4 + (FMT == SNNB_MXFP4 ? 0 : 4));
+constexpr int MX_PRODUCERS = 4;
+template <int BN> constexpr int mx_epilogue_warps() { return BN >= 128 ? 8 : 4; }
+template <int FMT, int BN> constexpr int mx_threads() {
+    return 32 * (MX_PRODUCERS + 1 + mx_epilogue_warps<BN>() + (FMT == SNNB_MXFP4 ? 0 : 4));
 }
 
-// STEP accumulator columns (tokens r0 .., the first `cols` of them inside) of this lane's
-// feature n.  16-bit outputs go out in pairs of features: neighbouring lanes swap a value, so
-// that the even lane stores both features of one token and the odd lane of the next.
-template <typename O, int STEP>
-__device__ __forceinline__ void store_cols16(const MxParams& p, const float (&r)[STEP], float bias,
-                                             int n, int64_t r0, int cols) {
-    O* out = static_cast<O*>(p.out);
-    const int odd = threadIdx.x & 1;
+// One accumulator column pair (tokens i, i + 1) of a feature, rounded, as one word.
+__device__ __forceinline__ uint32_t pack16(const MxParams& p, float a, float b) {
+    return p.out_dtype == SNNB_F16 ? mx::round_pair(a, b, (const __half*)nullptr)
+                                   : mx::round_pair(a, b, (const __nv_bfloat16*)nullptr);
+}
+__device__ __forceinline__ void store_one(const MxParams& p, int64_t i, float v) {
+    if (!SNNB_IN_BOUNDS(i, (int64_t)p.rows * p.N, p.status)) return;
+    if (p.out_dtype == SNNB_F32)
+        static_cast<float*>(p.out)[i] = v;
+    else if (p.out_dtype == SNNB_F16)
+        static_cast<__half*>(p.out)[i] = __float2half_rn(v);
+    else
+        static_cast<__nv_bfloat16*>(p.out)[i] = __float2bfloat16_rn(v);
+}
+template <int N>
+__device__ __forceinline__ void tmem_load(uint32_t t, float (&r)[N]) {
+    if constexpr (N == 32) tc::tmem_ld32(t, r);
+    else tc::tmem_ld16(t, r);
+    tc::tmem_wait_ld();
+}
+
+// The accumulator columns [0, CW) at TMEM address t: tokens r0 .., the first `cols` of them
+// inside; this lane's feature is n.  `release` hands the accumulator back.
+// 16-bit outputs with an even N go out two features at a time: every column pair is rounded into
+// one word (so the accumulator is free before the first store), neighbouring lanes exchange
+// their words, and the even lane stores both features of token i, the odd lane of token i + 1.
+template <int CW, typename Release>
+__device__ __forceinline__ void store_tile(const MxParams& p, uint32_t t, float bias, int n,
+                                           int64_t r0, int cols, Release release) {
+    constexpr int STEP = CW < 32 ? 16 : 32;
+    static_assert(CW % STEP == 0, "columns");
     if (p.pairs) {
-        O* o = out + (r0 + odd) * p.N + (n & ~1);
+        uint32_t v[CW / 2];
 #pragma unroll
-        for (int i = 0; i < STEP; i += 2) {
-            const float a = r[i] + bias, b = r[i + 1] + bias;
-            const float other = __shfl_xor_sync(0xffffffffu, odd ? a : b, 1);
-            const uint32_t v = odd ? mx::round_pair(other, b, out) : mx::round_pair(a, other, out);
-            if (n < p.N && i + odd < cols &&
+        for (int c = 0; c < CW; c += STEP) {
+            float r[STEP];
+            tmem_load(t + c, r);
+#pragma unroll
+            for (int i = 0; i < STEP; i += 2)
+                v[(c + i) / 2] = pack16(p, r[i] + bias, r[i + 1] + bias);
+        }
+        release();
+        const int odd = threadIdx.x & 1;
+        const uint32_t pick = odd ? 0x3276u : 0x5410u;
+        uint32_t* o = reinterpret_cast<uint32_t*>(
+            static_cast<uint16_t*>(p.out) + (r0 + odd) * p.N + (n & ~1));
+        const bool in = n < p.N;
+        const int64_t step = p.N;                    // two rows of 16-bit values, in words
+#pragma unroll
+        for (int i = 0; i < CW; i += 2) {
+            const uint32_t w = __byte_perm(v[i / 2], __shfl_xor_sync(0xffffffffu, v[i / 2], 1), pick);
+            if (in && i + odd < cols &&
                 SNNB_IN_BOUNDS((r0 + odd + i) * p.N + n, (int64_t)p.rows * p.N, p.status))
-                *reinterpret_cast<uint32_t*>(o + (int64_t)i * p.N) = v;
+                *o = w;
+            o += step;
         }
     } else {
-        O* o = out + r0 * p.N + n;
+#pragma unroll 1
+        for (int c = 0; c < cols; c += STEP) {
+            float r[STEP];
+            tmem_load(t + c, r);
 #pragma unroll
-        for (int i = 0; i < STEP; ++i)
-            if (n < p.N && i < cols &&
-                SNNB_IN_BOUNDS((r0 + i) * p.N + n, (int64_t)p.rows * p.N, p.status))
-                mx::round_to(r[i] + bias, o + (int64_t)i * p.N);
-    }
-}
-template <int STEP>
-__device__ __forceinline__ void store_cols(const MxParams& p, const float (&r)[STEP], float bias,
-                                           int n, int64_t r0, int cols) {
-    if (p.out_dtype == SNNB_F32) {
-        float* o = static_cast<float*>(p.out) + r0 * p.N + n;
-#pragma unroll
-        for (int i = 0; i < STEP; ++i)
-            if (n < p.N && i < cols &&
-                SNNB_IN_BOUNDS((r0 + i) * p.N + n, (int64_t)p.rows * p.N, p.status))
-                o[(int64_t)i * p.N] = r[i] + bias;
-    } else if (p.out_dtype == SNNB_F16) {
-        store_cols16<__half, STEP>(p, r, bias, n, r0, cols);
-    } else {
-        store_cols16<__nv_bfloat16, STEP>(p, r, bias, n, r0, cols);
+            for (int i = 0; i < STEP; ++i)
+                if (n < p.N && c + i < cols) store_one(p, (r0 + c + i) * p.N + n, r[i] + bias);
+        }
+        release();
     }
 }
 
@@ -217,12 +235,12 @@ __device__ __forceinline__ void store_cols(const MxParams& p, const float (&r)[S
 // of the tokens) and walk whole tiles.  Otherwise: one tile, its K range split over the CTAs of
 // a cluster, their float32 partial sums joined in rank order through distributed shared memory.
 template <int FMT, int BN, int STAGES, bool PAIR>
-__global__ void __launch_bounds__(mx_threads<FMT>(), 1)
+__global__ void __launch_bounds__(mx_threads<FMT, BN>(), 1)
 mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmA,
                  const __grid_constant__ CUtensorMap tmWS, const __grid_constant__ CUtensorMap tmAS,
                  const MxParams p) {
     using S = MxSmem<FMT, BN, STAGES, PAIR>;
-    constexpr int NP = mx_producers<FMT>();
+    constexpr int NP = MX_PRODUCERS, EW = mx_epilogue_warps<BN>();
     constexpr int CTAS = PAIR ? 2 : 1;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -237,18 +255,27 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
     auto w_tile = [&](int s) { return sbase + (uint32_t)(s * S::STAGE); };
     auto a_tile = [&](int s) { return sbase + (uint32_t)(s * S::STAGE + S::W_TILE); };
     auto scales_at = [&](int s) { return sbase + (uint32_t)(S::SCALES_OFF + s * S::SCALES); };
+    // the packed weights' own ring (E4M3 tokens)
+    auto packed = [&](int s) { return sbase + (uint32_t)(S::PACKED_OFF + s * S::PACKED); };
+    auto pfull_bar = [&](int s) { return done_bar + 8u * (1 + s); };
+    auto pempty_bar = [&](int s) { return done_bar + 8u * (1 + STAGES + s); };
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + S::TMEM_OFF);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int crank = PAIR ? (int)tc::cluster_rank() : 0;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
-            tc::mbar_init(full_bar(s), NP + (FMT == SNNB_MXFP4 ? 0 : 4 * CTAS));
+            // E2M1: four loads; E4M3: three, and the warp of each CTA that placed the weights
+            tc::mbar_init(full_bar(s), FMT == SNNB_MXFP4 ? 4 : 3 + CTAS);
             tc::mbar_init(empty_bar(s), 1);
+            if constexpr (S::PACKED > 0) {
+                tc::mbar_init(pfull_bar(s), 1);
+                tc::mbar_init(pempty_bar(s), 1);
+            }
         }
         for (int b = 0; b < S::ACCS; ++b) {
             tc::mbar_init(accf_bar(b), 1);
-            tc::mbar_init(acce_bar(b), 4 * CTAS);
+            tc::mbar_init(acce_bar(b), EW * CTAS);
         }
         tc::mbar_init(done_bar, 1);
         tc::fence_mbar_init();
@@ -287,20 +314,27 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
     if (warp < NP) {
         // ------------------------------------------------------------- copies
         // Issuing a tiled copy holds its thread for ~250 cycles, so each kind has a warp of its
-        // own: 0 tokens, 1 token scales, 2 weight scales, 3 weights (E2M1 tokens).  All bytes of
-        // a stage, a pair's both halves, complete the (even CTA's) full barrier.
+        // own.  All bytes of a stage, a pair's both halves, complete the (even CTA's) full
+        // barrier; packed weights their own ring's.
         constexpr uint32_t BYTES[4] = {S::A_TILE, S::A_SCALES, S::W_SCALES, S::W_TILE};
         const uint32_t mine = (warp == 0 ? BYTES[0] : warp == 1 ? BYTES[1] : warp == 2 ? BYTES[2]
                                                                                       : BYTES[3]) *
                               (uint32_t)CTAS;
+        const bool own_ring = S::PACKED > 0 && warp == 3;
         uint32_t it = 0, issued = 0;
         for (int tile = tile0; tile < p.tiles; tile += tile_step) {
             const int tw = (tile % p.tiles_w) * CTAS + crank, tt = tile / p.tiles_w;
             for (int ks = k0; ks < k1; ++ks, ++it) {
                 const int s = (int)(it % STAGES);
-                failed |= 1u - tc::mbar_wait_warp(empty_bar(s), ((it / STAGES) & 1u) ^ 1u, failed);
+                failed |= 1u - tc::mbar_wait_warp(own_ring ? pempty_bar(s) : empty_bar(s),
+                                                  ((it / STAGES) & 1u) ^ 1u, failed);
                 if (failed) break;
-                if (tc::elect_one()) {
+                if (own_ring) {
+                    if (tc::elect_one()) {
+                        tc::mbar_expect_tx(pfull_bar(s), (uint32_t)S::PACKED);
+                        tc::tma_load_2d(packed(s), &tmW, pfull_bar(s), ks * 64, tw * 128);
+                    }
+                } else if (tc::elect_one()) {
                     if (crank == 0) tc::mbar_expect_tx(full_bar(s), mine);
                     const uint32_t fb = PAIR ? tc::map_to_rank(full_bar(s), 0) : full_bar(s);
                     if (warp == 0)
@@ -323,7 +357,8 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
             // the odd CTA of a pair (whose copies complete the even CTA's) on the stage's release
             for (uint32_t k = 0; k < issued && k < (uint32_t)STAGES; ++k) {
                 const uint32_t g = issued - 1 - k;
-                tc::mbar_wait_warp<true>(crank ? empty_bar((int)(g % STAGES)) : full_bar((int)(g % STAGES)),
+                const int s = (int)(g % STAGES);
+                tc::mbar_wait_warp<true>(own_ring ? pfull_bar(s) : crank ? empty_bar(s) : full_bar(s),
                                          (g / STAGES) & 1u, 0);
             }
         }
@@ -394,9 +429,11 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
         }
         // every MMA of this CTA's (or its pair's) has completed
         failed |= 1u - tc::mbar_wait_warp<true>(done_bar, 0, 0);
-    } else if (warp < NP + 5) {
+    } else if (warp < NP + 1 + EW) {
         // ------------------------------------------------------------- epilogue
         const int q = warp & 3;
+        constexpr int CW = BN / (EW / 4);            // columns of a warp
+        const int c0 = (warp - NP - 1) / 4 * CW;
         uint32_t local = 0;
         for (int tile = tile0; tile < p.tiles; tile += tile_step, ++local) {
             const int tw = (tile % p.tiles_w) * CTAS + crank, tt = tile / p.tiles_w;
@@ -406,94 +443,79 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
             failed |= 1u - tc::mbar_wait_warp(accf_bar(b), (local / S::ACCS) & 1u, failed);
             tc::tc_fence_after();
             if (failed) break;
-            const uint32_t t = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(b * BN);
-            constexpr int STEP = BN < 32 ? 16 : 32;
+            const uint32_t t = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(b * BN + c0);
+            auto release = [&] {
+                tc::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (PAIR) tc::mbar_arrive_cluster(tc::map_to_rank(acce_bar(b), 0));
+                    else tc::mbar_arrive(acce_bar(b));
+                }
+            };
             if (!PAIR && splits > 1) {
                 // partial sums [column][lane] in the drained ring
-                float* part = reinterpret_cast<float*>(smem) + 32 * q + lane;
+                float* part = reinterpret_cast<float*>(smem) + c0 * 128 + 32 * q + lane;
 #pragma unroll 1
-                for (int c = 0; c < BN; c += 16) {
+                for (int c = 0; c < CW; c += 16) {
                     float r[16];
-                    tc::tmem_ld16(t + c, r);
-                    tc::tmem_wait_ld();
+                    tmem_load(t + c, r);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) part[(c + i) * 128] = r[i];
                 }
+                release();
             } else {
-                const int64_t left = (int64_t)p.rows - (int64_t)tt * BN;
-                const int cols = (int)(left < BN ? left : BN);
-#pragma unroll 1
-                for (int c = 0; c < cols; c += STEP) {
-                    float r[STEP];
-                    if constexpr (STEP == 32) tc::tmem_ld32(t + c, r);
-                    else tc::tmem_ld16(t + c, r);
-                    tc::tmem_wait_ld();
-                    store_cols<STEP>(p, r, bias, n, (int64_t)tt * BN + c, cols - c);
-                }
-            }
-            tc::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                if constexpr (PAIR) tc::mbar_arrive_cluster(tc::map_to_rank(acce_bar(b), 0));
-                else tc::mbar_arrive(acce_bar(b));
+                const int64_t r0 = (int64_t)tt * BN + c0;
+                const int64_t left = (int64_t)p.rows - r0;
+                store_tile<CW>(p, t, bias, n, r0, (int)(left < CW ? left : CW), release);
             }
         }
     } else {
         // ------------------------------------------------------------- weight pieces (E4M3)
-        // 16 codes (8 bytes) to the low half of a 16-byte slot; slot c of row r at c ^ (r % 8)
-        constexpr int AHEAD = STAGES - 2;
-        auto publish = [&](uint32_t g) {
-            if (lane != 0) return;
-            const uint32_t bar = full_bar((int)(g % STAGES));
-            if constexpr (PAIR) tc::mbar_arrive_cluster(tc::map_to_rank(bar, 0));
-            else tc::mbar_arrive(bar);
-        };
-        const int i = (warp - NP - 5) * 32 + lane;
-        const int c = i & 7;
+        // Warp w takes the stages w, w + 4, ...: 16 codes (8 bytes) to the low half of a
+        // 16-byte slot, slot c of row r at c ^ (r % 8).
+        static_assert(FMT == SNNB_MXFP4 || STAGES >= 4, "a warp never laps the ring");
+        const uint32_t w = (uint32_t)(warp - NP - 1 - EW);
         uint32_t it = 0;
-        for (int tile = tile0; tile < p.tiles; tile += tile_step) {
-            const int64_t n0 = (int64_t)((tile % p.tiles_w) * CTAS + crank) * 128;
+        for (int tile = tile0; tile < p.tiles && !failed; tile += tile_step) {
             for (int ks = k0; ks < k1; ++ks, ++it) {
+                if ((it & 3u) != w) continue;
                 const int s = (int)(it % STAGES);
-                failed |= 1u - tc::mbar_wait_warp(empty_bar(s), ((it / STAGES) & 1u) ^ 1u, failed);
+                const uint32_t ph = (it / STAGES) & 1u;
+                failed |= 1u - tc::mbar_wait_warp(pfull_bar(s), ph, failed);
+                failed |= 1u - tc::mbar_wait_warp(empty_bar(s), ph ^ 1u, failed);
                 if (failed) break;
-                const int64_t kb = (int64_t)ks * 64 + c * 8;
-                const uint32_t dst = w_tile(s);
+                const uint8_t* src = smem + S::PACKED_OFF + s * S::PACKED + lane * 16;
+                uint8_t* dst = smem + s * S::STAGE + (lane >> 2) * 128;
+                const int c = (lane & 3) * 2, x = lane >> 2;         // row u * 8 + x
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    const int r = u * 16 + (i >> 3);
-                    const bool in = n0 + r < p.N && kb < p.w_row_bytes;
-                    tc::cp_async_8(dst + r * 128 + ((c ^ (r & 7)) << 4),
-                                   p.w + (in ? (n0 + r) * p.w_row_bytes + kb : 0), in ? 8u : 0u);
+                for (int u = 0; u < 16; ++u) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(src + u * 512);
+                    *reinterpret_cast<uint2*>(dst + u * 1024 + ((c ^ x) << 4)) = make_uint2(v.x, v.y);
+                    *reinterpret_cast<uint2*>(dst + u * 1024 + (((c + 1) ^ x) << 4)) =
+                        make_uint2(v.z, v.w);
                 }
-                cp_async_commit();
-                if (it >= (uint32_t)AHEAD) {
-                    cp_async_wait_group<AHEAD>();
-                    tc::fence_proxy_async_smem();
-                    __syncwarp();
-                    publish(it - AHEAD);
+                tc::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    tc::mbar_arrive(pempty_bar(s));
+                    if constexpr (PAIR) tc::mbar_arrive_cluster(tc::map_to_rank(full_bar(s), 0));
+                    else tc::mbar_arrive(full_bar(s));
                 }
             }
-            if (failed) break;
         }
-        tc::cp_async_wait_all();
-        tc::fence_proxy_async_smem();
-        __syncwarp();
-        if (!failed)
-            for (uint32_t g = it > (uint32_t)AHEAD ? it - AHEAD : 0; g < it; ++g) publish(g);
     }
     if (failed && lane == 0) atomicExch(p.status, SNNB_ERR_TIMEOUT);
     if (!PAIR && splits > 1) {
         tc::cluster_sync();                          // every CTA's partial sums are in place
-        if (warp > NP && warp < NP + 5) {
-            const int q = warp & 3;
+        if (warp > NP && warp < NP + 1 + EW) {
+            const int q = warp & 3, half = (warp - NP - 1) / 4;
             const int tw = tile0 % p.tiles_w, tt = tile0 / p.tiles_w;
             const int n = tw * 128 + 32 * q + lane;
             const float bias = p.bias && n < p.N ? __ldg(p.bias + n) : 0.0f;
             const int64_t left = (int64_t)p.rows - (int64_t)tt * BN;
             const int cols = (int)(left < BN ? left : BN);
             const uint32_t mine = sbase + (uint32_t)(32 * q + lane) * 4u;
-            for (int c = rank; c < cols; c += splits) {
+            for (int c = rank * (EW / 4) + half; c < cols; c += splits * (EW / 4)) {
                 float x[8];
 #pragma unroll
                 for (int r = 0; r < 8; ++r) {
@@ -503,18 +525,10 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
                                      : "=f"(x[r])
                                      : "r"(tc::map_to_rank(mine + (uint32_t)c * 512u, (uint32_t)r)));
                 }
-                float v[1] = {x[0]};
+                float v = x[0];
 #pragma unroll
-                for (int r = 1; r < 8; ++r) v[0] += x[r];
-                const int64_t o = ((int64_t)tt * BN + c) * p.N + n;
-                if (n < p.N && SNNB_IN_BOUNDS(o, (int64_t)p.rows * p.N, p.status)) {
-                    if (p.out_dtype == SNNB_F32)
-                        static_cast<float*>(p.out)[o] = v[0] + bias;
-                    else if (p.out_dtype == SNNB_F16)
-                        static_cast<__half*>(p.out)[o] = __float2half_rn(v[0] + bias);
-                    else
-                        static_cast<__nv_bfloat16*>(p.out)[o] = __float2bfloat16_rn(v[0] + bias);
-                }
+                for (int r = 1; r < 8; ++r) v += x[r];
+                if (n < p.N) store_one(p, ((int64_t)tt * BN + c) * p.N + n, v + bias);
             }
         }
     }
@@ -542,12 +556,12 @@ int launch_mx(const void* a, const void* as, const void* w, const void* ws, int6
     MxMaps m;
     const uint64_t wrow = nb * 16, arow = nb * mx::Fmt<FMT>::BLOCK_BYTES;
     const uint64_t wdims[2] = {wrow, (uint64_t)p.N}, adims[2] = {arow, (uint64_t)p.rows};
-    const uint32_t wbox[2] = {128, 128}, abox[2] = {128, (uint32_t)S::A_ROWS};
+    const uint32_t wbox[2] = {FMT == SNNB_MXFP4 ? 128u : 64u, 128}, abox[2] = {128, (uint32_t)S::A_ROWS};
     int rc = encode_tmap(&m.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, a, adims, &arow, abox,
                          CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != SNNB_OK) return rc;
     rc = encode_tmap(&m.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, w, wdims, &wrow, wbox,
-                     CU_TENSOR_MAP_SWIZZLE_128B);
+                     FMT == SNNB_MXFP4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE);
     if (rc != SNNB_OK) return rc;
     // scale groups as [row tile][group][128 words]
     const uint64_t str[2] = {512, groups * 512};
@@ -580,7 +594,7 @@ int launch_mx(const void* a, const void* as, const void* w, const void* ws, int6
         grid = (unsigned)(tiles * splits);
         cluster = (unsigned)splits;
     }
-    return launch_kc(k, dim3(grid), dim3(mx_threads<FMT>()), S::DYN, s, cluster, m.w, m.a, m.ws,
+    return launch_kc(k, dim3(grid), dim3(mx_threads<FMT, BN>()), S::DYN, s, cluster, m.w, m.a, m.ws,
                      m.as, p);
 }
 
@@ -591,17 +605,17 @@ int run_mx(const void* a, const void* as, int64_t rows, int64_t K, const void* w
     p.status = device_status_ptr();
     if (!p.status) return SNNB_ERR_CUDA;
     p.rows = (int)rows; p.N = (int)N; p.groups = (int)mx::groups_of(K);
-    p.w_row_bytes = mx::blocks_of(K) * 16;
-    p.w = static_cast<const uint8_t*>(w);
     p.bias = bias; p.out = out; p.out_dtype = out_dtype;
-    p.pairs = N % 2 == 0 && reinterpret_cast<uintptr_t>(out) % 4 == 0;
+    p.pairs = out_dtype != SNNB_F32 && N % 2 == 0 && reinterpret_cast<uintptr_t>(out) % 4 == 0;
     const int64_t tiles128 = ((N + 127) / 128) * ((rows + 127) / 128);
-    if (rows <= 16) return launch_mx<FMT, 16, 5, false>(a, as, w, ws, K, p, s);
+    constexpr bool F4 = FMT == SNNB_MXFP4;
+    if (rows <= 16) return launch_mx<FMT, 16, F4 ? 5 : 4, false>(a, as, w, ws, K, p, s);
     if (rows <= 32) return launch_mx<FMT, 32, 4, false>(a, as, w, ws, K, p, s);
     if (rows <= 64) return launch_mx<FMT, 64, 4, false>(a, as, w, ws, K, p, s);
-    if (rows <= 128 || tiles128 <= 74) return launch_mx<FMT, 128, 6, false>(a, as, w, ws, K, p, s);
-    if (K <= 1024) return launch_mx<FMT, 128, 7, true>(a, as, w, ws, K, p, s);
-    return launch_mx<FMT, 256, 6, true>(a, as, w, ws, K, p, s);
+    if (rows <= 128 || tiles128 <= 74)
+        return launch_mx<FMT, 128, F4 ? 6 : 5, false>(a, as, w, ws, K, p, s);
+    if (K <= 1024) return launch_mx<FMT, 128, F4 ? 7 : 6, true>(a, as, w, ws, K, p, s);
+    return launch_mx<FMT, 256, F4 ? 6 : 5, true>(a, as, w, ws, K, p, s);
 }
 
 }  // namespace
