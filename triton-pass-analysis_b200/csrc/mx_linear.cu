@@ -19,8 +19,8 @@
 //
 //   warps 0-3  one kind of load each: tokens, their scales, the weights' scales, weights
 //   warp 4     MMA issuer
-//   warps 5-   epilogue (4, or 8 for 128 tokens and more, half of the columns each), thread =
-//              TMEM lane = feature; then, for E4M3, the 4 warps that place the weight pieces
+//   warps 5-   epilogue (4 per 64 tokens), thread = TMEM lane = feature; then, for E4M3, the 4
+//              warps that place the weight pieces
 #include "mx.cuh"
 #include "tc_common.cuh"
 
@@ -131,12 +131,13 @@ struct MxSmem {
     static constexpr int SCALE_COLS = 4 * GROUPS * (1 + TOKEN_TILES);
     static constexpr int COLS_USED = ACCS * BN + STAGES * SCALE_COLS;
     static constexpr int COLS = COLS_USED <= 128 ? 128 : (COLS_USED <= 256 ? 256 : 512);
+    static constexpr int CTAS_PER_SM = COLS <= 256 && (DYN + 1024) * 2 <= 228 * 1024 ? 2 : 1;
     static_assert(COLS_USED <= 512, "tensor memory");
     static_assert(DYN <= 227 * 1024, "shared memory");
 };
 
 constexpr int MX_PRODUCERS = 4;
-template <int BN> constexpr int mx_epilogue_warps() { return BN >= 128 ? 8 : 4; }
+template <int BN> constexpr int mx_epilogue_warps() { return BN <= 64 ? 4 : BN / 16; }
 template <int FMT, int BN> constexpr int mx_threads() {
     return 32 * (MX_PRODUCERS + 1 + mx_epilogue_warps<BN>() + (FMT == SNNB_MXFP4 ? 0 : 4));
 }
@@ -155,34 +156,37 @@ __device__ __forceinline__ void store_one(const MxParams& p, int64_t i, float v)
     else
         static_cast<__nv_bfloat16*>(p.out)[i] = __float2bfloat16_rn(v);
 }
+// N accumulator columns of this thread's lane; complete on return.
 template <int N>
 __device__ __forceinline__ void tmem_load(uint32_t t, float (&r)[N]) {
-    if constexpr (N == 32) tc::tmem_ld32(t, r);
-    else tc::tmem_ld16(t, r);
+    constexpr int STEP = N < 32 ? 16 : 32;
+    static_assert(N % STEP == 0, "columns");
+    float part[N / STEP][STEP];
+#pragma unroll
+    for (int i = 0; i < N / STEP; ++i) {
+        if constexpr (STEP == 32) tc::tmem_ld32(t + i * STEP, part[i]);
+        else tc::tmem_ld16(t + i * STEP, part[i]);
+    }
     tc::tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        asm volatile("" : "+f"(part[i / STEP][i % STEP]));       // no use moves before the wait
+        r[i] = part[i / STEP][i % STEP];
+    }
 }
 
 // The accumulator columns [0, CW) at TMEM address t: tokens r0 .., the first `cols` of them
-// inside; this lane's feature is n.  `release` hands the accumulator back.
-// 16-bit outputs with an even N go out two features at a time: every column pair is rounded into
-// one word (so the accumulator is free before the first store), neighbouring lanes exchange
-// their words, and the even lane stores both features of token i, the odd lane of token i + 1.
+// inside; this lane's feature is n.  `release` hands the accumulator back, as soon as it has been
+// read.  16-bit outputs with an even N go out two features at a time: a column pair is rounded
+// into one word, neighbouring lanes exchange their words, and the even lane stores both features
+// of token i, the odd lane of token i + 1.
 template <int CW, typename Release>
 __device__ __forceinline__ void store_tile(const MxParams& p, uint32_t t, float bias, int n,
                                            int64_t r0, int cols, Release release) {
-    constexpr int STEP = CW < 32 ? 16 : 32;
-    static_assert(CW % STEP == 0, "columns");
+    float r[CW];
+    tmem_load(t, r);
+    release();
     if (p.pairs) {
-        uint32_t v[CW / 2];
-#pragma unroll
-        for (int c = 0; c < CW; c += STEP) {
-            float r[STEP];
-            tmem_load(t + c, r);
-#pragma unroll
-            for (int i = 0; i < STEP; i += 2)
-                v[(c + i) / 2] = pack16(p, r[i] + bias, r[i + 1] + bias);
-        }
-        release();
         const int odd = threadIdx.x & 1;
         const uint32_t pick = odd ? 0x3276u : 0x5410u;
         uint32_t* o = reinterpret_cast<uint32_t*>(
@@ -191,22 +195,17 @@ __device__ __forceinline__ void store_tile(const MxParams& p, uint32_t t, float 
         const int64_t step = p.N;                    // two rows of 16-bit values, in words
 #pragma unroll
         for (int i = 0; i < CW; i += 2) {
-            const uint32_t w = __byte_perm(v[i / 2], __shfl_xor_sync(0xffffffffu, v[i / 2], 1), pick);
+            const uint32_t v = pack16(p, r[i] + bias, r[i + 1] + bias);
+            const uint32_t w = __byte_perm(v, __shfl_xor_sync(0xffffffffu, v, 1), pick);
             if (in && i + odd < cols &&
                 SNNB_IN_BOUNDS((r0 + odd + i) * p.N + n, (int64_t)p.rows * p.N, p.status))
                 *o = w;
             o += step;
         }
     } else {
-#pragma unroll 1
-        for (int c = 0; c < cols; c += STEP) {
-            float r[STEP];
-            tmem_load(t + c, r);
 #pragma unroll
-            for (int i = 0; i < STEP; ++i)
-                if (n < p.N && c + i < cols) store_one(p, (r0 + c + i) * p.N + n, r[i] + bias);
-        }
-        release();
+        for (int i = 0; i < CW; ++i)
+            if (n < p.N && i < cols) store_one(p, (r0 + i) * p.N + n, r[i] + bias);
     }
 }
 
@@ -214,7 +213,7 @@ __device__ __forceinline__ void store_tile(const MxParams& p, uint32_t t, float 
 // of the tokens) and walk whole tiles.  Otherwise: one tile, its K range split over the CTAs of
 // a cluster, their float32 partial sums joined in rank order through distributed shared memory.
 template <int FMT, int BN, int STAGES, bool PAIR>
-__global__ void __launch_bounds__(mx_threads<FMT, BN>(), 1)
+__global__ void __launch_bounds__(mx_threads<FMT, BN>(), MxSmem<FMT, BN, STAGES, PAIR>::CTAS_PER_SM)
 mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmA,
                  const __grid_constant__ CUtensorMap tmWS, const __grid_constant__ CUtensorMap tmAS,
                  const MxParams p) {
@@ -464,11 +463,17 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
                 uint8_t* dst = smem + s * S::STAGE + (lane >> 2) * 128;
                 const int c = (lane & 3) * 2, x = lane >> 2;         // row u * 8 + x
 #pragma unroll
-                for (int u = 0; u < 16; ++u) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(src + u * 512);
-                    *reinterpret_cast<uint2*>(dst + u * 1024 + ((c ^ x) << 4)) = make_uint2(v.x, v.y);
-                    *reinterpret_cast<uint2*>(dst + u * 1024 + (((c + 1) ^ x) << 4)) =
-                        make_uint2(v.z, v.w);
+                for (int h = 0; h < 16; h += 8) {
+                    uint4 v[8];                      // loads ahead of the stores
+#pragma unroll
+                    for (int u = 0; u < 8; ++u)
+                        v[u] = *reinterpret_cast<const uint4*>(src + (h + u) * 512);
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        uint8_t* d = dst + (h + u) * 1024;
+                        *reinterpret_cast<uint2*>(d + ((c ^ x) << 4)) = make_uint2(v[u].x, v[u].y);
+                        *reinterpret_cast<uint2*>(d + (((c + 1) ^ x) << 4)) = make_uint2(v[u].z, v[u].w);
+                    }
                 }
                 tc::fence_proxy_async_smem();
                 __syncwarp();
@@ -491,20 +496,29 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
             const int64_t left = (int64_t)p.rows - (int64_t)tt * BN;
             const int cols = (int)(left < BN ? left : BN);
             const uint32_t mine = sbase + (uint32_t)(32 * q + lane) * 4u;
-            for (int c = rank * (EW / 4) + half; c < cols; c += splits * (EW / 4)) {
-                float x[8];
+            // four columns of every rank in flight
+            const int step = splits * (EW / 4);
+            for (int c = rank * (EW / 4) + half; c < cols; c += 4 * step) {
+                float x[4][8];
 #pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    x[r] = 0.0f;
-                    if (r < splits)
-                        asm volatile("ld.shared::cluster.f32 %0, [%1];"
-                                     : "=f"(x[r])
-                                     : "r"(tc::map_to_rank(mine + (uint32_t)c * 512u, (uint32_t)r)));
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) {
+                        x[i][r] = 0.0f;
+                        if (r < splits && c + i * step < cols)
+                            asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                                         : "=f"(x[i][r])
+                                         : "r"(tc::map_to_rank(mine + (uint32_t)(c + i * step) * 512u,
+                                                               (uint32_t)r)));
+                    }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float v = x[i][0];
+#pragma unroll
+                    for (int r = 1; r < 8; ++r) v += x[i][r];
+                    if (n < p.N && c + i * step < cols)
+                        store_one(p, ((int64_t)tt * BN + c + i * step) * p.N + n, v + bias);
                 }
-                float v = x[0];
-#pragma unroll
-                for (int r = 1; r < 8; ++r) v += x[r];
-                if (n < p.N) store_one(p, ((int64_t)tt * BN + c) * p.N + n, v + bias);
             }
         }
     }
@@ -566,7 +580,8 @@ int launch_mx(const void* a, const void* as, const void* w, const void* ws, int6
     } else {
         const int nstages = (p.groups + S::GROUPS - 1) / S::GROUPS;
         int splits = 1;
-        while (splits < 8 && tiles * splits * 2 <= 296 && splits * 2 <= nstages) splits *= 2;
+        while (splits < 8 && tiles * splits * 2 <= 148 * S::CTAS_PER_SM && splits * 2 <= nstages)
+            splits *= 2;
         grid = (unsigned)(tiles * splits);
         cluster = (unsigned)splits;
     }
@@ -583,14 +598,17 @@ int run_mx(const void* a, const void* as, int64_t rows, int64_t K, const void* w
     p.rows = (int)rows; p.N = (int)N; p.groups = (int)mx::groups_of(K);
     p.bias = bias; p.out = out; p.out_dtype = out_dtype;
     p.pairs = out_dtype != SNNB_F32 && N % 2 == 0 && reinterpret_cast<uintptr_t>(out) % 4 == 0;
-    const int64_t tiles128 = ((N + 127) / 128) * ((rows + 127) / 128);
     constexpr bool F4 = FMT == SNNB_MXFP4;
     if (rows <= 16) return launch_mx<FMT, 16, F4 ? 5 : 4, false>(a, as, w, ws, K, p, s);
     if (rows <= 32) return launch_mx<FMT, 32, 4, false>(a, as, w, ws, K, p, s);
     if (rows <= 64) return launch_mx<FMT, 64, 4, false>(a, as, w, ws, K, p, s);
-    if (rows <= 128 || tiles128 <= 74)
-        return launch_mx<FMT, 128, F4 ? 6 : 5, false>(a, as, w, ws, K, p, s);
-    if (K <= 1024) return launch_mx<FMT, 128, F4 ? 7 : 6, true>(a, as, w, ws, K, p, s);
+    if (rows <= 128) return launch_mx<FMT, 128, F4 ? 6 : 5, false>(a, as, w, ws, K, p, s);
+    // Pairs, 74 at once.  128 tokens a tile where that still fits one round, and for short K,
+    // where the second accumulator hides the stores (8192 x 8192, K = 512: 35 us against 43 with
+    // 256; K = 2048: 78 against 68); 256 otherwise.
+    const int64_t pw = (N + 255) / 256;
+    if (pw * ((rows + 127) / 128) <= 74 || (K <= 768 && pw * ((rows + 255) / 256) > 74))
+        return launch_mx<FMT, 128, F4 ? 7 : 6, true>(a, as, w, ws, K, p, s);
     return launch_mx<FMT, 256, F4 ? 6 : 5, true>(a, as, w, ws, K, p, s);
 }
 
