@@ -35,6 +35,16 @@ template <> struct Fmt<SNNB_MXFP8> {
 __host__ __device__ __forceinline__ int64_t blocks_of(int64_t K) { return (K + BLOCK - 1) / BLOCK; }
 __host__ __device__ __forceinline__ int64_t groups_of(int64_t K) { return (blocks_of(K) + 3) / 4; }
 
+// Largest extents: indexes of blocks (rows padded to groups of 4) and of scale words stay below
+// 2^31, byte offsets are 64-bit; row strides up to 2^40 elements in all.
+inline bool sizes_ok(int64_t rows, int64_t K) {
+    return rows >= 0 && K >= 1 && K <= 0x7fffffff - 255 && rows <= 0x7fffffff - 127 &&
+           (rows + 127) * (groups_of(K) * 4) <= 0x7fffffff;
+}
+inline bool stride_ok(int64_t rows, int64_t ld) {
+    return ld >= 0 && (rows <= 1 || ld <= (int64_t(1) << 40) / rows);
+}
+
 // 8 floats, already multiplied by the inverse scale, to codes: round to nearest, ties to even,
 // magnitudes above the largest element become the largest.
 __device__ __forceinline__ void encode8(const float (&v)[8], uint32_t& c) {
@@ -99,28 +109,49 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
     return byte == 0 ? __int_as_float(0x00400000) : __int_as_float((int)(byte << 23));
 }
 
-// One block of 32 values held by 4 neighbouring lanes, 8 each: the scale byte is
-// floor(log2(largest magnitude)) - EMAX as an exponent, i.e. the exponent field of the largest
-// magnitude's float minus EMAX (0 for a block of zeros or float subnormals).  A block that holds
-// an infinity or a NaN gets the byte 255 (NaN) and zero codes.  Every lane of the warp calls.
-template <int FMT>
-__device__ __forceinline__ uint32_t quantise_block(const float (&x)[8],
-                                                   typename Fmt<FMT>::Codes8& codes) {
-    // magnitudes compare as integers, and an infinity or NaN is above every finite value
+// ---- quantising a block of 32 values held by 4 neighbouring lanes, 8 each ----------------
+// Every lane of the warp calls.  The scale byte is floor(log2(largest magnitude)) - EMAX as an
+// exponent: the exponent field of the largest magnitude's float minus EMAX, 0 for a block of
+// zeros or float subnormals.  A block that holds an infinity or a NaN gets the byte 255 (NaN)
+// and zero codes.
+
+// The largest magnitude's exponent field among 8 values.  Magnitudes compare as integers, and an
+// infinity or NaN is above every finite value.
+__device__ __forceinline__ uint32_t top_exponent(const float (&x)[8]) {
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = max(top, (uint32_t)__float_as_int(x[i]) & 0x7FFFFFFFu);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const uint32_t e = top >> 23;
-    const uint32_t byte = e == 255 ? 255u : (e > (uint32_t)Fmt<FMT>::EMAX ? e - Fmt<FMT>::EMAX : 0u);
-    // 1 / scale = 2^(127 - byte), exact and normal for byte <= 253; a product that leaves the
+    return top >> 23;
+}
+
+// The same from the raw values.  bfloat16 has float's exponent field: compare pairs.
+template <typename T> struct Raw8;
+template <typename T>
+__device__ __forceinline__ uint32_t top_exponent(const Raw8<T>&, const float (&x)[8]) {
+    return top_exponent(x);
+}
+__device__ __forceinline__ uint32_t top_exponent(const Raw8<__nv_bfloat16>& r, const float (&x)[8]);
+
+template <int FMT>
+__device__ __forceinline__ uint32_t quantise_block(const float (&x)[8], uint32_t exponent,
+                                                   typename Fmt<FMT>::Codes8& codes) {
+    uint32_t e = max(exponent, __shfl_xor_sync(0xffffffffu, exponent, 1));
+    e = max(e, __shfl_xor_sync(0xffffffffu, e, 2));
+    const bool bad = e == 255;
+    const uint32_t byte = bad ? 255u : (e > (uint32_t)Fmt<FMT>::EMAX ? e - Fmt<FMT>::EMAX : 0u);
+    // 1 / scale = 2^(127 - byte), exact and normal (byte <= 252); a product that leaves the
     // normal range is far below the smallest element and rounds to zero either way
     const float inv = __int_as_float((int)((254u - byte) << 23));
     float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = byte == 255 ? 0.0f : x[i] * inv;
+    for (int i = 0; i < 8; ++i) v[i] = x[i] * inv;
     encode8(v, codes);
+    if constexpr (FMT == SNNB_MXFP4) {
+        codes = bad ? 0u : codes;
+    } else {
+        codes.x = bad ? 0u : codes.x;
+        codes.y = bad ? 0u : codes.y;
+    }
     return byte;
 }
 
@@ -134,56 +165,35 @@ __device__ __forceinline__ uint32_t join_scales(uint32_t byte, int lane) {
 }
 
 // Index of the 4-byte word of row `row`, group `g` along K (blocks 4 g .. 4 g + 3).
-__device__ __forceinline__ int64_t scale_word(int64_t row, int64_t g, int64_t groups) {
+__device__ __forceinline__ uint32_t scale_word(uint32_t row, uint32_t g, uint32_t groups) {
     return ((row >> 7) * groups + g) * (GROUP_BYTES / 4) + (row & 31) * 4 + ((row >> 5) & 3);
 }
 
-// Walks the blocks of a tensor: block index q = row * per_row + j, advanced by a fixed step
-// with one division at the start.
-struct BlockWalk {
-    int64_t row, j, drow, dj, per_row;
-    __device__ BlockWalk(int64_t q, int64_t step, int64_t per_row_) : per_row(per_row_) {
-        row = q / per_row;
-        j = q - row * per_row;
-        drow = step / per_row;
-        dj = step - drow * per_row;
-    }
-    __device__ void next() {
-        row += drow;
-        j += dj;
-        if (j >= per_row) {
-            j -= per_row;
-            ++row;
-        }
-    }
-};
-
-// The scale bytes of rows past the tensor's last one, in its last row tile: zero.
-__device__ __forceinline__ void zero_row_padding(uint32_t* scales, int64_t rows, int64_t groups,
-                                                 int64_t thread, int64_t threads) {
-    const int64_t pad = ((rows + 127) & ~int64_t(127)) - rows;
-    const int64_t words = pad * groups;
-    if (thread >= words) return;
-    for (BlockWalk w(thread, threads, groups); w.row < pad; w.next())
-        scales[scale_word(rows + w.row, w.j, groups)] = 0;
+// The scale bytes of rows past the tensor's last one, in its last row tile: zero.  All threads
+// of the grid share the work.
+__device__ __forceinline__ void zero_row_padding(uint32_t* scales, uint32_t rows, uint32_t groups,
+                                                 uint64_t thread, uint64_t threads) {
+    const uint32_t pad = (0u - rows) & 127u;
+    for (uint64_t i = thread; i < (uint64_t)pad * groups; i += threads)
+        scales[scale_word(rows + (uint32_t)(i % pad), (uint32_t)(i / pad), groups)] = 0;
 }
 
-// 8 consecutive elements at p as floats; `n` of them lie inside the row (0..8; the others read
-// as zero).  VEC: p is 16-byte aligned and n is 0 or 8.
-template <bool VEC>
-__device__ __forceinline__ void load8(const float* p, int n, float (&v)[8]) {
-    if (VEC) {
-        float4 a = make_float4(0, 0, 0, 0), b = a;
-        if (n > 0) {
-            a = __ldg(reinterpret_cast<const float4*>(p));
-            b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-        }
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < n ? __ldg(p + i) : 0.0f;
-    }
+// ---- 8 values of a row -------------------------------------------------------------------
+template <typename T> struct Raw8 { uint4 v[sizeof(T) / 2]; };      // 16 bytes, 32 for float
+__device__ __forceinline__ uint32_t top_exponent(const Raw8<__nv_bfloat16>& r, const float (&)[8]) {
+    const uint32_t m = 0x7FFF7FFFu;
+    const uint32_t t = __vmaxu2(__vmaxu2(r.v[0].x & m, r.v[0].y & m),
+                                __vmaxu2(r.v[0].z & m, r.v[0].w & m));
+    return max(t >> 16, t & 0xFFFFu) >> 7;
+}
+
+// Streaming 16-byte load: read once, not kept in L1.
+__device__ __forceinline__ uint4 load16(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
 }
 __device__ __forceinline__ float2 pair_f32(uint32_t u, const __half*) {
     return __half22float2(*reinterpret_cast<const __half2*>(&u));
@@ -191,22 +201,22 @@ __device__ __forceinline__ float2 pair_f32(uint32_t u, const __half*) {
 __device__ __forceinline__ float2 pair_f32(uint32_t u, const __nv_bfloat16*) {
     return make_float2(__int_as_float((int)(u << 16)), __int_as_float((int)(u & 0xFFFF0000u)));
 }
-template <bool VEC, typename T>
-__device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]) {
-    if (VEC) {
-        uint4 a = make_uint4(0, 0, 0, 0);
-        if (n > 0) a = __ldg(reinterpret_cast<const uint4*>(p));
-        const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+template <typename T>
+__device__ __forceinline__ void to_floats(const Raw8<T>& r, float (&v)[8]) {
+    const uint32_t u[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = pair_f32(u[i], p);
-            v[2 * i] = f.x;
-            v[2 * i + 1] = f.y;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i]) : 0.0f;
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = pair_f32(u[i], (const T*)nullptr);
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
     }
+}
+template <>
+__device__ __forceinline__ void to_floats(const Raw8<float>& r, float (&v)[8]) {
+    const uint32_t u[8] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w,
+                           r.v[1].x, r.v[1].y, r.v[1].z, r.v[1].w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __int_as_float((int)u[i]);
 }
 
 __device__ __forceinline__ uint32_t round_pair(float a, float b, const __half*) {
@@ -217,36 +227,156 @@ __device__ __forceinline__ uint32_t round_pair(float a, float b, const __nv_bflo
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+template <typename T>
+__device__ __forceinline__ void from_floats(const float (&v)[8], Raw8<T>& r) {
+    const T* t = nullptr;
+    r.v[0] = make_uint4(round_pair(v[0], v[1], t), round_pair(v[2], v[3], t),
+                        round_pair(v[4], v[5], t), round_pair(v[6], v[7], t));
+}
+template <>
+__device__ __forceinline__ void from_floats(const float (&v)[8], Raw8<float>& r) {
+    uint32_t u[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u[i] = (uint32_t)__float_as_int(v[i]);
+    r.v[0] = make_uint4(u[0], u[1], u[2], u[3]);
+    r.v[1] = make_uint4(u[4], u[5], u[6], u[7]);
+}
+
+// 16-byte aligned p.
+template <typename T>
+__device__ __forceinline__ Raw8<T> load_aligned8(const T* p) {
+    Raw8<T> r;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.v[i] = load16(reinterpret_cast<const uint4*>(p) + i);
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void store_aligned8(T* p, const Raw8<T>& r) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = r.v[i];
+}
+template <typename T>
+__device__ __forceinline__ Raw8<T> zero8() {
+    Raw8<T> r;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.v[i] = make_uint4(0, 0, 0, 0);
+    return r;
+}
+
+// 8 values at p, only aligned to an element, the first n of them (0..8) inside the row, whose
+// elements are [row, row + K): two (float: three) aligned 16-byte loads around them where those
+// lie inside the row, else one load per element.  Values past n are zero.
+template <typename T>
+__device__ __forceinline__ Raw8<T> load_any8(const T* p, int n, const T* row, int64_t K) {
+    constexpr int W = (int)sizeof(T) * 2;                        // words of 8 values
+    uint32_t w[W + 4];
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p), down = at & ~uintptr_t(15);
+    const uint32_t off = (uint32_t)(at & 15);
+    if (n == 8 && down >= reinterpret_cast<uintptr_t>(row) &&
+        down + W * 4 + (off ? 16 : 0) <= reinterpret_cast<uintptr_t>(row + K)) {
+#pragma unroll
+        for (int i = 0; i < W / 4 + 1; ++i) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (i < W / 4 || off) v = __ldg(reinterpret_cast<const uint4*>(down) + i);
+            w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+        }
+        // shift right by off bytes: whole words first, then the odd half word
+#pragma unroll
+        for (int i = 0; i < W + 2; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
+#pragma unroll
+        for (int i = 0; i < W + 1; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
+        if (sizeof(T) == 2) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (off & 2) * 8);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (i >= n) continue;
+            if (sizeof(T) == 2)
+                w[i / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(p) + i) << (16 * (i & 1));
+            else
+                w[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
+        }
+    }
+    Raw8<T> r;
+#pragma unroll
+    for (int i = 0; i < W / 4; ++i)
+        r.v[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    return r;
+}
+
+// The counterpart store, of a whole warp: lane l holds 8 values for p (its own address, 8 l
+// elements after lane 0's), the first n inside the row; lanes past a partial one have n <= 0.
+// Aligned 16-byte pieces are put together from two neighbouring lanes, the one that holds a
+// piece's first value stores it; what no whole piece covers goes out by elements.
+template <typename T>
+__device__ __forceinline__ void store_any8(T* p, int n, const Raw8<T>& r, int lane) {
+    constexpr int W = (int)sizeof(T) * 2;
+    constexpr int PER = 16 / (int)sizeof(T);                     // elements of a piece
+    uint32_t w[W], t[W + 4];                 // own words; with the next lane's first 4
+#pragma unroll
+    for (int i = 0; i < W / 4; ++i) {
+        w[4 * i] = r.v[i].x; w[4 * i + 1] = r.v[i].y; w[4 * i + 2] = r.v[i].z; w[4 * i + 3] = r.v[i].w;
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) t[i] = w[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t[W + i] = __shfl_down_sync(0xffffffffu, w[i], 1);
+    const int next = max(0, __shfl_down_sync(0xffffffffu, n, 1));
+    if (n <= 0) return;
+    // elements before the first aligned address; the own and the next lane's values from there
+    const int head = (int)((0u - (uint32_t)reinterpret_cast<uintptr_t>(p)) & 15u) / (int)sizeof(T);
+    const int have = n < 8 ? n : 8 + (lane < 31 ? next : 0);
+    const int bytes = head * (int)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < W + 2; ++i) t[i] = bytes & 8 ? t[i + 2] : t[i];
+#pragma unroll
+    for (int i = 0; i < W + 1; ++i) t[i] = bytes & 4 ? t[i + 1] : t[i];
+    if (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) t[i] = __funnelshift_r(t[i], t[i + 1], (bytes & 2) * 8);
+    }
+    int taken = head;
+#pragma unroll
+    for (int i = 0; i < W / 4; ++i) {
+        if (head + (i + 1) * PER > have) continue;
+        *reinterpret_cast<uint4*>(p + head + i * PER) =
+            make_uint4(t[4 * i], t[4 * i + 1], t[4 * i + 2], t[4 * i + 3]);
+        taken = head + (i + 1) * PER;
+    }
+    // the lane before stored [0, head) with its last piece, unless there is none or the values
+    // here do not fill it
+    const bool start = lane == 0 || n < head;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (i >= n || !((i < head && start) || i >= taken)) continue;
+        if (sizeof(T) == 2)
+            reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+        else
+            reinterpret_cast<uint32_t*>(p)[i] = w[i];
+    }
+}
+
 __device__ __forceinline__ void round_to(float v, float* p) { *p = v; }
 __device__ __forceinline__ void round_to(float v, __half* p) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void round_to(float v, __nv_bfloat16* p) { *p = __float2bfloat16_rn(v); }
 
-template <bool VEC>
-__device__ __forceinline__ void store8(float* p, int n, const float (&v)[8]) {
-    if (VEC) {
-        if (n > 0) {
-            reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-            reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < n) p[i] = v[i];
+// n / d for n < 2^31 by a multiplication.
+struct FastDiv {
+    uint32_t d, mul, shift;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t d_) : d(d_) {
+        shift = 0;
+        while (shift < 31 && (uint64_t(1) << shift) < d) ++shift;
+        mul = (uint32_t)(((uint64_t(1) << 32) * ((uint64_t(1) << shift) - d)) / d + 1);
     }
-}
-template <bool VEC, typename T>
-__device__ __forceinline__ void store8(T* p, int n, const float (&v)[8]) {
-    if (VEC) {
-        if (n > 0)
-            *reinterpret_cast<uint4*>(p) =
-                make_uint4(round_pair(v[0], v[1], p), round_pair(v[2], v[3], p),
-                           round_pair(v[4], v[5], p), round_pair(v[6], v[7], p));
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < n) round_to(v[i], p + i);
+    __device__ __forceinline__ uint32_t div(uint32_t n) const {
+        return (__umulhi(n, mul) + n) >> shift;
     }
-}
+};
 
 }  // namespace mx
 }  // namespace snnb

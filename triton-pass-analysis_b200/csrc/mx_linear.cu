@@ -624,8 +624,7 @@ extern "C" int snnb_mx_linear(const void* a, const void* a_scales, int a_fmt, in
     if (a_fmt != SNNB_MXFP4 && a_fmt != SNNB_MXFP8) return SNNB_ERR_ARG;
     if (out_dtype != SNNB_F32 && out_dtype != SNNB_F16 && out_dtype != SNNB_BF16)
         return SNNB_ERR_ARG;
-    if (rows < 0 || N < 1 || K < 1 || rows > 0x7fffffff || N > 0x7fffffff || K > 0x7fffffff)
-        return SNNB_ERR_ARG;
+    if (N < 1 || !mx::sizes_ok(rows, K) || !mx::sizes_ok(N, K)) return SNNB_ERR_ARG;
     if (rows == 0) return SNNB_OK;
     if (!a || !a_scales || !w || !w_scales || !out || !aligned16(a) || !aligned16(a_scales) ||
         !aligned16(w) || !aligned16(w_scales))

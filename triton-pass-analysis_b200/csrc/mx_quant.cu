@@ -1,139 +1,241 @@
 // Quantisation to the microscaled formats and back (formats and layout: mx.cuh).
 //
 // Four neighbouring lanes hold one block of 32 values, 8 each: a 16-byte load of bf16 per lane,
-// the block's largest magnitude by two shuffles, one hardware conversion per pair of elements,
+// the block's largest exponent by two shuffles, one hardware conversion per pair of elements,
 // and the codes of a warp's 8 blocks as one contiguous store.  A row is padded to whole groups
 // of 4 blocks, so that the 16 lanes of a group join their scale bytes into the one word that
-// the group has in the scale layout.  The blocks of the whole tensor are numbered through, so
-// short rows fill a warp as well as long ones do.
+// the group has in the scale layout.
+//
+// Rows that are 16-byte aligned: the blocks of the whole tensor are numbered through, so short
+// rows fill a warp as well as long ones do.  Others: a warp takes 256 consecutive values of one
+// row, through aligned loads (or stores) around them that it shifts into place.
 //
 // Bound: HBM.  Every value is read once, its code written once; nothing is read again.
 #include "mx.cuh"
 
 namespace snnb {
-
-int* device_status_ptr();
-
 namespace {
 
 constexpr int Q_THREADS = 256;
-constexpr int Q_UNROLL = 4;                      // blocks per lane group in flight
+constexpr int Q_UNROLL = 4;                      // blocks (or row pieces) of a lane in flight
 
-template <typename T, int FMT, bool VEC>
+template <typename T, int FMT>
 __global__ void __launch_bounds__(Q_THREADS)
-mx_quantize_kernel(const T* __restrict__ x, int64_t rows, int64_t K, int64_t ldx,
+mx_quantize_kernel(const T* __restrict__ x, uint32_t rows, uint32_t K, int64_t ldx, uint32_t nb,
+                   uint32_t groups, mx::FastDiv per_row, uint32_t total,
                    uint8_t* __restrict__ data, uint32_t* __restrict__ scales) {
     using F = mx::Fmt<FMT>;
     using Codes = typename F::Codes8;
     pdl_wait();
     pdl_trigger();
-    const int lane = threadIdx.x & 31;
-    const int64_t nb = mx::blocks_of(K), groups = (nb + 3) / 4;
-    const int64_t thread = (int64_t)blockIdx.x * Q_THREADS + threadIdx.x;
-    const int64_t threads = (int64_t)gridDim.x * Q_THREADS;
-    const int sub = lane & 3;
-    mx::BlockWalk w(thread >> 2, threads >> 2, groups * 4);
-    // the 32 lanes of a warp leave together: the loop ends on the warp's first block
-    mx::BlockWalk first(thread >> 5 << 3, threads >> 2, groups * 4);
-    while (first.row < rows) {
-        float v[Q_UNROLL][8];
-        int64_t row[Q_UNROLL], j[Q_UNROLL];
+    const uint32_t lane = threadIdx.x & 31, sub = lane & 3;
+    const uint32_t thread = blockIdx.x * Q_THREADS + threadIdx.x;
+    const uint32_t step = gridDim.x * (Q_THREADS / 4);
+    // a warp's 32 lanes leave together: the loop goes by its first block
+    for (uint32_t first = (thread >> 5) * 8; first < total; first += Q_UNROLL * step) {
+        mx::Raw8<T> raw[Q_UNROLL];
+        uint32_t row[Q_UNROLL], j[Q_UNROLL];
 #pragma unroll
         for (int u = 0; u < Q_UNROLL; ++u) {
-            row[u] = w.row;
-            j[u] = w.j;
-            const int64_t k = w.j * 32 + sub * 8;
-            const int n = w.row < rows ? (int)max((int64_t)0, min((int64_t)8, K - k)) : 0;
-            mx::load8<VEC>(x + (n > 0 ? w.row * ldx + k : 0), n, v[u]);
-            w.next();
-            first.next();
+            const uint32_t q = first + u * step + (lane >> 2);
+            row[u] = per_row.div(q);
+            j[u] = q - row[u] * per_row.d;
+            const uint32_t k = j[u] * 32 + sub * 8;
+            raw[u] = q < total && k < K ? mx::load_aligned8(x + row[u] * ldx + k) : mx::zero8<T>();
         }
 #pragma unroll
         for (int u = 0; u < Q_UNROLL; ++u) {
+            float v[8];
+            mx::to_floats(raw[u], v);
             Codes c;
-            const uint32_t byte = mx::quantise_block<FMT>(v[u], c);
+            const uint32_t byte = mx::quantise_block<FMT>(v, mx::top_exponent(raw[u], v), c);
             const uint32_t word = mx::join_scales(byte, lane);
-            if (row[u] < rows) {
+            if (first + u * step + (lane >> 2) < total) {
                 if (j[u] < nb)
-                    *reinterpret_cast<Codes*>(data + (row[u] * nb + j[u]) * F::BLOCK_BYTES +
+                    *reinterpret_cast<Codes*>(data + (uint64_t)(row[u] * nb + j[u]) * F::BLOCK_BYTES +
                                               sub * sizeof(Codes)) = c;
-                if ((lane & 15) == 0)
-                    scales[mx::scale_word(row[u], j[u] >> 2, groups)] = word;
+                if ((lane & 15) == 0) scales[mx::scale_word(row[u], j[u] >> 2, groups)] = word;
             }
         }
     }
-    mx::zero_row_padding(scales, rows, groups, thread, threads);
+    mx::zero_row_padding(scales, rows, groups, thread, (uint64_t)gridDim.x * Q_THREADS);
 }
 
-template <typename T, int FMT, bool VEC>
+// total: pieces of 256 values, per_row.d = ceil(K / 256) of them a row.
+template <typename T, int FMT>
 __global__ void __launch_bounds__(Q_THREADS)
-mx_dequantize_kernel(const uint8_t* __restrict__ data, const uint32_t* __restrict__ scales,
-                     int64_t rows, int64_t K, T* __restrict__ out) {
+mx_quantize_any_kernel(const T* __restrict__ x, uint32_t rows, uint32_t K, int64_t ldx,
+                       uint32_t nb, uint32_t groups, mx::FastDiv per_row, uint32_t total,
+                       uint8_t* __restrict__ data, uint32_t* __restrict__ scales) {
     using F = mx::Fmt<FMT>;
     using Codes = typename F::Codes8;
     pdl_wait();
     pdl_trigger();
-    const int lane = threadIdx.x & 31;
-    const int64_t nb = mx::blocks_of(K), groups = (nb + 3) / 4;
-    const int64_t thread = (int64_t)blockIdx.x * Q_THREADS + threadIdx.x;
-    const int64_t threads = (int64_t)gridDim.x * Q_THREADS;
-    const int sub = lane & 3;
-    mx::BlockWalk w(thread >> 2, threads >> 2, nb);
-    while (w.row < rows) {
-        Codes c[Q_UNROLL];
-        uint32_t word[Q_UNROLL];
-        int64_t row[Q_UNROLL], j[Q_UNROLL];
+    const uint32_t lane = threadIdx.x & 31, sub = lane & 3;
+    const uint32_t thread = blockIdx.x * Q_THREADS + threadIdx.x;
+    const uint32_t step = gridDim.x * (Q_THREADS / 32);
+    for (uint32_t first = thread >> 5; first < total; first += Q_UNROLL * step) {
+        mx::Raw8<T> raw[Q_UNROLL];
+        uint32_t row[Q_UNROLL], k[Q_UNROLL];
 #pragma unroll
         for (int u = 0; u < Q_UNROLL; ++u) {
-            row[u] = w.row;
-            j[u] = w.j;
-            if (w.row < rows) {
-                c[u] = __ldg(reinterpret_cast<const Codes*>(
-                    data + (w.row * nb + w.j) * F::BLOCK_BYTES + sub * sizeof(Codes)));
-                word[u] = __ldg(scales + mx::scale_word(w.row, w.j >> 2, groups));
+            const uint32_t q = first + u * step;
+            row[u] = per_row.div(q);
+            k[u] = (q - row[u] * per_row.d) * 256 + lane * 8;
+            if (q < total && k[u] < K) {
+                const T* r = x + row[u] * ldx;
+                raw[u] = mx::load_any8(r + k[u], (int)min(8u, K - k[u]), r, (int64_t)K);
+            } else {
+                raw[u] = mx::zero8<T>();
             }
-            w.next();
         }
 #pragma unroll
         for (int u = 0; u < Q_UNROLL; ++u) {
-            if (row[u] >= rows) continue;
             float v[8];
-            mx::decode8(c[u], v);
-            const float s = mx::scale_value((word[u] >> (8 * (j[u] & 3))) & 255u);
+            mx::to_floats(raw[u], v);
+            Codes c;
+            const uint32_t byte = mx::quantise_block<FMT>(v, mx::top_exponent(raw[u], v), c);
+            const uint32_t word = mx::join_scales(byte, lane);
+            const uint32_t j = k[u] >> 5;
+            if (first + u * step < total) {
+                if (j < nb)
+                    *reinterpret_cast<Codes*>(data + (uint64_t)(row[u] * nb + j) * F::BLOCK_BYTES +
+                                              sub * sizeof(Codes)) = c;
+                if ((lane & 15) == 0 && (j >> 2) < groups)
+                    scales[mx::scale_word(row[u], j >> 2, groups)] = word;
+            }
+        }
+    }
+    mx::zero_row_padding(scales, rows, groups, thread, (uint64_t)gridDim.x * Q_THREADS);
+}
+
+template <typename T, int FMT>
+__device__ __forceinline__ mx::Raw8<T> decode_scaled(typename mx::Fmt<FMT>::Codes8 c,
+                                                     uint32_t byte) {
+    float v[8];
+    mx::decode8(c, v);
+    const float s = mx::scale_value(byte);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] *= s;
-            const int64_t k = j[u] * 32 + sub * 8;
-            const int n = (int)max((int64_t)0, min((int64_t)8, K - k));
-            mx::store8<VEC>(out + row[u] * K + k, n, v);
+    for (int i = 0; i < 8; ++i) v[i] *= s;
+    mx::Raw8<T> r;
+    mx::from_floats(v, r);
+    return r;
+}
+
+// total: blocks, per_row.d = nb of them a row; ALIGNED: K % 8 == 0 and out 16-byte aligned.
+template <typename T, int FMT>
+__global__ void __launch_bounds__(Q_THREADS)
+mx_dequantize_kernel(const uint8_t* __restrict__ data, const uint8_t* __restrict__ scales,
+                     uint32_t rows, uint32_t K, uint32_t groups, mx::FastDiv per_row,
+                     uint32_t total, T* __restrict__ out) {
+    using F = mx::Fmt<FMT>;
+    using Codes = typename F::Codes8;
+    pdl_wait();
+    pdl_trigger();
+    const uint32_t sub = threadIdx.x & 3;
+    const uint32_t thread = blockIdx.x * Q_THREADS + threadIdx.x;
+    const uint32_t step = gridDim.x * (Q_THREADS / 4);
+    for (uint32_t first = thread >> 2; first < total; first += Q_UNROLL * step) {
+        Codes c[Q_UNROLL];
+        uint32_t byte[Q_UNROLL], row[Q_UNROLL], j[Q_UNROLL];
+#pragma unroll
+        for (int u = 0; u < Q_UNROLL; ++u) {
+            const uint32_t q = first + u * step;
+            row[u] = per_row.div(q);
+            j[u] = q - row[u] * per_row.d;
+            if (q < total) {
+                c[u] = __ldg(reinterpret_cast<const Codes*>(data + (uint64_t)q * F::BLOCK_BYTES +
+                                                            sub * sizeof(Codes)));
+                byte[u] = __ldg(scales + 4 * (uint64_t)mx::scale_word(row[u], j[u] >> 2, groups) +
+                                (j[u] & 3));
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < Q_UNROLL; ++u) {
+            const uint32_t k = j[u] * 32 + sub * 8;
+            if (first + u * step < total && k < K)
+                mx::store_aligned8(out + (uint64_t)row[u] * K + k, decode_scaled<T, FMT>(c[u], byte[u]));
         }
     }
 }
 
-// Blocks for `quads` lane groups of 4, a full round of resident blocks at most (8 of 256
-// threads per SM).
-unsigned grid_for(int64_t quads) {
-    const int64_t need = (quads * 4 + Q_THREADS - 1) / Q_THREADS;
+// total: pieces of 256 values, per_row.d = ceil(K / 256) of them a row.
+template <typename T, int FMT>
+__global__ void __launch_bounds__(Q_THREADS)
+mx_dequantize_any_kernel(const uint8_t* __restrict__ data, const uint8_t* __restrict__ scales,
+                         uint32_t rows, uint32_t K, uint32_t nb, uint32_t groups,
+                         mx::FastDiv per_row, uint32_t total, T* __restrict__ out) {
+    using F = mx::Fmt<FMT>;
+    using Codes = typename F::Codes8;
+    pdl_wait();
+    pdl_trigger();
+    const uint32_t lane = threadIdx.x & 31, sub = lane & 3;
+    const uint32_t thread = blockIdx.x * Q_THREADS + threadIdx.x;
+    const uint32_t step = gridDim.x * (Q_THREADS / 32);
+    for (uint32_t first = thread >> 5; first < total; first += Q_UNROLL * step) {
+        Codes c[Q_UNROLL];
+        uint32_t byte[Q_UNROLL], row[Q_UNROLL], k[Q_UNROLL];
+#pragma unroll
+        for (int u = 0; u < Q_UNROLL; ++u) {
+            const uint32_t q = first + u * step;
+            row[u] = per_row.div(q);
+            k[u] = (q - row[u] * per_row.d) * 256 + lane * 8;
+            const uint32_t j = k[u] >> 5;
+            c[u] = Codes{};
+            byte[u] = 0;
+            if (q < total && j < nb) {
+                c[u] = __ldg(reinterpret_cast<const Codes*>(
+                    data + (uint64_t)(row[u] * nb + j) * F::BLOCK_BYTES + sub * sizeof(Codes)));
+                byte[u] = __ldg(scales + 4 * (uint64_t)mx::scale_word(row[u], j >> 2, groups) + (j & 3));
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < Q_UNROLL; ++u) {
+            const bool in = first + u * step < total && k[u] < K;
+            mx::store_any8(out + (in ? (uint64_t)row[u] * K + k[u] : 0),
+                           in ? (int)min(8u, K - k[u]) : 0, decode_scaled<T, FMT>(c[u], byte[u]),
+                           (int)lane);
+        }
+    }
+}
+
+// Blocks of 256 threads: what `warps` warps need, a full round of resident ones at most.
+unsigned grid_for(int64_t warps) {
+    const int64_t need = (warps + Q_THREADS / 32 - 1) / (Q_THREADS / 32);
     return (unsigned)(need < 1 ? 1 : (need > 148 * 8 ? 148 * 8 : need));
 }
 
 template <typename T, int FMT>
 int run_quantize(const void* x, int64_t rows, int64_t K, int64_t ldx, void* data, void* scales,
                  cudaStream_t s) {
-    const bool vec = K % 8 == 0 && aligned16(x) && ldx * (int64_t)sizeof(T) % 16 == 0;
-    const unsigned grid = grid_for(rows * mx::groups_of(K) * 4);
-    auto k = vec ? mx_quantize_kernel<T, FMT, true> : mx_quantize_kernel<T, FMT, false>;
-    return launch_k(k, dim3(grid), dim3(Q_THREADS), 0, s, static_cast<const T*>(x), rows, K, ldx,
-                    static_cast<uint8_t*>(data), static_cast<uint32_t*>(scales));
+    const uint32_t nb = (uint32_t)mx::blocks_of(K), groups = (uint32_t)mx::groups_of(K);
+    const bool aligned = K % 8 == 0 && aligned16(x) && (rows == 1 || ldx * (int64_t)sizeof(T) % 16 == 0);
+    const uint32_t per = aligned ? groups * 4 : (uint32_t)((K + 255) / 256);
+    const int64_t total = rows * per;
+    auto k = aligned ? mx_quantize_kernel<T, FMT> : mx_quantize_any_kernel<T, FMT>;
+    return launch_k(k, dim3(grid_for(aligned ? (total + 7) / 8 : total)), dim3(Q_THREADS), 0, s,
+                    static_cast<const T*>(x), (uint32_t)rows, (uint32_t)K, ldx, nb, groups,
+                    mx::FastDiv(per), (uint32_t)total, static_cast<uint8_t*>(data),
+                    static_cast<uint32_t*>(scales));
 }
 
 template <typename T, int FMT>
 int run_dequantize(const void* data, const void* scales, int64_t rows, int64_t K, void* out,
                    cudaStream_t s) {
-    const bool vec = K % 8 == 0 && aligned16(out);
-    const unsigned grid = grid_for(rows * mx::blocks_of(K));
-    auto k = vec ? mx_dequantize_kernel<T, FMT, true> : mx_dequantize_kernel<T, FMT, false>;
-    return launch_k(k, dim3(grid), dim3(Q_THREADS), 0, s, static_cast<const uint8_t*>(data),
-                    static_cast<const uint32_t*>(scales), rows, K, static_cast<T*>(out));
+    const uint32_t nb = (uint32_t)mx::blocks_of(K), groups = (uint32_t)mx::groups_of(K);
+    const uint8_t* d = static_cast<const uint8_t*>(data);
+    const uint8_t* sc = static_cast<const uint8_t*>(scales);
+    if (K % 8 == 0 && aligned16(out)) {
+        const int64_t total = rows * nb;
+        return launch_k(mx_dequantize_kernel<T, FMT>, dim3(grid_for((total + 7) / 8)),
+                        dim3(Q_THREADS), 0, s, d, sc, (uint32_t)rows, (uint32_t)K, groups,
+                        mx::FastDiv(nb), (uint32_t)total, static_cast<T*>(out));
+    }
+    const uint32_t per = (uint32_t)((K + 255) / 256);
+    const int64_t total = rows * per;
+    return launch_k(mx_dequantize_any_kernel<T, FMT>, dim3(grid_for(total)), dim3(Q_THREADS), 0, s,
+                    d, sc, (uint32_t)rows, (uint32_t)K, nb, groups, mx::FastDiv(per),
+                    (uint32_t)total, static_cast<T*>(out));
 }
 
 }  // namespace
@@ -151,23 +253,14 @@ using namespace snnb;
         default: return fn<__nv_bfloat16, SNNB_MXFP8>(__VA_ARGS__);                         \
     }
 
-// Largest extents: 2^40 elements a tensor keep every index and byte count far inside 64 bits.
-static bool mx_sizes_ok(int64_t rows, int64_t K) {
-    return rows >= 0 && K >= 1 && K <= 0x7fffffff && rows <= (int64_t(1) << 40) / K;
-}
-static bool mx_aligned(const void* data, const void* scales) {
-    return aligned16(data) && aligned16(scales);
-}
-
 extern "C" int snnb_mx_quantize(const void* x, int x_dtype, int64_t rows, int64_t K, int64_t ldx,
                                 int fmt, void* data, void* scales, snnb_stream_t stream) {
     if (const int inj = take_injected_status()) return inj;
     if (x_dtype != SNNB_F32 && x_dtype != SNNB_F16 && x_dtype != SNNB_BF16) return SNNB_ERR_ARG;
     if (fmt != SNNB_MXFP4 && fmt != SNNB_MXFP8) return SNNB_ERR_ARG;
-    if (!mx_sizes_ok(rows, K) || ldx < 0 || (rows > 1 && ldx > (int64_t(1) << 40) / rows))
-        return SNNB_ERR_ARG;
+    if (!mx::sizes_ok(rows, K) || !mx::stride_ok(rows, ldx)) return SNNB_ERR_ARG;
     if (rows == 0) return SNNB_OK;
-    if (!x || !data || !scales || !mx_aligned(data, scales)) return SNNB_ERR_ARG;
+    if (!x || !data || !scales || !aligned16(data) || !aligned16(scales)) return SNNB_ERR_ARG;
     if (reinterpret_cast<uintptr_t>(x) % (x_dtype == SNNB_F32 ? 4 : 2)) return SNNB_ERR_ARG;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     SNNB_MX_DISPATCH(x_dtype, fmt, run_quantize, x, rows, K, ldx, data, scales, s)
@@ -179,9 +272,9 @@ extern "C" int snnb_mx_dequantize(const void* data, const void* scales, int fmt,
     if (out_dtype != SNNB_F32 && out_dtype != SNNB_F16 && out_dtype != SNNB_BF16)
         return SNNB_ERR_ARG;
     if (fmt != SNNB_MXFP4 && fmt != SNNB_MXFP8) return SNNB_ERR_ARG;
-    if (!mx_sizes_ok(rows, K)) return SNNB_ERR_ARG;
+    if (!mx::sizes_ok(rows, K)) return SNNB_ERR_ARG;
     if (rows == 0) return SNNB_OK;
-    if (!out || !data || !scales || !mx_aligned(data, scales)) return SNNB_ERR_ARG;
+    if (!out || !data || !scales || !aligned16(data) || !aligned16(scales)) return SNNB_ERR_ARG;
     if (reinterpret_cast<uintptr_t>(out) % (out_dtype == SNNB_F32 ? 4 : 2)) return SNNB_ERR_ARG;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     SNNB_MX_DISPATCH(out_dtype, fmt, run_dequantize, data, scales, rows, K, out, s)

@@ -132,3 +132,13 @@ def ptr(t):
 def stream_of(t):
     import torch
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+
+def raw_stream(index: int) -> int:
+    """The current stream of CUDA device `index` as an integer handle."""
+    import torch
+    global raw_stream
+    raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+        (lambda i: torch.cuda.current_stream(i).cuda_stream)
+    return raw_stream(index)
