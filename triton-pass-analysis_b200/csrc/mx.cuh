@@ -115,13 +115,16 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
 // zeros or float subnormals.  A block that holds an infinity or a NaN gets the byte 255 (NaN)
 // and zero codes.
 
-// The largest magnitude's exponent field among 8 values.  Magnitudes compare as integers, and an
-// infinity or NaN is above every finite value.
+// The largest magnitude's exponent field among 8 values (255 where one is an infinity or NaN).
+__device__ __forceinline__ float max_abs3(float a, float b, float c) {
+    float d;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 __device__ __forceinline__ uint32_t top_exponent(const float (&x)[8]) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, (uint32_t)__float_as_int(x[i]) & 0x7FFFFFFFu);
-    return top >> 23;
+    const float m = max_abs3(max_abs3(x[0], x[1], x[2]), max_abs3(x[3], x[4], x[5]),
+                             max_abs3(x[6], x[7], x[7]));
+    return ((uint32_t)__float_as_int(m) >> 23) & 255u;
 }
 
 // The same from the raw values.  bfloat16 has float's exponent field: compare pairs.

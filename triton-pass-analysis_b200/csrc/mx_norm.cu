@@ -24,8 +24,6 @@ namespace snnb {
 namespace {
 
 struct NormParams {
-    const void* weight;
-    int w_f32;                   // weight is float32 (else of x's type)
     int fmt;
     float eps;
     double inv_k;
@@ -36,9 +34,11 @@ struct NormParams {
     int* status;
 };
 
-__device__ __forceinline__ double warp_sum(double v) {
+// Sum over aligned groups of LANES lanes of a warp.
+template <int LANES>
+__device__ __forceinline__ double lanes_sum(double v) {
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    for (int d = LANES / 2; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
     return v;
 }
 // Sum of 8 squares.
@@ -58,38 +58,13 @@ __device__ __forceinline__ double add_squares(const float (&h)[8]) {
     const float s = squares8(h);
     return s > 1e-30f && s < 1e38f ? (double)s : squares8_exact(h);
 }
+// 1 / sqrt(sum / K + eps): one Newton step in float64 on the float32 approximation (2^-22, so
+// ~2^-44 after it).
 __device__ __forceinline__ double rstd_of(const NormParams& p, double sum) {
-    return rsqrt(fma(sum, p.inv_k, (double)p.eps));
-}
-
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ void weights8(const NormParams& p, uint32_t k, int n, float (&w)[8]) {
-    if (p.w_f32) {
-        const float* q = static_cast<const float*>(p.weight);
-        mx::Raw8<float> r = mx::zero8<float>();
-        if (n > 0) {
-            if (ALIGNED) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) r.v[i] = __ldg(reinterpret_cast<const uint4*>(q + k) + i);
-            } else {
-                r = mx::load_any8(q + k, n, q, (int64_t)p.K);
-            }
-        }
-        mx::to_floats(r, w);
-    } else {
-        const T* q = static_cast<const T*>(p.weight);
-        mx::Raw8<T> r = mx::zero8<T>();
-        if (n > 0) {
-            if (ALIGNED) {
-#pragma unroll
-                for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-                    r.v[i] = __ldg(reinterpret_cast<const uint4*>(q + k) + i);
-            } else {
-                r = mx::load_any8(q + k, n, q, (int64_t)p.K);
-            }
-        }
-        mx::to_floats(r, w);
-    }
+    const double m = fma(sum, p.inv_k, (double)p.eps);
+    if (!(m > 1e-30 && m < 1e37)) return rsqrt(m);
+    const double r = (double)rsqrtf((float)m);
+    return fma(0.5 * r, fma(-m * r, r, 1.0), r);
 }
 
 // y of 8 values (see the top); values past n, whose h and w are 0, give 0.
@@ -113,26 +88,34 @@ __device__ __forceinline__ void normed8(const float (&h)[8], const float (&w)[8]
     }
 }
 
+// Where a row's codes and scale words go (nullptr: nowhere).
+struct RowOut {
+    uint8_t* data;
+    uint32_t* scales;
+    __device__ __forceinline__ RowOut(const NormParams& p, uint32_t row, bool in_row) {
+        data = in_row ? p.data + (uint64_t)(row * p.nb) * (p.fmt == SNNB_MXFP4 ? 16 : 32) : nullptr;
+        scales = p.scales + mx::scale_word(row, 0, p.groups);
+    }
+};
 // Codes and scale word of 8 values at column k of a row.  Every lane of the warp calls.
-__device__ __forceinline__ void emit8(const NormParams& p, uint32_t row, uint32_t k, bool in_row,
+__device__ __forceinline__ void emit8(const NormParams& p, const RowOut& o, uint32_t k,
                                       const float (&y)[8], int lane) {
-    const uint32_t j = k >> 5, sub = lane & 3;
-    const bool inside = in_row && j < p.nb;
+    const uint32_t j = k >> 5;
+    const bool inside = o.data && j < p.nb;
     const uint32_t e = mx::top_exponent(y);
-    const uint64_t block = (uint64_t)(row * p.nb + j);
     uint32_t byte;
     if (p.fmt == SNNB_MXFP4) {
         uint32_t c;
         byte = mx::quantise_block<SNNB_MXFP4>(y, e, c);
-        if (inside) *reinterpret_cast<uint32_t*>(p.data + block * 16 + sub * 4) = c;
+        if (inside) *reinterpret_cast<uint32_t*>(o.data + k / 2) = c;
     } else {
         uint2 c;
         byte = mx::quantise_block<SNNB_MXFP8>(y, e, c);
-        if (inside) *reinterpret_cast<uint2*>(p.data + block * 32 + sub * 8) = c;
+        if (inside) *reinterpret_cast<uint2*>(o.data + k) = c;
     }
     const uint32_t word = mx::join_scales(byte, lane);
-    if (in_row && (j >> 2) < p.groups && (lane & 15) == 0)
-        p.scales[mx::scale_word(row, j >> 2, p.groups)] = word;
+    if (o.data && (j >> 2) < p.groups && (lane & 15) == 0)
+        o.scales[(j >> 2) * (mx::GROUP_BYTES / 4)] = word;
 }
 
 // ---- rows through registers --------------------------------------------------------------
@@ -163,24 +146,41 @@ __device__ __forceinline__ void put_h8(const NormParams& p, T* h_out, uint32_t r
     else if (n > 0) mx::store_aligned8(q, o);
 }
 
+template <typename W, bool ALIGNED>
+__device__ __forceinline__ mx::Raw8<W> weights8(const NormParams& p, const W* weight, uint32_t k) {
+    if (k >= p.K) return mx::zero8<W>();
+    if (!ALIGNED) return mx::load_any8(weight + k, (int)min(8u, p.K - k), weight, (int64_t)p.K);
+    mx::Raw8<W> r;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(W) / 2; ++i)
+        r.v[i] = __ldg(reinterpret_cast<const uint4*>(weight + k) + i);
+    return r;
+}
+
 // LANES threads a row, CHUNKS x 8 values a thread: thread t holds columns (c * LANES + t) * 8 ..
 // + 7 of chunk c.  CHUNKS == 0: rows of any length, read twice.
-template <typename T, bool ALIGNED, int LANES, int CHUNKS>
-__global__ void __launch_bounds__(LANES == 32 ? 256 : LANES)
+constexpr int direct_threads(int lanes) { return lanes <= 32 ? 256 : lanes; }
+template <typename T, typename W, bool ALIGNED, int LANES, int CHUNKS>
+__global__ void __launch_bounds__(direct_threads(LANES))
 rms_norm_mx_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __restrict__ h_out,
-                   const NormParams p) {
-    constexpr uint32_t THREADS = LANES == 32 ? 256 : LANES;
+                   const W* __restrict__ weight, const NormParams p) {
+    constexpr uint32_t THREADS = direct_threads(LANES);
     __shared__ double shared[32];
     pdl_wait();
     pdl_trigger();
     const int lane = threadIdx.x & 31;
-    const uint32_t t = LANES == 32 ? lane : threadIdx.x;
-    const uint32_t row = LANES == 32 ? blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
+    const uint32_t t = threadIdx.x % LANES;
+    const uint32_t row = blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES;
     const bool in_row = row < p.rows;
+    const RowOut out(p, row, in_row);
     auto valid = [&](uint32_t k) { return in_row && k < p.K ? (int)min(8u, p.K - k) : 0; };
+    // whole warps: a chunk that begins past the row's end is left out
+    auto past = [&](uint32_t k, uint32_t end) {
+        return LANES >= 32 ? (k & ~255u) >= end : false;
+    };
     auto row_sum = [&](double v) {
-        v = warp_sum(v);
-        if (LANES == 32) return v;
+        v = lanes_sum<LANES < 32 ? LANES : 32>(v);
+        if (LANES <= 32) return v;
         if (lane == 0) shared[threadIdx.x >> 5] = v;
         __syncthreads();
         double s = 0.0;
@@ -190,9 +190,9 @@ rms_norm_mx_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __restri
     };
     auto finish = [&](uint32_t k, const float (&h)[8], float rstd, double rstd64) {
         float w[8], y[8];
-        weights8<T, ALIGNED>(p, k, valid(k), w);
+        mx::to_floats(weights8<W, ALIGNED>(p, weight, k), w);
         normed8(h, w, rstd, rstd64, y);
-        emit8(p, row, k, in_row, y, lane);
+        emit8(p, out, k, y, lane);
     };
     double sum = 0.0;
     if constexpr (CHUNKS > 0) {
@@ -205,6 +205,7 @@ rms_norm_mx_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __restri
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
             const uint32_t k = (c * LANES + t) * 8;
+            if (c > 0 && past(k, p.K)) break;
             if (h_out) put_h8<T, ALIGNED>(p, h_out, row, k, valid(k), h[c], lane);
             if (valid(k)) sum += add_squares(h[c]);
         }
@@ -212,12 +213,13 @@ rms_norm_mx_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __restri
         const float rstd = (float)rstd64;
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
-            if ((c * LANES + (t & ~31u)) * 8 >= p.groups * 128) break;       // whole warps
-            finish((c * LANES + t) * 8, h[c], rstd, rstd64);
+            const uint32_t k = (c * LANES + t) * 8;
+            if (c > 0 && past(k, p.groups * 128)) break;
+            finish(k, h[c], rstd, rstd64);
         }
     } else {
         float h[8];
-        for (uint32_t k = t * 8; (k & ~255u) < p.K; k += LANES * 8) {        // whole warps
+        for (uint32_t k = t * 8; !past(k, p.K); k += LANES * 8) {
             const int n = valid(k);
             take8<T, ALIGNED>(p, x, r, row, k, n, h);
             if (h_out) put_h8<T, ALIGNED>(p, h_out, row, k, n, h, lane);
@@ -225,7 +227,7 @@ rms_norm_mx_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __restri
         }
         const double rstd64 = rstd_of(p, row_sum(sum));
         const float rstd = (float)rstd64;
-        for (uint32_t k = t * 8; (k & ~255u) < p.groups * 128; k += LANES * 8) {
+        for (uint32_t k = t * 8; !past(k, p.groups * 128); k += LANES * 8) {
             take8<T, ALIGNED>(p, x, r, row, k, valid(k), h);
             finish(k, h, rstd, rstd64);
         }
@@ -253,19 +255,28 @@ __device__ __forceinline__ mx::Raw8<T> smem8(const uint8_t* row, uint32_t k) {
 
 constexpr int RING_MAX = 4;
 constexpr int RING_HEAD = 1024;              // barriers and sums, before the ring
+constexpr int RING_CHUNKS = 4;
+constexpr int ring_threads(int lanes) { return lanes < 256 ? 256 : lanes; }
+// Resident blocks to compile for: 80 registers a thread, 128 where values or weights are float32.
+template <typename T, typename W> constexpr int ring_blocks(int lanes) {
+    return (sizeof(T) == 4 || sizeof(W) == 4 ? 512 : 768) / ring_threads(lanes);
+}
 
 // Teams of LANES threads; team g of all walks the rows g, g + (number of teams), ...  A ring
-// stage holds one row of x and, `half` bytes behind it, of the residual.
-template <typename T, int LANES>
-__global__ void __launch_bounds__(LANES < 256 ? 256 : LANES)
+// stage holds one row of x and, `half` bytes behind it, of the residual (RES).  A thread holds
+// CHUNKS x 8 values of the row in registers, as in rms_norm_mx_kernel, and its columns' weights
+// for all rows.
+template <typename T, typename W, int LANES, bool RES>
+__global__ void __launch_bounds__(ring_threads(LANES), ring_blocks<T, W>(LANES))
 rms_norm_mx_ring_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __restrict__ h_out,
-                        const NormParams p, int stages, uint32_t half) {
-    constexpr int THREADS = LANES < 256 ? 256 : LANES, TEAMS = THREADS / LANES, WARPS = LANES / 32;
+                        const W* __restrict__ weight, const NormParams p, int stages,
+                        uint32_t half) {
+    constexpr int THREADS = ring_threads(LANES), TEAMS = THREADS / LANES, WARPS = LANES / 32;
     extern __shared__ __align__(128) uint8_t smem[];
     const int lane = threadIdx.x & 31;
     const int team = threadIdx.x / LANES;
     const uint32_t t = threadIdx.x % LANES;
-    const uint32_t stage_bytes = half * (r ? 2 : 1);
+    const uint32_t stage_bytes = half * (RES ? 2 : 1);
     const uint32_t bars = tc::smem_u32(smem) + (uint32_t)team * RING_MAX * 8;
     double* sums = reinterpret_cast<double*>(smem + TEAMS * RING_MAX * 8) + team * 2 * WARPS;
     uint8_t* ring = smem + RING_HEAD + (size_t)team * stages * stage_bytes;
@@ -281,9 +292,9 @@ rms_norm_mx_ring_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __r
     const uint32_t bytes = p.K * (uint32_t)sizeof(T);
     auto fetch = [&](uint32_t row, int s) {
         const uint32_t dst = ring32 + (uint32_t)s * stage_bytes;
-        tc::mbar_expect_tx(bars + 8 * s, bytes * (r ? 2u : 1u));
+        tc::mbar_expect_tx(bars + 8 * s, bytes * (RES ? 2u : 1u));
         bulk_load(dst, x + (int64_t)row * p.ldx, bytes, bars + 8 * s);
-        if (r) bulk_load(dst + half, r + (int64_t)row * p.ldr, bytes, bars + 8 * s);
+        if (RES) bulk_load(dst + half, r + (int64_t)row * p.ldr, bytes, bars + 8 * s);
     };
     auto team_sync = [&] {
         if constexpr (LANES == 32) __syncwarp();
@@ -292,6 +303,9 @@ rms_norm_mx_ring_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __r
     if (t == 0)
         for (int s = 0; s < stages; ++s)
             if (row0 + (uint64_t)s * step < p.rows) fetch(row0 + s * step, s);
+    mx::Raw8<W> w[RING_CHUNKS];
+#pragma unroll
+    for (int c = 0; c < RING_CHUNKS; ++c) w[c] = weights8<W, true>(p, weight, (c * LANES + t) * 8);
     uint32_t failed = 0;
     int s = 0;
     uint32_t parity = 0, odd = 0;
@@ -313,51 +327,56 @@ rms_norm_mx_ring_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __r
             if (lane == 0) atomicExch(p.status, SNNB_ERR_TIMEOUT);
         }
         const uint8_t* xs = ring + (size_t)s * stage_bytes;
-        const uint8_t* rs = xs + half;
-        auto take = [&](uint32_t k, float (&h)[8]) {
-            mx::to_floats(smem8<T>(xs, k), h);
-            if (r) {
-                float f[8];
-                mx::to_floats(smem8<T>(rs, k), f);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) h[i] += f[i];
-            }
-        };
+        T* hr = h_out ? h_out + (uint64_t)row * p.K : nullptr;
+        if (failed) hr = nullptr;
+        float h[RING_CHUNKS][8];
         double sum = 0.0;
-        for (uint32_t k = t * 8; k < p.K; k += LANES * 8) {
-            float h[8];
-            take(k, h);
-            if (h_out && !failed) {
-                mx::Raw8<T> o;
-                mx::from_floats(h, o);
-                mx::store_aligned8(h_out + (uint64_t)row * p.K + k, o);
+#pragma unroll
+        for (int c = 0; c < RING_CHUNKS; ++c) {
+            const uint32_t k = (c * LANES + t) * 8;
+            if (c > 0 && (k & ~255u) >= p.K) break;                           // whole warps
+            const bool in = k < p.K;
+            mx::to_floats(in ? smem8<T>(xs, k) : mx::zero8<T>(), h[c]);
+            if (RES) {
+                float f[8];
+                mx::to_floats(in ? smem8<T>(xs + half, k) : mx::zero8<T>(), f);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) h[c][i] += f[i];
             }
-            sum += add_squares(h);
+            if (hr && in) {
+                mx::Raw8<T> o;
+                mx::from_floats(h[c], o);
+                mx::store_aligned8(hr + k, o);
+            }
+            if (in) sum += add_squares(h[c]);
         }
-        sum = warp_sum(sum);
+        sum = lanes_sum<32>(sum);
         if constexpr (LANES > 32) {
             if (lane == 0) sums[odd * WARPS + (t >> 5)] = sum;
-            team_sync();
+        }
+        team_sync();                                  // sums written, the stage read by all
+        const uint64_t next = row64 + (uint64_t)stages * step;
+        if (t == 0 && !failed && next < p.rows) fetch((uint32_t)next, s);
+        if (++s == stages) {
+            s = 0;
+            parity ^= 1;
+        }
+        if constexpr (LANES > 32) {
             sum = 0.0;
 #pragma unroll
             for (int i = 0; i < WARPS; ++i) sum += sums[odd * WARPS + i];
         }
         const double rstd64 = rstd_of(p, sum);
         const float rstd = (float)rstd64;
-        for (uint32_t k = t * 8; (k & ~255u) < p.groups * 128; k += LANES * 8) {
-            float h[8] = {0, 0, 0, 0, 0, 0, 0, 0}, w[8], y[8];
-            const int n = k < p.K ? 8 : 0;
-            if (n) take(k, h);
-            weights8<T, true>(p, k, n, w);
-            normed8(h, w, rstd, rstd64, y);
-            emit8(p, row, k, !failed, y, lane);
-        }
-        team_sync();                                  // the stage has been read by all
-        const uint64_t next = row64 + (uint64_t)stages * step;
-        if (t == 0 && !failed && next < p.rows) fetch((uint32_t)next, s);
-        if (++s == stages) {
-            s = 0;
-            parity ^= 1;
+        const RowOut out(p, row, !failed);
+#pragma unroll
+        for (int c = 0; c < RING_CHUNKS; ++c) {
+            const uint32_t k = (c * LANES + t) * 8;
+            if (c > 0 && (k & ~255u) >= p.groups * 128) break;
+            float wf[8], y[8];
+            mx::to_floats(w[c], wf);
+            normed8(h[c], wf, rstd, rstd64, y);
+            emit8(p, out, k, y, lane);
         }
     }
     mx::zero_row_padding(p.scales, p.rows, p.groups, (uint64_t)blockIdx.x * THREADS + threadIdx.x,
@@ -365,67 +384,77 @@ rms_norm_mx_ring_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __r
 }
 
 // ---- host ------------------------------------------------------------------------------
-template <typename T, bool ALIGNED, int LANES, int CHUNKS>
-int launch_norm(const void* x, const void* r, void* h, const NormParams& p, cudaStream_t s) {
-    const uint32_t per = LANES == 32 ? 8 : 1;
-    return launch_k(rms_norm_mx_kernel<T, ALIGNED, LANES, CHUNKS>, dim3((p.rows + per - 1) / per),
-                    dim3(LANES == 32 ? 256 : LANES), 0, s, static_cast<const T*>(x),
-                    static_cast<const T*>(r), static_cast<T*>(h), p);
+struct NormArgs {
+    const void *x, *r, *weight;
+    void* h;
+    cudaStream_t s;
+};
+
+template <typename T, typename W, bool ALIGNED, int LANES, int CHUNKS>
+int launch_norm(const NormArgs& a, const NormParams& p) {
+    constexpr uint32_t THREADS = direct_threads(LANES), PER = THREADS / LANES;
+    return launch_k(rms_norm_mx_kernel<T, W, ALIGNED, LANES, CHUNKS>,
+                    dim3((p.rows + PER - 1) / PER), dim3(THREADS), 0, a.s,
+                    static_cast<const T*>(a.x), static_cast<const T*>(a.r), static_cast<T*>(a.h),
+                    static_cast<const W*>(a.weight), p);
 }
 
-constexpr uint32_t RING_BUDGET = 100 * 1024;         // two blocks an SM
-
-template <typename T, int LANES>
-bool ring_fits(const NormParams& p, bool res, uint32_t budget, int& stages) {
-    constexpr uint32_t TEAMS = LANES < 256 ? 256 / LANES : 1;
-    const uint64_t stage = ((uint64_t)p.K * sizeof(T) + 127) / 128 * 128 * (res ? 2 : 1);
-    const uint64_t fit = (budget - RING_HEAD) / (stage * TEAMS);
-    stages = (int)(fit > RING_MAX ? RING_MAX : fit);
-    return stages >= 2;
-}
-template <typename T, int LANES>
-int launch_ring(const void* x, const void* r, void* h, const NormParams& p, int stages,
-                int per_sm, cudaStream_t s) {
-    constexpr uint32_t TEAMS = LANES < 256 ? 256 / LANES : 1;
+// Shared memory of a ring of two stages sets the blocks per SM (as many as were compiled for at
+// most), what that leaves the stages.
+template <typename T, typename W, int LANES>
+int launch_ring(const NormArgs& a, const NormParams& p) {
+    constexpr uint32_t THREADS = ring_threads(LANES), TEAMS = THREADS / LANES;
+    constexpr uint32_t SM_BYTES = 224 * 1024, BLOCKS = ring_blocks<T, W>(LANES);
     const uint32_t half = (p.K * (uint32_t)sizeof(T) + 127) / 128 * 128;
-    const size_t smem = RING_HEAD + (size_t)TEAMS * stages * half * (r ? 2 : 1);
-    auto k = rms_norm_mx_ring_kernel<T, LANES>;
+    const uint32_t stage = TEAMS * half * (a.r ? 2 : 1);
+    uint32_t per_sm = SM_BYTES / (2 * stage + RING_HEAD + 1024);
+    if (per_sm < 1) return SNNB_ERR_UNSUPPORTED;
+    if (per_sm > BLOCKS) per_sm = BLOCKS;
+    uint32_t stages = (SM_BYTES / per_sm - RING_HEAD - 1024) / stage;
+    if (stages > RING_MAX) stages = RING_MAX;
+    const size_t smem = RING_HEAD + (size_t)stages * stage;
+    auto k = a.r ? rms_norm_mx_ring_kernel<T, W, LANES, true>
+                 : rms_norm_mx_ring_kernel<T, W, LANES, false>;
     const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return record_cuda_error(e);
     const uint32_t need = (p.rows + TEAMS - 1) / TEAMS, most = 148u * per_sm;
-    return launch_k(k, dim3(need < most ? need : most), dim3(LANES < 256 ? 256 : LANES), smem, s,
-                    static_cast<const T*>(x), static_cast<const T*>(r), static_cast<T*>(h), p,
-                    stages, half);
+    return launch_k(k, dim3(need < most ? need : most), dim3(THREADS), smem, a.s,
+                    static_cast<const T*>(a.x), static_cast<const T*>(a.r), static_cast<T*>(a.h),
+                    static_cast<const W*>(a.weight), p, (int)stages, half);
 }
 
-template <typename T>
-int run_norm(const void* x, const void* r, void* h, const NormParams& p, cudaStream_t s) {
+template <typename T, typename W>
+int run_norm(const NormArgs& a, const NormParams& p) {
     const int64_t es = sizeof(T);
     const uint32_t K = p.K;
     const bool one = p.rows == 1;
-    const bool aligned = K % 8 == 0 && aligned16(x) && (one || p.ldx * es % 16 == 0) &&
-                         (!r || (aligned16(r) && (one || p.ldr * es % 16 == 0))) &&
-                         (!h || aligned16(h)) && aligned16(p.weight);
+    const bool aligned = K % 8 == 0 && aligned16(a.x) && (one || p.ldx * es % 16 == 0) &&
+                         (!a.r || (aligned16(a.r) && (one || p.ldr * es % 16 == 0))) &&
+                         (!a.h || aligned16(a.h)) && aligned16(a.weight);
     if (!aligned) {
-        if (K <= 1024) return launch_norm<T, false, 32, 4>(x, r, h, p, s);
-        if (K <= 8192) return launch_norm<T, false, 256, 4>(x, r, h, p, s);
-        return launch_norm<T, false, 1024, 0>(x, r, h, p, s);
+        if (K <= 1024) return launch_norm<T, W, false, 32, 4>(a, p);
+        if (K <= 8192) return launch_norm<T, W, false, 256, 4>(a, p);
+        return launch_norm<T, W, false, 1024, 0>(a, p);
     }
+    // short rows: the copies of a ring cost more than they hide
+    if (K <= 128) return launch_norm<T, W, true, 16, 1>(a, p);
+    if (K <= 256) return launch_norm<T, W, true, 32, 1>(a, p);
     // Few rows (at most one per SM): as many threads as the row has groups of 8, for the shortest
     // chain of loads, sum and stores.
     if (p.rows <= 148) {
-        if (K <= 256) return launch_norm<T, true, 32, 1>(x, r, h, p, s);
-        if (K <= 2048) return launch_norm<T, true, 256, 1>(x, r, h, p, s);
-        if (K <= 4096) return launch_norm<T, true, 512, 1>(x, r, h, p, s);
-        if (K <= 8192) return launch_norm<T, true, 1024, 1>(x, r, h, p, s);
-        return launch_norm<T, true, 1024, 0>(x, r, h, p, s);
+        if (K <= 2048) return launch_norm<T, W, true, 256, 1>(a, p);
+        if (K <= 4096) return launch_norm<T, W, true, 512, 1>(a, p);
+        if (K <= 8192) return launch_norm<T, W, true, 1024, 1>(a, p);
+        return launch_norm<T, W, true, 1024, 0>(a, p);
     }
-    int st;
-    if (ring_fits<T, 32>(p, r, RING_BUDGET, st)) return launch_ring<T, 32>(x, r, h, p, st, 2, s);
-    if (ring_fits<T, 128>(p, r, RING_BUDGET, st)) return launch_ring<T, 128>(x, r, h, p, st, 2, s);
-    if (ring_fits<T, 256>(p, r, RING_BUDGET, st)) return launch_ring<T, 256>(x, r, h, p, st, 2, s);
-    if (ring_fits<T, 512>(p, r, 2 * RING_BUDGET, st)) return launch_ring<T, 512>(x, r, h, p, st, 1, s);
-    return launch_norm<T, true, 1024, 0>(x, r, h, p, s);
+    if (K <= 1024) return launch_norm<T, W, true, 32, 4>(a, p);
+    // 32 values a thread; a ring of two rows (and residuals) has to fit the SM
+    if (K <= 2048) return launch_ring<T, W, 64>(a, p);
+    if (K <= 4096) return launch_ring<T, W, 128>(a, p);
+    if (K <= 8192) return launch_ring<T, W, 256>(a, p);
+    if (K <= 16384 && (uint64_t)K * es * (a.r ? 2 : 1) <= 100 * 1024)
+        return launch_ring<T, W, 512>(a, p);
+    return launch_norm<T, W, true, 1024, 0>(a, p);
 }
 
 }  // namespace
@@ -454,8 +483,6 @@ extern "C" int snnb_rms_norm_mx(const void* x, int64_t ldx, const void* residual
     NormParams p = {};
     p.status = device_status_ptr();
     if (!p.status) return SNNB_ERR_CUDA;
-    p.weight = weight;
-    p.w_f32 = weight_dtype == SNNB_F32;
     p.fmt = fmt;
     p.eps = eps;
     p.inv_k = 1.0 / (double)K;
@@ -468,7 +495,11 @@ extern "C" int snnb_rms_norm_mx(const void* x, int64_t ldx, const void* residual
     p.data = static_cast<uint8_t*>(data);
     p.scales = static_cast<uint32_t*>(scales);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (x_dtype == SNNB_F32) return run_norm<float>(x, residual, h_out, p, s);
-    if (x_dtype == SNNB_F16) return run_norm<__half>(x, residual, h_out, p, s);
-    return run_norm<__nv_bfloat16>(x, residual, h_out, p, s);
+    const NormArgs a = {x, residual, weight, h_out, s};
+    if (x_dtype == SNNB_F32) return run_norm<float, float>(a, p);
+    if (x_dtype == SNNB_F16)
+        return weight_dtype == SNNB_F32 ? run_norm<__half, float>(a, p)
+                                        : run_norm<__half, __half>(a, p);
+    return weight_dtype == SNNB_F32 ? run_norm<__nv_bfloat16, float>(a, p)
+                                    : run_norm<__nv_bfloat16, __nv_bfloat16>(a, p);
 }
