@@ -69,6 +69,37 @@ __device__ __forceinline__ void encode8(const float (&v)[8], uint2& c) {
         : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
 }
 
+// Two float operations an instruction (each rounded as the scalar one is).
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+// v = a * s.
+__device__ __forceinline__ void scale8(const float (&a)[8], float s, float (&v)[8]) {
+    const uint64_t ss = pack2(s, s);
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) unpack2(mul2(pack2(a[i], a[i + 1]), ss), v[i], v[i + 1]);
+}
+
 // The values of 8 codes (exact: both element formats are subsets of f16).
 __device__ __forceinline__ void halves_to_f32(uint32_t h, float& a, float& b) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
@@ -105,8 +136,8 @@ __device__ __forceinline__ void decode8(uint2 c, float (&v)[8]) {
 
 // 2^(byte - 127); the value of byte 0 is subnormal, 255 is NaN.
 __device__ __forceinline__ float scale_value(uint32_t byte) {
-    if (byte == 255) return __int_as_float(0x7FC00000);
-    return byte == 0 ? __int_as_float(0x00400000) : __int_as_float((int)(byte << 23));
+    const uint32_t bits = byte << 23;
+    return __int_as_float((int)(byte == 0 ? 0x00400000u : byte == 255 ? 0x7FC00000u : bits));
 }
 
 // ---- quantising a block of 32 values held by 4 neighbouring lanes, 8 each ----------------
@@ -146,8 +177,7 @@ __device__ __forceinline__ uint32_t quantise_block(const float (&x)[8], uint32_t
     // normal range is far below the smallest element and rounds to zero either way
     const float inv = __int_as_float((int)((254u - byte) << 23));
     float v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = x[i] * inv;
+    scale8(x, inv, v);
     encode8(v, codes);
     if constexpr (FMT == SNNB_MXFP4) {
         codes = bad ? 0u : codes;

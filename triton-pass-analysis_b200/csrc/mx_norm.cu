@@ -34,6 +34,11 @@ struct NormParams {
     int* status;
 };
 
+__device__ __forceinline__ void add8(float (&a)[8], const float (&b)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2)
+        mx::unpack2(mx::add2(mx::pack2(a[i], a[i + 1]), mx::pack2(b[i], b[i + 1])), a[i], a[i + 1]);
+}
 // Sum over aligned groups of LANES lanes of a warp.
 template <int LANES>
 __device__ __forceinline__ double lanes_sum(double v) {
@@ -43,9 +48,11 @@ __device__ __forceinline__ double lanes_sum(double v) {
 }
 // Sum of 8 squares.
 __device__ __forceinline__ float squares8(const float (&h)[8]) {
-    const float a = fmaf(h[0], h[0], h[1] * h[1]), b = fmaf(h[2], h[2], h[3] * h[3]);
-    const float c = fmaf(h[4], h[4], h[5] * h[5]), d = fmaf(h[6], h[6], h[7] * h[7]);
-    return (a + b) + (c + d);
+    const uint64_t a = mx::pack2(h[0], h[1]), b = mx::pack2(h[2], h[3]);
+    const uint64_t c = mx::pack2(h[4], h[5]), d = mx::pack2(h[6], h[7]);
+    float x, y;
+    mx::unpack2(mx::add2(mx::fma2(a, a, mx::mul2(b, b)), mx::fma2(c, c, mx::mul2(d, d))), x, y);
+    return x + y;
 }
 // ... in float64 where float32 overflows or loses it: squares of values past 2^63 or below 2^-50.
 __device__ __forceinline__ double squares8_exact(const float (&h)[8]) {
@@ -70,12 +77,18 @@ __device__ __forceinline__ double rstd_of(const NormParams& p, double sum) {
 // y of 8 values (see the top); values past n, whose h and w are 0, give 0.
 __device__ __forceinline__ void normed8(const float (&h)[8], const float (&w)[8], float rstd,
                                         double rstd64, float (&y)[8]) {
-    uint32_t near = 0xffffffffu;
+    // two values' low halves at once (a carry out of the lower one only comes from a value that
+    // is near itself)
+    const uint64_t rr = mx::pack2(rstd, rstd);
+    uint32_t pairs = 0xffffffffu;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        y[i] = __fmul_rn(__fmul_rn(h[i], rstd), w[i]);
-        near = min(near, ((uint32_t)__float_as_int(y[i]) + 4u) & 0x7FFFFu);
+    for (int i = 0; i < 8; i += 2) {
+        mx::unpack2(mx::mul2(mx::mul2(mx::pack2(h[i], h[i + 1]), rr), mx::pack2(w[i], w[i + 1])), y[i],
+                    y[i + 1]);
+        pairs = __vminu2(pairs, __byte_perm((uint32_t)__float_as_int(y[i]),
+                                            (uint32_t)__float_as_int(y[i + 1]), 0x5410) + 0x00040004u);
     }
+    const uint32_t near = min(pairs & 0xffffu, pairs >> 16);
     if (near <= 8) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -132,8 +145,7 @@ __device__ __forceinline__ void take8(const NormParams& p, const T* x, const T* 
         if (n > 0) b = ALIGNED ? mx::load_aligned8(rr + k) : mx::load_any8(rr + k, n, rr, (int64_t)p.K);
         float f[8];
         mx::to_floats(b, f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) h[i] += f[i];
+        add8(h, f);
     }
 }
 template <typename T, bool ALIGNED>
@@ -266,7 +278,8 @@ template <typename T, typename W> constexpr int ring_blocks(int lanes) {
 // stage holds one row of x and, `half` bytes behind it, of the residual (RES).  A thread holds
 // CHUNKS x 8 values of the row in registers, as in rms_norm_mx_kernel, and its columns' weights
 // for all rows.
-template <typename T, typename W, int LANES, bool RES>
+// FULL: K is a multiple of 8 LANES, so no chunk ends inside a row.
+template <typename T, typename W, int LANES, bool RES, bool FULL>
 __global__ void __launch_bounds__(ring_threads(LANES), ring_blocks<T, W>(LANES))
 rms_norm_mx_ring_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __restrict__ h_out,
                         const W* __restrict__ weight, const NormParams p, int stages,
@@ -335,13 +348,12 @@ rms_norm_mx_ring_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __r
         for (int c = 0; c < RING_CHUNKS; ++c) {
             const uint32_t k = (c * LANES + t) * 8;
             if (c > 0 && (k & ~255u) >= p.K) break;                           // whole warps
-            const bool in = k < p.K;
+            const bool in = FULL || k < p.K;
             mx::to_floats(in ? smem8<T>(xs, k) : mx::zero8<T>(), h[c]);
             if (RES) {
                 float f[8];
                 mx::to_floats(in ? smem8<T>(xs + half, k) : mx::zero8<T>(), f);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) h[c][i] += f[i];
+                add8(h[c], f);
             }
             if (hr && in) {
                 mx::Raw8<T> o;
@@ -413,8 +425,11 @@ int launch_ring(const NormArgs& a, const NormParams& p) {
     uint32_t stages = (SM_BYTES / per_sm - RING_HEAD - 1024) / stage;
     if (stages > RING_MAX) stages = RING_MAX;
     const size_t smem = RING_HEAD + (size_t)stages * stage;
-    auto k = a.r ? rms_norm_mx_ring_kernel<T, W, LANES, true>
-                 : rms_norm_mx_ring_kernel<T, W, LANES, false>;
+    const bool full = p.K % (8 * LANES) == 0;
+    auto k = a.r ? full ? rms_norm_mx_ring_kernel<T, W, LANES, true, true>
+                        : rms_norm_mx_ring_kernel<T, W, LANES, true, false>
+                 : full ? rms_norm_mx_ring_kernel<T, W, LANES, false, true>
+                        : rms_norm_mx_ring_kernel<T, W, LANES, false, false>;
     const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return record_cuda_error(e);
     const uint32_t need = (p.rows + TEAMS - 1) / TEAMS, most = 148u * per_sm;

@@ -17,9 +17,14 @@ namespace snnb {
 namespace {
 
 constexpr int Q_THREADS = 256;
-constexpr int Q_UNROLL = 4;                      // blocks (or row pieces) of a lane in flight
 
-template <typename T, int FMT>
+// A thread block takes U x 64 consecutive blocks of 32 (or U x 8 row pieces of 256), so that a
+// thread has U loads in flight, and ends: with blocks resident for the whole launch that stride
+// through the tensor, 16384 x 8192 bf16 took 69 us (E2M1; 63 in this form) and 68 back (56).
+// U is 4 (2 for row pieces), or 1 for tensors too small to give every SM four blocks of those.
+
+// FLAT: K % 128 == 0 and contiguous rows, so values and codes lie at their block's index.
+template <typename T, int FMT, int U, bool FLAT>
 __global__ void __launch_bounds__(Q_THREADS)
 mx_quantize_kernel(const T* __restrict__ x, uint32_t rows, uint32_t K, int64_t ldx, uint32_t nb,
                    uint32_t groups, mx::FastDiv per_row, uint32_t total,
@@ -29,28 +34,41 @@ mx_quantize_kernel(const T* __restrict__ x, uint32_t rows, uint32_t K, int64_t l
     pdl_wait();
     pdl_trigger();
     const uint32_t lane = threadIdx.x & 31, sub = lane & 3;
-    const uint32_t thread = blockIdx.x * Q_THREADS + threadIdx.x;
-    const uint32_t step = gridDim.x * (Q_THREADS / 4);
-    // a warp's 32 lanes leave together: the loop goes by its first block
-    for (uint32_t first = (thread >> 5) * 8; first < total; first += Q_UNROLL * step) {
-        mx::Raw8<T> raw[Q_UNROLL];
-        uint32_t row[Q_UNROLL], j[Q_UNROLL];
+    const uint64_t thread = (uint64_t)blockIdx.x * Q_THREADS + threadIdx.x;
+    // of this warp; blocks past the last count as zeros
+    constexpr uint32_t step = Q_THREADS / 4;
+    const uint32_t first = blockIdx.x * (U * step) + (threadIdx.x >> 5) * 8;
+    {
+        mx::Raw8<T> raw[U];
+        uint32_t row[U], j[U];
 #pragma unroll
-        for (int u = 0; u < Q_UNROLL; ++u) {
+        for (int u = 0; u < U; ++u) {
             const uint32_t q = first + u * step + (lane >> 2);
-            row[u] = per_row.div(q);
-            j[u] = q - row[u] * per_row.d;
-            const uint32_t k = j[u] * 32 + sub * 8;
-            raw[u] = q < total && k < K ? mx::load_aligned8(x + row[u] * ldx + k) : mx::zero8<T>();
+            if (FLAT) {
+                raw[u] = q < total ? mx::load_aligned8(x + (uint64_t)q * 32 + sub * 8) : mx::zero8<T>();
+            } else {
+                row[u] = per_row.div(q);
+                j[u] = q - row[u] * per_row.d;
+                const uint32_t k = j[u] * 32 + sub * 8;
+                raw[u] = q < total && k < K ? mx::load_aligned8(x + row[u] * ldx + k) : mx::zero8<T>();
+            }
         }
 #pragma unroll
-        for (int u = 0; u < Q_UNROLL; ++u) {
+        for (int u = 0; u < U; ++u) {
             float v[8];
             mx::to_floats(raw[u], v);
             Codes c;
             const uint32_t byte = mx::quantise_block<FMT>(v, mx::top_exponent(raw[u], v), c);
             const uint32_t word = mx::join_scales(byte, lane);
-            if (first + u * step + (lane >> 2) < total) {
+            const uint32_t q = first + u * step + (lane >> 2);
+            if (q >= total) continue;
+            if (FLAT) {
+                *reinterpret_cast<Codes*>(data + (uint64_t)q * F::BLOCK_BYTES + sub * sizeof(Codes)) = c;
+                if ((lane & 15) == 0) {
+                    const uint32_t r = per_row.div(q);
+                    scales[mx::scale_word(r, (q - r * per_row.d) >> 2, groups)] = word;
+                }
+            } else {
                 if (j[u] < nb)
                     *reinterpret_cast<Codes*>(data + (uint64_t)(row[u] * nb + j[u]) * F::BLOCK_BYTES +
                                               sub * sizeof(Codes)) = c;
@@ -62,7 +80,7 @@ mx_quantize_kernel(const T* __restrict__ x, uint32_t rows, uint32_t K, int64_t l
 }
 
 // total: pieces of 256 values, per_row.d = ceil(K / 256) of them a row.
-template <typename T, int FMT>
+template <typename T, int FMT, int U>
 __global__ void __launch_bounds__(Q_THREADS)
 mx_quantize_any_kernel(const T* __restrict__ x, uint32_t rows, uint32_t K, int64_t ldx,
                        uint32_t nb, uint32_t groups, mx::FastDiv per_row, uint32_t total,
@@ -72,13 +90,14 @@ mx_quantize_any_kernel(const T* __restrict__ x, uint32_t rows, uint32_t K, int64
     pdl_wait();
     pdl_trigger();
     const uint32_t lane = threadIdx.x & 31, sub = lane & 3;
-    const uint32_t thread = blockIdx.x * Q_THREADS + threadIdx.x;
-    const uint32_t step = gridDim.x * (Q_THREADS / 32);
-    for (uint32_t first = thread >> 5; first < total; first += Q_UNROLL * step) {
-        mx::Raw8<T> raw[Q_UNROLL];
-        uint32_t row[Q_UNROLL], k[Q_UNROLL];
+    const uint64_t thread = (uint64_t)blockIdx.x * Q_THREADS + threadIdx.x;
+    constexpr uint32_t step = Q_THREADS / 32;
+    const uint32_t first = blockIdx.x * (U * step) + (threadIdx.x >> 5);
+    {
+        mx::Raw8<T> raw[U];
+        uint32_t row[U], k[U];
 #pragma unroll
-        for (int u = 0; u < Q_UNROLL; ++u) {
+        for (int u = 0; u < U; ++u) {
             const uint32_t q = first + u * step;
             row[u] = per_row.div(q);
             k[u] = (q - row[u] * per_row.d) * 256 + lane * 8;
@@ -90,7 +109,7 @@ mx_quantize_any_kernel(const T* __restrict__ x, uint32_t rows, uint32_t K, int64
             }
         }
 #pragma unroll
-        for (int u = 0; u < Q_UNROLL; ++u) {
+        for (int u = 0; u < U; ++u) {
             float v[8];
             mx::to_floats(raw[u], v);
             Codes c;
@@ -114,16 +133,15 @@ __device__ __forceinline__ mx::Raw8<T> decode_scaled(typename mx::Fmt<FMT>::Code
                                                      uint32_t byte) {
     float v[8];
     mx::decode8(c, v);
-    const float s = mx::scale_value(byte);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= s;
+    mx::scale8(v, mx::scale_value(byte), v);
     mx::Raw8<T> r;
     mx::from_floats(v, r);
     return r;
 }
 
-// total: blocks, per_row.d = nb of them a row; ALIGNED: K % 8 == 0 and out 16-byte aligned.
-template <typename T, int FMT>
+// K % 8 == 0 and out 16-byte aligned; FLAT: K % 32 == 0, so values lie at their block's index.
+// total: blocks, per_row.d = nb of them a row.
+template <typename T, int FMT, int U, bool FLAT>
 __global__ void __launch_bounds__(Q_THREADS)
 mx_dequantize_kernel(const uint8_t* __restrict__ data, const uint8_t* __restrict__ scales,
                      uint32_t rows, uint32_t K, uint32_t groups, mx::FastDiv per_row,
@@ -133,13 +151,13 @@ mx_dequantize_kernel(const uint8_t* __restrict__ data, const uint8_t* __restrict
     pdl_wait();
     pdl_trigger();
     const uint32_t sub = threadIdx.x & 3;
-    const uint32_t thread = blockIdx.x * Q_THREADS + threadIdx.x;
-    const uint32_t step = gridDim.x * (Q_THREADS / 4);
-    for (uint32_t first = thread >> 2; first < total; first += Q_UNROLL * step) {
-        Codes c[Q_UNROLL];
-        uint32_t byte[Q_UNROLL], row[Q_UNROLL], j[Q_UNROLL];
+    constexpr uint32_t step = Q_THREADS / 4;
+    const uint32_t first = blockIdx.x * (U * step) + (threadIdx.x >> 2);
+    {
+        Codes c[U];
+        uint32_t byte[U], row[U], j[U];
 #pragma unroll
-        for (int u = 0; u < Q_UNROLL; ++u) {
+        for (int u = 0; u < U; ++u) {
             const uint32_t q = first + u * step;
             row[u] = per_row.div(q);
             j[u] = q - row[u] * per_row.d;
@@ -151,16 +169,17 @@ mx_dequantize_kernel(const uint8_t* __restrict__ data, const uint8_t* __restrict
             }
         }
 #pragma unroll
-        for (int u = 0; u < Q_UNROLL; ++u) {
-            const uint32_t k = j[u] * 32 + sub * 8;
-            if (first + u * step < total && k < K)
-                mx::store_aligned8(out + (uint64_t)row[u] * K + k, decode_scaled<T, FMT>(c[u], byte[u]));
+        for (int u = 0; u < U; ++u) {
+            const uint32_t q = first + u * step, k = j[u] * 32 + sub * 8;
+            if (q < total && (FLAT || k < K))
+                mx::store_aligned8(out + (FLAT ? (uint64_t)q * 32 + sub * 8 : (uint64_t)row[u] * K + k),
+                                   decode_scaled<T, FMT>(c[u], byte[u]));
         }
     }
 }
 
 // total: pieces of 256 values, per_row.d = ceil(K / 256) of them a row.
-template <typename T, int FMT>
+template <typename T, int FMT, int U>
 __global__ void __launch_bounds__(Q_THREADS)
 mx_dequantize_any_kernel(const uint8_t* __restrict__ data, const uint8_t* __restrict__ scales,
                          uint32_t rows, uint32_t K, uint32_t nb, uint32_t groups,
@@ -170,13 +189,13 @@ mx_dequantize_any_kernel(const uint8_t* __restrict__ data, const uint8_t* __rest
     pdl_wait();
     pdl_trigger();
     const uint32_t lane = threadIdx.x & 31, sub = lane & 3;
-    const uint32_t thread = blockIdx.x * Q_THREADS + threadIdx.x;
-    const uint32_t step = gridDim.x * (Q_THREADS / 32);
-    for (uint32_t first = thread >> 5; first < total; first += Q_UNROLL * step) {
-        Codes c[Q_UNROLL];
-        uint32_t byte[Q_UNROLL], row[Q_UNROLL], k[Q_UNROLL];
+    constexpr uint32_t step = Q_THREADS / 32;
+    const uint32_t first = blockIdx.x * (U * step) + (threadIdx.x >> 5);
+    {
+        Codes c[U];
+        uint32_t byte[U], row[U], k[U];
 #pragma unroll
-        for (int u = 0; u < Q_UNROLL; ++u) {
+        for (int u = 0; u < U; ++u) {
             const uint32_t q = first + u * step;
             row[u] = per_row.div(q);
             k[u] = (q - row[u] * per_row.d) * 256 + lane * 8;
@@ -190,7 +209,7 @@ mx_dequantize_any_kernel(const uint8_t* __restrict__ data, const uint8_t* __rest
             }
         }
 #pragma unroll
-        for (int u = 0; u < Q_UNROLL; ++u) {
+        for (int u = 0; u < U; ++u) {
             const bool in = first + u * step < total && k[u] < K;
             mx::store_any8(out + (in ? (uint64_t)row[u] * K + k[u] : 0),
                            in ? (int)min(8u, K - k[u]) : 0, decode_scaled<T, FMT>(c[u], byte[u]),
@@ -199,21 +218,24 @@ mx_dequantize_any_kernel(const uint8_t* __restrict__ data, const uint8_t* __rest
     }
 }
 
-// Blocks of 256 threads: what `warps` warps need, a full round of resident ones at most.
-unsigned grid_for(int64_t warps) {
-    const int64_t need = (warps + Q_THREADS / 32 - 1) / (Q_THREADS / 32);
-    return (unsigned)(need < 1 ? 1 : (need > 148 * 8 ? 148 * 8 : need));
-}
+// Whether U = 1: `units` (per thread block and unit of U: `per`) do not fill four blocks an SM.
+bool small(int64_t units, int64_t per) { return units <= 148 * 4 * 4 * per; }
+unsigned blocks_for(int64_t units, int64_t per) { return (unsigned)((units + per - 1) / per); }
 
 template <typename T, int FMT>
 int run_quantize(const void* x, int64_t rows, int64_t K, int64_t ldx, void* data, void* scales,
                  cudaStream_t s) {
     const uint32_t nb = (uint32_t)mx::blocks_of(K), groups = (uint32_t)mx::groups_of(K);
     const bool aligned = K % 8 == 0 && aligned16(x) && (rows == 1 || ldx * (int64_t)sizeof(T) % 16 == 0);
+    const bool flat = K % 128 == 0 && (rows == 1 || ldx == K);
     const uint32_t per = aligned ? groups * 4 : (uint32_t)((K + 255) / 256);
-    const int64_t total = rows * per;
-    auto k = aligned ? mx_quantize_kernel<T, FMT> : mx_quantize_any_kernel<T, FMT>;
-    return launch_k(k, dim3(grid_for(aligned ? (total + 7) / 8 : total)), dim3(Q_THREADS), 0, s,
+    const int64_t total = rows * per, unit = aligned ? Q_THREADS / 4 : Q_THREADS / 32;
+    const bool one = small(total, unit);
+    auto k = !aligned ? (one ? mx_quantize_any_kernel<T, FMT, 1> : mx_quantize_any_kernel<T, FMT, 2>)
+             : flat   ? (one ? mx_quantize_kernel<T, FMT, 1, true> : mx_quantize_kernel<T, FMT, 4, true>)
+                      : (one ? mx_quantize_kernel<T, FMT, 1, false> : mx_quantize_kernel<T, FMT, 4, false>);
+    const int U = one ? 1 : aligned ? 4 : 2;
+    return launch_k(k, dim3(blocks_for(total, U * unit)), dim3(Q_THREADS), 0, s,
                     static_cast<const T*>(x), (uint32_t)rows, (uint32_t)K, ldx, nb, groups,
                     mx::FastDiv(per), (uint32_t)total, static_cast<uint8_t*>(data),
                     static_cast<uint32_t*>(scales));
@@ -226,16 +248,21 @@ int run_dequantize(const void* data, const void* scales, int64_t rows, int64_t K
     const uint8_t* d = static_cast<const uint8_t*>(data);
     const uint8_t* sc = static_cast<const uint8_t*>(scales);
     if (K % 8 == 0 && aligned16(out)) {
-        const int64_t total = rows * nb;
-        return launch_k(mx_dequantize_kernel<T, FMT>, dim3(grid_for((total + 7) / 8)),
-                        dim3(Q_THREADS), 0, s, d, sc, (uint32_t)rows, (uint32_t)K, groups,
-                        mx::FastDiv(nb), (uint32_t)total, static_cast<T*>(out));
+        const int64_t total = rows * nb, unit = Q_THREADS / 4;
+        const bool one = small(total, unit), flat = K % 32 == 0;
+        auto k = flat ? (one ? mx_dequantize_kernel<T, FMT, 1, true> : mx_dequantize_kernel<T, FMT, 4, true>)
+                      : (one ? mx_dequantize_kernel<T, FMT, 1, false> : mx_dequantize_kernel<T, FMT, 4, false>);
+        return launch_k(k, dim3(blocks_for(total, (one ? 1 : 4) * unit)), dim3(Q_THREADS), 0, s, d,
+                        sc, (uint32_t)rows, (uint32_t)K, groups, mx::FastDiv(nb), (uint32_t)total,
+                        static_cast<T*>(out));
     }
     const uint32_t per = (uint32_t)((K + 255) / 256);
-    const int64_t total = rows * per;
-    return launch_k(mx_dequantize_any_kernel<T, FMT>, dim3(grid_for(total)), dim3(Q_THREADS), 0, s,
-                    d, sc, (uint32_t)rows, (uint32_t)K, nb, groups, mx::FastDiv(per),
-                    (uint32_t)total, static_cast<T*>(out));
+    const int64_t total = rows * per, unit = Q_THREADS / 32;
+    const bool one = small(total, unit);
+    auto k = one ? mx_dequantize_any_kernel<T, FMT, 1> : mx_dequantize_any_kernel<T, FMT, 2>;
+    return launch_k(k, dim3(blocks_for(total, (one ? 1 : 2) * unit)), dim3(Q_THREADS), 0, s, d, sc,
+                    (uint32_t)rows, (uint32_t)K, nb, groups, mx::FastDiv(per), (uint32_t)total,
+                    static_cast<T*>(out));
 }
 
 }  // namespace
