@@ -287,7 +287,7 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
     const int nstages = (p.groups + S::GROUPS - 1) / S::GROUPS;
     const int k0 = (int)((int64_t)nstages * rank / splits);
     const int k1 = (int)((int64_t)nstages * (rank + 1) / splits);
-    uint32_t failed = 0;
+    uint32_t failed = 0, issued = 0;                 // issued: a producer warp's copies
 
     if (warp < NP) {
         // ------------------------------------------------------------- copies
@@ -299,8 +299,8 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
                                                                                       : BYTES[3]) *
                               (uint32_t)CTAS;
         const bool own_ring = S::PACKED > 0 && warp == 3;
-        uint32_t it = 0, issued = 0;
-        for (int tile = tile0; tile < p.tiles; tile += tile_step) {
+        uint32_t it = 0;
+        for (int tile = tile0; tile < p.tiles && !failed; tile += tile_step) {
             const int tw = (tile % p.tiles_w) * CTAS + crank, tt = tile / p.tiles_w;
             for (int ks = k0; ks < k1; ++ks, ++it) {
                 const int s = (int)(it % STAGES);
@@ -328,17 +328,6 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
                 __syncwarp();
                 ++issued;
             }
-            if (failed) break;
-        }
-        if (failed) {
-            // copies still in flight land before the CTA may exit: on the full barrier, or for
-            // the odd CTA of a pair (whose copies complete the even CTA's) on the stage's release
-            for (uint32_t k = 0; k < issued && k < (uint32_t)STAGES; ++k) {
-                const uint32_t g = issued - 1 - k;
-                const int s = (int)(g % STAGES);
-                tc::mbar_wait_warp<true>(own_ring ? pfull_bar(s) : crank ? empty_bar(s) : full_bar(s),
-                                         (g / STAGES) & 1u, 0);
-            }
         }
     } else if (warp == NP) {
         // ------------------------------------------------------------- MMA issuer
@@ -356,51 +345,51 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
         if (crank == 0) {
             if (tc::elect_one()) {
                 uint32_t it = 0, local = 0;
-                for (int tile = tile0; tile < p.tiles; tile += tile_step, ++local) {
+                for (int tile = tile0; tile < p.tiles && !failed; tile += tile_step, ++local) {
                     const int b = (int)(local % S::ACCS);
                     failed |= 1u - tc::mbar_wait_lane(acce_bar(b), ((local / S::ACCS) & 1u) ^ 1u, failed);
                     tc::tc_fence_after();
                     wait_full(it);
                     const uint32_t d = tmem + (uint32_t)(b * BN);
-                    for (int ks = k0; ks < k1; ++ks, ++it) {
+                    // after a wait that ran out: no more MMAs and nothing handed on, so that
+                    // every other role's wait runs out too
+                    for (int ks = k0; ks < k1 && !failed; ++ks, ++it) {
                         const int s = (int)(it % STAGES);
-                        if (!failed) {
-                            const uint32_t sw = tmem + (uint32_t)(S::ACCS * BN + s * S::SCALE_COLS);
-                            const uint32_t sa = sw + 4 * S::GROUPS;
-                            const uint32_t sc = scales_at(s);
-                            const uint64_t dw = tc::sdesc_k_sw128(w_tile(s));
-                            const uint64_t da = tc::sdesc_k_sw128(a_tile(s));
-                            constexpr int PER_GROUP = 4 / S::GROUPS;     // MMAs per 128 of K
+                        const uint32_t sw = tmem + (uint32_t)(S::ACCS * BN + s * S::SCALE_COLS);
+                        const uint32_t sa = sw + 4 * S::GROUPS;
+                        const uint32_t sc = scales_at(s);
+                        const uint64_t dw = tc::sdesc_k_sw128(w_tile(s));
+                        const uint64_t da = tc::sdesc_k_sw128(a_tile(s));
+                        constexpr int PER_GROUP = 4 / S::GROUPS;     // MMAs per 128 of K
 #pragma unroll
-                            for (int g = 0; g < S::GROUPS; ++g) {
-                                if (g > 0 && ks * S::GROUPS + g >= p.groups) break;
-                                copy_scales<PAIR>(sw + 4 * g, sc + g * mx::GROUP_BYTES);
+                        for (int g = 0; g < S::GROUPS; ++g) {
+                            if (g > 0 && ks * S::GROUPS + g >= p.groups) break;
+                            copy_scales<PAIR>(sw + 4 * g, sc + g * mx::GROUP_BYTES);
 #pragma unroll
-                                for (int h = 0; h < S::TOKEN_TILES; ++h)
-                                    copy_scales<PAIR>(sa + 4 * (g * S::TOKEN_TILES + h),
-                                                      sc + S::W_SCALES +
-                                                          (h * S::GROUPS + g) * mx::GROUP_BYTES);
+                            for (int h = 0; h < S::TOKEN_TILES; ++h)
+                                copy_scales<PAIR>(sa + 4 * (g * S::TOKEN_TILES + h),
+                                                  sc + S::W_SCALES +
+                                                      (h * S::GROUPS + g) * mx::GROUP_BYTES);
 #pragma unroll
-                                for (int m = 0; m < PER_GROUP; ++m) {
-                                    const int k = g * PER_GROUP + m;
-                                    umma_mx<FMT, PAIR>(d, dw + 2 * k, da + 2 * k,
-                                                       IDESC | idesc_scale_byte(m * S::GROUPS),
-                                                       sw + 4 * g, sa + 4 * g * S::TOKEN_TILES,
-                                                       (ks != k0) || (k != 0));
-                                }
+                            for (int m = 0; m < PER_GROUP; ++m) {
+                                const int k = g * PER_GROUP + m;
+                                umma_mx<FMT, PAIR>(d, dw + 2 * k, da + 2 * k,
+                                                   IDESC | idesc_scale_byte(m * S::GROUPS),
+                                                   sw + 4 * g, sa + 4 * g * S::TOKEN_TILES,
+                                                   (ks != k0) || (k != 0));
                             }
                         }
                         // the next stage before this one's commit: a wait behind a commit
                         // returns only once the tensor pipe has drained
                         if (ks + 1 < k1) wait_full(it + 1);
-                        commit(empty_bar(s));
+                        if (!failed) commit(empty_bar(s));
                     }
-                    commit(accf_bar(b));
+                    if (!failed) commit(accf_bar(b));
                 }
                 commit(done_bar);
             }
             __syncwarp();
-            failed = __shfl_sync(0xffffffffu, failed, 0);
+            failed = __any_sync(0xffffffffu, (int)failed);
         }
         // every MMA of this CTA's (or its pair's) has completed
         failed |= 1u - tc::mbar_wait_warp<true>(done_bar, 0, 0);
@@ -523,7 +512,21 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
         }
     }
     tc::tc_fence_before();
-    __syncthreads();
+    if (__syncthreads_or((int)failed)) {
+        // copies still in flight land before the CTA may exit: waits on the full barrier, or for
+        // the odd CTA of a pair (whose copies complete the even CTA's) on the stage's release,
+        // with the limit that outlasts any copy
+        if (warp < NP)
+            for (uint32_t k = 0; k < issued && k < (uint32_t)STAGES; ++k) {
+                const uint32_t g = issued - 1 - k;
+                const int s = (int)(g % STAGES);
+                tc::mbar_wait_warp<true>(S::PACKED > 0 && warp == 3 ? pfull_bar(s)
+                                         : crank                    ? empty_bar(s)
+                                                                    : full_bar(s),
+                                         (g / STAGES) & 1u, 0);
+            }
+        __syncthreads();
+    }
     // neither CTA of a pair leaves while the other may signal its barriers or have its memory
     // read by the tensor pipe; nor one of a split cluster while its partial sums are read
     if (PAIR || splits > 1) tc::cluster_sync();

@@ -3,12 +3,11 @@
 //   y = (h / sqrt(mean(h^2) + eps)) * weight
 //   codes, scales = y in E2M1 or E4M3, one scale per 32 values
 //
-// Rounding.  The norm is taken of the unrounded sum h.  Squares are summed in float32 within 8
-// values and in float64 beyond, and 1 / sqrt is float64, so that rstd is good to ~1e-9: an error
-// of one float32 ulp (6e-8) in y already moves ~7e-7 of the codes to a neighbour.  y itself is
-// float32 unless it lies within 4 ulp of a value that a code boundary could be (its low 19 bits
-// zero: 3 mantissa bits and the half step), where it is formed again in float64 and rounded to
-// odd, which keeps it on its side of the boundary.
+// Rounding.  The norm is taken of the unrounded sum h.  An error of one float32 ulp (6e-8) in y
+// already moves ~7e-7 of the codes to a neighbour, so the squares are summed and 1 / sqrt is
+// taken in float64.  y itself is float32 unless it lies within 4 ulp of a value that a code
+// boundary could be (its low 19 bits zero: 3 mantissa bits and the half step), where it is formed
+// again in float64 and rounded to odd, which keeps it on its side of the boundary.
 //
 // Two forms.  Many aligned rows: a team of LANES threads walks rows, whose x and residual come
 // by bulk copies into a ring in shared memory while earlier rows are worked on; both passes over
@@ -46,24 +45,44 @@ __device__ __forceinline__ double lanes_sum(double v) {
     for (int d = LANES / 2; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
     return v;
 }
-// Sum of 8 squares.
-__device__ __forceinline__ float squares8(const float (&h)[8]) {
-    const uint64_t a = mx::pack2(h[0], h[1]), b = mx::pack2(h[2], h[3]);
-    const uint64_t c = mx::pack2(h[4], h[5]), d = mx::pack2(h[6], h[7]);
-    float x, y;
-    mx::unpack2(mx::add2(mx::fma2(a, a, mx::mul2(b, b)), mx::fma2(c, c, mx::mul2(d, d))), x, y);
-    return x + y;
-}
-// ... in float64 where float32 overflows or loses it: squares of values past 2^63 or below 2^-50.
-__device__ __forceinline__ double squares8_exact(const float (&h)[8]) {
-    double s = 0.0;
+// Sum of N x 8 squares, as if in float64 (~2^-40).  Two float32 sums start at a power of two M
+// above all they will reach: t = fl(a a + s) is then a multiple of M 2^-23, s - t is exact, and
+// fl(a a + (s - t)) is what t lost, summed apart; 4 operations for two squares (converting every
+// value to float64 took 27 us more of a 16384 x 8192 launch's 197).  Values whose squares leave
+// float32's range, infinities and NaN go through float64.
+template <int N>
+__device__ __forceinline__ double squares(const float (&h)[N][8]) {
+    float m = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s = fma((double)h[i], (double)h[i], s);
-    return s;
-}
-__device__ __forceinline__ double add_squares(const float (&h)[8]) {
-    const float s = squares8(h);
-    return s > 1e-30f && s < 1e38f ? (double)s : squares8_exact(h);
+    for (int c = 0; c < N; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) m = mx::max_abs3(m, h[c][i], h[c][i + 1]);
+    if (m == 0.0f) return 0.0;
+    if (!(m > 1e-15f && m < 1e15f)) {
+        double d = 0.0;
+        for (int c = 0; c < N; ++c)
+            for (int i = 0; i < 8; ++i) d = fma((double)h[c][i], (double)h[c][i], d);
+        return d;
+    }
+    // 4 N squares a sum, each below 2^(2 e + 2) for e the exponent of m
+    constexpr int UP = N <= 1 ? 5 : N <= 2 ? 6 : 7;
+    const int e = (int)((uint32_t)__float_as_int(m) >> 23) - 127;
+    const float M = __int_as_float((2 * e + UP + 127) << 23);
+    const uint64_t minus = mx::pack2(-1.0f, -1.0f);
+    uint64_t s = mx::pack2(M, M), lost = mx::pack2(0.0f, 0.0f);
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const uint64_t a = mx::pack2(h[c][i], h[c][i + 1]);
+            const uint64_t t = mx::fma2(a, a, s);
+            lost = mx::add2(lost, mx::fma2(a, a, mx::fma2(t, minus, s)));
+            s = t;
+        }
+    float s0, s1, l0, l1;
+    mx::unpack2(s, s0, s1);
+    mx::unpack2(lost, l0, l1);
+    return (double)(s0 - M) + (double)(s1 - M) + (double)(l0 + l1);
 }
 // 1 / sqrt(sum / K + eps): one Newton step in float64 on the float32 approximation (2^-22, so
 // ~2^-44 after it).
@@ -219,8 +238,8 @@ rms_norm_mx_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __restri
             const uint32_t k = (c * LANES + t) * 8;
             if (c > 0 && past(k, p.K)) break;
             if (h_out) put_h8<T, ALIGNED>(p, h_out, row, k, valid(k), h[c], lane);
-            if (valid(k)) sum += add_squares(h[c]);
         }
+        sum = squares(h);
         const double rstd64 = rstd_of(p, row_sum(sum));
         const float rstd = (float)rstd64;
 #pragma unroll
@@ -230,12 +249,13 @@ rms_norm_mx_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __restri
             finish(k, h[c], rstd, rstd64);
         }
     } else {
-        float h[8];
+        float h1[1][8];
+        float (&h)[8] = h1[0];
         for (uint32_t k = t * 8; !past(k, p.K); k += LANES * 8) {
             const int n = valid(k);
             take8<T, ALIGNED>(p, x, r, row, k, n, h);
             if (h_out) put_h8<T, ALIGNED>(p, h_out, row, k, n, h, lane);
-            if (n) sum += add_squares(h);
+            sum += squares(h1);
         }
         const double rstd64 = rstd_of(p, row_sum(sum));
         const float rstd = (float)rstd64;
@@ -278,7 +298,8 @@ template <typename T, typename W> constexpr int ring_blocks(int lanes) {
 // stage holds one row of x and, `half` bytes behind it, of the residual (RES).  A thread holds
 // CHUNKS x 8 values of the row in registers, as in rms_norm_mx_kernel, and its columns' weights
 // for all rows.
-// FULL: K is a multiple of 8 LANES, so no chunk ends inside a row.
+// FULL: K is all that a team holds, so that no value needs a bounds test (8192 x 8192 float32:
+// 148 us with the tests, 130 without).
 template <typename T, typename W, int LANES, bool RES, bool FULL>
 __global__ void __launch_bounds__(ring_threads(LANES), ring_blocks<T, W>(LANES))
 rms_norm_mx_ring_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __restrict__ h_out,
@@ -343,11 +364,10 @@ rms_norm_mx_ring_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __r
         T* hr = h_out ? h_out + (uint64_t)row * p.K : nullptr;
         if (failed) hr = nullptr;
         float h[RING_CHUNKS][8];
-        double sum = 0.0;
+        double sum;
 #pragma unroll
         for (int c = 0; c < RING_CHUNKS; ++c) {
             const uint32_t k = (c * LANES + t) * 8;
-            if (c > 0 && (k & ~255u) >= p.K) break;                           // whole warps
             const bool in = FULL || k < p.K;
             mx::to_floats(in ? smem8<T>(xs, k) : mx::zero8<T>(), h[c]);
             if (RES) {
@@ -360,9 +380,8 @@ rms_norm_mx_ring_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __r
                 mx::from_floats(h[c], o);
                 mx::store_aligned8(hr + k, o);
             }
-            if (in) sum += add_squares(h[c]);
         }
-        sum = lanes_sum<32>(sum);
+        sum = lanes_sum<32>(squares(h));
         if constexpr (LANES > 32) {
             if (lane == 0) sums[odd * WARPS + (t >> 5)] = sum;
         }
@@ -384,7 +403,7 @@ rms_norm_mx_ring_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __r
 #pragma unroll
         for (int c = 0; c < RING_CHUNKS; ++c) {
             const uint32_t k = (c * LANES + t) * 8;
-            if (c > 0 && (k & ~255u) >= p.groups * 128) break;
+            if (!FULL && c > 0 && (k & ~255u) >= p.groups * 128) break;       // whole warps
             float wf[8], y[8];
             mx::to_floats(w[c], wf);
             normed8(h[c], wf, rstd, rstd64, y);
@@ -425,7 +444,7 @@ int launch_ring(const NormArgs& a, const NormParams& p) {
     uint32_t stages = (SM_BYTES / per_sm - RING_HEAD - 1024) / stage;
     if (stages > RING_MAX) stages = RING_MAX;
     const size_t smem = RING_HEAD + (size_t)stages * stage;
-    const bool full = p.K % (8 * LANES) == 0;
+    const bool full = p.K == 8 * LANES * RING_CHUNKS;
     auto k = a.r ? full ? rms_norm_mx_ring_kernel<T, W, LANES, true, true>
                         : rms_norm_mx_ring_kernel<T, W, LANES, true, false>
                  : full ? rms_norm_mx_ring_kernel<T, W, LANES, false, true>

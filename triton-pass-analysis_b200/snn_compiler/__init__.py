@@ -7,11 +7,12 @@ runs in libsnnb200.so: hand-written sm_100a CUDA kernels behind a C ABI
 """
 from .kernels import (if_lif, plif, cuba_lif, eif, fused_bias_if_lif, fused_bias_if_lif_rate,
                       fused_bias_if_lif_stateful, fold_conv_bn, conv_neuron, linear_neuron,
-                      conv_bn_neuron)
+                      conv_bn_neuron, MXTensor, mx_quantize, mx_dequantize, mx_linear,
+                      rms_norm_mx)
 from .nn import (IFNode, LIFNode, PLIFNode, CubaLIFNode, EIFNode, FusedAddNeuron,
                  RateCodedIFNode, RateCodedLIFNode, StatefulLIFNode, FusedConvNeuron,
                  FusedLinearNeuron, FusedConvBNNeuron, FusedConvBNAddNeuron, ChunkedForward,
-                 run_chunked)
+                 run_chunked, MXLinear, RMSNormMX, SpikingMLP)
 
 __all__ = [
     "if_lif", "plif", "cuba_lif", "eif", "fused_bias_if_lif", "fused_bias_if_lif_rate",
@@ -20,5 +21,6 @@ __all__ = [
     "FusedConvBNAddNeuron",
     "IFNode", "LIFNode", "PLIFNode", "FusedAddNeuron", "RateCodedIFNode",
     "RateCodedLIFNode", "StatefulLIFNode", "CubaLIFNode", "EIFNode", "ChunkedForward",
-    "run_chunked",
+    "run_chunked", "MXTensor", "mx_quantize", "mx_dequantize", "mx_linear", "rms_norm_mx",
+    "MXLinear", "RMSNormMX", "SpikingMLP",
 ]

@@ -48,9 +48,9 @@ class MXTensor:
     """Codes and scales of a tensor of `shape` (any leading axes, flattened to rows):
     data uint8 [rows, 16 ceil(K/32)] (mxfp4, the even element in the low four bits) or
     [rows, 32 ceil(K/32)] (mxfp8), scales uint8 of mx_scales_shape(rows, K).  Elements past K and
-    scale bytes that no block owns are zero.  Neither is to be resized or moved while in use."""
+    scale bytes that no block owns are zero."""
 
-    __slots__ = ("shape", "fmt", "rows", "device", "_code", "_data", "_scales", "_dp", "_sp")
+    __slots__ = ("shape", "fmt", "rows", "device", "_code", "_data", "_scales", "_size")
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor, shape, fmt: str):
         code = _fmt(fmt)
@@ -65,8 +65,7 @@ class MXTensor:
             scales.numel() == (rows + 127) // 128 * ((nb + 3) // 4) * 512, \
             (tuple(scales.shape), tuple(shape))
         self.shape, self.fmt, self.rows, self.device = tuple(shape), fmt, rows, data.device
-        self._code, self._data, self._scales = code, data, scales
-        self._dp, self._sp = data.data_ptr(), scales.data_ptr()
+        self._code, self._data, self._scales, self._size = code, data, scales, 0
 
     @classmethod
     def _new(cls, like: torch.Tensor, rows: int, shape, fmt: str, code: int):
@@ -77,19 +76,20 @@ class MXTensor:
         buf = like.new_empty(size + (rows + 127) // 128 * ((nb + 3) // 4) * 512,
                              dtype=torch.uint8)
         self.shape, self.fmt, self.rows, self.device = tuple(shape), fmt, rows, like.device
-        self._code, self._data, self._scales = code, buf, None
-        self._dp = buf.data_ptr()
-        self._sp = self._dp + size
+        self._code, self._data, self._scales, self._size = code, buf, None, size
         return self
+
+    def _pointers(self):
+        """Addresses of the codes and the scales."""
+        p = self._data.data_ptr()
+        return p, p + self._size if self._scales is None else self._scales.data_ptr()
 
     def _split(self):
         """The one allocation of _new as two tensors."""
         if self._scales is None:
-            buf, nb = self._data, (self.shape[-1] + 31) // 32
-            width = nb * _BLOCK_BYTES[self._code]
-            size = self.rows * width
-            self._scales = buf[size:].view(mx_scales_shape(self.rows, self.shape[-1]))
-            self._data = buf[:size].view(self.rows, width)
+            buf, size, K = self._data, self._size, self.shape[-1]
+            self._scales = buf[size:].view(mx_scales_shape(self.rows, K))
+            self._data = buf[:size].view(self.rows, (K + 31) // 32 * _BLOCK_BYTES[self._code])
 
     @property
     def data(self) -> torch.Tensor:
@@ -167,7 +167,7 @@ def mx_quantize(x: torch.Tensor, fmt: str = "mxfp4") -> MXTensor:
     x2, ld = _rows_of(x)
     rows = x2.shape[0]
     t = MXTensor._new(x, rows, shape, fmt, code)
-    _launch("snnb_mx_quantize", t.device, x2.data_ptr(), dt, rows, K, ld, code, t._dp, t._sp)
+    _launch("snnb_mx_quantize", t.device, x2.data_ptr(), dt, rows, K, ld, code, *t._pointers())
     return t
 
 
@@ -175,7 +175,7 @@ def mx_dequantize(t: MXTensor, dtype=torch.bfloat16) -> torch.Tensor:
     """The values that t's codes stand for, rounded once to dtype (bfloat16 holds them all)."""
     dt = _dtype(dtype)
     out = torch.empty(t.shape, dtype=dtype, device=t.device)
-    _launch("snnb_mx_dequantize", t.device, t._dp, t._sp, t._code, t.rows, t.shape[-1],
+    _launch("snnb_mx_dequantize", t.device, *t._pointers(), t._code, t.rows, t.shape[-1],
             out.data_ptr(), dt)
     return out
 
@@ -202,7 +202,7 @@ def mx_linear(a: MXTensor, w: MXTensor, bias: torch.Tensor | None = None, *,
     else:
         dt = _dtype(out.dtype)
         assert out.device == device and out.is_contiguous() and tuple(out.shape) == shape
-    _launch("snnb_mx_linear", device, a._dp, a._sp, a._code, a.rows, K, w._dp, w._sp, N,
+    _launch("snnb_mx_linear", device, *a._pointers(), a._code, a.rows, K, *w._pointers(), N,
             None if bias is None else bias.data_ptr(), out.data_ptr(), dt)
     return out
 
@@ -234,5 +234,5 @@ def rms_norm_mx(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | 
     t = MXTensor._new(x, rows, shape, fmt, code)
     _launch("snnb_rms_norm_mx", device, x2.data_ptr(), ldx,
             None if r2 is None else r2.data_ptr(), ldr, dt, weight.data_ptr(), _DTYPES[wd], eps,
-            rows, K, code, t._dp, t._sp, hp)
+            rows, K, code, *t._pointers(), hp)
     return t, h

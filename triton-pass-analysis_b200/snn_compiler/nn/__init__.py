@@ -6,9 +6,11 @@ from .fused_layers import (FusedConvNeuron, FusedLinearNeuron, FusedConvBNNeuron
                            FusedConvBNAddNeuron, FusedConvBN, tune_convs)
 from .attention import (FusedSpikeAttention, SpikeAttentionBlock, is_spiking_self_attention,
                         is_ms_attention, is_spiking_attention)
+from .mx import MXLinear, RMSNormMX, SpikingMLP
 
 __all__ = ["IFNode", "LIFNode", "PLIFNode", "CubaLIFNode", "EIFNode", "ChunkedForward",
            "run_chunked", "FusedAddNeuron", "FusedConvNeuron",
            "FusedLinearNeuron", "FusedConvBNNeuron", "FusedConvBNAddNeuron", "FusedConvBN", "tune_convs", "RateCodedIFNode",
            "RateCodedLIFNode", "StatefulLIFNode", "FusedSpikeAttention", "SpikeAttentionBlock",
-           "is_spiking_self_attention", "is_ms_attention", "is_spiking_attention"]
+           "is_spiking_self_attention", "is_ms_attention", "is_spiking_attention",
+           "MXLinear", "RMSNormMX", "SpikingMLP"]
