@@ -107,7 +107,7 @@ __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_add
 }
 
 // ---- shared memory -----------------------------------------------------------------------
-template <int FMT, int BN, int STAGES, bool PAIR>
+template <int FMT, int BN, int STAGES, bool PAIR, int PACKED_STAGES>
 struct MxSmem {
     static constexpr int GROUPS = FMT == SNNB_MXFP4 ? 2 : 1;     // 128-wide groups of K a stage
     static constexpr int TOKEN_TILES = (BN + 127) / 128;         // scale tiles of the tokens
@@ -121,9 +121,9 @@ struct MxSmem {
     static constexpr int SCALES = W_SCALES + A_SCALES;           // per stage
     static constexpr int PACKED = FMT == SNNB_MXFP4 ? 0 : 128 * 64;  // packed weights, per stage
     static constexpr int PACKED_OFF = SCALES_OFF + STAGES * SCALES;
-    static constexpr int BAR_OFF = PACKED_OFF + STAGES * PACKED;
+    static constexpr int BAR_OFF = PACKED_OFF + PACKED_STAGES * PACKED;
     static constexpr int ACCS = BN <= 128 ? 2 : 1;               // accumulators in TMEM
-    static constexpr int NBARS = (PACKED ? 4 : 2) * STAGES + 2 * ACCS + 1;
+    static constexpr int NBARS = 2 * STAGES + 2 * ACCS + 1 + 2 * PACKED_STAGES;
     static constexpr int TMEM_OFF = BAR_OFF + NBARS * 8;
     static constexpr int TOTAL = TMEM_OFF + 8;
     static constexpr int DYN = TOTAL + 1024;
@@ -138,8 +138,13 @@ struct MxSmem {
 
 constexpr int MX_PRODUCERS = 4;
 template <int BN> constexpr int mx_epilogue_warps() { return BN <= 64 ? 4 : BN / 16; }
+// Warps that place one stage's weight pieces (4 stages in turn): 2 where a block has an SM for
+// itself and threads to spare.
+template <int FMT, int BN> constexpr int mx_placers() {
+    return FMT == SNNB_MXFP4 ? 0 : BN <= 128 ? 2 : 1;
+}
 template <int FMT, int BN> constexpr int mx_threads() {
-    return 32 * (MX_PRODUCERS + 1 + mx_epilogue_warps<BN>() + (FMT == SNNB_MXFP4 ? 0 : 4));
+    return 32 * (MX_PRODUCERS + 1 + mx_epilogue_warps<BN>() + 4 * mx_placers<FMT, BN>());
 }
 
 // One accumulator column pair (tokens i, i + 1) of a feature, rounded, as one word.
@@ -209,16 +214,73 @@ __device__ __forceinline__ void store_tile(const MxParams& p, uint32_t t, float 
     }
 }
 
+// The cluster's partial sums [column][128 features] at `part` of every CTA, added in rank order:
+// CTA `rank` finishes BN / SPLITS of the columns (tokens), four features a thread.  Every load of
+// a thread is in flight before the first sum: read one column after the other, the join took
+// 4 us of a 64 x 2048 x 2048 product's 9.5.
+template <int BN, int SPLITS>
+__device__ __forceinline__ void join_splits(const MxParams& p, uint32_t part, int rank, int n0,
+                                            int64_t r0) {
+    constexpr int COLS = BN / SPLITS;
+    constexpr int AHEAD = 16 / SPLITS;                           // units in flight
+    uint32_t from[SPLITS];
+#pragma unroll
+    for (int r = 0; r < SPLITS; ++r) from[r] = tc::map_to_rank(part, (uint32_t)r);
+    for (int u0 = threadIdx.x; u0 < COLS * 32; u0 += AHEAD * blockDim.x) {
+        float4 x[AHEAD][SPLITS];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int u = u0 + i * blockDim.x;
+            if (u < COLS * 32 && r0 + rank * COLS + (u >> 5) < p.rows) {
+                const uint32_t at = (uint32_t)(((rank * COLS + (u >> 5)) * 32 + (u & 31)) * 16);
+#pragma unroll
+                for (int r = 0; r < SPLITS; ++r) x[i][r] = tc::ld_dsmem_f4(from[r] + at);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int u = u0 + i * blockDim.x;
+            const int64_t row = r0 + rank * COLS + (u >> 5);
+            const int n = n0 + (u & 31) * 4;
+            if (u >= COLS * 32 || row >= p.rows || n >= p.N) continue;
+            float v[4] = {x[i][0].x, x[i][0].y, x[i][0].z, x[i][0].w};
+#pragma unroll
+            for (int r = 1; r < SPLITS; ++r) {
+                v[0] += x[i][r].x; v[1] += x[i][r].y; v[2] += x[i][r].z; v[3] += x[i][r].w;
+            }
+            const int have = p.N - n < 4 ? p.N - n : 4;
+            if (p.bias) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (e < have) v[e] += __ldg(p.bias + n + e);
+            }
+            if (p.pairs) {                                       // 16 bits, N even
+                uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + row * p.N + n);
+                if (SNNB_IN_BOUNDS(row * p.N + n + have - 1, (int64_t)p.rows * p.N, p.status)) {
+                    o[0] = pack16(p, v[0], v[1]);
+                    if (have > 2) o[1] = pack16(p, v[2], v[3]);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (e < have) store_one(p, row * p.N + n + e, v[e]);
+            }
+        }
+    }
+}
+
 // PAIR: two CTAs share a 256-feature x BN-token tile (each stages its own 128 features and half
 // of the tokens) and walk whole tiles.  Otherwise: one tile, its K range split over the CTAs of
 // a cluster, their float32 partial sums joined in rank order through distributed shared memory.
-template <int FMT, int BN, int STAGES, bool PAIR>
-__global__ void __launch_bounds__(mx_threads<FMT, BN>(), MxSmem<FMT, BN, STAGES, PAIR>::CTAS_PER_SM)
+// PACKED_STAGES: of the packed weights' ring (E4M3 tokens), 0 for E2M1.
+template <int FMT, int BN, int STAGES, bool PAIR, int PACKED_STAGES>
+__global__ void __launch_bounds__(mx_threads<FMT, BN>(),
+                                  MxSmem<FMT, BN, STAGES, PAIR, PACKED_STAGES>::CTAS_PER_SM)
 mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmA,
                  const __grid_constant__ CUtensorMap tmWS, const __grid_constant__ CUtensorMap tmAS,
                  const MxParams p) {
-    using S = MxSmem<FMT, BN, STAGES, PAIR>;
-    constexpr int NP = MX_PRODUCERS, EW = mx_epilogue_warps<BN>();
+    using S = MxSmem<FMT, BN, STAGES, PAIR, PACKED_STAGES>;
+    constexpr int NP = MX_PRODUCERS, EW = mx_epilogue_warps<BN>(), PLACERS = mx_placers<FMT, BN>();
     constexpr int CTAS = PAIR ? 2 : 1;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -236,20 +298,20 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
     // the packed weights' own ring (E4M3 tokens)
     auto packed = [&](int s) { return sbase + (uint32_t)(S::PACKED_OFF + s * S::PACKED); };
     auto pfull_bar = [&](int s) { return done_bar + 8u * (1 + s); };
-    auto pempty_bar = [&](int s) { return done_bar + 8u * (1 + STAGES + s); };
+    auto pempty_bar = [&](int s) { return done_bar + 8u * (1 + PACKED_STAGES + s); };
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + S::TMEM_OFF);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int crank = PAIR ? (int)tc::cluster_rank() : 0;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
-            // E2M1: four loads; E4M3: three, and the warp of each CTA that placed the weights
-            tc::mbar_init(full_bar(s), FMT == SNNB_MXFP4 ? 4 : 3 + CTAS);
+            // E2M1: four loads; E4M3: three, and the warps of each CTA that placed the weights
+            tc::mbar_init(full_bar(s), FMT == SNNB_MXFP4 ? 4 : 3 + PLACERS * CTAS);
             tc::mbar_init(empty_bar(s), 1);
-            if constexpr (S::PACKED > 0) {
-                tc::mbar_init(pfull_bar(s), 1);
-                tc::mbar_init(pempty_bar(s), 1);
-            }
+        }
+        for (int s = 0; s < PACKED_STAGES; ++s) {
+            tc::mbar_init(pfull_bar(s), 1);
+            tc::mbar_init(pempty_bar(s), PLACERS);
         }
         for (int b = 0; b < S::ACCS; ++b) {
             tc::mbar_init(accf_bar(b), 1);
@@ -299,13 +361,14 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
                                                                                       : BYTES[3]) *
                               (uint32_t)CTAS;
         const bool own_ring = S::PACKED > 0 && warp == 3;
+        const int ring = own_ring ? PACKED_STAGES : STAGES;
         uint32_t it = 0;
         for (int tile = tile0; tile < p.tiles && !failed; tile += tile_step) {
             const int tw = (tile % p.tiles_w) * CTAS + crank, tt = tile / p.tiles_w;
             for (int ks = k0; ks < k1; ++ks, ++it) {
-                const int s = (int)(it % STAGES);
+                const int s = (int)(it % ring);
                 failed |= 1u - tc::mbar_wait_warp(own_ring ? pempty_bar(s) : empty_bar(s),
-                                                  ((it / STAGES) & 1u) ^ 1u, failed);
+                                                  ((it / ring) & 1u) ^ 1u, failed);
                 if (failed) break;
                 if (own_ring) {
                     if (tc::elect_one()) {
@@ -435,24 +498,27 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
         }
     } else {
         // ------------------------------------------------------------- weight pieces (E4M3)
-        // Warp w takes the stages w, w + 4, ...: 16 codes (8 bytes) to the low half of a
-        // 16-byte slot, slot c of row r at c ^ (r % 8).
-        static_assert(FMT == SNNB_MXFP4 || STAGES >= 4, "a warp never laps the ring");
-        const uint32_t w = (uint32_t)(warp - NP - 1 - EW);
+        // The warps w, w + 4 take the stages w, w + 4, ... (each a part of the rows): 16 codes
+        // (8 bytes) to the low half of a 16-byte slot, slot c of row r at c ^ (r % 8).
+        static_assert(FMT == SNNB_MXFP4 || (STAGES >= 4 && PACKED_STAGES >= 4),
+                      "a warp that takes every fourth stage never laps a ring");
+        constexpr int ROWS = PLACERS > 0 ? 16 / PLACERS : 0;         // groups of 8 rows a warp
+        const uint32_t w = (uint32_t)(warp - NP - 1 - EW) & 3u;
+        const int part = (warp - NP - 1 - EW) >> 2;
         uint32_t it = 0;
         for (int tile = tile0; tile < p.tiles && !failed; tile += tile_step) {
             for (int ks = k0; ks < k1; ++ks, ++it) {
                 if ((it & 3u) != w) continue;
-                const int s = (int)(it % STAGES);
-                const uint32_t ph = (it / STAGES) & 1u;
-                failed |= 1u - tc::mbar_wait_warp(pfull_bar(s), ph, failed);
-                failed |= 1u - tc::mbar_wait_warp(empty_bar(s), ph ^ 1u, failed);
+                const int s = (int)(it % STAGES), ps = PLACERS > 0 ? (int)(it % PACKED_STAGES) : 0;
+                failed |= 1u - tc::mbar_wait_warp(pfull_bar(ps), PLACERS > 0 ? (it / PACKED_STAGES) & 1u : 0,
+                                                  failed);
+                failed |= 1u - tc::mbar_wait_warp(empty_bar(s), ((it / STAGES) & 1u) ^ 1u, failed);
                 if (failed) break;
-                const uint8_t* src = smem + S::PACKED_OFF + s * S::PACKED + lane * 16;
-                uint8_t* dst = smem + s * S::STAGE + (lane >> 2) * 128;
+                const uint8_t* src = smem + S::PACKED_OFF + ps * S::PACKED + part * ROWS * 512 + lane * 16;
+                uint8_t* dst = smem + s * S::STAGE + part * ROWS * 1024 + (lane >> 2) * 128;
                 const int c = (lane & 3) * 2, x = lane >> 2;         // row u * 8 + x
 #pragma unroll
-                for (int h = 0; h < 16; h += 8) {
+                for (int h = 0; h < ROWS; h += 8) {
                     uint4 v[8];                      // loads ahead of the stores
 #pragma unroll
                     for (int u = 0; u < 8; ++u)
@@ -467,7 +533,7 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
                 tc::fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) {
-                    tc::mbar_arrive(pempty_bar(s));
+                    tc::mbar_arrive(pempty_bar(ps));
                     if (crank) mbar_arrive_cluster_relaxed(tc::map_to_rank(full_bar(s), 0));
                     else tc::mbar_arrive(full_bar(s));
                 }
@@ -477,54 +543,26 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
     if (failed && lane == 0) atomicExch(p.status, SNNB_ERR_TIMEOUT);
     if (!PAIR && splits > 1) {
         tc::cluster_sync();                          // every CTA's partial sums are in place
-        if (warp > NP && warp < NP + 1 + EW) {
-            const int q = warp & 3, half = (warp - NP - 1) / 4;
-            const int tw = tile0 % p.tiles_w, tt = tile0 / p.tiles_w;
-            const int n = tw * 128 + 32 * q + lane;
-            const float bias = p.bias && n < p.N ? __ldg(p.bias + n) : 0.0f;
-            const int64_t left = (int64_t)p.rows - (int64_t)tt * BN;
-            const int cols = (int)(left < BN ? left : BN);
-            const uint32_t mine = sbase + (uint32_t)(32 * q + lane) * 4u;
-            // four columns of every rank in flight
-            const int step = splits * (EW / 4);
-            for (int c = rank * (EW / 4) + half; c < cols; c += 4 * step) {
-                float x[4][8];
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int r = 0; r < 8; ++r) {
-                        x[i][r] = 0.0f;
-                        if (r < splits && c + i * step < cols)
-                            asm volatile("ld.shared::cluster.f32 %0, [%1];"
-                                         : "=f"(x[i][r])
-                                         : "r"(tc::map_to_rank(mine + (uint32_t)(c + i * step) * 512u,
-                                                               (uint32_t)r)));
-                    }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float v = x[i][0];
-#pragma unroll
-                    for (int r = 1; r < 8; ++r) v += x[i][r];
-                    if (n < p.N && c + i * step < cols)
-                        store_one(p, ((int64_t)tt * BN + c + i * step) * p.N + n, v + bias);
-                }
-            }
-        }
+        const int tw = tile0 % p.tiles_w, tt = tile0 / p.tiles_w;
+        if (splits == 2) join_splits<BN, 2>(p, sbase, rank, tw * 128, (int64_t)tt * BN);
+        else if (splits == 4) join_splits<BN, 4>(p, sbase, rank, tw * 128, (int64_t)tt * BN);
+        else join_splits<BN, 8>(p, sbase, rank, tw * 128, (int64_t)tt * BN);
     }
     tc::tc_fence_before();
     if (__syncthreads_or((int)failed)) {
         // copies still in flight land before the CTA may exit: waits on the full barrier, or for
         // the odd CTA of a pair (whose copies complete the even CTA's) on the stage's release,
         // with the limit that outlasts any copy
-        if (warp < NP)
-            for (uint32_t k = 0; k < issued && k < (uint32_t)STAGES; ++k) {
+        if (warp < NP) {
+            const bool own_ring = S::PACKED > 0 && warp == 3;
+            const uint32_t ring = own_ring ? PACKED_STAGES : STAGES;
+            for (uint32_t k = 0; k < issued && k < ring; ++k) {
                 const uint32_t g = issued - 1 - k;
-                const int s = (int)(g % STAGES);
-                tc::mbar_wait_warp<true>(S::PACKED > 0 && warp == 3 ? pfull_bar(s)
-                                         : crank                    ? empty_bar(s)
-                                                                    : full_bar(s),
-                                         (g / STAGES) & 1u, 0);
+                const int s = (int)(g % ring);
+                tc::mbar_wait_warp<true>(own_ring ? pfull_bar(s) : crank ? empty_bar(s) : full_bar(s),
+                                         (g / ring) & 1u, 0);
             }
+        }
         __syncthreads();
     }
     // neither CTA of a pair leaves while the other may signal its barriers or have its memory
@@ -541,16 +579,86 @@ struct MxMaps {
     CUtensorMap w, a, ws, as;
 };
 
-template <int FMT, int BN, int STAGES, bool PAIR>
+// One instantiation's launch settings on the current device, asked for once: the shared-memory
+// opt-in, and how many clusters of 1, 2, 4, 8 CTAs are resident at once.
+struct MxDevice {
+    bool ready;
+    int clusters[4];
+};
+template <typename Kernel>
+int mx_device(Kernel k, int threads, int smem, bool pair, MxDevice (&cache)[64], const MxDevice*& out) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return record_cuda_error(e);
+    if (dev < 0 || dev >= 64) return SNNB_ERR_UNSUPPORTED;
+    MxDevice& d = cache[dev];
+    if (!__atomic_load_n(&d.ready, __ATOMIC_ACQUIRE)) {
+        e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return record_cuda_error(e);
+        for (int i = 0; i < 4 && !pair; ++i) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(1u << i);
+            cfg.blockDim = dim3((unsigned)threads);
+            cfg.dynamicSmemBytes = (size_t)smem;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = 1u << i;
+            attr[0].val.clusterDim.y = 1;
+            attr[0].val.clusterDim.z = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            int n = 0;
+            e = cudaOccupancyMaxActiveClusters(&n, k, &cfg);
+            if (e != cudaSuccess) return record_cuda_error(e);
+            __atomic_store_n(&d.clusters[i], n, __ATOMIC_RELAXED);
+        }
+        __atomic_store_n(&d.ready, true, __ATOMIC_RELEASE);
+    }
+    out = &d;
+    return SNNB_OK;
+}
+
+// Launches one form.  min_split > 0: only if the K range can be split at least that much with
+// every cluster resident at once, else SNNB_ERR_UNSUPPORTED.
+template <int FMT, int BN, int STAGES, bool PAIR, int PACKED_STAGES>
 int launch_mx(const void* a, const void* as, const void* w, const void* ws, int64_t K, MxParams p,
-              cudaStream_t s) {
-    using S = MxSmem<FMT, BN, STAGES, PAIR>;
+              cudaStream_t s, int min_split = 0) {
+    using S = MxSmem<FMT, BN, STAGES, PAIR, PACKED_STAGES>;
+    static MxDevice cache[64];
+    auto k = mx_linear_kernel<FMT, BN, STAGES, PAIR, PACKED_STAGES>;
+    const MxDevice* dev = nullptr;
+    int rc = mx_device(k, mx_threads<FMT, BN>(), S::DYN, PAIR, cache, dev);
+    if (rc != SNNB_OK) return rc;
+    const int64_t width = PAIR ? 256 : 128;
+    p.tiles_w = (int)((p.N + width - 1) / width);
+    const int64_t tiles = p.tiles_w * (((int64_t)p.rows + BN - 1) / BN);
+    if (tiles > 0x7fffffff / 8) return SNNB_ERR_ARG;
+    p.tiles = (int)tiles;
+    unsigned grid, cluster;
+    if (PAIR) {
+        grid = 2 * (unsigned)(tiles < 74 ? tiles : 74);
+        cluster = 2;
+    } else {
+        // The largest split that leaves every cluster resident at once (the occupancy call counts
+        // one CTA an SM) and saves 6 stages of ~0.25 us, which pay for its join (1.4 us); none
+        // where the tiles alone nearly fill the SMs, unless K is long.  1 x 16384 x 4096 in 4
+        // bits: 9.3 us, 9.8 split in 2; 1 x 8192 x 8192: 12.7, 10.6 in 2, 9.2 in 4;
+        // 64 x 2048 x 2048: 5.2, 6.4 in 4; 1 x 16384 x 16384: 27.8, 25.7 in 2.
+        const int nstages = (p.groups + S::GROUPS - 1) / S::GROUPS;
+        int log = 0;
+        for (int l = 1; l <= 3 && (tiles < 100 || nstages >= 48); ++l)
+            if (tiles <= (int64_t)dev->clusters[l] * S::CTAS_PER_SM && nstages - (nstages >> l) >= 6)
+                log = l;
+        if ((1 << log) < min_split) return SNNB_ERR_UNSUPPORTED;
+        grid = (unsigned)(tiles << log);
+        cluster = 1u << log;
+    }
     const uint64_t nb = (uint64_t)mx::blocks_of(K), groups = (uint64_t)p.groups;
     MxMaps m;
     const uint64_t wrow = nb * 16, arow = nb * mx::Fmt<FMT>::BLOCK_BYTES;
     const uint64_t wdims[2] = {wrow, (uint64_t)p.N}, adims[2] = {arow, (uint64_t)p.rows};
     const uint32_t wbox[2] = {FMT == SNNB_MXFP4 ? 128u : 64u, 128}, abox[2] = {128, (uint32_t)S::A_ROWS};
-    int rc = encode_tmap(&m.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, a, adims, &arow, abox,
+    rc = encode_tmap(&m.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, a, adims, &arow, abox,
                          CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != SNNB_OK) return rc;
     rc = encode_tmap(&m.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, w, wdims, &wrow, wbox,
@@ -567,27 +675,6 @@ int launch_mx(const void* a, const void* as, const void* w, const void* ws, int6
     rc = encode_tmap(&m.ws, CU_TENSOR_MAP_DATA_TYPE_INT32, 3, ws, wsdims, str, wsbox,
                      CU_TENSOR_MAP_SWIZZLE_NONE);
     if (rc != SNNB_OK) return rc;
-    const int64_t width = PAIR ? 256 : 128;
-    p.tiles_w = (int)((p.N + width - 1) / width);
-    const int64_t tiles = p.tiles_w * (((int64_t)p.rows + BN - 1) / BN);
-    if (tiles > 0x7fffffff / 8) return SNNB_ERR_ARG;
-    p.tiles = (int)tiles;
-    auto k = mx_linear_kernel<FMT, BN, STAGES, PAIR>;
-    const cudaError_t e =
-        cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::DYN);
-    if (e != cudaSuccess) return record_cuda_error(e);
-    unsigned grid, cluster;
-    if (PAIR) {
-        grid = 2 * (unsigned)(tiles < 74 ? tiles : 74);
-        cluster = 2;
-    } else {
-        const int nstages = (p.groups + S::GROUPS - 1) / S::GROUPS;
-        int splits = 1;
-        while (splits < 8 && tiles * splits * 2 <= 148 * S::CTAS_PER_SM && splits * 2 <= nstages)
-            splits *= 2;
-        grid = (unsigned)(tiles * splits);
-        cluster = (unsigned)splits;
-    }
     return launch_kc(k, dim3(grid), dim3(mx_threads<FMT, BN>()), S::DYN, s, cluster, m.w, m.a, m.ws,
                      m.as, p);
 }
@@ -602,17 +689,29 @@ int run_mx(const void* a, const void* as, int64_t rows, int64_t K, const void* w
     p.bias = bias; p.out = out; p.out_dtype = out_dtype;
     p.pairs = out_dtype != SNNB_F32 && N % 2 == 0 && reinterpret_cast<uintptr_t>(out) % 4 == 0;
     constexpr bool F4 = FMT == SNNB_MXFP4;
-    if (rows <= 16) return launch_mx<FMT, 16, F4 ? 5 : 4, false>(a, as, w, ws, K, p, s);
-    if (rows <= 32) return launch_mx<FMT, 32, 4, false>(a, as, w, ws, K, p, s);
-    if (rows <= 64) return launch_mx<FMT, 64, 4, false>(a, as, w, ws, K, p, s);
-    if (rows <= 128) return launch_mx<FMT, 128, F4 ? 6 : 5, false>(a, as, w, ws, K, p, s);
+    // Up to 128 tokens: one token tile, K split.  Two CTAs an SM for E2M1; one for E4M3, whose
+    // packed ring then covers the latency of HBM.
+    if (rows <= 16) return launch_mx<FMT, 16, F4 ? 5 : 4, false, F4 ? 0 : 16>(a, as, w, ws, K, p, s);
+    if (rows <= 32) return launch_mx<FMT, 32, 4, false, F4 ? 0 : 14>(a, as, w, ws, K, p, s);
+    if (rows <= 64) return launch_mx<FMT, 64, 4, false, F4 ? 0 : 12>(a, as, w, ws, K, p, s);
+    if (rows <= 128) return launch_mx<FMT, 128, F4 ? 6 : 4, false, F4 ? 0 : 8>(a, as, w, ws, K, p, s);
     // Pairs, 74 at once.  128 tokens a tile where that still fits one round, and for short K,
     // where the second accumulator hides the stores (8192 x 8192, K = 512: 35 us against 43 with
     // 256; K = 2048: 78 against 68); 256 otherwise.
-    const int64_t pw = (N + 255) / 256;
-    if (pw * ((rows + 127) / 128) <= 74 || (K <= 768 && pw * ((rows + 255) / 256) > 74))
-        return launch_mx<FMT, 128, F4 ? 7 : 6, true>(a, as, w, ws, K, p, s);
-    return launch_mx<FMT, 256, F4 ? 6 : 5, true>(a, as, w, ws, K, p, s);
+    const int64_t pw = (N + 255) / 256, nstages = (p.groups + (F4 ? 1 : 0)) / (F4 ? 2 : 1);
+    if (pw * ((rows + 127) / 128) <= 74) {
+        // One round that leaves SMs idle over a long K: split K instead (200 x 512 x 16384 in 4
+        // bits: 8.5 us against 20; 1024 x 1024 x 1024: 10 against 4.4).
+        if (nstages >= 12) {
+            const int rc = launch_mx<FMT, 128, F4 ? 6 : 4, false, F4 ? 0 : 8>(
+                a, as, w, ws, K, p, s, nstages >= 48 ? 2 : 4);
+            if (rc != SNNB_ERR_UNSUPPORTED) return rc;
+        }
+        return launch_mx<FMT, 128, F4 ? 7 : 6, true, F4 ? 0 : 6>(a, as, w, ws, K, p, s);
+    }
+    if (K <= 768 && pw * ((rows + 255) / 256) > 74)
+        return launch_mx<FMT, 128, F4 ? 7 : 6, true, F4 ? 0 : 6>(a, as, w, ws, K, p, s);
+    return launch_mx<FMT, 256, F4 ? 6 : 5, true, F4 ? 0 : 5>(a, as, w, ws, K, p, s);
 }
 
 }  // namespace
