@@ -50,7 +50,7 @@ class MXTensor:
     [rows, 32 ceil(K/32)] (mxfp8), scales uint8 of mx_scales_shape(rows, K).  Elements past K and
     scale bytes that no block owns are zero."""
 
-    __slots__ = ("shape", "fmt", "rows", "device", "_code", "_data", "_scales", "_size")
+    __slots__ = ("shape", "fmt", "rows", "_code", "_data", "_scales", "_size")
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor, shape, fmt: str):
         code = _fmt(fmt)
@@ -58,13 +58,14 @@ class MXTensor:
         rows = shape[0] if len(shape) == 2 else math.prod(shape[:-1])
         nb = (K + 31) // 32
         assert K >= 1, shape
-        assert data.dtype == scales.dtype == torch.uint8 and data.device == scales.device
+        assert data.dtype == scales.dtype == torch.uint8
+        assert data.get_device() == scales.get_device()
         assert data.is_contiguous() and data.numel() == rows * nb * _BLOCK_BYTES[code], \
             (tuple(data.shape), tuple(shape), fmt)
         assert scales.is_contiguous() and \
             scales.numel() == (rows + 127) // 128 * ((nb + 3) // 4) * 512, \
             (tuple(scales.shape), tuple(shape))
-        self.shape, self.fmt, self.rows, self.device = tuple(shape), fmt, rows, data.device
+        self.shape, self.fmt, self.rows = tuple(shape), fmt, rows
         self._code, self._data, self._scales, self._size = code, data, scales, 0
 
     @classmethod
@@ -75,7 +76,7 @@ class MXTensor:
         size = rows * nb * _BLOCK_BYTES[code]
         buf = like.new_empty(size + (rows + 127) // 128 * ((nb + 3) // 4) * 512,
                              dtype=torch.uint8)
-        self.shape, self.fmt, self.rows, self.device = tuple(shape), fmt, rows, like.device
+        self.shape, self.fmt, self.rows = shape, fmt, rows
         self._code, self._data, self._scales, self._size = code, buf, None, size
         return self
 
@@ -90,6 +91,10 @@ class MXTensor:
             buf, size, K = self._data, self._size, self.shape[-1]
             self._scales = buf[size:].view(mx_scales_shape(self.rows, K))
             self._data = buf[:size].view(self.rows, (K + 31) // 32 * _BLOCK_BYTES[self._code])
+
+    @property
+    def device(self) -> torch.device:
+        return self._data.device
 
     @property
     def data(self) -> torch.Tensor:
@@ -139,12 +144,15 @@ def _rows_of(x: torch.Tensor):
     return x, ld
 
 
-def _launch(name: str, device: torch.device, *args) -> None:
-    """One library call on the current stream of `device`, which becomes the current device for
-    it (launches go to the current device)."""
-    assert device.type == "cuda", f"a CUDA tensor is needed, got {device}"
-    index = device.index
-    fn = getattr(_lib.lib(), name)
+_entries = {}
+
+
+def _launch(name: str, index: int, *args) -> None:
+    """One library call on the current stream of CUDA device `index`, which becomes the current
+    device for it (launches go to the current device)."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(_lib.lib(), name)
     if index == torch.cuda.current_device():
         st = fn(*args, _lib.raw_stream(index))
     else:
@@ -152,6 +160,12 @@ def _launch(name: str, device: torch.device, *args) -> None:
             st = fn(*args, _lib.raw_stream(index))
     if st:
         _lib.check(st, name)
+
+
+def _index(t: torch.Tensor) -> int:
+    index = t.get_device()
+    assert index >= 0, f"a CUDA tensor is needed, got {t.device}"
+    return index
 
 
 def mx_quantize(x: torch.Tensor, fmt: str = "mxfp4") -> MXTensor:
@@ -164,18 +178,20 @@ def mx_quantize(x: torch.Tensor, fmt: str = "mxfp4") -> MXTensor:
     K = shape[-1]
     if K < 1:
         raise ValueError("mx_quantize: the last axis is empty")
+    index = _index(x)
     x2, ld = _rows_of(x)
     rows = x2.shape[0]
-    t = MXTensor._new(x, rows, shape, fmt, code)
-    _launch("snnb_mx_quantize", t.device, x2.data_ptr(), dt, rows, K, ld, code, *t._pointers())
+    t = MXTensor._new(x, rows, tuple(shape), fmt, code)
+    _launch("snnb_mx_quantize", index, x2.data_ptr(), dt, rows, K, ld, code, *t._pointers())
     return t
 
 
 def mx_dequantize(t: MXTensor, dtype=torch.bfloat16) -> torch.Tensor:
     """The values that t's codes stand for, rounded once to dtype (bfloat16 holds them all)."""
     dt = _dtype(dtype)
-    out = torch.empty(t.shape, dtype=dtype, device=t.device)
-    _launch("snnb_mx_dequantize", t.device, *t._pointers(), t._code, t.rows, t.shape[-1],
+    index = _index(t._data)
+    out = t._data.new_empty(t.shape, dtype=dtype)
+    _launch("snnb_mx_dequantize", index, *t._pointers(), t._code, t.rows, t.shape[-1],
             out.data_ptr(), dt)
     return out
 
@@ -188,21 +204,21 @@ def mx_linear(a: MXTensor, w: MXTensor, bias: torch.Tensor | None = None, *,
         raise ValueError(f"mx_linear: the weights are held in mxfp4, got {w.fmt}")
     assert len(w.shape) == 2 and a.shape[-1] == w.shape[1], (a.shape, w.shape)
     N, K = w.shape
-    device = a.device
-    assert w.device == device, (w.device, device)
+    index = _index(a._data)
+    assert w._data.get_device() == index, (w.device, a.device)
     if N < 1:
         raise ValueError("mx_linear: no output features")
     if bias is not None:
         assert bias.dtype == torch.float32 and bias.is_contiguous() and \
-            bias.numel() == N and bias.device == device, (tuple(bias.shape), bias.dtype)
-    shape = (*a.shape[:-1], N)
+            bias.numel() == N and bias.get_device() == index, (tuple(bias.shape), bias.dtype)
+    shape = a.shape[:-1] + (N,)
     if out is None:
         dt = _dtype(dtype)
-        out = torch.empty(shape, dtype=dtype, device=device)
+        out = a._data.new_empty(shape, dtype=dtype)
     else:
         dt = _dtype(out.dtype)
-        assert out.device == device and out.is_contiguous() and tuple(out.shape) == shape
-    _launch("snnb_mx_linear", device, *a._pointers(), a._code, a.rows, K, *w._pointers(), N,
+        assert out.get_device() == index and out.is_contiguous() and tuple(out.shape) == shape
+    _launch("snnb_mx_linear", index, *a._pointers(), a._code, a.rows, K, *w._pointers(), N,
             None if bias is None else bias.data_ptr(), out.data_ptr(), dt)
     return out
 
@@ -219,20 +235,20 @@ def rms_norm_mx(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | 
         raise ValueError("rms_norm_mx: the last axis is empty")
     if not eps >= 0.0:
         raise ValueError(f"rms_norm_mx: eps is {eps}")
-    device, wd = x.device, weight.dtype
+    index, wd = _index(x), weight.dtype
     assert (wd == x.dtype or wd == torch.float32) and weight.is_contiguous() and \
-        weight.numel() == K and weight.device == device, (tuple(weight.shape), wd)
+        weight.numel() == K and weight.get_device() == index, (tuple(weight.shape), wd)
     x2, ldx = _rows_of(x)
     rows = x2.shape[0]
     r2, ldr, h, hp = None, 0, x, None
     if residual is not None:
         assert residual.shape == shape and residual.dtype == x.dtype and \
-            residual.device == device, (tuple(residual.shape), residual.dtype)
+            residual.get_device() == index, (tuple(residual.shape), residual.dtype)
         r2, ldr = _rows_of(residual)
-        h = torch.empty(shape, dtype=x.dtype, device=device)
+        h = x.new_empty(shape)
         hp = h.data_ptr()
-    t = MXTensor._new(x, rows, shape, fmt, code)
-    _launch("snnb_rms_norm_mx", device, x2.data_ptr(), ldx,
+    t = MXTensor._new(x, rows, tuple(shape), fmt, code)
+    _launch("snnb_rms_norm_mx", index, x2.data_ptr(), ldx,
             None if r2 is None else r2.data_ptr(), ldr, dt, weight.data_ptr(), _DTYPES[wd], eps,
             rows, K, code, *t._pointers(), hp)
     return t, h
