@@ -119,7 +119,7 @@ struct MxSmem {
     static constexpr int STAGE = W_TILE + A_TILE;                // operand tiles, 1024-aligned
     static constexpr int SCALES_OFF = STAGES * STAGE;
     static constexpr int SCALES = W_SCALES + A_SCALES;           // per stage
-    static constexpr int PACKED = FMT == SNNB_MXFP4 ? 0 : 128 * 64;  // packed weights, per stage
+    static constexpr int PACKED = PACKED_STAGES > 0 ? 128 * 64 : 0;  // packed weights, per stage
     static constexpr int PACKED_OFF = SCALES_OFF + STAGES * SCALES;
     static constexpr int BAR_OFF = PACKED_OFF + PACKED_STAGES * PACKED;
     static constexpr int ACCS = BN <= 128 ? 2 : 1;               // accumulators in TMEM
@@ -140,11 +140,11 @@ constexpr int MX_PRODUCERS = 4;
 template <int BN> constexpr int mx_epilogue_warps() { return BN <= 64 ? 4 : BN / 16; }
 // Warps that place one stage's weight pieces (4 stages in turn): 2 where a block has an SM for
 // itself and threads to spare.
-template <int FMT, int BN> constexpr int mx_placers() {
-    return FMT == SNNB_MXFP4 ? 0 : BN <= 128 ? 2 : 1;
+template <int BN, int PACKED_STAGES> constexpr int mx_placers() {
+    return PACKED_STAGES == 0 ? 0 : BN <= 128 ? 2 : 1;
 }
-template <int FMT, int BN> constexpr int mx_threads() {
-    return 32 * (MX_PRODUCERS + 1 + mx_epilogue_warps<BN>() + 4 * mx_placers<FMT, BN>());
+template <int BN, int PACKED_STAGES> constexpr int mx_threads() {
+    return 32 * (MX_PRODUCERS + 1 + mx_epilogue_warps<BN>() + 4 * mx_placers<BN, PACKED_STAGES>());
 }
 
 // One accumulator column pair (tokens i, i + 1) of a feature, rounded, as one word.
@@ -274,13 +274,13 @@ __device__ __forceinline__ void join_splits(const MxParams& p, uint32_t part, in
 // a cluster, their float32 partial sums joined in rank order through distributed shared memory.
 // PACKED_STAGES: of the packed weights' ring (E4M3 tokens), 0 for E2M1.
 template <int FMT, int BN, int STAGES, bool PAIR, int PACKED_STAGES>
-__global__ void __launch_bounds__(mx_threads<FMT, BN>(),
+__global__ void __launch_bounds__(mx_threads<BN, PACKED_STAGES>(),
                                   MxSmem<FMT, BN, STAGES, PAIR, PACKED_STAGES>::CTAS_PER_SM)
 mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmA,
                  const __grid_constant__ CUtensorMap tmWS, const __grid_constant__ CUtensorMap tmAS,
                  const MxParams p) {
     using S = MxSmem<FMT, BN, STAGES, PAIR, PACKED_STAGES>;
-    constexpr int NP = MX_PRODUCERS, EW = mx_epilogue_warps<BN>(), PLACERS = mx_placers<FMT, BN>();
+    constexpr int NP = MX_PRODUCERS, EW = mx_epilogue_warps<BN>(), PLACERS = mx_placers<BN, PACKED_STAGES>();
     constexpr int CTAS = PAIR ? 2 : 1;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -305,8 +305,8 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
-            // E2M1: four loads; E4M3: three, and the warps of each CTA that placed the weights
-            tc::mbar_init(full_bar(s), FMT == SNNB_MXFP4 ? 4 : 3 + PLACERS * CTAS);
+            // four loads, or three and the warps of each CTA that placed the weights
+            tc::mbar_init(full_bar(s), PACKED_STAGES == 0 ? 4 : 3 + PLACERS * CTAS);
             tc::mbar_init(empty_bar(s), 1);
         }
         for (int s = 0; s < PACKED_STAGES; ++s) {
@@ -356,7 +356,9 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
         // Issuing a tiled copy holds its thread for ~250 cycles, so each kind has a warp of its
         // own.  All bytes of a stage, a pair's both halves, complete the (even CTA's) full
         // barrier; packed weights their own ring's.
-        constexpr uint32_t BYTES[4] = {S::A_TILE, S::A_SCALES, S::W_SCALES, S::W_TILE};
+        // (an unpacking copy counts the packed bytes)
+        constexpr uint32_t BYTES[4] = {S::A_TILE, S::A_SCALES, S::W_SCALES,
+                                       FMT == SNNB_MXFP4 ? S::W_TILE : S::W_TILE / 2};
         const uint32_t mine = (warp == 0 ? BYTES[0] : warp == 1 ? BYTES[1] : warp == 2 ? BYTES[2]
                                                                                       : BYTES[3]) *
                               (uint32_t)CTAS;
@@ -386,6 +388,7 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
                     else if (warp == 2)
                         load_3d<PAIR>(scales_at(s), &tmWS, fb, 0, ks * S::GROUPS, tw);
                     else
+                        // E2M1: bytes; unpacked: elements (128 of either a stage)
                         load_2d<PAIR>(w_tile(s), &tmW, fb, ks * 128, tw * 128);
                 }
                 __syncwarp();
@@ -500,7 +503,7 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
         // ------------------------------------------------------------- weight pieces (E4M3)
         // The warps w, w + 4 take the stages w, w + 4, ... (each a part of the rows): 16 codes
         // (8 bytes) to the low half of a 16-byte slot, slot c of row r at c ^ (r % 8).
-        static_assert(FMT == SNNB_MXFP4 || (STAGES >= 4 && PACKED_STAGES >= 4),
+        static_assert(PACKED_STAGES == 0 || (STAGES >= 4 && PACKED_STAGES >= 4),
                       "a warp that takes every fourth stage never laps a ring");
         constexpr int ROWS = PLACERS > 0 ? 16 / PLACERS : 0;         // groups of 8 rows a warp
         const uint32_t w = (uint32_t)(warp - NP - 1 - EW) & 3u;
@@ -627,7 +630,7 @@ int launch_mx(const void* a, const void* as, const void* w, const void* ws, int6
     static MxDevice cache[64];
     auto k = mx_linear_kernel<FMT, BN, STAGES, PAIR, PACKED_STAGES>;
     const MxDevice* dev = nullptr;
-    int rc = mx_device(k, mx_threads<FMT, BN>(), S::DYN, PAIR, cache, dev);
+    int rc = mx_device(k, mx_threads<BN, PACKED_STAGES>(), S::DYN, PAIR, cache, dev);
     if (rc != SNNB_OK) return rc;
     const int64_t width = PAIR ? 256 : 128;
     p.tiles_w = (int)((p.N + width - 1) / width);
@@ -657,12 +660,19 @@ int launch_mx(const void* a, const void* as, const void* w, const void* ws, int6
     MxMaps m;
     const uint64_t wrow = nb * 16, arow = nb * mx::Fmt<FMT>::BLOCK_BYTES;
     const uint64_t wdims[2] = {wrow, (uint64_t)p.N}, adims[2] = {arow, (uint64_t)p.rows};
-    const uint32_t wbox[2] = {FMT == SNNB_MXFP4 ? 128u : 64u, 128}, abox[2] = {128, (uint32_t)S::A_ROWS};
+    const uint32_t wbox[2] = {PACKED_STAGES > 0 ? 64u : 128u, 128}, abox[2] = {128, (uint32_t)S::A_ROWS};
     rc = encode_tmap(&m.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, a, adims, &arow, abox,
                          CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != SNNB_OK) return rc;
-    rc = encode_tmap(&m.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, w, wdims, &wrow, wbox,
-                     FMT == SNNB_MXFP4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE);
+    if (FMT == SNNB_MXFP8 && PACKED_STAGES == 0) {
+        // 16 codes to the low half of a 16-byte slot, by the copy itself
+        const uint64_t wels[2] = {wrow * 2, (uint64_t)p.N};
+        rc = encode_tmap(&m.w, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 2, w, wels, &wrow, wbox,
+                         CU_TENSOR_MAP_SWIZZLE_128B);
+    } else {
+        rc = encode_tmap(&m.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, w, wdims, &wrow, wbox,
+                         PACKED_STAGES > 0 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B);
+    }
     if (rc != SNNB_OK) return rc;
     // scale groups as [row tile][group][128 words]
     const uint64_t str[2] = {512, groups * 512};
@@ -675,26 +685,21 @@ int launch_mx(const void* a, const void* as, const void* w, const void* ws, int6
     rc = encode_tmap(&m.ws, CU_TENSOR_MAP_DATA_TYPE_INT32, 3, ws, wsdims, str, wsbox,
                      CU_TENSOR_MAP_SWIZZLE_NONE);
     if (rc != SNNB_OK) return rc;
-    return launch_kc(k, dim3(grid), dim3(mx_threads<FMT, BN>()), S::DYN, s, cluster, m.w, m.a, m.ws,
+    return launch_kc(k, dim3(grid), dim3(mx_threads<BN, PACKED_STAGES>()), S::DYN, s, cluster, m.w, m.a, m.ws,
                      m.as, p);
 }
 
-template <int FMT>
-int run_mx(const void* a, const void* as, int64_t rows, int64_t K, const void* w, const void* ws,
-           int64_t N, const float* bias, void* out, int out_dtype, cudaStream_t s) {
-    MxParams p = {};
-    p.status = device_status_ptr();
-    if (!p.status) return SNNB_ERR_CUDA;
-    p.rows = (int)rows; p.N = (int)N; p.groups = (int)mx::groups_of(K);
-    p.bias = bias; p.out = out; p.out_dtype = out_dtype;
-    p.pairs = out_dtype != SNNB_F32 && N % 2 == 0 && reinterpret_cast<uintptr_t>(out) % 4 == 0;
-    constexpr bool F4 = FMT == SNNB_MXFP4;
-    // Up to 128 tokens: one token tile, K split.  Two CTAs an SM for E2M1; one for E4M3, whose
-    // packed ring then covers the latency of HBM.
-    if (rows <= 16) return launch_mx<FMT, 16, F4 ? 5 : 4, false, F4 ? 0 : 16>(a, as, w, ws, K, p, s);
-    if (rows <= 32) return launch_mx<FMT, 32, 4, false, F4 ? 0 : 14>(a, as, w, ws, K, p, s);
-    if (rows <= 64) return launch_mx<FMT, 64, 4, false, F4 ? 0 : 12>(a, as, w, ws, K, p, s);
-    if (rows <= 128) return launch_mx<FMT, 128, F4 ? 6 : 4, false, F4 ? 0 : 8>(a, as, w, ws, K, p, s);
+// UNPACK: the copies unpack the weights beside E4M3 tokens.
+template <int FMT, bool UNPACK>
+int pick_mx(const void* a, const void* as, const void* w, const void* ws, int64_t rows, int64_t N,
+            int64_t K, const MxParams& p, cudaStream_t s) {
+    constexpr bool F4 = FMT == SNNB_MXFP4, P = !F4 && !UNPACK;      // P: a packed ring
+    // Up to 128 tokens: one token tile, K split.  Two CTAs an SM, or one whose packed ring covers
+    // the latency of HBM.
+    if (rows <= 16) return launch_mx<FMT, 16, P ? 4 : 5, false, P ? 16 : 0>(a, as, w, ws, K, p, s);
+    if (rows <= 32) return launch_mx<FMT, 32, 4, false, P ? 14 : 0>(a, as, w, ws, K, p, s);
+    if (rows <= 64) return launch_mx<FMT, 64, 4, false, P ? 12 : 0>(a, as, w, ws, K, p, s);
+    if (rows <= 128) return launch_mx<FMT, 128, P ? 4 : 6, false, P ? 8 : 0>(a, as, w, ws, K, p, s);
     // Pairs, 74 at once.  128 tokens a tile where that still fits one round, and for short K,
     // where the second accumulator hides the stores (8192 x 8192, K = 512: 35 us against 43 with
     // 256; K = 2048: 78 against 68); 256 otherwise.
@@ -703,15 +708,30 @@ int run_mx(const void* a, const void* as, int64_t rows, int64_t K, const void* w
         // One round that leaves SMs idle over a long K: split K instead (200 x 512 x 16384 in 4
         // bits: 8.5 us against 20; 1024 x 1024 x 1024: 10 against 4.4).
         if (nstages >= 12) {
-            const int rc = launch_mx<FMT, 128, F4 ? 6 : 4, false, F4 ? 0 : 8>(
+            const int rc = launch_mx<FMT, 128, P ? 4 : 6, false, P ? 8 : 0>(
                 a, as, w, ws, K, p, s, nstages >= 48 ? 2 : 4);
             if (rc != SNNB_ERR_UNSUPPORTED) return rc;
         }
-        return launch_mx<FMT, 128, F4 ? 7 : 6, true, F4 ? 0 : 6>(a, as, w, ws, K, p, s);
+        return launch_mx<FMT, 128, P ? 6 : 7, true, P ? 6 : 0>(a, as, w, ws, K, p, s);
     }
     if (K <= 768 && pw * ((rows + 255) / 256) > 74)
-        return launch_mx<FMT, 128, F4 ? 7 : 6, true, F4 ? 0 : 6>(a, as, w, ws, K, p, s);
-    return launch_mx<FMT, 256, F4 ? 6 : 5, true, F4 ? 0 : 5>(a, as, w, ws, K, p, s);
+        return launch_mx<FMT, 128, P ? 6 : 7, true, P ? 6 : 0>(a, as, w, ws, K, p, s);
+    return launch_mx<FMT, 256, P ? 5 : 6, true, P ? 5 : 0>(a, as, w, ws, K, p, s);
+}
+
+int run_mx(const void* a, const void* as, int a_fmt, int64_t rows, int64_t K, const void* w,
+           const void* ws, int64_t N, const float* bias, void* out, int out_dtype, cudaStream_t s) {
+    MxParams p = {};
+    p.status = device_status_ptr();
+    if (!p.status) return SNNB_ERR_CUDA;
+    p.rows = (int)rows; p.N = (int)N; p.groups = (int)mx::groups_of(K);
+    p.bias = bias; p.out = out; p.out_dtype = out_dtype;
+    p.pairs = out_dtype != SNNB_F32 && N % 2 == 0 && reinterpret_cast<uintptr_t>(out) % 4 == 0;
+    if (a_fmt == SNNB_MXFP4) return pick_mx<SNNB_MXFP4, false>(a, as, w, ws, rows, N, K, p, s);
+    // an unpacking copy wants whole groups of 128 elements a row and a base on 32 bytes
+    if (mx::blocks_of(K) % 4 == 0 && reinterpret_cast<uintptr_t>(w) % 32 == 0)
+        return pick_mx<SNNB_MXFP8, true>(a, as, w, ws, rows, N, K, p, s);
+    return pick_mx<SNNB_MXFP8, false>(a, as, w, ws, rows, N, K, p, s);
 }
 
 }  // namespace
@@ -735,7 +755,5 @@ extern "C" int snnb_mx_linear(const void* a, const void* a_scales, int a_fmt, in
     if (reinterpret_cast<uintptr_t>(out) % es || reinterpret_cast<uintptr_t>(bias) % 4)
         return SNNB_ERR_ARG;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return a_fmt == SNNB_MXFP4
-               ? run_mx<SNNB_MXFP4>(a, a_scales, rows, K, w, w_scales, N, bias, out, out_dtype, s)
-               : run_mx<SNNB_MXFP8>(a, a_scales, rows, K, w, w_scales, N, bias, out, out_dtype, s);
+    return run_mx(a, a_scales, a_fmt, rows, K, w, w_scales, N, bias, out, out_dtype, s);
 }
