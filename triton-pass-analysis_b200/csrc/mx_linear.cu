@@ -644,12 +644,13 @@ int launch_mx(const void* a, const void* as, const void* w, const void* ws, int6
     } else {
         // The largest split that leaves every cluster resident at once (the occupancy call counts
         // one CTA an SM) and saves 6 stages of ~0.25 us, which pay for its join (1.4 us); none
-        // where the tiles alone nearly fill the SMs, unless K is long.  1 x 16384 x 4096 in 4
-        // bits: 9.3 us, 9.8 split in 2; 1 x 8192 x 8192: 12.7, 10.6 in 2, 9.2 in 4;
-        // 64 x 2048 x 2048: 5.2, 6.4 in 4; 1 x 16384 x 16384: 27.8, 25.7 in 2.
+        // where the tiles alone nearly fill the SMs, unless K is long.  Tokens x features x K in
+        // 4 bits: 1 x 16384 x 4096: 9.3 us, 9.8 split in 2; 1 x 8192 x 8192: 12.7, 10.6 in 2, 9.2
+        // in 4; 64 x 2048 x 2048: 5.2, 6.4 in 4; with tokens in 8 bits 16 x 16384 x 4096: 12.7,
+        // 11.9 in 2; 1 x 2048 x 2048: 6.4, 5.3 in 4, 4.6 in 8.
         const int nstages = (p.groups + S::GROUPS - 1) / S::GROUPS;
         int log = 0;
-        for (int l = 1; l <= 3 && (tiles < 100 || nstages >= 48); ++l)
+        for (int l = 1; l <= 3 && (tiles < 100 || nstages >= 24); ++l)
             if (tiles <= (int64_t)dev->clusters[l] * S::CTAS_PER_SM && nstages - (nstages >> l) >= 6)
                 log = l;
         if ((1 << log) < min_split) return SNNB_ERR_UNSUPPORTED;
