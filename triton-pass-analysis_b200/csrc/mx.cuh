@@ -296,38 +296,42 @@ __device__ __forceinline__ Raw8<T> zero8() {
     return r;
 }
 
-// 8 values at p, only aligned to an element, the first n of them (0..8) inside the row, whose
-// elements are [row, row + K): two (float: three) aligned 16-byte loads around them where those
-// lie inside the row, else one load per element.  Values past n are zero.
+// w[0 ..] shifted right by `bytes` (0 .. 15, a multiple of sizeof(T)) over its first N words.
+template <typename T, int N>
+__device__ __forceinline__ void shift_right(uint32_t (&w)[N + 4], uint32_t bytes) {
+#pragma unroll
+    for (int i = 0; i < N + 2; ++i) w[i] = bytes & 8 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < N + 1; ++i) w[i] = bytes & 4 ? w[i + 1] : w[i];
+    if (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (bytes & 2) * 8);
+    }
+}
+
+// The values k .. k + 7 of a row of K at `row`, aligned to an element only; values past K are
+// zero.  Inside the row: two (float: three) aligned 16-byte loads around them, shifted into
+// place; at its ends one load per element, so that nothing outside the row is read.
 template <typename T>
-__device__ __forceinline__ Raw8<T> load_any8(const T* p, int n, const T* row, int64_t K) {
+__device__ __forceinline__ Raw8<T> load_any8(const T* row, uint32_t k, uint32_t K) {
     constexpr int W = (int)sizeof(T) * 2;                        // words of 8 values
     uint32_t w[W + 4];
-    const uintptr_t at = reinterpret_cast<uintptr_t>(p), down = at & ~uintptr_t(15);
-    const uint32_t off = (uint32_t)(at & 15);
-    if (n == 8 && down >= reinterpret_cast<uintptr_t>(row) &&
-        down + W * 4 + (off ? 16 : 0) <= reinterpret_cast<uintptr_t>(row + K)) {
+    const T* p = row + k;
+    if (k >= 8 && k + 16 <= K) {                                 // 16 bytes to spare either way
+        const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+        const uint4* down = reinterpret_cast<const uint4*>(at & ~uintptr_t(15));
 #pragma unroll
         for (int i = 0; i < W / 4 + 1; ++i) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (i < W / 4 || off) v = __ldg(reinterpret_cast<const uint4*>(down) + i);
+            const uint4 v = __ldg(down + i);
             w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
         }
-        // shift right by off bytes: whole words first, then the odd half word
-#pragma unroll
-        for (int i = 0; i < W + 2; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
-#pragma unroll
-        for (int i = 0; i < W + 1; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
-        if (sizeof(T) == 2) {
-#pragma unroll
-            for (int i = 0; i < W; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (off & 2) * 8);
-        }
+        shift_right<T, W>(w, (uint32_t)(at & 15));
     } else {
 #pragma unroll
         for (int i = 0; i < W; ++i) w[i] = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            if (i >= n) continue;
+            if (k + i >= K) continue;
             if (sizeof(T) == 2)
                 w[i / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(p) + i) << (16 * (i & 1));
             else
@@ -364,14 +368,7 @@ __device__ __forceinline__ void store_any8(T* p, int n, const Raw8<T>& r, int la
     const int head = (int)((0u - (uint32_t)reinterpret_cast<uintptr_t>(p)) & 15u) / (int)sizeof(T);
     const int have = n < 8 ? n : 8 + (lane < 31 ? next : 0);
     const int bytes = head * (int)sizeof(T);
-#pragma unroll
-    for (int i = 0; i < W + 2; ++i) t[i] = bytes & 8 ? t[i + 2] : t[i];
-#pragma unroll
-    for (int i = 0; i < W + 1; ++i) t[i] = bytes & 4 ? t[i + 1] : t[i];
-    if (sizeof(T) == 2) {
-#pragma unroll
-        for (int i = 0; i < W; ++i) t[i] = __funnelshift_r(t[i], t[i + 1], (bytes & 2) * 8);
-    }
+    shift_right<T, W>(t, (uint32_t)bytes);
     int taken = head;
 #pragma unroll
     for (int i = 0; i < W / 4; ++i) {

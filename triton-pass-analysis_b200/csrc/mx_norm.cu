@@ -156,12 +156,12 @@ __device__ __forceinline__ void take8(const NormParams& p, const T* x, const T* 
                                       uint32_t k, int n, float (&h)[8]) {
     mx::Raw8<T> a = mx::zero8<T>();
     const T* xr = x + (int64_t)row * p.ldx;
-    if (n > 0) a = ALIGNED ? mx::load_aligned8(xr + k) : mx::load_any8(xr + k, n, xr, (int64_t)p.K);
+    if (n > 0) a = ALIGNED ? mx::load_aligned8(xr + k) : mx::load_any8(xr, k, p.K);
     mx::to_floats(a, h);
     if (r) {
         mx::Raw8<T> b = mx::zero8<T>();
         const T* rr = r + (int64_t)row * p.ldr;
-        if (n > 0) b = ALIGNED ? mx::load_aligned8(rr + k) : mx::load_any8(rr + k, n, rr, (int64_t)p.K);
+        if (n > 0) b = ALIGNED ? mx::load_aligned8(rr + k) : mx::load_any8(rr, k, p.K);
         float f[8];
         mx::to_floats(b, f);
         add8(h, f);
@@ -177,10 +177,10 @@ __device__ __forceinline__ void put_h8(const NormParams& p, T* h_out, uint32_t r
     else if (n > 0) mx::store_aligned8(q, o);
 }
 
-template <typename W, bool ALIGNED>
+template <typename W>
 __device__ __forceinline__ mx::Raw8<W> weights8(const NormParams& p, const W* weight, uint32_t k) {
     if (k >= p.K) return mx::zero8<W>();
-    if (!ALIGNED) return mx::load_any8(weight + k, (int)min(8u, p.K - k), weight, (int64_t)p.K);
+    if (k + 8 > p.K || (reinterpret_cast<uintptr_t>(weight) & 15)) return mx::load_any8(weight, k, p.K);
     mx::Raw8<W> r;
 #pragma unroll
     for (int i = 0; i < (int)sizeof(W) / 2; ++i)
@@ -221,7 +221,7 @@ rms_norm_mx_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __restri
     };
     auto finish = [&](uint32_t k, const float (&h)[8], float rstd, double rstd64) {
         float w[8], y[8];
-        mx::to_floats(weights8<W, ALIGNED>(p, weight, k), w);
+        mx::to_floats(weights8<W>(p, weight, k), w);
         normed8(h, w, rstd, rstd64, y);
         emit8(p, out, k, y, lane);
     };
@@ -339,7 +339,7 @@ rms_norm_mx_ring_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __r
             if (row0 + (uint64_t)s * step < p.rows) fetch(row0 + s * step, s);
     mx::Raw8<W> w[RING_CHUNKS];
 #pragma unroll
-    for (int c = 0; c < RING_CHUNKS; ++c) w[c] = weights8<W, true>(p, weight, (c * LANES + t) * 8);
+    for (int c = 0; c < RING_CHUNKS; ++c) w[c] = weights8<W>(p, weight, (c * LANES + t) * 8);
     uint32_t failed = 0;
     int s = 0;
     uint32_t parity = 0, odd = 0;
@@ -467,6 +467,8 @@ int run_norm(const NormArgs& a, const NormParams& p) {
                          (!a.h || aligned16(a.h)) && aligned16(a.weight);
     if (!aligned) {
         if (K <= 1024) return launch_norm<T, W, false, 32, 4>(a, p);
+        if (K <= 2048) return launch_norm<T, W, false, 64, 4>(a, p);
+        if (K <= 4096) return launch_norm<T, W, false, 128, 4>(a, p);
         if (K <= 8192) return launch_norm<T, W, false, 256, 4>(a, p);
         return launch_norm<T, W, false, 1024, 0>(a, p);
     }

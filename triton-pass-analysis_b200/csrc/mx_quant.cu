@@ -101,12 +101,7 @@ mx_quantize_any_kernel(const T* __restrict__ x, uint32_t rows, uint32_t K, int64
             const uint32_t q = first + u * step;
             row[u] = per_row.div(q);
             k[u] = (q - row[u] * per_row.d) * 256 + lane * 8;
-            if (q < total && k[u] < K) {
-                const T* r = x + row[u] * ldx;
-                raw[u] = mx::load_any8(r + k[u], (int)min(8u, K - k[u]), r, (int64_t)K);
-            } else {
-                raw[u] = mx::zero8<T>();
-            }
+            raw[u] = q < total && k[u] < K ? mx::load_any8(x + row[u] * ldx, k[u], K) : mx::zero8<T>();
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
