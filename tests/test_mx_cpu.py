@@ -36,6 +36,19 @@ def test_scale_layout_round_trip(rows, K):
     assert np.array_equal(OM.row_scales(t.scales.numpy(), rows, nb), s.numpy())
 
 
+@pytest.mark.parametrize("K", [1, 31, 32, 33, 40, 96, 127])
+@pytest.mark.parametrize("fmt", ["mxfp4", "mxfp8"])
+def test_from_rows_clears_codes_past_the_last_column(K, fmt):
+    mx = _mx()
+    nb, size = -(-K // 32), 16 if fmt == "mxfp4" else 32
+    data = torch.full((3, nb, size), 0x77, dtype=torch.uint8)
+    t = mx.MXTensor.from_rows(data, torch.full((3, nb), 127, dtype=torch.uint8), K, fmt)
+    flat = t.data.reshape(3, -1)
+    codes = torch.stack([flat & 15, flat >> 4], -1).flatten(1) if fmt == "mxfp4" else flat
+    assert (codes[:, :K] != 0).all() and not codes[:, K:].any()
+    assert (data == 0x77).all()                               # the caller's bytes stay
+
+
 @pytest.mark.parametrize("fmt", ["mxfp4", "mxfp8"])
 def test_oracle_formats(fmt):
     """Every value of the format is a fixed point of the oracle's rounding, midpoints go to the

@@ -109,7 +109,8 @@ class MXTensor:
     @classmethod
     def from_rows(cls, data: torch.Tensor, row_scales: torch.Tensor, K: int, fmt: str):
         """From codes [rows, ...] and row-major scale bytes [rows, ceil(K/32)] (uint8), the form
-        in which checkpoints hold them; the scales are laid out once."""
+        in which checkpoints hold them; the scales are laid out once.  Codes past K become zero."""
+        _fmt(fmt)
         rows, nb = row_scales.shape
         assert row_scales.dtype == torch.uint8 and nb == (K + 31) // 32, \
             (tuple(row_scales.shape), K)
@@ -117,7 +118,15 @@ class MXTensor:
         full = torch.zeros(tr * 128, tb * 4, dtype=torch.uint8, device=row_scales.device)
         full[:rows, :nb] = row_scales
         tiled = full.view(tr, 4, 32, tb, 4).permute(0, 3, 2, 1, 4).contiguous()
-        return cls(data.contiguous(), tiled, (rows, K), fmt)
+        data = data.contiguous()
+        if K % 32:
+            per_byte = 2 if fmt == "mxfp4" else 1
+            used = -(-K // per_byte)                              # bytes of a row that hold codes
+            data = data.reshape(rows, nb * 32 // per_byte).clone()
+            data[:, used:] = 0
+            if K % per_byte:
+                data[:, used - 1] &= 15
+        return cls(data, tiled, (rows, K), fmt)
 
     def row_scales(self) -> torch.Tensor:
         """The scale bytes row-major, [rows, ceil(K/32)]."""
@@ -226,8 +235,9 @@ def mx_linear(a: MXTensor, w: MXTensor, bias: torch.Tensor | None = None, *,
 def rms_norm_mx(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, *,
                 eps: float = 1e-6, fmt: str = "mxfp8"):
     """h = x + residual; (h / sqrt(mean(h^2) + eps)) * weight over the last axis, quantised to
-    `fmt` -> (MXTensor, h).  The sum and the norm are float32; the returned h, the next residual,
-    is rounded to x's dtype (x itself without a residual).  weight [K] of x's dtype or float32."""
+    `fmt` -> (MXTensor, h).  The sum and the norm are held in float32 or more; the returned h, the
+    next residual, is rounded to x's dtype (x itself without a residual).  weight [K] of x's dtype or
+    float32."""
     code, dt, shape = _fmt(fmt), _dtype(x.dtype), x.shape
     assert len(shape) >= 1, "rms_norm_mx: x has no axis"
     K = shape[-1]
