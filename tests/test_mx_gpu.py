@@ -499,6 +499,19 @@ def test_mx_linear_module():
     assert ((m(x) - y).norm() / y.norm()).item() < 0.25
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_linear_module_whose_bias_was_cast(dtype):
+    """model.to(dtype) casts the bias buffer; the product takes it at that value."""
+    from snn_compiler.nn import MXLinear
+    torch.manual_seed(4)
+    m = MXLinear.from_linear(torch.nn.Linear(200, 96).to(DEV), dtype=torch.float32)
+    x = torch.randn(5, 200, device=DEV)
+    without = MXLinear(m.weight, None, dtype=torch.float32)(x)
+    m = m.to(dtype)
+    assert m.bias.dtype == dtype
+    assert torch.equal(m(x), without + m.bias.float())
+
+
 def test_spiking_mlp_block():
     """norm -> fc1 -> LIF -> fc2 over [T, B, N, D]: each stage against the oracle on the stage's
     own input, and two chained blocks through the residual."""

@@ -53,7 +53,10 @@ class MXLinear(nn.Module):
     def forward(self, x):
         if not isinstance(x, MXTensor):
             x = mx_quantize(x, self.act)
-        return mx_linear(x, self.weight, self.bias, dtype=self.dtype)
+        bias = self.bias
+        if bias is not None and bias.dtype != torch.float32:      # after .half() or .to(bfloat16)
+            bias = bias.float()
+        return mx_linear(x, self.weight, bias, dtype=self.dtype)
 
     def extra_repr(self):
         return (f"{self.in_features}, {self.out_features}, bias={self.bias is not None}, "
