@@ -402,6 +402,36 @@ def test_norm_slices_of_wider_tensors(rows, K, cols, at, dtype):
     _check_norm(q, h, x, w, r, 1e-6, "mxfp4")
 
 
+@pytest.mark.parametrize("K", [1, 7, 9, 34, 100, 128, 129, 189, 250, 257, 404, 500, 777, 3001])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_norm_of_unaligned_rows_between_nans(K, dtype):
+    """Rows inside a wider tensor whose other columns are NaN: loads may cover them, results do
+    not.  The first row starts the storage, the last ends it."""
+    mx = _mx()
+    g = _gen(K)
+    rows = 37
+    for fmt, ld, at in (("mxfp4", K + 3, 0), ("mxfp8", K + 3, 3), ("mxfp8", K + 17, 5)):
+        hold = [torch.full((rows, ld), float("nan"), dtype=dtype) for _ in range(2)]
+        x, r = (t[:, at:at + K] for t in hold)
+        x.copy_(torch.randn(rows, K, generator=g))
+        r.copy_(torch.randn(rows, K, generator=g))
+        w = torch.rand(K, generator=g).to(dtype) + 0.5
+        xd, rd = (t.to(DEV)[:, at:at + K] for t in hold)
+        q, h = mx.rms_norm_mx(xd, w.to(DEV), rd, eps=1e-6, fmt=fmt)
+        _check_norm(q, h, x, w, r, 1e-6, fmt)
+
+
+@pytest.mark.parametrize("K", [5, 100, 189, 500, 1003])
+def test_norm_of_one_row_for_all(K):
+    """Row stride 0."""
+    mx = _mx()
+    g = _gen(K)
+    x, w = torch.randn(1, K, generator=g), torch.rand(K, generator=g) + 0.5
+    r = torch.randn(40, K, generator=g)
+    q, h = mx.rms_norm_mx(x.to(DEV).expand(40, K), w.to(DEV), r.to(DEV), eps=1e-6, fmt="mxfp8")
+    _check_norm(q, h, x.expand(40, K), w, r, 1e-6, "mxfp8")
+
+
 def test_norm_rows_of_extremes():
     """Zero rows (eps alone), values whose squares leave float32, and NaN or infinite rows, which
     stay NaN (or zero around an infinity) and leave their neighbours alone."""

@@ -309,15 +309,29 @@ __device__ __forceinline__ void shift_right(uint32_t (&w)[N + 4], uint32_t bytes
     }
 }
 
+// Whether aligned loads around a row's values may reach past its two ends: the bytes there belong
+// to the tensor's span, from its first value to its last (gaps between its rows included).
+struct RowEnds {
+    bool before = false, after = false;
+    __device__ __forceinline__ RowEnds() {}
+    template <typename T>
+    __device__ __forceinline__ RowEnds(const T* x, uint32_t rows, int64_t ld, uint32_t K, uint32_t row) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(x + (int64_t)row * ld);
+        before = (at & ~uintptr_t(15)) >= reinterpret_cast<uintptr_t>(x);
+        after = at + K * (uint64_t)sizeof(T) + 16 * (sizeof(T) / 2 + 1) <=
+                reinterpret_cast<uintptr_t>(x + (int64_t)(rows - 1) * ld + K);
+    }
+};
+
 // The values k .. k + 7 of a row of K at `row`, aligned to an element only; values past K are
-// zero.  Inside the row: two (float: three) aligned 16-byte loads around them, shifted into
-// place; at its ends one load per element, so that nothing outside the row is read.
+// zero.  Two (float: three) aligned 16-byte loads around them, shifted into place, where those
+// stay inside the row or the tensor's span; elsewhere one load per element.
 template <typename T>
-__device__ __forceinline__ Raw8<T> load_any8(const T* row, uint32_t k, uint32_t K) {
+__device__ __forceinline__ Raw8<T> load_any8(const T* row, uint32_t k, uint32_t K, RowEnds ends = RowEnds()) {
     constexpr int W = (int)sizeof(T) * 2;                        // words of 8 values
     uint32_t w[W + 4];
     const T* p = row + k;
-    if (k >= 8 && k + 16 <= K) {                                 // 16 bytes to spare either way
+    if ((k >= 8 || ends.before) && (k + 16 <= K || ends.after)) {
         const uintptr_t at = reinterpret_cast<uintptr_t>(p);
         const uint4* down = reinterpret_cast<const uint4*>(at & ~uintptr_t(15));
 #pragma unroll
@@ -326,6 +340,14 @@ __device__ __forceinline__ Raw8<T> load_any8(const T* row, uint32_t k, uint32_t 
             w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
         }
         shift_right<T, W>(w, (uint32_t)(at & 15));
+        if (k + 8 > K) {                                         // the row's end
+            const int n = (int)(K - k);
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                if (sizeof(T) == 4) w[i] = i < n ? w[i] : 0;
+                else w[i] = 2 * i + 1 < n ? w[i] : 2 * i < n ? w[i] & 0xFFFFu : 0;
+            }
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < W; ++i) w[i] = 0;
@@ -345,11 +367,12 @@ __device__ __forceinline__ Raw8<T> load_any8(const T* row, uint32_t k, uint32_t 
     return r;
 }
 
-// The counterpart store, of a whole warp: lane l holds 8 values for p (its own address, 8 l
-// elements after lane 0's), the first n inside the row; lanes past a partial one have n <= 0.
+// The counterpart store, of a whole warp in teams of TEAM lanes, one row each: a team's lane l
+// holds 8 values for p (its own address, 8 l elements after lane 0's), the first n inside the row;
+// lanes past a partial one have n <= 0.
 // Aligned 16-byte pieces are put together from two neighbouring lanes, the one that holds a
 // piece's first value stores it; what no whole piece covers goes out by elements.
-template <typename T>
+template <typename T, int TEAM = 32>
 __device__ __forceinline__ void store_any8(T* p, int n, const Raw8<T>& r, int lane) {
     constexpr int W = (int)sizeof(T) * 2;
     constexpr int PER = 16 / (int)sizeof(T);                     // elements of a piece
@@ -366,7 +389,7 @@ __device__ __forceinline__ void store_any8(T* p, int n, const Raw8<T>& r, int la
     if (n <= 0) return;
     // elements before the first aligned address; the own and the next lane's values from there
     const int head = (int)((0u - (uint32_t)reinterpret_cast<uintptr_t>(p)) & 15u) / (int)sizeof(T);
-    const int have = n < 8 ? n : 8 + (lane < 31 ? next : 0);
+    const int have = n < 8 ? n : 8 + ((lane & (TEAM - 1)) < TEAM - 1 ? next : 0);
     const int bytes = head * (int)sizeof(T);
     shift_right<T, W>(t, (uint32_t)bytes);
     int taken = head;
@@ -379,7 +402,7 @@ __device__ __forceinline__ void store_any8(T* p, int n, const Raw8<T>& r, int la
     }
     // the lane before stored [0, head) with its last piece, unless there is none or the values
     // here do not fill it
-    const bool start = lane == 0 || n < head;
+    const bool start = (lane & (TEAM - 1)) == 0 || n < head;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         if (i >= n || !((i < head && start) || i >= taken)) continue;

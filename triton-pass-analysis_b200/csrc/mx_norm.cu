@@ -153,27 +153,28 @@ __device__ __forceinline__ void emit8(const NormParams& p, const RowOut& o, uint
 // ---- rows through registers --------------------------------------------------------------
 template <typename T, bool ALIGNED>
 __device__ __forceinline__ void take8(const NormParams& p, const T* x, const T* r, uint32_t row,
-                                      uint32_t k, int n, float (&h)[8]) {
+                                      uint32_t k, int n, mx::RowEnds xs, mx::RowEnds rs,
+                                      float (&h)[8]) {
     mx::Raw8<T> a = mx::zero8<T>();
     const T* xr = x + (int64_t)row * p.ldx;
-    if (n > 0) a = ALIGNED ? mx::load_aligned8(xr + k) : mx::load_any8(xr, k, p.K);
+    if (n > 0) a = ALIGNED ? mx::load_aligned8(xr + k) : mx::load_any8(xr, k, p.K, xs);
     mx::to_floats(a, h);
     if (r) {
         mx::Raw8<T> b = mx::zero8<T>();
         const T* rr = r + (int64_t)row * p.ldr;
-        if (n > 0) b = ALIGNED ? mx::load_aligned8(rr + k) : mx::load_any8(rr, k, p.K);
+        if (n > 0) b = ALIGNED ? mx::load_aligned8(rr + k) : mx::load_any8(rr, k, p.K, rs);
         float f[8];
         mx::to_floats(b, f);
         add8(h, f);
     }
 }
-template <typename T, bool ALIGNED>
+template <typename T, bool ALIGNED, int LANES>
 __device__ __forceinline__ void put_h8(const NormParams& p, T* h_out, uint32_t row, uint32_t k,
                                        int n, const float (&h)[8], int lane) {
     mx::Raw8<T> o;
     mx::from_floats(h, o);
     T* q = h_out + (n > 0 ? (uint64_t)row * p.K + k : 0);
-    if (!ALIGNED) mx::store_any8(q, n, o, lane);
+    if (!ALIGNED) mx::store_any8<T, LANES < 32 ? LANES : 32>(q, n, o, lane);
     else if (n > 0) mx::store_aligned8(q, o);
 }
 
@@ -204,6 +205,11 @@ rms_norm_mx_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __restri
     const uint32_t row = blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES;
     const bool in_row = row < p.rows;
     const RowOut out(p, row, in_row);
+    mx::RowEnds xs, rs;
+    if (!ALIGNED && LANES <= 128 && in_row) {           // longer rows: not worth the tests
+        xs = mx::RowEnds(x, p.rows, p.ldx, p.K, row);
+        if (r) rs = mx::RowEnds(r, p.rows, p.ldr, p.K, row);
+    }
     auto valid = [&](uint32_t k) { return in_row && k < p.K ? (int)min(8u, p.K - k) : 0; };
     // whole warps: a chunk that begins past the row's end is left out
     auto past = [&](uint32_t k, uint32_t end) {
@@ -231,13 +237,13 @@ rms_norm_mx_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __restri
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
             const uint32_t k = (c * LANES + t) * 8;
-            take8<T, ALIGNED>(p, x, r, row, k, valid(k), h[c]);
+            take8<T, ALIGNED>(p, x, r, row, k, valid(k), xs, rs, h[c]);
         }
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
             const uint32_t k = (c * LANES + t) * 8;
             if (c > 0 && past(k, p.K)) break;
-            if (h_out) put_h8<T, ALIGNED>(p, h_out, row, k, valid(k), h[c], lane);
+            if (h_out) put_h8<T, ALIGNED, LANES>(p, h_out, row, k, valid(k), h[c], lane);
         }
         sum = squares(h);
         const double rstd64 = rstd_of(p, row_sum(sum));
@@ -253,14 +259,14 @@ rms_norm_mx_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __restri
         float (&h)[8] = h1[0];
         for (uint32_t k = t * 8; !past(k, p.K); k += LANES * 8) {
             const int n = valid(k);
-            take8<T, ALIGNED>(p, x, r, row, k, n, h);
-            if (h_out) put_h8<T, ALIGNED>(p, h_out, row, k, n, h, lane);
+            take8<T, ALIGNED>(p, x, r, row, k, n, xs, rs, h);
+            if (h_out) put_h8<T, ALIGNED, LANES>(p, h_out, row, k, n, h, lane);
             sum += squares(h1);
         }
         const double rstd64 = rstd_of(p, row_sum(sum));
         const float rstd = (float)rstd64;
         for (uint32_t k = t * 8; !past(k, p.groups * 128); k += LANES * 8) {
-            take8<T, ALIGNED>(p, x, r, row, k, valid(k), h);
+            take8<T, ALIGNED>(p, x, r, row, k, valid(k), xs, rs, h);
             finish(k, h, rstd, rstd64);
         }
     }
@@ -466,10 +472,17 @@ int run_norm(const NormArgs& a, const NormParams& p) {
                          (!a.r || (aligned16(a.r) && (one || p.ldr * es % 16 == 0))) &&
                          (!a.h || aligned16(a.h)) && aligned16(a.weight);
     if (!aligned) {
+        // a team with as many lanes as the row needs: 63025 x 34 bf16 with residual 24 us (57 with
+        // a warp a row), 15646 x 189 11 (16), 34225 x 404 45 (57; float32, 10000 x 500: 23, 21);
+        // from 8192 columns on, one read instead of two: 3000 x 16001 123 us (175)
+        if (K <= 128) return launch_norm<T, W, false, 16, 1>(a, p);
+        if (K <= 256) return launch_norm<T, W, false, 16, 2>(a, p);
+        if (K <= 512 && es == 2) return launch_norm<T, W, false, 16, 4>(a, p);
         if (K <= 1024) return launch_norm<T, W, false, 32, 4>(a, p);
         if (K <= 2048) return launch_norm<T, W, false, 64, 4>(a, p);
         if (K <= 4096) return launch_norm<T, W, false, 128, 4>(a, p);
         if (K <= 8192) return launch_norm<T, W, false, 256, 4>(a, p);
+        if (K <= 16384) return launch_norm<T, W, false, 512, 4>(a, p);
         return launch_norm<T, W, false, 1024, 0>(a, p);
     }
     // short rows: the copies of a ring cost more than they hide
