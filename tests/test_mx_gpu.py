@@ -510,6 +510,27 @@ def test_status_word_stays_clear():
     assert KC.device_status() == 0
 
 
+@pytest.mark.parametrize("rows,N,K", [(1, 1, 32), (2, 3, 32), (15, 31, 40), (17, 33, 64), (64, 129, 96),
+                                      (101, 255, 33), (301, 257, 64), (1001, 1023, 40),
+                                      (1300, 2051, 160)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fmt", ["mxfp4", "mxfp8"])
+def test_linear_odd_features_in_16_bits(rows, N, K, dtype, fmt):
+    """An odd number of features: words of two that begin at even or odd features by the row, at
+    either alignment of `out`.  The same product in float32, rounded once, is the same bits."""
+    mx = _mx()
+    g = _gen(rows + N)
+    a = mx.mx_quantize(torch.randn(rows, K, generator=g).to(DEV), fmt)
+    w = mx.mx_quantize(torch.randn(N, K, generator=g).to(DEV))
+    bias = torch.randn(N, generator=g).to(DEV)
+    want = mx.mx_linear(a, w, bias, dtype=torch.float32).to(dtype)
+    for at in (0, 1, 2):
+        hold = torch.full((rows * N + 4,), 7.0, dtype=dtype, device=DEV)
+        mx.mx_linear(a, w, bias, out=hold[at: at + rows * N].view(rows, N))
+        assert torch.equal(hold[at: at + rows * N].view(rows, N), want)
+        assert (hold[:at] == 7).all() and (hold[at + rows * N:] == 7).all()
+
+
 def test_mx_linear_module():
     from snn_compiler.nn import MXLinear
     mx = _mx()

@@ -33,7 +33,7 @@ struct MxParams {
     const float* bias;
     void* out;
     int out_dtype;
-    int pairs;                       // 16-bit outputs may be stored two features at a time
+    int pairs, odd_pairs;            // 16-bit outputs may be stored two features at a time: N even, odd
     int* status;
 };
 
@@ -185,7 +185,7 @@ __device__ __forceinline__ void tmem_load(uint32_t t, float (&r)[N]) {
 // read.  16-bit outputs with an even N go out two features at a time: a column pair is rounded
 // into one word, neighbouring lanes exchange their words, and the even lane stores both features
 // of token i, the odd lane of token i + 1.
-template <int CW, typename Release>
+template <int CW, bool ODD_PAIRS, typename Release>
 __device__ __forceinline__ void store_tile(const MxParams& p, uint32_t t, float bias, int n,
                                            int64_t r0, int cols, Release release) {
     float r[CW];
@@ -206,6 +206,35 @@ __device__ __forceinline__ void store_tile(const MxParams& p, uint32_t t, float 
                 SNNB_IN_BOUNDS((r0 + odd + i) * p.N + n, (int64_t)p.rows * p.N, p.status))
                 *o = w;
             o += step;
+        }
+    } else if (ODD_PAIRS && p.odd_pairs) {
+        // N is odd, r0 + i even: token i's words begin at even features, token i + 1's at odd
+        // ones, so either half takes the next lane's value.  Lanes 0 and 31 hold halves of token
+        // i + 1's words that neighbouring warps share, the last feature half of token i's.
+        // (4096 x 8191 x 512: 35 us, 47 by single values; 4223 x 14243 x 33: 69, 91.  Tiles of 256
+        // tokens have 16 warps for it, whose registers this would spill: 4096 x 4097 x 4096 33 us
+        // by single values, 35 to 37 so.)
+        uint32_t v[CW / 2];
+#pragma unroll
+        for (int i = 0; i < CW / 2; ++i) v[i] = pack16(p, r[2 * i] + bias, r[2 * i + 1] + bias);
+        const int lane = threadIdx.x & 31, odd = lane & 1;
+        const uint32_t pick = odd ? 0x7632u : 0x5410u;
+        uint16_t* o = static_cast<uint16_t*>(p.out) + (r0 + odd) * p.N + n;
+        const bool pair = lane < 31 && n + 1 < p.N, last = n == p.N - 1;
+        const bool half = (lane == 0 || lane == 31) && n < p.N;
+#pragma unroll
+        for (int i = 0; i < CW; i += 2) {
+            const uint32_t x = v[i / 2];
+            const uint32_t w = __byte_perm(x, __shfl_down_sync(0xffffffffu, x, 1), pick);
+            if (pair && i + odd < cols &&
+                SNNB_IN_BOUNDS((r0 + i + odd) * p.N + n + 1, (int64_t)p.rows * p.N, p.status))
+                *reinterpret_cast<uint32_t*>(o) = w;
+            if (half && i + 1 < cols &&
+                SNNB_IN_BOUNDS((r0 + i + 1) * p.N + n, (int64_t)p.rows * p.N, p.status))
+                o[(1 - odd) * p.N] = (uint16_t)(x >> 16);
+            if (last && i < cols && SNNB_IN_BOUNDS((r0 + i) * p.N + n, (int64_t)p.rows * p.N, p.status))
+                *o = (uint16_t)x;
+            o += 2 * (int64_t)p.N;
         }
     } else {
 #pragma unroll
@@ -496,7 +525,7 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
             } else {
                 const int64_t r0 = (int64_t)tt * BN + c0;
                 const int64_t left = (int64_t)p.rows - r0;
-                store_tile<CW>(p, t, bias, n, r0, (int)(left < CW ? left : CW), release);
+                store_tile<CW, BN != 256>(p, t, bias, n, r0, (int)(left < CW ? left : CW), release);
             }
         }
     } else {
@@ -730,7 +759,9 @@ int run_mx(const void* a, const void* as, int a_fmt, int64_t rows, int64_t K, co
     if (!p.status) return SNNB_ERR_CUDA;
     p.rows = (int)rows; p.N = (int)N; p.groups = (int)mx::groups_of(K);
     p.bias = bias; p.out = out; p.out_dtype = out_dtype;
-    p.pairs = out_dtype != SNNB_F32 && N % 2 == 0 && reinterpret_cast<uintptr_t>(out) % 4 == 0;
+    const bool words = out_dtype != SNNB_F32 && reinterpret_cast<uintptr_t>(out) % 4 == 0;
+    p.pairs = words && N % 2 == 0;
+    p.odd_pairs = words && N % 2 == 1;
     if (a_fmt == SNNB_MXFP4) return pick_mx<SNNB_MXFP4, false>(a, as, w, ws, rows, N, K, p, s);
     // an unpacking copy wants whole groups of 128 elements a row and a base on 32 bytes
     if (mx::blocks_of(K) % 4 == 0 && reinterpret_cast<uintptr_t>(w) % 32 == 0)
