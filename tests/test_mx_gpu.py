@@ -421,6 +421,30 @@ def test_norm_of_unaligned_rows_between_nans(K, dtype):
         _check_norm(q, h, x, w, r, 1e-6, fmt)
 
 
+@pytest.mark.parametrize("K", [1, 8, 31, 34, 48, 63, 64, 65, 120, 127, 129, 260, 300, 511, 513])
+@pytest.mark.parametrize("rows", [1, 9, 301])
+def test_short_rows(K, rows):
+    """Quantise, back and norm at every team width of short rows, aligned or not, the gap between
+    rows NaN."""
+    mx = _mx()
+    g = _gen(rows * 1000 + K)
+    for gap, at, dtype, fmt in ((0, 0, torch.float32, "mxfp4"), (16, 8, torch.bfloat16, "mxfp8"),
+                                (3, 1, torch.float16, "mxfp4"), (5, 2, torch.float32, "mxfp8")):
+        hold = torch.full((rows, K + gap), float("nan"), dtype=dtype)
+        x = hold[:, at:at + K]
+        x.copy_(torch.randn(rows, K, generator=g))
+        d = hold.to(DEV)[:, at:at + K]
+        t = mx.mx_quantize(d, fmt)
+        _check_quantised(t, x.double().numpy(), fmt)
+        back = mx.mx_dequantize(t, torch.float32).cpu()
+        codes, scales = OM.quantize(x.double().numpy(), fmt)
+        want = OM.values(codes, scales, fmt).reshape(rows, -1)[:, :K]
+        assert np.array_equal(back.double().numpy(), want)
+        w = (torch.rand(K, generator=g) + 0.5).to(dtype)
+        q, h = mx.rms_norm_mx(d, w.to(DEV), None, eps=1e-6, fmt=fmt)
+        _check_norm(q, h, x, w, None, 1e-6, fmt)
+
+
 @pytest.mark.parametrize("K", [5, 100, 189, 500, 1003])
 def test_norm_of_one_row_for_all(K):
     """Row stride 0."""

@@ -189,11 +189,12 @@ __device__ __forceinline__ uint32_t quantise_block(const float (&x)[8], uint32_t
 }
 
 // The four scale bytes of 4 neighbouring blocks (16 lanes, one byte per 4 lanes) as one word,
-// in every one of the 16 lanes.
+// in every one of the 16 lanes; of a row of two blocks that 8 lanes hold, in those.
+template <int LANES = 32>
 __device__ __forceinline__ uint32_t join_scales(uint32_t byte, int lane) {
-    uint32_t w = byte << (8 * ((lane >> 2) & 3));
+    uint32_t w = byte << (8 * ((lane >> 2) & (LANES >= 16 ? 3 : 1)));
     w |= __shfl_xor_sync(0xffffffffu, w, 4);
-    w |= __shfl_xor_sync(0xffffffffu, w, 8);
+    if (LANES >= 16) w |= __shfl_xor_sync(0xffffffffu, w, 8);
     return w;
 }
 

@@ -130,6 +130,7 @@ struct RowOut {
     }
 };
 // Codes and scale word of 8 values at column k of a row.  Every lane of the warp calls.
+template <int LANES = 32>
 __device__ __forceinline__ void emit8(const NormParams& p, const RowOut& o, uint32_t k,
                                       const float (&y)[8], int lane) {
     const uint32_t j = k >> 5;
@@ -145,8 +146,8 @@ __device__ __forceinline__ void emit8(const NormParams& p, const RowOut& o, uint
         byte = mx::quantise_block<SNNB_MXFP8>(y, e, c);
         if (inside) *reinterpret_cast<uint2*>(o.data + k) = c;
     }
-    const uint32_t word = mx::join_scales(byte, lane);
-    if (o.data && (j >> 2) < p.groups && (lane & 15) == 0)
+    const uint32_t word = mx::join_scales<LANES>(byte, lane);
+    if (o.data && (j >> 2) < p.groups && (lane & (LANES < 16 ? 7 : 15)) == 0)
         o.scales[(j >> 2) * (mx::GROUP_BYTES / 4)] = word;
 }
 
@@ -229,7 +230,7 @@ rms_norm_mx_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __restri
         float w[8], y[8];
         mx::to_floats(weights8<W>(p, weight, k), w);
         normed8(h, w, rstd, rstd64, y);
-        emit8(p, out, k, y, lane);
+        emit8<LANES < 32 ? LANES : 32>(p, out, k, y, lane);
     };
     double sum = 0.0;
     if constexpr (CHUNKS > 0) {
@@ -472,9 +473,10 @@ int run_norm(const NormArgs& a, const NormParams& p) {
                          (!a.r || (aligned16(a.r) && (one || p.ldr * es % 16 == 0))) &&
                          (!a.h || aligned16(a.h)) && aligned16(a.weight);
     if (!aligned) {
-        // a team with as many lanes as the row needs: 63025 x 34 bf16 with residual 24 us (57 with
+        // a team with as many lanes as the row needs: 63025 x 34 bf16 with residual 13 us (57 with
         // a warp a row), 15646 x 189 11 (16), 34225 x 404 45 (57; float32, 10000 x 500: 23, 21);
         // from 8192 columns on, one read instead of two: 3000 x 16001 123 us (175)
+        if (K <= 64) return launch_norm<T, W, false, 8, 1>(a, p);
         if (K <= 128) return launch_norm<T, W, false, 16, 1>(a, p);
         if (K <= 256) return launch_norm<T, W, false, 16, 2>(a, p);
         if (K <= 512 && es == 2) return launch_norm<T, W, false, 16, 4>(a, p);
@@ -485,7 +487,9 @@ int run_norm(const NormArgs& a, const NormParams& p) {
         if (K <= 16384) return launch_norm<T, W, false, 512, 4>(a, p);
         return launch_norm<T, W, false, 1024, 0>(a, p);
     }
-    // short rows: the copies of a ring cost more than they hide
+    // short rows: the copies of a ring cost more than they hide (57885 x 32 bf16 with residual: 7.1
+    // us with 8 lanes a row, 12.8 with 16)
+    if (K <= 64) return launch_norm<T, W, true, 8, 1>(a, p);
     if (K <= 128) return launch_norm<T, W, true, 16, 1>(a, p);
     if (K <= 256) return launch_norm<T, W, true, 32, 1>(a, p);
     // Few rows (at most one per SM): as many threads as the row has groups of 8, for the shortest

@@ -79,8 +79,9 @@ mx_quantize_kernel(const T* __restrict__ x, uint32_t rows, uint32_t K, int64_t l
     mx::zero_row_padding(scales, rows, groups, thread, (uint64_t)gridDim.x * Q_THREADS);
 }
 
-// total: pieces of 256 values, per_row.d = ceil(K / 256) of them a row.
-template <typename T, int FMT, int U>
+// LANES threads a piece of 8 LANES values.  total: pieces, per_row.d of them a row (LANES = 8:
+// rows of one piece).
+template <typename T, int FMT, int U, int LANES>
 __global__ void __launch_bounds__(Q_THREADS)
 mx_quantize_any_kernel(const T* __restrict__ x, uint32_t rows, uint32_t K, int64_t ldx,
                        uint32_t nb, uint32_t groups, mx::FastDiv per_row, uint32_t total,
@@ -91,8 +92,8 @@ mx_quantize_any_kernel(const T* __restrict__ x, uint32_t rows, uint32_t K, int64
     pdl_trigger();
     const uint32_t lane = threadIdx.x & 31, sub = lane & 3;
     const uint64_t thread = (uint64_t)blockIdx.x * Q_THREADS + threadIdx.x;
-    constexpr uint32_t step = Q_THREADS / 32;
-    const uint32_t first = blockIdx.x * (U * step) + (threadIdx.x >> 5);
+    constexpr uint32_t step = Q_THREADS / LANES;
+    const uint32_t first = blockIdx.x * (U * step) + threadIdx.x / LANES;
     {
         mx::Raw8<T> raw[U];
         uint32_t row[U], k[U];
@@ -100,8 +101,12 @@ mx_quantize_any_kernel(const T* __restrict__ x, uint32_t rows, uint32_t K, int64
         for (int u = 0; u < U; ++u) {
             const uint32_t q = first + u * step;
             row[u] = per_row.div(q);
-            k[u] = (q - row[u] * per_row.d) * 256 + lane * 8;
-            raw[u] = q < total && k[u] < K ? mx::load_any8(x + row[u] * ldx, k[u], K) : mx::zero8<T>();
+            k[u] = ((q - row[u] * per_row.d) * LANES + (lane & (LANES - 1))) * 8;
+            // short rows are mostly ends; in longer ones the test costs more than it gives
+            mx::RowEnds ends;
+            if (LANES < 32 && q < total) ends = mx::RowEnds(x, rows, ldx, K, row[u]);
+            raw[u] = q < total && k[u] < K ? mx::load_any8(x + row[u] * ldx, k[u], K, ends)
+                                           : mx::zero8<T>();
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -109,13 +114,13 @@ mx_quantize_any_kernel(const T* __restrict__ x, uint32_t rows, uint32_t K, int64
             mx::to_floats(raw[u], v);
             Codes c;
             const uint32_t byte = mx::quantise_block<FMT>(v, mx::top_exponent(raw[u], v), c);
-            const uint32_t word = mx::join_scales(byte, lane);
+            const uint32_t word = mx::join_scales<LANES>(byte, lane);
             const uint32_t j = k[u] >> 5;
             if (first + u * step < total) {
                 if (j < nb)
                     *reinterpret_cast<Codes*>(data + (uint64_t)(row[u] * nb + j) * F::BLOCK_BYTES +
                                               sub * sizeof(Codes)) = c;
-                if ((lane & 15) == 0 && (j >> 2) < groups)
+                if ((lane & (LANES < 16 ? 7 : 15)) == 0 && (j >> 2) < groups)
                     scales[mx::scale_word(row[u], j >> 2, groups)] = word;
             }
         }
@@ -173,8 +178,8 @@ mx_dequantize_kernel(const uint8_t* __restrict__ data, const uint8_t* __restrict
     }
 }
 
-// total: pieces of 256 values, per_row.d = ceil(K / 256) of them a row.
-template <typename T, int FMT, int U>
+// LANES threads a piece of 8 LANES values.  total: pieces, per_row.d of them a row.
+template <typename T, int FMT, int U, int LANES>
 __global__ void __launch_bounds__(Q_THREADS)
 mx_dequantize_any_kernel(const uint8_t* __restrict__ data, const uint8_t* __restrict__ scales,
                          uint32_t rows, uint32_t K, uint32_t nb, uint32_t groups,
@@ -184,8 +189,8 @@ mx_dequantize_any_kernel(const uint8_t* __restrict__ data, const uint8_t* __rest
     pdl_wait();
     pdl_trigger();
     const uint32_t lane = threadIdx.x & 31, sub = lane & 3;
-    constexpr uint32_t step = Q_THREADS / 32;
-    const uint32_t first = blockIdx.x * (U * step) + (threadIdx.x >> 5);
+    constexpr uint32_t step = Q_THREADS / LANES;
+    const uint32_t first = blockIdx.x * (U * step) + threadIdx.x / LANES;
     {
         Codes c[U];
         uint32_t byte[U], row[U], k[U];
@@ -193,7 +198,7 @@ mx_dequantize_any_kernel(const uint8_t* __restrict__ data, const uint8_t* __rest
         for (int u = 0; u < U; ++u) {
             const uint32_t q = first + u * step;
             row[u] = per_row.div(q);
-            k[u] = (q - row[u] * per_row.d) * 256 + lane * 8;
+            k[u] = ((q - row[u] * per_row.d) * LANES + (lane & (LANES - 1))) * 8;
             const uint32_t j = k[u] >> 5;
             c[u] = Codes{};
             byte[u] = 0;
@@ -206,7 +211,7 @@ mx_dequantize_any_kernel(const uint8_t* __restrict__ data, const uint8_t* __rest
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const bool in = first + u * step < total && k[u] < K;
-            mx::store_any8(out + (in ? (uint64_t)row[u] * K + k[u] : 0),
+            mx::store_any8<T, LANES>(out + (in ? (uint64_t)row[u] * K + k[u] : 0),
                            in ? (int)min(8u, K - k[u]) : 0, decode_scaled<T, FMT>(c[u], byte[u]),
                            (int)lane);
         }
@@ -215,6 +220,10 @@ mx_dequantize_any_kernel(const uint8_t* __restrict__ data, const uint8_t* __rest
 
 // Whether U = 1: `units` (per thread block and unit of U: `per`) do not fill four blocks an SM.
 bool small(int64_t units, int64_t per) { return units <= 148 * 4 * 4 * per; }
+// Lanes a piece of an unaligned row: what short rows fill (63025 x 34 bf16 -> E2M1: 5.0 us, 13.2
+// with 32; 27336 x 113: 4.6, 6.6; 27997 x 344: 9.0, 12.2), 32 beyond (3000 x 16001: 34 us, 37
+// with 16).
+int any_lanes(int64_t K) { return K <= 64 ? 8 : K <= 128 || (K > 256 && K <= 512) ? 16 : 32; }
 unsigned blocks_for(int64_t units, int64_t per) { return (unsigned)((units + per - 1) / per); }
 
 template <typename T, int FMT>
@@ -223,10 +232,13 @@ int run_quantize(const void* x, int64_t rows, int64_t K, int64_t ldx, void* data
     const uint32_t nb = (uint32_t)mx::blocks_of(K), groups = (uint32_t)mx::groups_of(K);
     const bool aligned = K % 8 == 0 && aligned16(x) && (rows == 1 || ldx * (int64_t)sizeof(T) % 16 == 0);
     const bool flat = K % 128 == 0 && (rows == 1 || ldx == K);
-    const uint32_t per = aligned ? groups * 4 : (uint32_t)((K + 255) / 256);
-    const int64_t total = rows * per, unit = aligned ? Q_THREADS / 4 : Q_THREADS / 32;
+    const int lanes = aligned ? 4 : any_lanes(K);
+    const uint32_t per = aligned ? groups * 4 : (uint32_t)((K + 8 * lanes - 1) / (8 * lanes));
+    const int64_t total = rows * per, unit = Q_THREADS / lanes;
     const bool one = small(total, unit);
-    auto k = !aligned ? (one ? mx_quantize_any_kernel<T, FMT, 1> : mx_quantize_any_kernel<T, FMT, 2>)
+    auto k = lanes == 8  ? (one ? mx_quantize_any_kernel<T, FMT, 1, 8> : mx_quantize_any_kernel<T, FMT, 2, 8>)
+             : lanes == 16 ? (one ? mx_quantize_any_kernel<T, FMT, 1, 16> : mx_quantize_any_kernel<T, FMT, 2, 16>)
+             : lanes == 32 ? (one ? mx_quantize_any_kernel<T, FMT, 1, 32> : mx_quantize_any_kernel<T, FMT, 2, 32>)
              : flat   ? (one ? mx_quantize_kernel<T, FMT, 1, true> : mx_quantize_kernel<T, FMT, 4, true>)
                       : (one ? mx_quantize_kernel<T, FMT, 1, false> : mx_quantize_kernel<T, FMT, 4, false>);
     const int U = one ? 1 : aligned ? 4 : 2;
@@ -251,10 +263,13 @@ int run_dequantize(const void* data, const void* scales, int64_t rows, int64_t K
                         sc, (uint32_t)rows, (uint32_t)K, groups, mx::FastDiv(nb), (uint32_t)total,
                         static_cast<T*>(out));
     }
-    const uint32_t per = (uint32_t)((K + 255) / 256);
-    const int64_t total = rows * per, unit = Q_THREADS / 32;
+    const int lanes = any_lanes(K);
+    const uint32_t per = (uint32_t)((K + 8 * lanes - 1) / (8 * lanes));
+    const int64_t total = rows * per, unit = Q_THREADS / lanes;
     const bool one = small(total, unit);
-    auto k = one ? mx_dequantize_any_kernel<T, FMT, 1> : mx_dequantize_any_kernel<T, FMT, 2>;
+    auto k = lanes == 8    ? (one ? mx_dequantize_any_kernel<T, FMT, 1, 8> : mx_dequantize_any_kernel<T, FMT, 2, 8>)
+             : lanes == 16 ? (one ? mx_dequantize_any_kernel<T, FMT, 1, 16> : mx_dequantize_any_kernel<T, FMT, 2, 16>)
+                           : (one ? mx_dequantize_any_kernel<T, FMT, 1, 32> : mx_dequantize_any_kernel<T, FMT, 2, 32>);
     return launch_k(k, dim3(blocks_for(total, (one ? 1 : 2) * unit)), dim3(Q_THREADS), 0, s, d, sc,
                     (uint32_t)rows, (uint32_t)K, nb, groups, mx::FastDiv(per), (uint32_t)total,
                     static_cast<T*>(out));
