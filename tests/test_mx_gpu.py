@@ -534,6 +534,29 @@ def test_status_word_stays_clear():
     assert KC.device_status() == 0
 
 
+@pytest.mark.parametrize("stages", list(range(1, 27)))
+@pytest.mark.parametrize("fmt", ["mxfp4", "mxfp8"])
+def test_linear_every_number_of_stages(stages, fmt):
+    """Few tiles and a K of 1 to 26 ring stages (256 of K in mxfp4, 128 in mxfp8), whole or ragged:
+    K is split over as many thread blocks as pay, and each has work."""
+    from snn_compiler.kernels import conv as KC
+    mx = _mx()
+    step = 256 if fmt == "mxfp4" else 128
+    for rows, N, K in ((2, 16, stages * step), (2, 16, stages * step - step // 2 - 32),
+                       (40, 200, stages * step - 7), (140, 100, stages * step - 32)):
+        if K < 1:
+            continue
+        g = _gen(K)
+        a = mx.mx_quantize(torch.randn(rows, K, generator=g).to(DEV), fmt)
+        w = mx.mx_quantize(torch.randn(N, K, generator=g).to(DEV))
+        out = mx.mx_linear(a, w, dtype=torch.float32).double().cpu()
+        va = torch.from_numpy(OM.values(*_held(a), fmt)[:, :K])
+        vw = torch.from_numpy(OM.values(*_held(w), "mxfp4")[:, :K])
+        tol = (2 * K / 32 + 16) * 2.0 ** -23 * (va.abs() @ vw.abs().t()) + 2.0 ** -24 * (va @ vw.t()).abs()
+        assert ((out - va @ vw.t()).abs() <= tol).all(), (rows, N, K)
+    assert KC.device_status() == 0
+
+
 @pytest.mark.parametrize("rows,N,K", [(1, 1, 32), (2, 3, 32), (15, 31, 40), (17, 33, 64), (64, 129, 96),
                                       (101, 255, 33), (301, 257, 64), (1001, 1023, 40),
                                       (1300, 2051, 160)])

@@ -298,6 +298,27 @@ __device__ __forceinline__ void join_splits(const MxParams& p, uint32_t part, in
     }
 }
 
+// The stages of K of CTA `rank` of `splits`: from its first to the next rank's first.  Its MMA
+// thread waits for at least one.
+__host__ __device__ constexpr int first_stage(int nstages, int rank, int splits) {
+    return (int)((int64_t)nstages * rank / splits);
+}
+// Whether 2^log ways save 6 stages of ~0.25 us, which pay for the join (1.4 us), and leave every
+// CTA a stage.
+constexpr bool split_pays(int nstages, int log) {
+    return (nstages >> log) >= 1 && nstages - (nstages >> log) >= 6;
+}
+constexpr bool every_rank_has_stages() {
+    for (int n = 1; n <= 64; ++n)
+        for (int log = 0; log <= 3; ++log)
+            for (int r = 0; r < 1 << log; ++r)
+                if ((log == 0 || split_pays(n, log)) &&
+                    first_stage(n, r, 1 << log) >= first_stage(n, r + 1, 1 << log))
+                    return false;
+    return true;
+}
+static_assert(every_rank_has_stages(), "a CTA without a stage would wait for one");
+
 // PAIR: two CTAs share a 256-feature x BN-token tile (each stages its own 128 features and half
 // of the tokens) and walk whole tiles.  Otherwise: one tile, its K range split over the CTAs of
 // a cluster, their float32 partial sums joined in rank order through distributed shared memory.
@@ -376,8 +397,7 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
     const int tile0 = PAIR ? (int)blockIdx.x / 2 : (int)blockIdx.x / splits;
     const int tile_step = PAIR ? (int)gridDim.x / 2 : p.tiles;
     const int nstages = (p.groups + S::GROUPS - 1) / S::GROUPS;
-    const int k0 = (int)((int64_t)nstages * rank / splits);
-    const int k1 = (int)((int64_t)nstages * (rank + 1) / splits);
+    const int k0 = first_stage(nstages, rank, splits), k1 = first_stage(nstages, rank + 1, splits);
     uint32_t failed = 0, issued = 0;                 // issued: a producer warp's copies
 
     if (warp < NP) {
@@ -672,15 +692,14 @@ int launch_mx(const void* a, const void* as, const void* w, const void* ws, int6
         cluster = 2;
     } else {
         // The largest split that leaves every cluster resident at once (the occupancy call counts
-        // one CTA an SM) and saves 6 stages of ~0.25 us, which pay for its join (1.4 us); none
-        // where the tiles alone nearly fill the SMs, unless K is long.  Tokens x features x K in
-        // 4 bits: 1 x 16384 x 4096: 9.3 us, 9.8 split in 2; 1 x 8192 x 8192: 12.7, 10.6 in 2, 9.2
-        // in 4; 64 x 2048 x 2048: 5.2, 6.4 in 4; with tokens in 8 bits 16 x 16384 x 4096: 12.7,
-        // 11.9 in 2; 1 x 2048 x 2048: 6.4, 5.3 in 4, 4.6 in 8.
+        // one CTA an SM) and pays; none where the tiles alone nearly fill the SMs, unless K is
+        // long.  Tokens x features x K in 4 bits: 1 x 16384 x 4096: 9.3 us, 9.8 split in 2; 1 x
+        // 8192 x 8192: 12.7, 10.6 in 2, 9.2 in 4; 64 x 2048 x 2048: 5.2, 6.4 in 4; with tokens in
+        // 8 bits 16 x 16384 x 4096: 12.7, 11.9 in 2; 1 x 2048 x 2048: 6.4, 5.3 in 4, 4.6 in 8.
         const int nstages = (p.groups + S::GROUPS - 1) / S::GROUPS;
         int log = 0;
         for (int l = 1; l <= 3 && (tiles < 100 || nstages >= 24); ++l)
-            if (tiles <= (int64_t)dev->clusters[l] * S::CTAS_PER_SM && nstages - (nstages >> l) >= 6)
+            if (tiles <= (int64_t)dev->clusters[l] * S::CTAS_PER_SM && split_pays(nstages, l))
                 log = l;
         if ((1 << log) < min_split) return SNNB_ERR_UNSUPPORTED;
         grid = (unsigned)(tiles << log);
