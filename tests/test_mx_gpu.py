@@ -534,6 +534,26 @@ def test_status_word_stays_clear():
     assert KC.device_status() == 0
 
 
+@pytest.mark.parametrize("rows,N,K", [(6523, 4000, 32), (2000, 4000, 96), (2000, 3000, 1000)])
+def test_linear_of_packed_weights_repeated(rows, N, K):
+    """Rows of K that are no whole groups of 128 beside 8-bit tokens: weights pass through a ring of
+    their own, whose copies may land in any order.  Every repetition gives the first one's bits,
+    and those are the oracle's within the bound."""
+    mx = _mx()
+    g = _gen(K)
+    a = mx.mx_quantize(torch.randn(rows, K, generator=g).to(DEV), "mxfp8")
+    ws = [mx.mx_quantize(torch.randn(N, K, generator=g).to(DEV)) for _ in range(3)]
+    first = [mx.mx_linear(a, w, dtype=torch.float32) for w in ws]
+    va = torch.from_numpy(OM.values(*_held(a), "mxfp8")[:, :K]).to(DEV)
+    for w, out in zip(ws, first):
+        vw = torch.from_numpy(OM.values(*_held(w), "mxfp4")[:, :K]).to(DEV)
+        tol = (2 * K / 32 + 16) * 2.0 ** -23 * (va.abs() @ vw.abs().t()) + 2.0 ** -24 * (va @ vw.t()).abs()
+        assert ((out.double() - va @ vw.t()).abs() <= tol).all()
+    for _ in range(300):
+        for w, out in zip(ws, first):
+            assert torch.equal(mx.mx_linear(a, w, dtype=torch.float32), out)
+
+
 @pytest.mark.parametrize("stages", list(range(1, 27)))
 @pytest.mark.parametrize("fmt", ["mxfp4", "mxfp8"])
 def test_linear_every_number_of_stages(stages, fmt):

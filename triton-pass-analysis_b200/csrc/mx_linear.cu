@@ -552,8 +552,12 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
         // ------------------------------------------------------------- weight pieces (E4M3)
         // The warps w, w + 4 take the stages w, w + 4, ... (each a part of the rows): 16 codes
         // (8 bytes) to the low half of a 16-byte slot, slot c of row r at c ^ (r % 8).
-        static_assert(PACKED_STAGES == 0 || (STAGES >= 4 && PACKED_STAGES >= 4),
-                      "a warp that takes every fourth stage never laps a ring");
+        // A wait by parity needs the phase before to have completed, and a slot's phase before is
+        // another warp's stage, whose copy may land after a later one.  So the stage's release
+        // is waited for first: every MMA up to stage it - STAGES is done, hence every copy up to
+        // there has landed, which covers the packed slot's last use.
+        static_assert(PACKED_STAGES == 0 || (STAGES >= 4 && PACKED_STAGES >= STAGES),
+                      "a wait of a warp that takes every fourth stage is at most one phase ahead");
         constexpr int ROWS = PLACERS > 0 ? 16 / PLACERS : 0;         // groups of 8 rows a warp
         const uint32_t w = (uint32_t)(warp - NP - 1 - EW) & 3u;
         const int part = (warp - NP - 1 - EW) >> 2;
@@ -562,9 +566,9 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
             for (int ks = k0; ks < k1; ++ks, ++it) {
                 if ((it & 3u) != w) continue;
                 const int s = (int)(it % STAGES), ps = PLACERS > 0 ? (int)(it % PACKED_STAGES) : 0;
+                failed |= 1u - tc::mbar_wait_warp(empty_bar(s), ((it / STAGES) & 1u) ^ 1u, failed);
                 failed |= 1u - tc::mbar_wait_warp(pfull_bar(ps), PLACERS > 0 ? (it / PACKED_STAGES) & 1u : 0,
                                                   failed);
-                failed |= 1u - tc::mbar_wait_warp(empty_bar(s), ((it / STAGES) & 1u) ^ 1u, failed);
                 if (failed) break;
                 const uint8_t* src = smem + S::PACKED_OFF + ps * S::PACKED + part * ROWS * 512 + lane * 16;
                 uint8_t* dst = smem + s * S::STAGE + part * ROWS * 1024 + (lane >> 2) * 128;
