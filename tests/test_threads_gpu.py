@@ -1,0 +1,70 @@
+"""Kernels whose shared memory depends on the sizes, called from several host threads at once.  How
+much a kernel may use is a setting of the kernel, not of the launch: no thread's call may take it
+from another's, so every call launches and gives the results of a call alone.
+
+The threads call the C entries, which leave them little to do between two launches."""
+import threading
+
+import pytest
+import torch
+
+from snn_compiler import _lib
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+class _Case:
+    """One call of the C entry `name`; `args` without the stream, `outs` its output tensors."""
+
+    def __init__(self, name, args, outs):
+        self.fn, self.args, self.outs = getattr(_lib.lib(), name), args, outs
+        _lib.check(self.fn(*args, torch.cuda.current_stream().cuda_stream), name)
+        torch.cuda.synchronize()
+        self.want = [o.clone() for o in outs]
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+
+
+def _together(cases, calls=20000):
+    """One thread for each case, on a stream of its own."""
+    failed = []
+
+    def work(case):
+        stream = torch.cuda.Stream()
+        at = stream.cuda_stream
+        for i in range(calls):
+            status = case.fn(*case.args, at)
+            if status:
+                failed.append((case.args, status, i))
+                break
+        stream.synchronize()
+    threads = [threading.Thread(target=work, args=(c,)) for c in cases]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    for c in cases:
+        assert all(torch.equal(a, b) for a, b in zip(c.outs, c.want))
+
+
+def test_norms_of_several_lengths():
+    """Rows of 2256 and 3256 values share a kernel (128 threads a row), of 4104 and 8184 another."""
+    from snn_compiler.kernels import mx
+    g = torch.Generator().manual_seed(9)
+
+    def case(K):
+        rows = 200
+        x, r = (torch.randn(rows, K, generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+        w = (torch.rand(K, generator=g) + 0.5).to(torch.bfloat16).to(DEV)
+        data = torch.empty(rows, (K + 31) // 32 * 32, dtype=torch.uint8, device=DEV)
+        scales = torch.empty(mx.mx_scales_shape(rows, K), dtype=torch.uint8, device=DEV)
+        h = torch.empty_like(x)
+        c = _Case("snnb_rms_norm_mx",
+                  (x.data_ptr(), K, r.data_ptr(), K, _lib.BF16, w.data_ptr(), _lib.BF16, 1e-6, rows,
+                   K, 1, data.data_ptr(), scales.data_ptr(), h.data_ptr()), (data, scales, h))
+        c.inputs = x, r, w
+        return c
+    _together([case(K) for K in (2256, 3256, 8184, 4104)])

@@ -439,16 +439,33 @@ int launch_norm(const NormArgs& a, const NormParams& p) {
 
 // Shared memory of a ring of two stages sets the blocks per SM (as many as were compiled for at
 // most), what that leaves the stages.
+constexpr uint32_t RING_SM_BYTES = 224 * 1024;
+// Lets `k` use as much shared memory as any ring asks for, once per device.  The setting is the
+// kernel's, not the launch's: set to each call's own size, another host thread could lower it
+// between this thread's setting and launch.
+template <typename Kernel>
+int allow_ring(Kernel k, bool (&ready)[64]) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return record_cuda_error(e);
+    if (dev < 0 || dev >= 64) return SNNB_ERR_UNSUPPORTED;
+    if (__atomic_load_n(&ready[dev], __ATOMIC_ACQUIRE)) return SNNB_OK;
+    e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)RING_SM_BYTES);
+    if (e != cudaSuccess) return record_cuda_error(e);
+    __atomic_store_n(&ready[dev], true, __ATOMIC_RELEASE);
+    return SNNB_OK;
+}
+
 template <typename T, typename W, int LANES>
 int launch_ring(const NormArgs& a, const NormParams& p) {
     constexpr uint32_t THREADS = ring_threads(LANES), TEAMS = THREADS / LANES;
-    constexpr uint32_t SM_BYTES = 224 * 1024, BLOCKS = ring_blocks<T, W>(LANES);
+    constexpr uint32_t BLOCKS = ring_blocks<T, W>(LANES);
     const uint32_t half = (p.K * (uint32_t)sizeof(T) + 127) / 128 * 128;
     const uint32_t stage = TEAMS * half * (a.r ? 2 : 1);
-    uint32_t per_sm = SM_BYTES / (2 * stage + RING_HEAD + 1024);
+    uint32_t per_sm = RING_SM_BYTES / (2 * stage + RING_HEAD + 1024);
     if (per_sm < 1) return SNNB_ERR_UNSUPPORTED;
     if (per_sm > BLOCKS) per_sm = BLOCKS;
-    uint32_t stages = (SM_BYTES / per_sm - RING_HEAD - 1024) / stage;
+    uint32_t stages = (RING_SM_BYTES / per_sm - RING_HEAD - 1024) / stage;
     if (stages > RING_MAX) stages = RING_MAX;
     const size_t smem = RING_HEAD + (size_t)stages * stage;
     const bool full = p.K == 8 * LANES * RING_CHUNKS;
@@ -456,8 +473,9 @@ int launch_ring(const NormArgs& a, const NormParams& p) {
                         : rms_norm_mx_ring_kernel<T, W, LANES, true, false>
                  : full ? rms_norm_mx_ring_kernel<T, W, LANES, false, true>
                         : rms_norm_mx_ring_kernel<T, W, LANES, false, false>;
-    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return record_cuda_error(e);
+    static bool ready[4][64];
+    const int rc = allow_ring(k, ready[(a.r ? 2 : 0) + full]);
+    if (rc != SNNB_OK) return rc;
     const uint32_t need = (p.rows + TEAMS - 1) / TEAMS, most = 148u * per_sm;
     return launch_k(k, dim3(need < most ? need : most), dim3(THREADS), smem, a.s,
                     static_cast<const T*>(a.x), static_cast<const T*>(a.r), static_cast<T*>(a.h),
