@@ -68,3 +68,35 @@ def test_norms_of_several_lengths():
         c.inputs = x, r, w
         return c
     _together([case(K) for K in (2256, 3256, 8184, 4104)])
+
+
+@pytest.mark.parametrize("op", ["conv", "linear"])
+def test_first_cuda_call_of_a_thread(op):
+    """A host thread whose first CUDA call is one of the entries that describe tensors to the
+    copy engine: it has no context of its own yet."""
+    from snn_compiler.kernels import conv as C, mx
+    g = torch.Generator().manual_seed(14)
+    if op == "linear":
+        a = mx.mx_quantize(torch.randn(8, 256, generator=g).to(DEV), "mxfp8")
+        w = mx.mx_quantize(torch.randn(64, 256, generator=g).to(DEV))
+        call = lambda: mx.mx_linear(a, w)
+    else:
+        x = (torch.rand(4, 2, 8, 8, 64, generator=g) < 0.2).to(torch.bfloat16).to(DEV)
+        w = (torch.randn(64, 3, 3, 64, generator=g) * 0.06).to(torch.bfloat16).to(DEV)
+        b = (torch.rand(64, generator=g) * 0.9).to(DEV)
+        call = lambda: C.conv3x3_lif(x, w, b, tau=2.0, v_threshold=1.0)
+    want = call()
+    torch.cuda.synchronize()
+    got = []
+
+    def work():
+        try:
+            got.append(call())
+        except Exception as e:                     # reported by the main thread
+            got.append(repr(e))
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    assert isinstance(got[0], torch.Tensor), got
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want)

@@ -1195,9 +1195,21 @@ int encode_tmap(CUtensorMap* map, CUtensorMapDataType dtype, int rank, const voi
         es[i] = elem_strides ? elem_strides[i] : 1;
         if (i < rank - 1) st[i] = strides_bytes[i];
     }
-    CUresult r = fn(map, dtype, (cuuint32_t)rank, const_cast<void*>(base), d, st, b, es,
-                    CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    auto encode = [&] {
+        return fn(map, dtype, (cuuint32_t)rank, const_cast<void*>(base), d, st, b, es,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = encode();
+    if (r == CUDA_ERROR_INVALID_CONTEXT || r == CUDA_ERROR_NOT_INITIALIZED) {
+        // a host thread that has made no runtime call yet has no context, which this driver
+        // entry does not give it; setting its device does
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e == cudaSuccess) e = cudaSetDevice(dev);
+        if (e != cudaSuccess) return record_cuda_error(e);
+        r = encode();
+    }
     return r == CUDA_SUCCESS ? SNNB_OK : SNNB_ERR_ARG;
 }
 
