@@ -100,3 +100,37 @@ def test_first_cuda_call_of_a_thread(op):
     assert isinstance(got[0], torch.Tensor), got
     torch.cuda.synchronize()
     assert torch.equal(got[0], want)
+
+
+def _first_conv(g, cin, cout, size, pool=False):
+    T, B = 4, 2
+    x = torch.rand(1, B, cin, size, size, generator=g).to(DEV)
+    w = (torch.randn(cout, cin, 3, 3, generator=g) * 0.2).to(DEV)
+    b = (torch.rand(cout, generator=g) * 0.6).to(DEV)
+    side = size // 2 if pool else size
+    out = torch.empty(T, B, side, side, cout, device=DEV, dtype=torch.bfloat16)
+    c = _Case("snnb_first_conv_lif",
+              (x.data_ptr(), 1, T, B, cin, size, size, w.data_ptr(), b.data_ptr(), cout, 0.5, 0.5,
+               1.0, 0.0, 1, int(pool), out.data_ptr()), (out,))
+    c.inputs = x, w, b
+    return c
+
+
+def test_first_convs_of_several_sizes():
+    """The image layer over quads of pixels, whose shared memory goes by channels and width."""
+    g = torch.Generator().manual_seed(10)
+    _together([_first_conv(g, 3, 64, 32), _first_conv(g, 1, 16, 16), _first_conv(g, 2, 64, 32),
+               _first_conv(g, 1, 32, 32)])
+
+
+def test_first_convs_of_bands_of_several_sizes():
+    """Over bands of rows, with weights that a quad's shared memory does not hold."""
+    g = torch.Generator().manual_seed(12)
+    _together([_first_conv(g, 16, 128, 32), _first_conv(g, 14, 128, 8), _first_conv(g, 16, 128, 64),
+               _first_conv(g, 15, 128, 16)])
+
+
+def test_pooled_first_convs_of_several_sizes():
+    g = torch.Generator().manual_seed(13)
+    _together([_first_conv(g, 3, 64, 32, True), _first_conv(g, 1, 16, 16, True),
+               _first_conv(g, 8, 64, 16, True), _first_conv(g, 2, 32, 16, True)])

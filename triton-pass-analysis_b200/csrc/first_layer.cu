@@ -343,6 +343,11 @@ __global__ void __launch_bounds__(QUAD_THREADS, DIRECT ? 4 : 3) first_conv_quad_
     }
 }
 
+// Most shared memory of a launch.  The kernels are allowed this much whatever a call asks for:
+// the setting is the kernel's, and a call's own size there could take it from another host
+// thread's larger launch.
+constexpr int SMEM_MAX = 200 * 1024, QUAD_SMEM_MAX = 64 * 1024;
+
 }  // namespace
 }  // namespace snnb
 
@@ -361,7 +366,7 @@ extern "C" int snnb_first_conv_lif(const float* x, int64_t Ti, int64_t T, int64_
     const int CG = (!pool && Cout % 64 == 0) ? 64 : 16;
     if (pool && ((H % 2) || (W % 2))) return SNNB_ERR_UNSUPPORTED;
     const int64_t smem = Cin * 9 * Cout * 4;
-    if (smem > 200 * 1024) return SNNB_ERR_UNSUPPORTED;
+    if (smem > SMEM_MAX) return SNNB_ERR_UNSUPPORTED;
     if (T * B * Cin * H * W > ((int64_t)1 << 40) || T > 0x7fffffff) return SNNB_ERR_ARG;
     const int Ho = pool ? (int)H / 2 : (int)H, Wo = pool ? (int)W / 2 : (int)W;
     const int64_t total = B * Ho * Wo * (Cout / CG);
@@ -375,10 +380,10 @@ extern "C" int snnb_first_conv_lif(const float* x, int64_t Ti, int64_t T, int64_
         const int R = per_row <= QUAD_THREADS ? QUAD_THREADS / per_row : 0;
         const int64_t nblk = B * ((H + (R ? R : 1) - 1) / (R ? R : 1));
         const int64_t qsmem = (9 * Cin * Cout + Cout + 2 * Cin * (R + 2) * (W + 2)) * 4;
-        if (R >= 1 && nblk <= 0x7fffffffll && qsmem <= 64 * 1024) {
+        if (R >= 1 && nblk <= 0x7fffffffll && qsmem <= QUAD_SMEM_MAX) {
             auto quad = [&](auto kernel) -> int {
                 cudaError_t e = cudaFuncSetAttribute(
-                    kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)qsmem);
+                    kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, QUAD_SMEM_MAX);
                 if (e != cudaSuccess) return record_cuda_error(e);
                 return launch_k(kernel, dim3((unsigned)nblk), dim3(QUAD_THREADS), qsmem, s, x,
                                 (int)Ti, (int)T, (int)B, (int)Cin, (int)H, (int)W, R, w, bias,
@@ -396,11 +401,11 @@ extern "C" int snnb_first_conv_lif(const float* x, int64_t Ti, int64_t T, int64_
         const int R = 128 / (int)W;
         const int64_t nblk = B * ((H + R - 1) / R);
         const int64_t bsmem = (9 * Cin * Cout + Cout + Cin * (R + 2) * (W + 2)) * 4;
-        if (nblk <= 0x7fffffffll && bsmem <= 200 * 1024) {
+        if (nblk <= 0x7fffffffll && bsmem <= SMEM_MAX) {
             const int threads = 128 * (int)(Cout / BAND_CG);
             auto band = [&](auto kernel) -> int {
                 cudaError_t e = cudaFuncSetAttribute(
-                    kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bsmem);
+                    kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
                 if (e != cudaSuccess) return record_cuda_error(e);
                 return launch_k(kernel, dim3((unsigned)nblk), dim3(threads), bsmem, s, x, (int)Ti,
                                 (int)T, (int)B, (int)Cin, (int)H, (int)W, w, bias, (int)Cout,
@@ -412,7 +417,7 @@ extern "C" int snnb_first_conv_lif(const float* x, int64_t Ti, int64_t T, int64_
     }
     auto run = [&](auto kernel) -> int {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int)smem);
+                                             SMEM_MAX);
         if (e != cudaSuccess) return record_cuda_error(e);
         return launch_k(kernel, dim3((unsigned)blocks), dim3(THREADS), smem, s, x, (int)Ti, (int)T,
                         (int)B, (int)Cin, (int)H, (int)W, w, bias, (int)Cout, decay, input_scale,
