@@ -134,3 +134,21 @@ def test_pooled_first_convs_of_several_sizes():
     g = torch.Generator().manual_seed(13)
     _together([_first_conv(g, 3, 64, 32, True), _first_conv(g, 1, 16, 16, True),
                _first_conv(g, 8, 64, 16, True), _first_conv(g, 2, 32, 16, True)])
+
+
+def test_band_convs_of_several_sizes():
+    """Row-band convolutions of 64 and 128 input channels over rows of 8 and 32 pixels."""
+    g = torch.Generator().manual_seed(11)
+
+    def case(cin, W, variant):
+        T, B = 4, 2
+        x = (torch.rand(T, B, W, W, cin, generator=g) < 0.2).to(torch.bfloat16).to(DEV)
+        w = (torch.randn(64, 3, 3, cin, generator=g) * 0.06).to(torch.bfloat16).to(DEV)
+        b = (torch.rand(64, generator=g) * 0.9).to(DEV)
+        out = torch.empty(T, B, W, W, 64, device=DEV, dtype=torch.bfloat16)
+        c = _Case("snnb_conv3x3_lif",
+                  (x.data_ptr(), T, B, W, W, cin, w.data_ptr(), b.data_ptr(), 64, 0.5, 0.5, 1.0,
+                   0.0, 1, 0, variant, 32, 1, None, 0, out.data_ptr()), (out,))
+        c.inputs = x, w, b
+        return c
+    _together([case(64, 8, 3), case(128, 32, 3), case(64, 8, 7), case(128, 32, 7)])

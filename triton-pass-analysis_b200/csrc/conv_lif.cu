@@ -1013,10 +1013,12 @@ int sm_count() {
 
 namespace {
 
+// allowed: the most shared memory of any of the kernel's launches.  The setting is the kernel's:
+// a call's own size there could take it from another host thread's larger launch.
 template <typename K>
 int launch_persistent(K kernel, int smem, const CUtensorMap& ta, const CUtensorMap& tb,
-                      const ConvParams& p, cudaStream_t s, int threads = THREADS) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+                      const ConvParams& p, cudaStream_t s, int threads, int allowed) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, allowed);
     if (e != cudaSuccess) return record_cuda_error(e);
     int occ = 0;
     e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kernel, threads, smem);
@@ -1026,6 +1028,13 @@ int launch_persistent(K kernel, int smem, const CUtensorMap& ta, const CUtensorM
     const int64_t items = (int64_t)p.num_tiles * (p.splits > 1 ? p.splits : 1);
     const int grid = (int)(items < cap ? items : cap);
     return launch_k(kernel, dim3(grid), dim3(threads), smem, s, ta, tb, p);
+}
+
+// The same for a kernel whose launches all have the same size.
+template <typename K>
+int launch_persistent(K kernel, int smem, const CUtensorMap& ta, const CUtensorMap& tb,
+                      const ConvParams& p, cudaStream_t s, int threads = THREADS) {
+    return launch_persistent(kernel, smem, ta, tb, p, s, threads, smem);
 }
 
 // Persistent launch of a CTA-pair kernel: clusters of 2, as many as can be resident at
@@ -1296,18 +1305,19 @@ int run_band_layer(const void* x, int T, int B, int H, int W, int Cin, const voi
     p.ring = ring; p.a_bytes = a_bytes; p.w_bytes = w_bytes;
     const int dyn = BN == 64 ? SmemBand<64>::dyn_bytes(w_bytes, ring, a_bytes, copies)
                              : SmemBand<32>::dyn_bytes(w_bytes, ring, a_bytes, copies);
+    const int most = smem_optin();
     if (xs) {
         if (BN == 64)
-            return hard ? launch_persistent(conv_lif_band_kernel<64, true, true>, dyn, ta, tb, p, s, BAND_THREADS)
-                        : launch_persistent(conv_lif_band_kernel<64, false, true>, dyn, ta, tb, p, s, BAND_THREADS);
-        return hard ? launch_persistent(conv_lif_band_kernel<32, true, true>, dyn, ta, tb, p, s, BAND_THREADS)
-                    : launch_persistent(conv_lif_band_kernel<32, false, true>, dyn, ta, tb, p, s, BAND_THREADS);
+            return hard ? launch_persistent(conv_lif_band_kernel<64, true, true>, dyn, ta, tb, p, s, BAND_THREADS, most)
+                        : launch_persistent(conv_lif_band_kernel<64, false, true>, dyn, ta, tb, p, s, BAND_THREADS, most);
+        return hard ? launch_persistent(conv_lif_band_kernel<32, true, true>, dyn, ta, tb, p, s, BAND_THREADS, most)
+                    : launch_persistent(conv_lif_band_kernel<32, false, true>, dyn, ta, tb, p, s, BAND_THREADS, most);
     }
     if (BN == 64)
-        return hard ? launch_persistent(conv_lif_band_kernel<64, true, false>, dyn, ta, tb, p, s, BAND_THREADS)
-                    : launch_persistent(conv_lif_band_kernel<64, false, false>, dyn, ta, tb, p, s, BAND_THREADS);
-    return hard ? launch_persistent(conv_lif_band_kernel<32, true, false>, dyn, ta, tb, p, s, BAND_THREADS)
-                : launch_persistent(conv_lif_band_kernel<32, false, false>, dyn, ta, tb, p, s, BAND_THREADS);
+        return hard ? launch_persistent(conv_lif_band_kernel<64, true, false>, dyn, ta, tb, p, s, BAND_THREADS, most)
+                    : launch_persistent(conv_lif_band_kernel<64, false, false>, dyn, ta, tb, p, s, BAND_THREADS, most);
+    return hard ? launch_persistent(conv_lif_band_kernel<32, true, false>, dyn, ta, tb, p, s, BAND_THREADS, most)
+                : launch_persistent(conv_lif_band_kernel<32, false, false>, dyn, ta, tb, p, s, BAND_THREADS, most);
 }
 
 // Bytes of the split-K partial sums, splits * T * B * H * W * Cout float32 values, or -1
