@@ -662,3 +662,27 @@ def test_spiking_mlp_block():
     y2, h2 = block(y, h)
     assert torch.equal(h2, (x.float() + y.float()).to(torch.bfloat16))
     assert torch.isfinite(y2.float()).all()
+
+
+# every form of the packed ring: one tile of 16, 32, 64 and 128 tokens with K split, pairs of 128
+# tokens (few tiles; short K) and of 256
+@pytest.mark.parametrize("rows,N,K", [(1, 512, 8100), (20, 640, 4000), (60, 1001, 4050),
+                                      (128, 256, 4016), (300, 1000, 1100),
+                                      (2000, 4000, 416), (2000, 3000, 1100), (1300, 4097, 2500)])
+def test_linear_forms_of_the_packed_ring_repeated(rows, N, K):
+    """Weights placed by warps, of which one CTA of a pair reads the other's: every repetition
+    gives the first one's bits, and those are the oracle's within the bound."""
+    mx = _mx()
+    assert -(-K // 32) % 4, "rows of whole groups of 128 are unpacked by the copies instead"
+    g = _gen(K + rows)
+    a = mx.mx_quantize(torch.randn(rows, K, generator=g).to(DEV), "mxfp8")
+    ws = [mx.mx_quantize(torch.randn(N, K, generator=g).to(DEV)) for _ in range(3)]
+    first = [mx.mx_linear(a, w, dtype=torch.float32) for w in ws]
+    va = torch.from_numpy(OM.values(*_held(a), "mxfp8")[:, :K]).to(DEV)
+    for w, out in zip(ws, first):
+        vw = torch.from_numpy(OM.values(*_held(w), "mxfp4")[:, :K]).to(DEV)
+        tol = (2 * K / 32 + 16) * 2.0 ** -23 * (va.abs() @ vw.abs().t()) + 2.0 ** -24 * (va @ vw.t()).abs()
+        assert ((out.double() - va @ vw.t()).abs() <= tol).all()
+    for _ in range(200):
+        for w, out in zip(ws, first):
+            assert torch.equal(mx.mx_linear(a, w, dtype=torch.float32), out)

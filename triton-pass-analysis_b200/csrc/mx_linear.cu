@@ -96,11 +96,10 @@ __device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* tm, uin
     if constexpr (PAIR) tc::tma_load_3d_pair(dst, tm, bar, c0, c1, c2);
     else tc::tma_load_3d(dst, tm, bar, c0, c1, c2);
 }
-// Arrival on a barrier of the pair's even CTA, relaxed: no data crosses the CTAs with it.  It
-// reports TMEM reads that have completed (tcgen05.wait::ld, fence::before_thread_sync), or
-// weight pieces that fence.proxy.async has completed in this SM's own shared memory, where the
-// tensor core reads them.  A release at cluster scope would wait for every earlier write of the
-// SM instead (~1900 cycles, where a stage takes 540).
+// Arrival on a barrier of the pair's even CTA, relaxed: it reports TMEM reads that have completed
+// (tcgen05.wait::ld, fence::before_thread_sync) and no data in memory crosses the CTAs with it.  A
+// release at cluster scope would wait for every earlier write of the SM instead (~1900 cycles,
+// where a stage takes 540), the epilogue's stores among them.
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
                  : "memory");
@@ -454,7 +453,11 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
         };
         auto wait_full = [&](uint32_t it) {
             const uint32_t bar = full_bar((int)(it % STAGES)), ph = (it / STAGES) & 1u;
-            failed |= 1u - tc::mbar_wait_lane(bar, ph, failed);
+            // the odd CTA's warps arrive here as well once they have placed weight pieces
+            if constexpr (PAIR && PACKED_STAGES > 0)
+                failed |= 1u - tc::mbar_wait_lane_cluster(bar, ph, failed);
+            else
+                failed |= 1u - tc::mbar_wait_lane(bar, ph, failed);
             tc::tc_fence_after();
         };
         if (crank == 0) {
@@ -590,7 +593,12 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
                 __syncwarp();
                 if (lane == 0) {
                     tc::mbar_arrive(pempty_bar(ps));
-                    if (crank) mbar_arrive_cluster_relaxed(tc::map_to_rank(full_bar(s), 0));
+                    // the even CTA's thread issues the MMA that reads the odd CTA's pieces: the
+                    // one thing that orders it after their stores is a release at cluster scope.
+                    // (It costs 4096 x 8192 x 4000 128 us against 111 with a relaxed arrival, 2300
+                    // x 2304 x 1100 16.4 against 14.5, 6523 x 4000 x 32 24.0 against 22.0; tiles of
+                    // one CTA, which need none, take 215, 21.9 and 57.)
+                    if (crank) tc::mbar_arrive_cluster(tc::map_to_rank(full_bar(s), 0));
                     else tc::mbar_arrive(full_bar(s));
                 }
             }

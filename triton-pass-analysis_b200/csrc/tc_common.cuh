@@ -431,6 +431,36 @@ __device__ __forceinline__ uint32_t mbar_wait_warp_cluster(uint32_t bar, uint32_
         : "memory");
     return ok;
 }
+// mbar_wait_lane with cluster-scope acquire, for the same kind of barrier.
+__device__ __forceinline__ uint32_t mbar_wait_lane_cluster(uint32_t bar, uint32_t parity,
+                                                           uint32_t skip) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .u64 t0, t1, lim;\n\t"
+        "setp.ne.u32 q, %3, 0;\n\t"
+        "@q bra DFAIL_%=;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "@p bra DOK_%=;\n\t"
+        "ld.volatile.u64 lim, [%4];\n\t"
+        "mov.u64 t0, %%clock64;\n\t"
+        "DLOOP_%=:\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "@p bra DOK_%=;\n\t"
+        "mov.u64 t1, %%clock64;\n\t"
+        "sub.u64 t1, t1, t0;\n\t"
+        "setp.lt.u64 q, t1, lim;\n\t"
+        "@q bra DLOOP_%=;\n\t"
+        "DFAIL_%=:\n\t"
+        "mov.u32 %0, 0;\n\t"
+        "bra.uni DEND_%=;\n\t"
+        "DOK_%=:\n\t"
+        "mov.u32 %0, 1;\n\t"
+        "DEND_%=:\n\t}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(skip), "l"(&g_wait_limit)
+        : "memory");
+    return ok;
+}
 // Tiled loads into this CTA's shared memory whose completion bytes are counted on the
 // mbarrier at `bar` (a shared::cluster address: the pair's even CTA); no multicast.
 __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* tm, uint32_t bar,
