@@ -200,3 +200,39 @@ def test_c_entries_reject_bad_arguments_without_a_device():
                 dict(data=None), dict(scales=None), dict(x=odd), dict(r=odd), dict(h=odd),
                 dict(w=odd), dict(data=by8), dict(ldx=-1), dict(ldr=-1), dict(rows=1 << 31)):
         assert n(**bad) == -1, bad
+
+
+@pytest.mark.parametrize("step", [0, 1])
+def test_another_thread_reads_a_tensor_while_it_is_split(monkeypatch, step):
+    """Codes and scales of one allocation become two tensors at their first use.  Whichever step of
+    that another thread's read falls on, it sees whole codes and whole scales."""
+    import threading
+    mx = _mx()
+    rows, K = 130, 200
+    sizes, scales_shape = mx._BLOCK_BYTES, mx.mx_scales_shape(rows, K)
+    t = mx.MXTensor._new(torch.empty(0), rows, (rows, K), "mxfp4", 0)
+    main, steps, seen = threading.current_thread(), [], []
+
+    def read():
+        try:
+            seen.append((tuple(t.data.shape), tuple(t.scales.shape)))
+        except Exception as e:                     # reported by the main thread
+            seen.append(repr(e))
+
+    def pause():
+        if threading.current_thread() is main:
+            steps.append(1)
+            if len(steps) == step + 1:
+                other = threading.Thread(target=read)
+                other.start()
+                other.join()
+
+    class Sizes:
+        def __getitem__(self, i):
+            pause()
+            return sizes[i]
+    monkeypatch.setattr(mx, "_BLOCK_BYTES", Sizes())
+    monkeypatch.setattr(mx, "mx_scales_shape", lambda *a: (pause(), scales_shape)[1])
+    whole = ((rows, 7 * 16), scales_shape)
+    assert (tuple(t.data.shape), tuple(t.scales.shape)) == whole
+    assert seen == [whole]

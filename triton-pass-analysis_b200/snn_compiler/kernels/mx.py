@@ -50,7 +50,9 @@ class MXTensor:
     [rows, 32 ceil(K/32)] (mxfp8), scales uint8 of mx_scales_shape(rows, K).  Elements past K and
     scale bytes that no block owns are zero."""
 
-    __slots__ = ("shape", "fmt", "rows", "_code", "_data", "_scales", "_size")
+    # _data holds the codes, or codes and scales in one allocation (_size: where the scales start,
+    # -1 where they lie apart); _parts the two as tensors, once they are known
+    __slots__ = ("shape", "fmt", "rows", "_code", "_data", "_size", "_parts")
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor, shape, fmt: str):
         code = _fmt(fmt)
@@ -66,7 +68,7 @@ class MXTensor:
             scales.numel() == (rows + 127) // 128 * ((nb + 3) // 4) * 512, \
             (tuple(scales.shape), tuple(shape))
         self.shape, self.fmt, self.rows = tuple(shape), fmt, rows
-        self._code, self._data, self._scales, self._size = code, data, scales, 0
+        self._code, self._data, self._size, self._parts = code, data, -1, (data, scales)
 
     @classmethod
     def _new(cls, like: torch.Tensor, rows: int, shape, fmt: str, code: int):
@@ -77,20 +79,23 @@ class MXTensor:
         buf = like.new_empty(size + (rows + 127) // 128 * ((nb + 3) // 4) * 512,
                              dtype=torch.uint8)
         self.shape, self.fmt, self.rows = shape, fmt, rows
-        self._code, self._data, self._scales, self._size = code, buf, None, size
+        self._code, self._data, self._size, self._parts = code, buf, size, None
         return self
 
     def _pointers(self):
         """Addresses of the codes and the scales."""
         p = self._data.data_ptr()
-        return p, p + self._size if self._scales is None else self._scales.data_ptr()
+        return p, p + self._size if self._size >= 0 else self._parts[1].data_ptr()
 
     def _split(self):
-        """The one allocation of _new as two tensors."""
-        if self._scales is None:
+        """Codes and scales as two tensors.  Set together: other threads see both or neither."""
+        parts = self._parts
+        if parts is None:
             buf, size, K = self._data, self._size, self.shape[-1]
-            self._scales = buf[size:].view(mx_scales_shape(self.rows, K))
-            self._data = buf[:size].view(self.rows, (K + 31) // 32 * _BLOCK_BYTES[self._code])
+            scales = buf[size:].view(mx_scales_shape(self.rows, K))
+            data = buf[:size].view(self.rows, (K + 31) // 32 * _BLOCK_BYTES[self._code])
+            parts = self._parts = (data, scales)
+        return parts
 
     @property
     def device(self) -> torch.device:
@@ -98,13 +103,11 @@ class MXTensor:
 
     @property
     def data(self) -> torch.Tensor:
-        self._split()
-        return self._data
+        return self._split()[0]
 
     @property
     def scales(self) -> torch.Tensor:
-        self._split()
-        return self._scales
+        return self._split()[1]
 
     @classmethod
     def from_rows(cls, data: torch.Tensor, row_scales: torch.Tensor, K: int, fmt: str):
