@@ -589,7 +589,9 @@ int snnb_set_wait_limit(int64_t cycles);
  *   snnb_debug_inject_stall(count): in the next `count` launches of the T-sequential conv
  *     kernel (snnb_conv3x3_lif variant 1), the producer warp of CTA 0 withholds every
  *     stage; that CTA's MMA warp then waits until the wait limit runs out and the launch
- *     reports SNNB_ERR_TIMEOUT (CTA 0's output is left unspecified).
+ *     reports SNNB_ERR_TIMEOUT (CTA 0's output is left unspecified).  Launches of
+ *     snnb_rms_norm_mx's ring kernel (many rows of more than 1024 values) count as well: there
+ *     block 0 never fetches its teams' second rows.
  * Both are process-wide; count 0 cancels.
  */
 int snnb_debug_inject_status(int status, int count);

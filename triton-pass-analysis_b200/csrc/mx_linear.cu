@@ -616,15 +616,17 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
     if (__syncthreads_or((int)failed)) {
         // copies still in flight land before the CTA may exit: waits on the full barrier, or for
         // the odd CTA of a pair (whose copies complete the even CTA's) on the stage's release,
-        // with the limit that outlasts any copy
+        // with the limit that outlasts any copy.  The newest copy first: once that limit has run
+        // out, which it does where a stage is never handed on, it has done so for the older ones.
         if (warp < NP) {
             const bool own_ring = S::PACKED > 0 && warp == 3;
             const uint32_t ring = own_ring ? PACKED_STAGES : STAGES;
             for (uint32_t k = 0; k < issued && k < ring; ++k) {
                 const uint32_t g = issued - 1 - k;
                 const int s = (int)(g % ring);
-                tc::mbar_wait_warp<true>(own_ring ? pfull_bar(s) : crank ? empty_bar(s) : full_bar(s),
-                                         (g / ring) & 1u, 0);
+                if (!tc::mbar_wait_warp<true>(own_ring ? pfull_bar(s) : crank ? empty_bar(s) : full_bar(s),
+                                              (g / ring) & 1u, 0))
+                    break;
             }
         }
         __syncthreads();

@@ -31,6 +31,7 @@ struct NormParams {
     uint8_t* data;
     uint32_t* scales;
     int* status;
+    int stall;                   // test hook: the ring kernel's block 0 never fetches its second rows
 };
 
 __device__ __forceinline__ void add8(float (&a)[8], const float (&b)[8]) {
@@ -343,7 +344,8 @@ rms_norm_mx_ring_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __r
     };
     if (t == 0)
         for (int s = 0; s < stages; ++s)
-            if (row0 + (uint64_t)s * step < p.rows) fetch(row0 + s * step, s);
+            if (row0 + (uint64_t)s * step < p.rows && !(p.stall && blockIdx.x == 0 && s == 1))
+                fetch(row0 + s * step, s);
     mx::Raw8<W> w[RING_CHUNKS];
 #pragma unroll
     for (int c = 0; c < RING_CHUNKS; ++c) w[c] = weights8<W>(p, weight, (c * LANES + t) * 8);
@@ -353,13 +355,14 @@ rms_norm_mx_ring_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __r
     for (uint64_t row64 = row0; row64 < p.rows; row64 += step, odd ^= 1) {
         const uint32_t row = (uint32_t)row64;
         if (!failed && !tc::mbar_wait_warp(bars + 8 * s, parity, 0)) {
-            // a wait ran out: this warp works on and stores nothing; the copies in flight land
-            // before the block may exit
+            // a wait ran out: this warp works on and stores nothing.  The copies in flight, all of
+            // them by the team's first warp, land before the block may exit; a wait of that limit
+            // that runs out has outlasted those behind it as well
             failed = 1;
             int fs = s;
             uint32_t fp = parity;
-            for (int i = 0; i < stages; ++i) {
-                if (row64 + (uint64_t)i * step < p.rows) tc::mbar_wait_warp<true>(bars + 8 * fs, fp, 0);
+            for (int i = 0; t < 32 && i < stages && row64 + (uint64_t)i * step < p.rows; ++i) {
+                if (!tc::mbar_wait_warp<true>(bars + 8 * fs, fp, 0)) break;
                 if (++fs == stages) {
                     fs = 0;
                     fp ^= 1;
@@ -457,7 +460,7 @@ int allow_ring(Kernel k, bool (&ready)[64]) {
 }
 
 template <typename T, typename W, int LANES>
-int launch_ring(const NormArgs& a, const NormParams& p) {
+int launch_ring(const NormArgs& a, NormParams p) {
     constexpr uint32_t THREADS = ring_threads(LANES), TEAMS = THREADS / LANES;
     constexpr uint32_t BLOCKS = ring_blocks<T, W>(LANES);
     const uint32_t half = (p.K * (uint32_t)sizeof(T) + 127) / 128 * 128;
@@ -477,6 +480,7 @@ int launch_ring(const NormArgs& a, const NormParams& p) {
     const int rc = allow_ring(k, ready[(a.r ? 2 : 0) + full]);
     if (rc != SNNB_OK) return rc;
     const uint32_t need = (p.rows + TEAMS - 1) / TEAMS, most = 148u * per_sm;
+    p.stall = take_injected_stall();
     return launch_k(k, dim3(need < most ? need : most), dim3(THREADS), smem, a.s,
                     static_cast<const T*>(a.x), static_cast<const T*>(a.r), static_cast<T*>(a.h),
                     static_cast<const W*>(a.weight), p, (int)stages, half);
