@@ -668,7 +668,8 @@ def test_spiking_mlp_block():
 # tokens (few tiles; short K) and of 256
 @pytest.mark.parametrize("rows,N,K", [(1, 512, 8100), (20, 640, 4000), (60, 1001, 4050),
                                       (128, 256, 4016), (300, 1000, 1100),
-                                      (2000, 4000, 416), (2000, 3000, 1100), (1300, 4097, 2500)])
+                                      (2000, 4000, 416), (2000, 3000, 1100), (1300, 4097, 2500),
+                                      (256, 2304, 4000)])
 def test_linear_forms_of_the_packed_ring_repeated(rows, N, K):
     """Weights placed by warps, of which one CTA of a pair reads the other's: every repetition
     gives the first one's bits, and those are the oracle's within the bound."""

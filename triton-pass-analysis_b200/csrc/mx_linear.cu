@@ -771,11 +771,11 @@ int pick_mx(const void* a, const void* as, const void* w, const void* ws, int64_
         // One round that leaves SMs idle over a long K: split K instead (200 x 512 x 16384 in 4
         // bits: 8.5 us against 20; 1024 x 1024 x 1024: 10 against 4.4).  Only 2 ways fit: from 24
         // stages (256 x 2304 x 8192: 10.1 against 11.8; x 4096: 8.1 against 7.5; 512 x 2048 x
-        // 5632 with tokens in 8 bits: 11.5 against 14.2; x 2048: 8.2 against 7.3), with a packed
-        // ring from 48 (256 x 2304 x 4000, 32 stages: 14.0 against 12.8).
+        // 5632 with tokens in 8 bits: 11.5 against 14.2; x 2048: 8.2 against 7.3; with a packed
+        // ring 256 x 2304 x 4000: 14.3 against 17.4; x 1936: 11.5 against 10.9).
         if (nstages >= 12) {
             const int rc = launch_mx<FMT, 128, P ? 4 : 6, false, P ? 8 : 0>(
-                a, as, w, ws, K, p, s, nstages >= (P ? 48 : 24) ? 2 : 4);
+                a, as, w, ws, K, p, s, nstages >= 24 ? 2 : 4);
             if (rc != SNNB_ERR_UNSUPPORTED) return rc;
         }
         return launch_mx<FMT, 128, P ? 6 : 7, true, P ? 6 : 0>(a, as, w, ws, K, p, s);
