@@ -545,6 +545,9 @@ int snnb_mx_dequantize(const void* data, const void* scales, int fmt, int64_t ro
 /*
  * out [rows, N] = a [rows, K] * w [N, K]^T + bias: a of a_fmt, w of SNNB_MXFP4, both as above;
  * bias [N] float32 or NULL; float32 sums, rounded once to out_dtype (F32 / F16 / BF16).
+ * Here and in snnb_rms_norm_mx a bounded wait that gives up leaves the outputs unspecified and
+ * SNNB_ERR_TIMEOUT in the device status word (snnb_read_device_status); the call has returned by
+ * then.
  */
 int snnb_mx_linear(const void* a, const void* a_scales, int a_fmt, int64_t rows, int64_t K,
                    const void* w, const void* w_scales, int64_t N, const float* bias, void* out,

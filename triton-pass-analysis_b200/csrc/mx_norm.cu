@@ -3,19 +3,24 @@
 //   y = (h / sqrt(mean(h^2) + eps)) * weight
 //   codes, scales = y in E2M1 or E4M3, one scale per 32 values
 //
-// Rounding.  The norm is taken of the unrounded sum h.  An error of one float32 ulp (6e-8) in y
+// Rounding.  The norm is taken of the float32 h, before it is rounded to x's type.  An error of one float32 ulp (6e-8) in y
 // already moves ~7e-7 of the codes to a neighbour, so the squares are summed and 1 / sqrt is
 // taken in float64.  y itself is float32 unless it lies within 4 ulp of a value that a code
 // boundary could be (its low 19 bits zero: 3 mantissa bits and the half step), where it is formed
 // again in float64 and rounded to odd, which keeps it on its side of the boundary.
 //
-// Two forms.  Many aligned rows: a team of LANES threads walks rows, whose x and residual come
-// by bulk copies into a ring in shared memory while earlier rows are worked on; both passes over
-// a row (squares, output) read it there.  Few rows, unaligned rows or rows too long for the ring:
-// a row's values stay in registers between the passes (or are read twice past 1024 threads x 32).
-// Four neighbouring lanes hold one block of 32, as in the quantisation kernel.
+// Two forms.  Many aligned rows of more than 1024 values: a team of LANES threads walks rows, whose
+// x and residual come by bulk copies into a ring in shared memory while earlier rows are worked on.
+// Others: teams of one row each, straight from memory.  In both a row's values stay in registers
+// between the passes (squares, output); only rows that a team cannot hold are read twice: past 8192
+// values where the aligned rows are few, past 16384 (aligned float32 with a residual: 12800)
+// elsewhere.  Four neighbouring lanes hold one block of 32, as in the quantisation kernel.
 //
-// Bound: HBM for many rows; for few, the latency of one load, one sum over the block, one store.
+// Bound: HBM for many wide aligned rows (16384 x 8192 bf16 with residual 165 us, 5.7 TB/s); for few
+// rows the latency of one load, one sum over the block, one store.  Short rows (12544 x 384: 12.3
+// us, 2.7 TB/s) wait for loads, as nothing is in flight while a team sums and stores; unaligned
+// ones (8192 x 4096 at odd starts: 83 us, 2.8 TB/s) take 55% of the issue slots besides, for the
+// shifts.
 #include "mx.cuh"
 #include "tc_common.cuh"
 

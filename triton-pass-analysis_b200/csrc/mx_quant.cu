@@ -10,7 +10,9 @@
 // rows fill a warp as well as long ones do.  Others: a warp takes 256 consecutive values of one
 // row, through aligned loads (or stores) around them that it shifts into place.
 //
-// Bound: HBM.  Every value is read once, its code written once; nothing is read again.
+// Bound: HBM for aligned rows: every value is read once, its code written once.  Unaligned ones
+// (8192 x 4099 bf16 -> E2M1: 26 us, 3.3 TB/s; back 29) are bound by instructions: the shifts leave
+// two thirds of the issue slots taken and the integer pipe full.
 #include "mx.cuh"
 
 namespace snnb {
@@ -20,8 +22,8 @@ constexpr int Q_THREADS = 256;
 
 // A thread block takes U x 64 consecutive blocks of 32 (or U x 8 row pieces of 256), so that a
 // thread has U loads in flight, and ends: with blocks resident for the whole launch that stride
-// through the tensor, 16384 x 8192 bf16 took 69 us (E2M1; 63 in this form) and 68 back (56).
-// U is 4 (2 for row pieces), or 1 for tensors too small to give every SM four blocks of those.
+// through the tensor, 16384 x 8192 bf16 took 69 us (E2M1; 63 in this form) and 68 back (52).
+// U is 4 (2 for row pieces), or 1 for tensors too small for four (eight) such blocks an SM.
 
 // FLAT: K % 128 == 0 and contiguous rows, so values and codes lie at their block's index.
 template <typename T, int FMT, int U, bool FLAT>
@@ -218,7 +220,8 @@ mx_dequantize_any_kernel(const uint8_t* __restrict__ data, const uint8_t* __rest
     }
 }
 
-// Whether U = 1: `units` (per thread block and unit of U: `per`) do not fill four blocks an SM.
+// Whether U = 1: `units` (per thread block and unit of U: `per`) do not fill four blocks an SM at U
+// = 4, eight at U = 2.
 bool small(int64_t units, int64_t per) { return units <= 148 * 4 * 4 * per; }
 // Lanes a piece of an unaligned row: what short rows fill (63025 x 34 bf16 -> E2M1: 5.0 us, 13.2
 // with 32; 27336 x 113: 4.6, 6.6; 27997 x 344: 9.0, 12.2), 32 beyond (3000 x 16001: 34 us, 37

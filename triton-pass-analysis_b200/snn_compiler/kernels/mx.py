@@ -10,7 +10,9 @@ Spikes {0, 1} are exact in either.
   mx_linear(a, w, bias, dtype=...) -> tensor             a w^T + bias, float32 sums, w in mxfp4
   rms_norm_mx(x, weight, residual, ...) -> MXTensor, h   norm of h = x + residual, quantised
 
-Each call is one launch of libsnnb200.so on the current stream of its input's device.
+Each call is one launch of libsnnb200.so on the current stream of its input's device.  Waits inside
+mx_linear and rms_norm_mx are bounded: one that gives up leaves the output unspecified and is
+reported by the device status word (kernels.conv.raise_on_device_status), not by the call.
 """
 from __future__ import annotations
 
@@ -199,7 +201,8 @@ def mx_quantize(x: torch.Tensor, fmt: str = "mxfp4") -> MXTensor:
 
 
 def mx_dequantize(t: MXTensor, dtype=torch.bfloat16) -> torch.Tensor:
-    """The values that t's codes stand for, rounded once to dtype (bfloat16 holds them all)."""
+    """The values that t's codes stand for, rounded once to dtype (bfloat16 holds them all but some
+    of E4M3's under the scale bytes 0 to 2, which lie below its smallest)."""
     dt = _dtype(dtype)
     index = _index(t._data)
     out = t._data.new_empty(t.shape, dtype=dtype)
