@@ -564,6 +564,70 @@ int snnb_rms_norm_mx(const void* x, int64_t ldx, const void* residual, int64_t l
                      int fmt, void* data, void* scales, void* h_out, snnb_stream_t stream);
 
 /*
+ * Operators of a causal linear-attention block (no counterpart in the reference, whose spiking
+ * attention has neither positions nor a causal order).  Strides are in elements, columns have
+ * unit stride; host arrays are read before the call returns.
+ *
+ * snnb_rotary_axes: queries [B, N, q_heads, d] and keys [B, N, k_heads, d] (either may have no
+ * heads) turned by positions with several axes.  Pair i < pairs, columns (i, i + pairs), or
+ * (2i, 2i + 1) when interleaved, turns by positions[b, n, axis[i]] * turns[i] whole turns
+ * (backwards when inverse); columns from 2 * pairs on are copied.  q_strides, k_strides (host, 6):
+ * batch, token, head of the input, then of the output, which may be the input itself; positions
+ * int32 (0), int64 (1) or float32 (2) with positions_strides (host, 3): batch, token, axis; turns,
+ * axis (host) [pairs]: frequency / 2 pi, row of positions; pairs <= 256.
+ */
+int snnb_rotary_axes(const void* q, void* q_out, int64_t q_heads, const int64_t* q_strides,
+                     const void* k, void* k_out, int64_t k_heads, const int64_t* k_strides,
+                     int dtype, int64_t B, int64_t N, int64_t d, const void* positions,
+                     int positions_dtype, const int64_t* positions_strides, const double* turns,
+                     const uint8_t* axis, int pairs, int interleaved, int inverse,
+                     snnb_stream_t stream);
+
+/*
+ * Linear attention with a decay for each head, q [B, N, H, dk], k [B, N, Hkv, dk],
+ * v [B, N, Hkv, dv] (query head h reads key head h / (H / Hkv)), dk and dv up to 256:
+ *   S_t = decay[h] S_{t-1} + k_t v_t^T,   out_t = scale q_t S_t
+ * decay [H] float32; state_in (NULL: zero) and state_out (NULL: not wanted) [B, H, dk, dv]
+ * float32, which may be the same; lengths [B] int32 (0) or int64 (1) or NULL: tokens of each
+ * sequence, clamped to [0, N]; rows of `out` [B, N, H, dv] (contiguous) behind them are zero.
+ * q_strides, k_strides, v_strides (host, 3): batch, token, head.  workspace: 16-byte aligned, of
+ * snnb_decay_attention_workspace_bytes (negative: bad sizes; 0: none), for this call alone.
+ */
+int64_t snnb_decay_attention_workspace_bytes(int dtype, int64_t B, int64_t N, int64_t H,
+                                             int64_t dk, int64_t dv);
+int snnb_decay_attention(const void* q, const int64_t* q_strides, const void* k,
+                         const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                         int dtype, int64_t B, int64_t N, int64_t H, int64_t Hkv, int64_t dk,
+                         int64_t dv, const float* decay, float scale, const float* state_in,
+                         const void* lengths, int lengths_dtype, void* out, float* state_out,
+                         void* workspace, int64_t workspace_bytes, snnb_stream_t stream);
+
+/* The same for one token of each sequence: q [B, H, dk], k, v [B, Hkv, d] with strides (host, 2):
+ * batch, head; out [B, H, dv] contiguous; state_out may be state_in. */
+int snnb_decay_attention_step(const void* q, const int64_t* q_strides, const void* k,
+                              const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                              int dtype, int64_t B, int64_t H, int64_t Hkv, int64_t dk, int64_t dv,
+                              const float* decay, float scale, const float* state_in, void* out,
+                              float* state_out, snnb_stream_t stream);
+
+/* activations of snnb_group_norm_act */
+#define SNNB_ACT_NONE 0
+#define SNNB_ACT_SILU 1
+#define SNNB_ACT_RELU 2
+#define SNNB_ACT_GELU 3   /* y * Phi(y), the exact form */
+
+/*
+ * out = act((x - mean) / sqrt(var + eps) * weight + bias) of channels-last x [B, S, C], mean and
+ * biased variance over the S * C / groups values of each group of channels of a sample.  weight
+ * and bias [C] of weight_dtype (x's or F32), either may be NULL; out [B, S, C] contiguous, of x's
+ * type.
+ */
+int snnb_group_norm_act(const void* x, int64_t x_batch_stride, int64_t x_row_stride, int dtype,
+                        int64_t B, int64_t S, int64_t C, int64_t groups, const void* weight,
+                        const void* bias, int weight_dtype, float eps, int act, void* out,
+                        snnb_stream_t stream);
+
+/*
  * Reads and clears the device status word that kernels with bounded waits write
  * (SNNB_ERR_TIMEOUT after a wait gave up).  Synchronises `stream`.
  */

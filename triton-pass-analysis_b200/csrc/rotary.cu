@@ -1,0 +1,130 @@
+// Rotary positions with several axes (time, height, width ...) for queries and keys.
+//
+//   pair i of a head, columns (i, i + R) or (2i, 2i + 1) of its first 2R, turns by the angle
+//   t = positions[axis(i)] * f(i):   (a, b) -> (a cos t - b sin t, a sin t + b cos t)
+//
+// The angle is held in turns: positions are exact in float64, f / 2 pi comes in float64 and the
+// product's whole turns are dropped there, so a far position loses nothing (in float32 a position
+// of 2^20 would be off by 0.06 rad); what remains of it, in [-1/2, 1/2], is exact enough in
+// float32 for the sine and the cosine.
+#include "common.cuh"
+#include "mx.cuh"
+
+namespace snnb {
+namespace {
+
+constexpr int R_THREADS = 256;
+constexpr int MAX_PAIRS = 256;
+
+// The pairs' frequencies and axes, passed by value: a launch holds its own copy.
+struct Ladder {
+    double turns[MAX_PAIRS];       // frequency / 2 pi
+    uint8_t axis[MAX_PAIRS];
+};
+
+struct Heads {                     // [B, N, heads, d], strides in elements, unit column stride
+    const void* in;
+    void* out;
+    int64_t ib, in_, ih, ob, on, oh;
+};
+
+struct Positions {
+    const void* p;
+    int64_t sb, sn, sa;            // strides of batch, token, axis
+    int type;                      // 0 int32, 1 int64, 2 float32
+    __device__ __forceinline__ double at(int64_t b, int64_t n, int a) const {
+        const int64_t i = b * sb + n * sn + a * sa;
+        if (type == 0) return (double)static_cast<const int32_t*>(p)[i];
+        if (type == 1) return (double)static_cast<const int64_t*>(p)[i];
+        return (double)static_cast<const float*>(p)[i];
+    }
+};
+
+// One thread per token and pair (or column that is not turned); it goes through the heads.
+template <typename T>
+__global__ void __launch_bounds__(R_THREADS)
+rotary_kernel(Heads q, Heads k, uint32_t hq, uint32_t hk, uint32_t N, uint32_t units,
+              int64_t total, uint32_t pairs, uint32_t d, int interleaved, int inverse,
+              Positions pos, const __grid_constant__ Ladder ladder) {
+    pdl_wait();
+    pdl_trigger();
+    const int64_t at = (int64_t)blockIdx.x * R_THREADS + threadIdx.x;
+    if (at >= total) return;
+    const int64_t token = at / units;
+    const uint32_t u = (uint32_t)(at - token * units);
+    const int64_t b = token / N, n = token - b * N;
+    const bool turn = u < pairs;
+    const uint32_t c0 = !turn ? u + pairs : interleaved ? 2 * u : u;
+    const uint32_t c1 = !turn ? c0 : interleaved ? 2 * u + 1 : u + pairs;
+    float cs = 1.0f, sn = 0.0f;
+    if (turn) {
+        const double t = pos.at(b, n, ladder.axis[u]) * ladder.turns[u];
+        sincospif(2.0f * (float)(t - rint(t)), &sn, &cs);
+        if (inverse) sn = -sn;
+    }
+    for (uint32_t h = 0; h < hq + hk; ++h) {
+        const Heads& x = h < hq ? q : k;
+        const uint32_t hh = h < hq ? h : h - hq;
+        const T* in = static_cast<const T*>(x.in) + b * x.ib + n * x.in_ + hh * x.ih;
+        T* out = static_cast<T*>(x.out) + b * x.ob + n * x.on + hh * x.oh;
+        const float a0 = to_f32(in[c0]), a1 = to_f32(in[c1]);
+        if (turn) {
+            mx::round_to(a0 * cs - a1 * sn, out + c0);
+            mx::round_to(a0 * sn + a1 * cs, out + c1);
+        } else {
+            out[c0] = in[c0];
+        }
+    }
+}
+
+}  // namespace
+}  // namespace snnb
+
+using namespace snnb;
+
+extern "C" int snnb_rotary_axes(const void* q, void* q_out, int64_t q_heads,
+                                const int64_t* q_strides, const void* k, void* k_out,
+                                int64_t k_heads, const int64_t* k_strides, int dtype, int64_t B,
+                                int64_t N, int64_t d, const void* positions, int positions_dtype,
+                                const int64_t* positions_strides, const double* turns,
+                                const uint8_t* axis, int pairs, int interleaved, int inverse,
+                                snnb_stream_t stream) {
+    if (const int inj = take_injected_status()) return inj;
+    if (dtype != SNNB_F32 && dtype != SNNB_F16 && dtype != SNNB_BF16) return SNNB_ERR_ARG;
+    if (positions_dtype < 0 || positions_dtype > 2) return SNNB_ERR_ARG;
+    if (B < 0 || N < 0 || q_heads < 0 || k_heads < 0 || d < 1 || d > 0x7fffffff) return SNNB_ERR_ARG;
+    if (pairs < 1 || pairs > MAX_PAIRS || 2 * (int64_t)pairs > d) return SNNB_ERR_ARG;
+    if (q_heads > 0x3fffffff || k_heads > 0x3fffffff || N > 0x7fffffff) return SNNB_ERR_ARG;
+    if (B == 0 || N == 0 || q_heads + k_heads == 0) return SNNB_OK;
+    if (!positions || !positions_strides || !turns || !axis) return SNNB_ERR_ARG;
+    if (q_heads && (!q || !q_out || !q_strides)) return SNNB_ERR_ARG;
+    if (k_heads && (!k || !k_out || !k_strides)) return SNNB_ERR_ARG;
+    const int size = dtype == SNNB_F32 ? 4 : 2, psize = positions_dtype == 1 ? 8 : 4;
+    const void* ptrs[4] = {q_heads ? q : nullptr, q_heads ? q_out : nullptr,
+                           k_heads ? k : nullptr, k_heads ? k_out : nullptr};
+    for (const void* p : ptrs)
+        if (reinterpret_cast<uintptr_t>(p) % size) return SNNB_ERR_ARG;
+    if (reinterpret_cast<uintptr_t>(positions) % psize) return SNNB_ERR_ARG;
+    const int64_t units = d - pairs;
+    if (B > (int64_t(1) << 38) / N / units) return SNNB_ERR_ARG;
+    Ladder ladder = {};
+    for (int i = 0; i < pairs; ++i) {
+        ladder.turns[i] = turns[i];
+        ladder.axis[i] = axis[i];
+    }
+    auto heads = [](const void* in, void* out, const int64_t* s) {
+        return s ? Heads{in, out, s[0], s[1], s[2], s[3], s[4], s[5]} : Heads{};
+    };
+    const Heads hq = heads(q, q_out, q_heads ? q_strides : nullptr);
+    const Heads hk = heads(k, k_out, k_heads ? k_strides : nullptr);
+    const Positions pos{positions, positions_strides[0], positions_strides[1],
+                        positions_strides[2], positions_dtype};
+    const int64_t total = B * N * units;
+    auto kernel = dtype == SNNB_F32   ? rotary_kernel<float>
+                  : dtype == SNNB_F16 ? rotary_kernel<__half>
+                                      : rotary_kernel<__nv_bfloat16>;
+    return launch_k(kernel, dim3((unsigned)((total + R_THREADS - 1) / R_THREADS)), dim3(R_THREADS),
+                    0, static_cast<cudaStream_t>(stream), hq, hk, (uint32_t)q_heads,
+                    (uint32_t)k_heads, (uint32_t)N, (uint32_t)units, total, (uint32_t)pairs,
+                    (uint32_t)d, interleaved, inverse, pos, ladder);
+}

@@ -69,6 +69,13 @@ SIGNATURES = {
     "snnb_mx_dequantize": [P, P, I32, I64, I64, P, I32, P],
     "snnb_mx_linear": [P, P, I32, I64, I64, P, P, I64, P, P, I32, P],
     "snnb_rms_norm_mx": [P, I64, P, I64, I32, P, I32, F, I64, I64, I32, P, P, P, P],
+    "snnb_rotary_axes": [P, P, I64, P, P, P, I64, P, I32, I64, I64, I64, P, I32, P, P, P, I32, I32,
+                         I32, P],
+    "snnb_decay_attention_workspace_bytes": [I32, I64, I64, I64, I64, I64],
+    "snnb_decay_attention": [P, P, P, P, P, P, I32, I64, I64, I64, I64, I64, I64, P, F, P, P, I32, P,
+                             P, P, I64, P],
+    "snnb_decay_attention_step": [P, P, P, P, P, P, I32, I64, I64, I64, I64, I64, P, F, P, P, P, P],
+    "snnb_group_norm_act": [P, I64, I64, I32, I64, I64, I64, I64, P, P, I32, F, I32, P, P],
     "snnb_conv3x3_lif_static_scratch": [P, I64, I64, I64, I64, I64, P, P, I64, F, F, F, F, I32,
                                         I32, I32, I32, P, P],
 }
@@ -102,6 +109,7 @@ def lib():
             fn = getattr(L, name)
             fn.argtypes = args
             fn.restype = ctypes.c_int
+        L.snnb_decay_attention_workspace_bytes.restype = ctypes.c_int64
         _lib = L
     return _lib
 
