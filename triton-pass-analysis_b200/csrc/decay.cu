@@ -208,6 +208,7 @@ extern "C" int snnb_decay_attention(const void* q, const int64_t* q_strides, con
     (void)workspace;
     (void)workspace_bytes;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (tc_takes(a, dtype)) return tc_run(a, s);
     if (dtype == SNNB_F32) return run_any<float>(a, s);
     if (dtype == SNNB_F16) return run_any<__half>(a, s);
     return run_any<__nv_bfloat16>(a, s);

@@ -50,5 +50,9 @@ int allow_smem(int bytes) {
     return SNNB_OK;
 }
 
+// The tensor cores' form (decay_tc.cu): whether it takes these arguments, and its launches.
+bool tc_takes(const Args& a, int dtype);
+int tc_run(const Args& a, cudaStream_t s);
+
 }  // namespace decay
 }  // namespace snnb
