@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(G_THREADS) decay_any_kernel(Args a, uint32_t t
     const int64_t b = bh / a.H, h = bh - b * a.H, hk = h / (a.H / a.Hk);
     const int c0 = tile * GV, nv = min(GV, a.dv - c0), t = threadIdx.x;
     const int64_t len = a.length(b);
-    if (t <= GC) pw[t] = power(a.decay[h], t);
+    if (t <= GC) pw[t] = (float)power(a.decay[h], t);
     const float* s_in = a.state_in ? a.state_in + (b * a.H + h) * dk * a.dv + c0 : nullptr;
     for (int i = t; i < dk * GV; i += G_THREADS)
         S[i] = s_in && i % GV < nv ? s_in[(int64_t)(i / GV) * a.dv + i % GV] : 0.0f;
@@ -175,7 +175,7 @@ using namespace snnb;
 extern "C" int64_t snnb_decay_attention_workspace_bytes(int dtype, int64_t B, int64_t N, int64_t H,
                                                         int64_t dk, int64_t dv) {
     if (!heads_ok(dtype, B, H, H, dk, dv) || N < 0) return -1;
-    return 0;
+    return decay::tc_workspace(dtype, B, N, H, dk, dv);
 }
 
 extern "C" int snnb_decay_attention(const void* q, const int64_t* q_strides, const void* k,
@@ -205,10 +205,8 @@ extern "C" int snnb_decay_attention(const void* q, const int64_t* q_strides, con
         a.ks[i] = k_strides[i];
         a.vs[i] = v_strides[i];
     }
-    (void)workspace;
-    (void)workspace_bytes;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (tc_takes(a, dtype)) return tc_run(a, s);
+    if (tc_takes(a, dtype)) return tc_run(a, workspace, workspace_bytes, s);
     if (dtype == SNNB_F32) return run_any<float>(a, s);
     if (dtype == SNNB_F16) return run_any<__half>(a, s);
     return run_any<__nv_bfloat16>(a, s);

@@ -31,9 +31,14 @@ struct Args {
     }
 };
 
-// base^n for whole n >= 0, with 0^0 = 1.
-__device__ __forceinline__ float power(float base, int n) {
-    return n == 0 ? 1.0f : (float)exp((double)n * log((double)base));
+// base^n for whole 0 <= n < 2^31, with 0^0 = 1, by squaring in float64: powers compound over the
+// chunks.
+__device__ __forceinline__ double power(float base, int n) {
+    double r = 1.0, x = base;
+#pragma unroll 1
+    for (; n; n >>= 1, x *= x)
+        if (n & 1) r *= x;
+    return r;
 }
 
 // Allows `kernel` `bytes` of shared memory, once per device.
@@ -50,9 +55,11 @@ int allow_smem(int bytes) {
     return SNNB_OK;
 }
 
-// The tensor cores' form (decay_tc.cu): whether it takes these arguments, and its launches.
+// The tensor cores' form (decay_tc.cu): whether it takes these arguments, the workspace that it may
+// need for them, and its launches.
 bool tc_takes(const Args& a, int dtype);
-int tc_run(const Args& a, cudaStream_t s);
+int64_t tc_workspace(int dtype, int64_t B, int64_t N, int64_t H, int64_t dk, int64_t dv);
+int tc_run(const Args& a, void* work, int64_t bytes, cudaStream_t s);
 
 }  // namespace decay
 }  // namespace snnb

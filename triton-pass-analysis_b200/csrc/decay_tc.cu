@@ -1,4 +1,5 @@
 // Decay attention of 16-bit inputs on the tensor cores (formulas: decay.cu).
+#include <stdlib.h>
 #include "decay.cuh"
 #include "tc_common.cuh"
 
@@ -10,37 +11,81 @@ constexpr int C = 128;             // tokens of a chunk
 constexpr int DV = 64;             // columns of v, and of the state, that a thread block takes
 
 template <int DK> struct Smem {
-    static constexpr int STAGES = DK == 64 ? 1 : 2;
-    static constexpr int QKB = DK == 64 ? 1 : 2;               // score buffers in TMEM
     static constexpr int KB = DK / 64;                         // 64-column blocks of q and k
     static constexpr int BLOCK = C * 128;                      // 128 rows of 128 bytes
-    static constexpr int Q = 0, K = KB * BLOCK, V = 2 * KB * BLOCK, STAGE = (2 * KB + 1) * BLOCK;
-    static constexpr int S_OFF = STAGES * STAGE;               // state: high and low terms
+    static constexpr int QK_STAGES = DK == 64 ? 3 : 2, V_STAGES = DK == 64 ? 3 : 2;
+    static constexpr int QK_STAGE = 2 * KB * BLOCK;            // q, then k
+    static constexpr int V_OFF = QK_STAGES * QK_STAGE;
+    static constexpr int S_OFF = V_OFF + V_STAGES * BLOCK;     // state: high and low terms
     static constexpr int S_TERM = DK * 128;
-    static constexpr int VT_OFF = S_OFF + 2 * S_TERM;          // two slots for the scaled v's terms
-    static constexpr int PW_OFF = VT_OFF + 2 * BLOCK;          // decay^0 .. decay^C
-    static constexpr int RW_OFF = PW_OFF + 132 * 4;            // decay^31 .. decay^0
-    static constexpr int CP_OFF = RW_OFF + 32 * 4;             // decay^C, decay^last as two floats
-    static constexpr int BAD_OFF = CP_OFF + 16;                // [2][DV] rows, [2] chunk numbers
+    static constexpr int VT_OFF = S_OFF + 2 * S_TERM;          // scaled v: half a chunk's three terms
+    static constexpr int VT_TERM = BLOCK / 2;
+    static constexpr bool STAGED = DK == 64;                   // outputs leave by bulk copies
+    static constexpr int O_OFF = VT_OFF + 3 * VT_TERM;         // 32 rows for each warp
+    static constexpr int PW_OFF = O_OFF + (STAGED ? BLOCK : 0);  // 0 (31 times), decay^0 .. ^127
+    static constexpr int RW_OFF = PW_OFF + 160 * 4;            // decay^31 .. decay^0
+    static constexpr int WV_OFF = RW_OFF + 32 * 4;             // the factors of v's rows
+    static constexpr int BAD_OFF = WV_OFF + C * 4;             // [2][DV] rows, [2] chunk numbers
     static constexpr int BAR_OFF = BAD_OFF + (2 * DV + 2) * 4;
-    static constexpr int NBARS = 2 * STAGES + 2 * QKB + 8;
+    static constexpr int NBARS = 2 * QK_STAGES + 2 * V_STAGES + 11;
     static constexpr int TMEM_OFF = BAR_OFF + NBARS * 8;
     static constexpr int DYN = TMEM_OFF + 8 + 1024;
-    // TMEM columns: scores (and over their first half the rounded scores), q S, scores V, K^T V
-    static constexpr int COLS = DK == 64 ? 256 : 512;
-    static constexpr int T_QS = QKB * 128, T_PV = T_QS + 64, T_KV = DK == 64 ? 64 : T_PV + 64;
-    static constexpr int CTAS_PER_SM = DK == 64 ? 2 : 1;
-    static_assert(DYN <= 227 * 1024 && (DYN + 1024) * CTAS_PER_SM <= 228 * 1024, "shared memory");
+    static_assert(DYN <= 227 * 1024, "shared memory");
     static_assert(BAR_OFF % 8 == 0 && RW_OFF % 16 == 0, "alignment");
 };
 
-constexpr int THREADS = 14 * 32;   // scores and outputs, state, scaled v: 4 warps each; copies; MMAs
+// TMEM columns: scores (and over their first half P), q times the state's two terms, P V, K^T
+// times the scaled v's three terms.
+constexpr int T_QK = 0, T_QS = 128, T_PV = 256, T_KV = 320, T_COLS = 512;
+
+// Warps 0-3 scores to P, 4-7 outputs, 8-11 the state, 12-15 scaled v, 16 copies, 17 MMAs, 18 and 19
+// with warps 2 and 3, whose rows have the most scores.
+constexpr int THREADS = 20 * 32;
+// Registers a thread of each group of four warps: no more than 96 on the average, the launch's.
+constexpr int REGS_P = 88, REGS_O = 80, REGS_S = 128, REGS_V = 96;      // P: warps 16-19 too
+static_assert(2 * REGS_P + REGS_O + REGS_S + REGS_V <= 5 * 96, "registers");
+template <int N> __device__ __forceinline__ void fewer_regs() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N> __device__ __forceinline__ void more_regs() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
 
 struct TcArgs {
     Args a;
     int tiles;                     // of DV columns
+    int segs, cps;                 // segments of each sequence, chunks of a segment
+    uint32_t items;                // of this launch
+    float* work;                   // [segs][B H tiles][DK][DV] states (slot segs - 1: the start)
     int* status;
-    bool al_state, al_out;         // 16-byte aligned rows
+    bool out32;                    // the output's rows are 32-byte aligned
+};
+
+// A thread block's unit of work: a segment of a sequence, a head, DV columns.
+struct Item {
+    int64_t len;
+    int b, h, hk, bht, tile, seg;
+    int c0, n, last;               // first chunk, chunks, tokens of the last one
+    bool end;                      // of the sequence
+    float lam;
+    __device__ __forceinline__ Item(const TcArgs& p, uint32_t it) {
+        const Args& a = p.a;
+        const uint32_t H = (uint32_t)a.H, tiles = p.tiles, rest = it / tiles;
+        tile = (int)(it - rest * tiles);
+        const uint32_t sb = rest / H;                          // segment and sequence
+        h = (int)(rest - sb * H);
+        seg = (int)(sb / (uint32_t)a.B);
+        b = (int)(sb - (uint32_t)seg * (uint32_t)a.B);
+        bht = (int)(it - (uint32_t)seg * (uint32_t)a.B * H * tiles);
+        hk = (int)((uint32_t)h / (uint32_t)(a.H / a.Hk));
+        len = a.length(b);
+        lam = a.decay[h];
+        const int all = (int)((len + C - 1) / C);
+        c0 = min(seg * p.cps, all);
+        n = min(p.cps, all - c0);
+        end = c0 + n == all && (n > 0 || seg == 0);
+        last = n > 0 && c0 + n == all ? (int)(len - (int64_t)(all - 1) * C) : C;
+    }
 };
 
 // Operand with its rows (128 bytes, 128-byte swizzle) along K: `mn` bytes to the next 64 of M or N.
@@ -96,52 +141,77 @@ __device__ __forceinline__ uint32_t swizzled(int row, int piece) {
 __device__ __forceinline__ uint32_t bf2(float a, float b) {
     return mx::round_pair(a, b, (const __nv_bfloat16*)nullptr);
 }
+// 16 outputs of a row, the first `cols` (a multiple of 8) inside.
+__device__ __forceinline__ void store16(__nv_bfloat16* o, const uint32_t (&w)[8], int cols, bool al32) {
+    if (al32) {                                      // then cols is a multiple of 16
+        if (cols > 0)
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(o), "r"(w[0]),
+                         "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                         : "memory");
+        return;
+    }
+    if (cols > 0) reinterpret_cast<uint4*>(o)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    if (cols > 8) reinterpret_cast<uint4*>(o)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+}
 __device__ __forceinline__ float lo_f(uint32_t u) { return __int_as_float((int)(u << 16)); }
+// The upper halves of two floats as bf16 (cut, not rounded), and a float's upper half as a float.
+__device__ __forceinline__ uint32_t tops(float a, float b) {
+    return __byte_perm((uint32_t)__float_as_int(a), (uint32_t)__float_as_int(b), 0x7632);
+}
+__device__ __forceinline__ float top_f(float a) {
+    return __int_as_float(__float_as_int(a) & (int)0xFFFF0000u);
+}
 __device__ __forceinline__ float hi_f(uint32_t u) { return __int_as_float((int)(u & 0xFFFF0000u)); }
 
-template <int DK>
-__global__ void __launch_bounds__(THREADS, Smem<DK>::CTAS_PER_SM)
+// STATES: only the states that the segments leave, each from zero (the first: from state_in).
+template <int DK, bool STATES>
+__global__ void __launch_bounds__(THREADS, 1)
 decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                const __grid_constant__ CUtensorMap tmV, const __grid_constant__ TcArgs p) {
+                const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
+                const __grid_constant__ TcArgs p) {
     using L = Smem<DK>;
-    constexpr int ST = L::STAGES, QKB = L::QKB;
+    constexpr int NQ = L::QK_STAGES, NV = L::V_STAGES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sbase = tc::smem_u32(smem);
     float* pw = reinterpret_cast<float*>(smem + L::PW_OFF);
     float* rw = reinterpret_cast<float*>(smem + L::RW_OFF);
-    float* cp = reinterpret_cast<float*>(smem + L::CP_OFF);
+    float* wv = reinterpret_cast<float*>(smem + L::WV_OFF);
     int* bad_row = reinterpret_cast<int*>(smem + L::BAD_OFF);
     volatile int* bad_chunk = bad_row + 2 * DV;
     const uint32_t bar0 = sbase + L::BAR_OFF;
-    auto full = [&](int s) { return bar0 + 8u * s; };
-    auto empty = [&](int s) { return bar0 + 8u * (ST + s); };
-    auto qk_ready = [&](int i) { return bar0 + 8u * (2 * ST + i); };
-    auto p_ready = [&](int i) { return bar0 + 8u * (2 * ST + QKB + i); };
-    const uint32_t misc = bar0 + 8u * (2 * ST + 2 * QKB);
-    const uint32_t o_ready = misc, o_free = misc + 8, vt_ready = misc + 16, vt_free = misc + 24,
-                   vt3_ready = misc + 32, kv_ready = misc + 40, s_ready = misc + 48,
-                   done = misc + 56;
+    auto qk_full = [&](uint32_t s) { return bar0 + 8u * s; };
+    auto qk_empty = [&](uint32_t s) { return bar0 + 8u * (NQ + s); };
+    auto v_full = [&](uint32_t s) { return bar0 + 8u * (2 * NQ + s); };
+    auto v_empty = [&](uint32_t s) { return bar0 + 8u * (2 * NQ + NV + s); };
+    const uint32_t misc = bar0 + 8u * (2 * NQ + 2 * NV);
+    const uint32_t qk_ready = misc, p_ready = misc + 8, o_ready = misc + 16, o_free = misc + 24,
+                   vt_ready = misc + 32, kv_ready = misc + 40, kv_read = misc + 48,
+                   s_ready = misc + 56, qs_done = misc + 64, vt_free = misc + 72,
+                   done = misc + 80;
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + L::TMEM_OFF);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Args& a = p.a;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < ST; ++s) {
-            tc::mbar_init(full(s), 1);
-            tc::mbar_init(empty(s), 1);
+        for (int s = 0; s < NQ; ++s) {
+            tc::mbar_init(qk_full(s), 1);
+            tc::mbar_init(qk_empty(s), 1);
         }
-        for (int i = 0; i < QKB; ++i) {
-            tc::mbar_init(qk_ready(i), 1);
-            tc::mbar_init(p_ready(i), 4);
+        for (int s = 0; s < NV; ++s) {
+            tc::mbar_init(v_full(s), 1);
+            tc::mbar_init(v_empty(s), 1);
         }
+        tc::mbar_init(qk_ready, 1);
+        tc::mbar_init(p_ready, 6);
         tc::mbar_init(o_ready, 1);
         tc::mbar_init(o_free, 4);
         tc::mbar_init(vt_ready, 4);
-        tc::mbar_init(vt_free, 1);
-        tc::mbar_init(vt3_ready, 4);
         tc::mbar_init(kv_ready, 1);
+        tc::mbar_init(kv_read, 4);
+        tc::mbar_init(qs_done, 1);
+        tc::mbar_init(vt_free, 1);
         tc::mbar_init(s_ready, 4);
         tc::mbar_init(done, 1);
         tc::fence_mbar_init();
@@ -150,8 +220,8 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         tc::prefetch_tmap(&tmV);
         bad_chunk[0] = bad_chunk[1] = -1;
     }
-    if (warp == 13) {
-        tc::tmem_alloc(sbase + L::TMEM_OFF, L::COLS);
+    if (warp == 17) {
+        tc::tmem_alloc(sbase + L::TMEM_OFF, T_COLS);
         tc::tmem_relinquish();
     }
     tc::tc_fence_before();
@@ -161,411 +231,520 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     pdl_trigger();
     pdl_wait();
 
-    const int tile = (int)(blockIdx.x % (uint32_t)p.tiles);
-    const int64_t bh = blockIdx.x / (uint32_t)p.tiles;
-    const int64_t b = bh / a.H, h = bh - b * a.H, hk = h / (a.H / a.Hk);
-    const int64_t len = a.length(b);
-    const int nc = (int)((len + C - 1) / C);
-    const int last = nc ? (int)(len - (int64_t)(nc - 1) * C) : 0;     // tokens of the last chunk
-    if (warp < 12) {
-        const float lam = a.decay[h];
-        const int t = threadIdx.x;
-        if (t <= C) {
-            const float x = power(lam, t);
-            pw[t] = x;
-            if (t < 32) rw[31 - t] = x;
-        } else if (t >= 192 && t < 194) {
-            const int n = t == 192 ? C : last;
-            const double d = n == 0 ? 1.0 : exp((double)n * log((double)lam));
-            cp[2 * (t - 192)] = (float)d;
-            cp[2 * (t - 192) + 1] = (float)(d - (double)(float)d);
-        }
-        tc::named_bar_sync(2, 12 * 32);
-    }
-    uint32_t failed = 0;
-
-    if (warp < 4) {
-        // ---------------------------------------------------- scores to P, outputs
-        const int row = threadIdx.x;                 // of the chunk, and lane of TMEM
-        const uint32_t tl = tmem + ((uint32_t)(32 * warp) << 16);
-        auto scores = [&](int c) {
-            const int buf = c % QKB;
-            failed |= 1u - tc::mbar_wait_warp(qk_ready(buf), (uint32_t)(c / QKB) & 1u, failed);
-            tc::tc_fence_after();
-            const uint32_t t = tl + buf * 128;
-#pragma unroll 1
-            for (int blk = 0; blk < 4; ++blk) {
-                uint32_t w[16];
-                if (blk > warp) {                    // later tokens
+    // Every role walks the block's items and their chunks; g counts the chunks of all.
+    uint32_t failed = 0, g = 0;
+    if (warp < 4 || warp >= 16) {
+        fewer_regs<REGS_P>();
+        if (warp == 16) {
+            // ------------------------------------------------ copies
+            uint32_t issued_qk = 0, issued_v = 0;
+            for (uint32_t it = blockIdx.x; it < p.items; it += gridDim.x) {
+                const Item x(p, it);
+                for (int c = 0; c < x.n; ++c, ++g) {
+                    const uint32_t s = g % NQ, sv = g % NV;
+                    const int n0 = (x.c0 + c) * C;
+                    failed |= 1u - tc::mbar_wait_warp(qk_empty(s), ((g / NQ) & 1u) ^ 1u, failed);
+                    if (!failed && tc::elect_one()) {
+                        const uint32_t q = sbase + s * L::QK_STAGE, k = q + L::KB * L::BLOCK;
+                        tc::mbar_expect_tx(qk_full(s), (uint32_t)(L::QK_STAGE / (STATES ? 2 : 1)));
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) w[i] = 0;
-                } else {
-                    float x[32];
-                    tc::tmem_ld32(t + blk * 32, x);
-                    tc::tmem_wait_ld();
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(x[i]));
-                    if (blk == warp) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            x[i] = i <= lane ? x[i] * pw[lane - i] : 0.0f;
-                    } else {
-                        const float f = pw[row - 32 * blk - 31];
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            const float4 r = *reinterpret_cast<const float4*>(rw + i);
-                            x[i] *= f * r.x;
-                            x[i + 1] *= f * r.y;
-                            x[i + 2] *= f * r.z;
-                            x[i + 3] *= f * r.w;
+                        for (int i = 0; i < L::KB; ++i) {
+                            if (!STATES)
+                                tc::tma_load_4d(q + i * L::BLOCK, &tmQ, qk_full(s), 64 * i, x.h, n0, x.b);
+                            tc::tma_load_4d(k + i * L::BLOCK, &tmK, qk_full(s), 64 * i, x.hk, n0, x.b);
                         }
                     }
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) w[i] = bf2(x[2 * i], x[2 * i + 1]);
-                }
-                tmem_st16(t + blk * 16, w);
-            }
-            tmem_wait_st();
-            tc::tc_fence_before();
-            if (lane == 0) tc::mbar_arrive(p_ready(buf));
-            __syncwarp();
-        };
-        const float fq = pw[row + 1];
-        const int cols = min(DV, a.dv - tile * DV);
-        __nv_bfloat16* out =
-            static_cast<__nv_bfloat16*>(a.out) + (b * a.N * a.H + h) * a.dv + tile * DV;
-        const int64_t ld = a.H * a.dv;
-        auto store_row = [&](int64_t n, const uint32_t (&w)[32]) {
-            __nv_bfloat16* o = out + n * ld;
-            if (!SNNB_IN_BOUNDS(n, a.N, p.status)) return;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (8 * i < cols) {                  // dv is a multiple of 8
-                    if (p.al_out) {
-                        reinterpret_cast<uint4*>(o)[i] =
-                            make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            reinterpret_cast<uint16_t*>(o)[8 * i + e] =
-                                (uint16_t)(w[4 * i + e / 2] >> (16 * (e & 1)));
+                    __syncwarp();
+                    if (!failed) ++issued_qk;
+                    failed |= 1u - tc::mbar_wait_warp(v_empty(sv), ((g / NV) & 1u) ^ 1u, failed);
+                    if (!failed && tc::elect_one()) {
+                        tc::mbar_expect_tx(v_full(sv), (uint32_t)L::BLOCK);
+                        tc::tma_load_4d(sbase + L::V_OFF + sv * L::BLOCK, &tmV, v_full(sv), DV * x.tile,
+                                        x.hk, n0, x.b);
                     }
+                    __syncwarp();
+                    if (!failed) ++issued_v;
                 }
-        };
-        auto outputs = [&](int c) {
-            failed |= 1u - tc::mbar_wait_warp(o_ready, (uint32_t)c & 1u, failed);
-            tc::tc_fence_after();
-            uint32_t w[32];
-            const bool spoiled = bad_chunk[c & 1] == c;
-#pragma unroll
-            for (int i = 0; i < DV; i += 16) {
-                float s[16], v[16];
-                tc::tmem_ld16(tl + L::T_QS + i, s);
-                tc::tmem_ld16(tl + L::T_PV + i, v);
-                tc::tmem_wait_ld();
-                tc::reg_fence16(s);
-                tc::reg_fence16(v);
-#pragma unroll
-                for (int j = 0; j < 16; ++j) v[j] = (v[j] + fq * s[j]) * a.scale;
-                if (spoiled) {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        if (row >= bad_row[(c & 1) * DV + i + j]) v[j] = __int_as_float(0x7fffffff);
-                }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) w[i / 2 + j] = bf2(v[2 * j], v[2 * j + 1]);
             }
-            tc::tc_fence_before();
-            if (lane == 0) tc::mbar_arrive(o_free);
+            if (failed) {                            // copies in flight land before the block ends
+                for (uint32_t k = 0; k < issued_qk && k < (uint32_t)NQ; ++k) {
+                    const uint32_t i = issued_qk - 1 - k;
+                    tc::mbar_wait_warp<true>(qk_full(i % NQ), (i / NQ) & 1u, 0);
+                }
+                for (uint32_t k = 0; k < issued_v && k < (uint32_t)NV; ++k) {
+                    const uint32_t i = issued_v - 1 - k;
+                    tc::mbar_wait_warp<true>(v_full(i % NV), (i / NV) & 1u, 0);
+                }
+            }
+        } else if (warp == 17) {
+            // ------------------------------------------------ MMAs
+            if (tc::elect_one()) {
+                auto wait = [&](uint32_t bar, uint32_t parity) {
+                    failed |= 1u - tc::mbar_wait_lane(bar, parity, failed);
+                    tc::tc_fence_after();
+                };
+                uint32_t chunks = 0;
+                for (uint32_t it = blockIdx.x; it < p.items; it += gridDim.x) chunks += Item(p, it).n;
+                auto issue_qk = [&](uint32_t c) {
+                    const uint32_t q = sbase + (c % NQ) * L::QK_STAGE, k = q + L::KB * L::BLOCK;
+                    wait(qk_full(c % NQ), (c / NQ) & 1u);
+                    if (failed || STATES) return;
+#pragma unroll
+                    for (int i = 0; i < 4 * L::KB; ++i)
+                        tc::umma_bf16(tmem + T_QK, tc::sdesc_k_sw128(q + i / 4 * L::BLOCK) + 2 * (i % 4),
+                                      tc::sdesc_k_sw128(k + i / 4 * L::BLOCK) + 2 * (i % 4),
+                                      tc::idesc_bf16_f32(128, 128), i != 0);
+                    tc::umma_commit(qk_ready);
+                };
+#pragma unroll 1
+                for (g = 0; g < chunks && !failed; ++g) {
+                    const uint32_t ph = g & 1u, s = g % NQ, sv = g % NV;
+                    const uint32_t q = sbase + s * L::QK_STAGE, k = q + L::KB * L::BLOCK;
+                    issue_qk(g);
+                    if (g) wait(kv_read, ph ^ 1u);
+                    // k^T times the three terms of the scaled v, side by side, by half chunks
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        wait(vt_ready, (uint32_t)half);
+                        if (failed) break;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            tc::umma_bf16(tmem + T_KV,
+                                          sdesc_mn_sw128(k, DK == 64 ? 0 : L::BLOCK) + 128 * (4 * half + i),
+                                          sdesc_mn_sw128(sbase + L::VT_OFF, L::VT_TERM) + 128 * i,
+                                          tc::idesc_bf16_f32(128, 192) | A_MN | B_MN, (half | i) != 0);
+                        tc::umma_commit(half ? kv_ready : vt_free);
+                    }
+                    wait(s_ready, ph);
+                    if (!STATES) {
+                        if (g) wait(o_free, ph ^ 1u);
+                        if (failed) break;
+                        // q times both terms of the state, side by side
+#pragma unroll
+                        for (int i = 0; i < DK / 16; ++i)
+                            tc::umma_bf16(tmem + T_QS, tc::sdesc_k_sw128(q + i / 4 * L::BLOCK) + 2 * (i % 4),
+                                          sdesc_mn_sw128(sbase + L::S_OFF, L::S_TERM) + 128 * i,
+                                          tc::idesc_bf16_f32(128, 128) | B_MN, i != 0);
+                        tc::umma_commit(qs_done);
+                    }
+                    tc::umma_commit(qk_empty(s));
+                    if (!STATES) {
+                        wait(p_ready, ph);
+                        if (failed) break;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            umma_ts(tmem + T_PV, tmem + T_QK + 8 * i,
+                                    sdesc_mn_sw128(sbase + L::V_OFF + sv * L::BLOCK, 0) + 128 * i,
+                                    tc::idesc_bf16_f32(128, 64) | B_MN, i != 0);
+                        tc::umma_commit(o_ready);
+                    }
+                    tc::umma_commit(v_empty(sv));
+                }
+                tc::umma_commit(done);
+            }
             __syncwarp();
-            const int64_t n = (int64_t)c * C + row;
-            if (n >= len) {
+            failed = __any_sync(0xffffffffu, failed);
+            failed |= 1u - tc::mbar_wait_warp<true>(done, 0, 0);
+        } else {
+            // ------------------------------------------------ scores to P
+            // Blocks of 32 x 32: a warp has those of its rows (its lanes of TMEM) up to the
+            // diagonal one; the third and the fourth of the last two warps' rows go to warps 18
+            // and 19.
+            const int q = warp & 3, first = warp >= 18 ? 2 : 0, row = 32 * q + lane;
+            const bool two = q == 3 || (q >= 1 && first == 0);     // of these two blocks
+            const int diag = q >= 2 && first == 0 ? -1 : q - first;     // which of the two, if any
+            const uint32_t tl = tmem + ((uint32_t)(32 * q) << 16) + T_QK;
+            for (uint32_t it = blockIdx.x; !STATES && it < p.items; it += gridDim.x) {
+                const Item x(p, it);
+                if (x.n == 0) continue;
+                tc::named_bar_sync(2, 6 * 32);       // the last item's table has been read
+                if (warp < 4) {
+                    const float f = (float)power(x.lam, row);
+                    pw[31 + row] = f;
+                    if (row < 32) rw[31 - row] = f;
+                    if (row < 31) pw[row] = 0.0f;
+                }
+                tc::named_bar_sync(2, 6 * 32);
+                float f0 = diag == 0 ? 0.0f : pw[row - 32 * first],
+                      f1 = diag == 1 || !two ? 0.0f : pw[row - 32 * first - 32];
+#pragma unroll 1
+                for (int c = 0; c < x.n; ++c, ++g) {
+                    failed |= 1u - tc::mbar_wait_warp(qk_ready, g & 1u, failed);
+                    tc::tc_fence_after();
+                    float s[32], s1[32];
+                    tc::tmem_ld32(tl + first * 32, s);
+                    if (two) tc::tmem_ld32(tl + first * 32 + 32, s1);
+                    tc::tmem_wait_ld();
 #pragma unroll
-                for (int j = 0; j < 32; ++j) w[j] = 0;
-            }
-            if (n < a.N && !failed) store_row(n, w);
-        };
-        if (nc) {
-            scores(0);
-            for (int c = 0; c < nc; ++c) {
-                if (QKB == 2 && c + 1 < nc) scores(c + 1);
-                outputs(c);
-                if (QKB == 1 && c + 1 < nc) scores(c + 1);
+                    for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(s[i]), "+f"(s1[i]));
+                    // P takes the place of scores that the other warp of these rows reads
+                    if (q >= 2) tc::named_bar_sync(3 + q, 64);
+#pragma unroll 1
+                    for (int blk = 0; blk < 2; ++blk) {
+                        uint32_t w[16];
+                        if (blk == 0 || two) {
+                            if (blk == diag) {
+                                // later tokens count nothing, whatever their scores
+                                const float* d = pw + 31 + lane;
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) {
+                                    const float y = s[i] * d[-i];
+                                    s[i] = i <= lane ? y : 0.0f;
+                                }
+                            } else {
+                                const float f = blk ? f1 : f0;
+                                const uint64_t ff = mx::pack2(f, f);
+#pragma unroll
+                                for (int i = 0; i < 32; i += 4) {
+                                    const float4 r = *reinterpret_cast<const float4*>(rw + i);
+                                    mx::unpack2(mx::mul2(mx::pack2(s[i], s[i + 1]),
+                                                         mx::mul2(ff, mx::pack2(r.x, r.y))), s[i], s[i + 1]);
+                                    mx::unpack2(mx::mul2(mx::pack2(s[i + 2], s[i + 3]),
+                                                         mx::mul2(ff, mx::pack2(r.z, r.w))), s[i + 2], s[i + 3]);
+                                }
+                            }
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) w[i] = bf2(s[2 * i], s[2 * i + 1]);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) w[i] = 0;
+                        }
+                        tmem_st16(tl + (first + blk) * 16, w);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) s[i] = s1[i];
+                    }
+                    if (q < 2) {                     // blocks of later tokens
+                        const uint32_t zero[16] = {};
+                        tmem_st16(tl + 32, zero);
+                        tmem_st16(tl + 48, zero);
+                    }
+                    tmem_wait_st();
+                    tc::tc_fence_before();
+                    if (lane == 0) tc::mbar_arrive(p_ready);
+                    __syncwarp();
+                }
             }
         }
-        // rows behind the last chunk
-        const uint32_t zero[32] = {};
-        for (int64_t n = (int64_t)nc * C + row; n < a.N; n += C) store_row(n, zero);
     } else if (warp < 8) {
+        // ---------------------------------------------------- outputs
+        fewer_regs<REGS_O>();
+        const int q = warp & 3, row = 32 * q + lane;
+        const uint32_t tl = tmem + ((uint32_t)(32 * q) << 16);
+        const uint32_t stage = sbase + L::O_OFF + q * 32 * 128;
+        for (uint32_t it = blockIdx.x; !STATES && it < p.items; it += gridDim.x) {
+            const Item x(p, it);
+            const float fq = (float)power(x.lam, row + 1) * a.scale;
+            const uint64_t fq2 = mx::pack2(fq, fq), sc2 = mx::pack2(a.scale, a.scale);
+            const int cols = min(DV, a.dv - x.tile * DV);
+            const int64_t ld = a.H * a.dv;
+            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) +
+                                 ((int64_t)x.b * a.N * a.H + x.h) * a.dv + x.tile * DV +
+                                 ((int64_t)x.c0 * C + row) * ld;
+#pragma unroll 1
+            for (int c = 0; c < x.n; ++c, ++g, out += C * ld) {
+                const int64_t n = (int64_t)(x.c0 + c) * C + row;
+                if (L::STAGED) {                     // the last copy has read its rows
+                    if (lane == 0) tc::bulk_wait_group_read<0>();
+                    __syncwarp();
+                }
+                failed |= 1u - tc::mbar_wait_warp(o_ready, g & 1u, failed);
+                tc::tc_fence_after();
+                const bool spoiled = bad_chunk[g & 1] == (int)g, alive = n < x.len;
+                const bool write = n < a.N && !failed && SNNB_IN_BOUNDS(n, a.N, p.status);
+#pragma unroll 1
+                for (int i = 0; i < DV; i += 16) {
+                    float s[16], l[16], v[16];
+                    tc::tmem_ld16(tl + T_QS + i, s);
+                    tc::tmem_ld16(tl + T_QS + 64 + i, l);
+                    tc::tmem_ld16(tl + T_PV + i, v);
+                    tc::tmem_wait_ld();
+                    tc::reg_fence16(s);
+                    tc::reg_fence16(l);
+                    tc::reg_fence16(v);
+                    if (i + 16 == DV) {
+                        tc::tc_fence_before();
+                        if (lane == 0) tc::mbar_arrive(o_free);
+                        __syncwarp();
+                    }
+                    uint32_t w[8];
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2) {
+                        const uint64_t y = mx::add2(mx::pack2(s[j], s[j + 1]), mx::pack2(l[j], l[j + 1]));
+                        mx::unpack2(mx::fma2(fq2, y, mx::mul2(sc2, mx::pack2(v[j], v[j + 1]))), v[j],
+                                    v[j + 1]);
+                    }
+                    if (spoiled) {
+                        const int* rows = bad_row + (g & 1) * DV + i;
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (row >= rows[j]) v[j] = __int_as_float(0x7fffffff);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) w[j] = alive ? bf2(v[2 * j], v[2 * j + 1]) : 0u;
+                    if (L::STAGED) {
+                        sts128(stage + swizzled(lane, i / 8), make_uint4(w[0], w[1], w[2], w[3]));
+                        sts128(stage + swizzled(lane, i / 8 + 1), make_uint4(w[4], w[5], w[6], w[7]));
+                    } else if (write) {
+                        store16(out + i, w, cols - i, p.out32);
+                    }
+                }
+                if (L::STAGED) {
+                    tc::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0 && write) {        // rows behind N are not written
+                        asm volatile(
+                            "cp.async.bulk.tensor.4d.global.shared::cta.bulk_group "
+                            "[%0, {%2, %3, %4, %5}], [%1];" ::"l"(&tmO),
+                            "r"(stage), "r"(DV * x.tile), "r"(x.h), "r"((int)n), "r"(x.b)
+                            : "memory");
+                        tc::bulk_commit_group();
+                    }
+                }
+            }
+            if (x.end) {                             // rows behind the last chunk
+                const uint32_t zero[8] = {};
+#pragma unroll 1
+                for (int64_t n = (int64_t)(x.c0 + x.n) * C + row; n < a.N; n += C, out += C * ld)
+#pragma unroll 1
+                    for (int i = 0; i < cols; i += 16) store16(out + i, zero, cols - i, p.out32);
+            }
+        }
+        if (lane == 0) tc::bulk_wait_group<0>();     // the copies have left shared memory
+    } else if (warp < 12) {
         // ---------------------------------------------------- the state
         // This thread's row and columns: DK = 64 products have 128 rows, the second 64 the
         // first's copy, so that each half of the threads takes half of the columns.
-        const int t = threadIdx.x - 128;
+        more_regs<REGS_S>();
+        const int t = threadIdx.x - 256;
         constexpr int W = DK == 64 ? 32 : 64;
-        const int row = t % DK, c0 = DK == 64 ? t / 64 * 32 : 0;
-        const uint32_t tl = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + L::T_KV + c0;
-        const int64_t at = (bh * a.dk + row) * a.dv + tile * DV + c0;
-        const int cols = row < a.dk ? min(W, a.dv - tile * DV - c0) : 0;
-        float S[W];
+        const int row = t % DK, col = DK == 64 ? t / 64 * 32 : 0;
+        const uint32_t tl = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + T_KV + col;
+        for (uint32_t it = blockIdx.x; it < p.items; it += gridDim.x) {
+            const Item x(p, it);
+            if (x.n == 0 && (STATES ? x.seg > 0 : !x.end)) continue;
+            const int64_t at = (((int64_t)x.b * a.H + x.h) * a.dk + row) * a.dv + x.tile * DV + col;
+            const int cols = row < a.dk ? min(W, a.dv - x.tile * DV - col) : 0;
+            const int64_t slot = a.B * a.H * p.tiles * (DK * DV);
+            float* work = p.work + (int64_t)x.bht * (DK * DV) + row * DV + col;
+            float S[W];
+            // what there is before the first chunk
+            const bool segs = !STATES && p.segs > 1;
+            const float* from = x.seg > 0 ? (segs ? work : nullptr)
+                                : !a.state_in ? nullptr
+                                : segs        ? work + (p.segs - 1) * slot
+                                              : a.state_in + at;
+            const int have = segs ? W : cols;
 #pragma unroll
-        for (int i = 0; i < W; ++i) S[i] = 0.0f;
-        if (a.state_in) {
-#pragma unroll
-            for (int i = 0; i < W; i += 4)
-                if (i < cols) {
-                    if (p.al_state) {
-                        const float4 x = *reinterpret_cast<const float4*>(a.state_in + at + i);
-                        S[i] = x.x; S[i + 1] = x.y; S[i + 2] = x.z; S[i + 3] = x.w;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) S[i + e] = a.state_in[at + i + e];
-                    }
-                }
-        }
-        auto publish = [&]() {
-#pragma unroll
-            for (int i = 0; i < W; i += 8) {
-                uint32_t hi[4], lo[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float x = S[i + 2 * j], y = S[i + 2 * j + 1];
-                    hi[j] = bf2(x, y);
-                    lo[j] = bf2(x - lo_f(hi[j]), y - hi_f(hi[j]));
-                }
-                const uint32_t o = sbase + L::S_OFF + swizzled(row, (c0 + i) / 8);
-                sts128(o, make_uint4(hi[0], hi[1], hi[2], hi[3]));
-                sts128(o + L::S_TERM, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+            for (int i = 0; i < W; i += 4) {
+                const float4 y = from && i < have ? *reinterpret_cast<const float4*>(from + i)
+                                                  : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                S[i] = y.x; S[i + 1] = y.y; S[i + 2] = y.z; S[i + 3] = y.w;
             }
-            tc::fence_proxy_async_smem();
-            tc::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(s_ready);
-        };
-        publish();
-        for (int c = 0; c < nc; ++c) {
-            failed |= 1u - tc::mbar_wait_warp(kv_ready, (uint32_t)c & 1u, failed);
-            tc::tc_fence_after();
-            const float2 f = reinterpret_cast<const float2*>(cp)[c + 1 == nc];
-#pragma unroll
-            for (int i = 0; i < W; i += 16) {
-                float x[16];
-                tc::tmem_ld16(tl + i, x);
-                tc::tmem_wait_ld();
-                tc::reg_fence16(x);
-#pragma unroll
-                for (int j = 0; j < 16; ++j) S[i + j] = fmaf(S[i + j], f.x, fmaf(S[i + j], f.y, x[j]));
-            }
-            if (c + 1 < nc) publish();
-        }
-        if (a.state_out && !failed) {
-#pragma unroll
-            for (int i = 0; i < W; i += 4)
-                if (i < cols) {
-                    if (p.al_state) {
-                        *reinterpret_cast<float4*>(a.state_out + at + i) =
-                            make_float4(S[i], S[i + 1], S[i + 2], S[i + 3]);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) a.state_out[at + i + e] = S[i + e];
-                    }
-                }
-        }
-    } else if (warp < 12) {
-        // ---------------------------------------------------- v scaled, as three bf16 terms
-        const int t = threadIdx.x - 256, piece = t & 7, r0 = t >> 3;
-        const uint32_t slot0 = sbase + L::VT_OFF, slot1 = slot0 + L::BLOCK;
-        for (int c = 0; c < nc; ++c) {
-            const int s = c % ST, m = c + 1 == nc ? last : C;
-            failed |= 1u - tc::mbar_wait_warp(full(s), (uint32_t)(c / ST) & 1u, failed);
-            const uint32_t stage = sbase + s * L::STAGE, vs = stage + L::V;
-            uint32_t low[8][4], top = 0;
-            // the slots' last readers
-            if (c) failed |= 1u - tc::mbar_wait_warp(kv_ready, (uint32_t)(c - 1) & 1u, failed);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = r0 + 16 * i;
-                const uint32_t o = swizzled(r, piece);
-                uint4 raw = lds128(vs + o);
-                const float w = r < m ? pw[m - 1 - r] : 0.0f;
-                if (r >= m) {
-                    // rows behind the sequence, whatever they hold (beyond the tensor: zeros)
-                    raw = make_uint4(0, 0, 0, 0);
-                    sts128(vs + o, raw);
-#pragma unroll
-                    for (int k = 0; k < L::KB; ++k) sts128(stage + L::K + k * L::BLOCK + o, raw);
-                }
-                const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
-                uint32_t hi[4], mid[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    top = __vmaxu2(top, u[j] & 0x7FFF7FFFu);
-                    float x = lo_f(u[j]) * w, y = hi_f(u[j]) * w;
-                    hi[j] = bf2(x, y);
-                    x -= lo_f(hi[j]);
-                    y -= hi_f(hi[j]);
-                    mid[j] = bf2(x, y);
-                    low[i][j] = bf2(x - lo_f(mid[j]), y - hi_f(mid[j]));
-                }
-                sts128(slot0 + o, make_uint4(hi[0], hi[1], hi[2], hi[3]));
-                sts128(slot1 + o, make_uint4(mid[0], mid[1], mid[2], mid[3]));
-            }
-            if (tc::named_bar_any(1, 128, (top & 0xFFFFu) >= 0x7F80u || (top >> 16) >= 0x7F80u)) {
-                // Values that are not finite: 0 * inf in the product of scores and v would reach
-                // the chunk's earlier rows.  There they become zero, and the outputs of their
-                // columns NaN from their row on.
-                if (t < DV) bad_row[(c & 1) * DV + t] = C;
-                tc::named_bar_sync(1, 128);
+            if (segs && x.seg > 1) {
+                const double d = power(x.lam, p.cps * C);
+                const float fh = (float)d, fl = (float)(d - (double)fh);
 #pragma unroll 1
-                for (int r = r0; r < C; r += 16) {
-                    const uint32_t o = swizzled(r, piece);
-                    uint4 raw = lds128(vs + o);
-                    uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+                for (int s = 1; s < x.seg; ++s) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if ((u[j] & 0x7F80u) == 0x7F80u) {
-                            atomicMin(&bad_row[(c & 1) * DV + 8 * piece + 2 * j], r);
-                            u[j] &= 0xFFFF0000u;
-                        }
-                        if ((u[j] & 0x7F800000u) == 0x7F800000u) {
-                            atomicMin(&bad_row[(c & 1) * DV + 8 * piece + 2 * j + 1], r);
-                            u[j] &= 0xFFFFu;
-                        }
+                    for (int i = 0; i < W; i += 4) {
+                        const float4 y = *reinterpret_cast<const float4*>(work + s * slot + i);
+                        S[i] = fmaf(S[i], fh, fmaf(S[i], fl, y.x));
+                        S[i + 1] = fmaf(S[i + 1], fh, fmaf(S[i + 1], fl, y.y));
+                        S[i + 2] = fmaf(S[i + 2], fh, fmaf(S[i + 2], fl, y.z));
+                        S[i + 3] = fmaf(S[i + 3], fh, fmaf(S[i + 3], fl, y.w));
                     }
-                    sts128(vs + o, make_uint4(u[0], u[1], u[2], u[3]));
                 }
-                if (t == 0) bad_chunk[c & 1] = c;
             }
-            tc::fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(vt_ready);
-            failed |= 1u - tc::mbar_wait_warp(vt_free, (uint32_t)c & 1u, failed);
+            auto put = [&](float* to, int n) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                sts128(slot0 + swizzled(r0 + 16 * i, piece),
-                       make_uint4(low[i][0], low[i][1], low[i][2], low[i][3]));
-            tc::fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(vt3_ready);
-        }
-    } else if (warp == 12) {
-        // ---------------------------------------------------- copies
-        uint32_t issued = 0;
-        for (int c = 0; c < nc; ++c) {
-            const int s = c % ST;
-            failed |= 1u - tc::mbar_wait_warp(empty(s), ((uint32_t)(c / ST) & 1u) ^ 1u, failed);
-            const uint32_t stage = sbase + s * L::STAGE;
-            if (!failed && tc::elect_one()) {
-                tc::mbar_expect_tx(full(s), (uint32_t)L::STAGE);
-                const int n0 = c * C;
+                for (int i = 0; i < W; i += 4)
+                    if (i < n)
+                        *reinterpret_cast<float4*>(to + i) =
+                            make_float4(S[i], S[i + 1], S[i + 2], S[i + 3]);
+            };
+            if (STATES && x.seg == 0 && a.state_in)  // state_out may be state_in
+                put(work + (p.segs - 1) * slot, W);
+            const double dc = power(x.lam, C), dl = power(x.lam, x.last);
+            const float ch = (float)dc, cl = (float)(dc - (double)ch), lh = (float)dl,
+                        ll = (float)(dl - (double)lh);
+#pragma unroll 1
+            for (int c = 0; c < x.n; ++c, ++g) {
+                if (!STATES) {
+                    // the state before this chunk, once q times the last one is done
+                    if (g) failed |= 1u - tc::mbar_wait_warp(qs_done, (g - 1) & 1u, failed);
 #pragma unroll
-                for (int k = 0; k < L::KB; ++k) {
-                    tc::tma_load_4d(stage + L::Q + k * L::BLOCK, &tmQ, full(s), 64 * k, (int)h, n0, (int)b);
-                    tc::tma_load_4d(stage + L::K + k * L::BLOCK, &tmK, full(s), 64 * k, (int)hk, n0, (int)b);
+                    for (int i = 0; i < W; i += 8) {
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float y = S[i + 2 * j], z = S[i + 2 * j + 1];
+                            hi[j] = bf2(y, z);
+                            lo[j] = bf2(y - lo_f(hi[j]), z - hi_f(hi[j]));
+                        }
+                        const uint32_t o = sbase + L::S_OFF + swizzled(row, (col + i) / 8);
+                        sts128(o, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+                        sts128(o + L::S_TERM, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+                    }
+                    tc::fence_proxy_async_smem();
                 }
-                tc::tma_load_4d(stage + L::V, &tmV, full(s), DV * tile, (int)hk, n0, (int)b);
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(s_ready);
+                failed |= 1u - tc::mbar_wait_warp(kv_ready, g & 1u, failed);
+                tc::tc_fence_after();
+                const bool end = c + 1 == x.n;
+                const float fh = end ? lh : ch, fl = end ? ll : cl;
+                const uint64_t fh2 = mx::pack2(fh, fh), fl2 = mx::pack2(fl, fl);
+#pragma unroll
+                for (int i = 0; i < W; i += 16) {
+                    float y[16], z[16], u[16];
+                    tc::tmem_ld16(tl + i, y);
+                    tc::tmem_ld16(tl + 64 + i, z);
+                    tc::tmem_ld16(tl + 128 + i, u);
+                    tc::tmem_wait_ld();
+                    tc::reg_fence16(y);
+                    tc::reg_fence16(z);
+                    tc::reg_fence16(u);
+                    if (i + 16 == W) {
+                        tc::tc_fence_before();
+                        if (lane == 0) tc::mbar_arrive(kv_read);
+                        __syncwarp();
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2) {
+                        const uint64_t sum = mx::add2(mx::pack2(y[j], y[j + 1]),
+                                                      mx::add2(mx::pack2(z[j], z[j + 1]),
+                                                               mx::pack2(u[j], u[j + 1])));
+                        const uint64_t old = mx::pack2(S[i + j], S[i + j + 1]);
+                        mx::unpack2(mx::fma2(old, fh2, mx::fma2(old, fl2, sum)), S[i + j], S[i + j + 1]);
+                    }
+                }
             }
-            __syncwarp();
-            if (!failed) ++issued;
-        }
-        if (failed) {                                // copies in flight land before the block ends
-            for (uint32_t k = 0; k < issued && k < (uint32_t)ST; ++k) {
-                const int c = (int)issued - 1 - (int)k;
-                tc::mbar_wait_warp<true>(full(c % ST), (uint32_t)(c / ST) & 1u, 0);
-            }
+            if (!failed && (STATES || (x.end && a.state_out)))
+                put(STATES ? work + x.seg * slot : a.state_out + at, STATES ? W : cols);
         }
     } else {
-        // ---------------------------------------------------- MMAs
-        if (tc::elect_one()) {
-            constexpr uint32_t I_QK = tc::idesc_bf16_f32(128, 128), I_64 = tc::idesc_bf16_f32(128, 64);
-            auto wait = [&](uint32_t bar, uint32_t parity) {
-                failed |= 1u - tc::mbar_wait_lane(bar, parity, failed);
-                tc::tc_fence_after();
-            };
-            auto issue_qk = [&](int c) {
-                const int s = c % ST, buf = c % QKB;
-                wait(full(s), (uint32_t)(c / ST) & 1u);
-                const uint32_t stage = sbase + s * L::STAGE;
-                if (failed) return;
-#pragma unroll
-                for (int k = 0; k < L::KB; ++k) {
-                    const uint64_t da = tc::sdesc_k_sw128(stage + L::Q + k * L::BLOCK);
-                    const uint64_t db = tc::sdesc_k_sw128(stage + L::K + k * L::BLOCK);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        tc::umma_bf16(tmem + buf * 128, da + 2 * i, db + 2 * i, I_QK, (k | i) != 0);
+        // ---------------------------------------------------- v scaled, as three bf16 terms
+        const int t = threadIdx.x - 384, piece = t & 7, r0 = t >> 3;
+        const uint32_t vt = sbase + L::VT_OFF + swizzled(r0, piece);
+        const uint64_t minus = mx::pack2(-1.0f, -1.0f);
+        for (uint32_t it = blockIdx.x; it < p.items; it += gridDim.x) {
+            const Item x(p, it);
+            int held = -1;                           // tokens that the factors are for
+#pragma unroll 1
+            for (int c = 0; c < x.n; ++c, ++g) {
+                const uint32_t s = g % NV, sq = g % NQ;
+                const int m = c + 1 == x.n ? x.last : C;
+                if (m != held) {
+                    tc::named_bar_sync(1, 128);
+                    wv[t] = t < m ? (float)power(x.lam, m - 1 - t) : 0.0f;
+                    held = m;
+                    tc::named_bar_sync(1, 128);
                 }
-                tc::umma_commit(qk_ready(buf));
-            };
-            if (nc) issue_qk(0);
-            for (int c = 0; c < nc && !failed; ++c) {
-                const int s = c % ST, buf = c % QKB;
-                const uint32_t stage = sbase + s * L::STAGE, ph = (uint32_t)c & 1u;
-                if (QKB == 2 && c + 1 < nc) issue_qk(c + 1);
-                if (QKB == 2 || c == 0) wait(s_ready, ph);
-                if (c) wait(o_free, ph ^ 1u);
-                if (failed) break;
-                // q S
+                failed |= 1u - tc::mbar_wait_warp(v_full(s), (g / NV) & 1u, failed);
+                const uint32_t vs = sbase + L::V_OFF + s * L::BLOCK + swizzled(r0, piece);
+                if (m < C) {
+                    // rows behind the sequence, whatever they hold (beyond the tensor: zeros)
+                    failed |= 1u - tc::mbar_wait_warp(qk_full(sq), (g / NQ) & 1u, failed);
+                    const uint32_t ks = sbase + sq * L::QK_STAGE + L::KB * L::BLOCK + swizzled(r0, piece);
+                    const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+                    for (int i = 0; i < 8; ++i)
+                        if (r0 + 16 * i >= m) {
+                            sts128(vs + 2048 * i, zero);
 #pragma unroll
-                for (int term = 0; term < 2; ++term)
+                            for (int k = 0; k < L::KB; ++k) sts128(ks + k * L::BLOCK + 2048 * i, zero);
+                        }
+                }
+                uint32_t top = 0;
+#pragma unroll 1
+                for (int half = 0; half < 2; ++half) {
+                    uint4 raw[4];
+                    float f[4];
 #pragma unroll
-                    for (int k = 0; k < DK / 16; ++k)
-                        tc::umma_bf16(tmem + L::T_QS,
-                                      tc::sdesc_k_sw128(stage + L::Q + k / 4 * L::BLOCK) + 2 * (k % 4),
-                                      sdesc_mn_sw128(sbase + L::S_OFF + term * L::S_TERM, 0) + 128 * k,
-                                      I_64 | B_MN, (term | k) != 0);
-                if (QKB == 1) wait(p_ready(buf), (uint32_t)(c / QKB) & 1u);
-                wait(vt_ready, ph);
-                if (failed) break;
-                auto kv = [&](uint32_t slot, bool first) {
-                    const uint64_t da = sdesc_mn_sw128(stage + L::K, DK == 64 ? 0 : L::BLOCK);
-                    const uint64_t db = sdesc_mn_sw128(sbase + L::VT_OFF + slot * L::BLOCK, 0);
+                    for (int i = 0; i < 4; ++i) {
+                        raw[i] = lds128(vs + 2048 * (4 * half + i));
+                        f[i] = wv[r0 + 16 * (4 * half + i)];
+                    }
+                    uint32_t hi[4][4], mid[4][4], low[4][4];
 #pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        tc::umma_bf16(tmem + L::T_KV, da + 128 * k, db + 128 * k, I_64 | A_MN | B_MN,
-                                      !first || k != 0);
-                };
-                kv(0, true);
-                tc::umma_commit(vt_free);
-                kv(1, false);
-                if (QKB == 2) wait(p_ready(buf), (uint32_t)(c / QKB) & 1u);
-                if (failed) break;
-                const uint64_t dv = sdesc_mn_sw128(stage + L::V, 0);
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                        const uint64_t ff = mx::pack2(f[i], f[i]);
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    umma_ts(tmem + L::T_PV, tmem + buf * 128 + 8 * k, dv + 128 * k, I_64 | B_MN, k != 0);
-                tc::umma_commit(o_ready);
-                wait(vt3_ready, ph);
-                if (failed) break;
-                kv(0, false);
-                tc::umma_commit(kv_ready);
-                tc::umma_commit(empty(s));
-                if (QKB == 1 && c + 1 < nc) {
-                    wait(s_ready, ph ^ 1u);          // K^T V has been read: its columns are scores'
-                    if (!failed) issue_qk(c + 1);
+                        for (int j = 0; j < 4; ++j) {
+                            top = __vmaxu2(top, u[j] & 0x7FFF7FFFu);
+                            // 24 bits, cut into three times 8: exact
+                            uint64_t yz = mx::mul2(mx::pack2(lo_f(u[j]), hi_f(u[j])), ff);
+                            float y, z;
+                            mx::unpack2(yz, y, z);
+                            hi[i][j] = tops(y, z);
+                            yz = mx::fma2(mx::pack2(top_f(y), top_f(z)), minus, yz);
+                            mx::unpack2(yz, y, z);
+                            mid[i][j] = tops(y, z);
+                            yz = mx::fma2(mx::pack2(top_f(y), top_f(z)), minus, yz);
+                            mx::unpack2(yz, y, z);
+                            low[i][j] = tops(y, z);
+                        }
+                    }
+                    // the products have read the half before
+                    if (half) failed |= 1u - tc::mbar_wait_warp(vt_free, g & 1u, failed);
+                    else if (g) failed |= 1u - tc::mbar_wait_warp(kv_ready, (g - 1) & 1u, failed);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t o = vt + 2048 * i;
+                        sts128(o, make_uint4(hi[i][0], hi[i][1], hi[i][2], hi[i][3]));
+                        sts128(o + L::VT_TERM, make_uint4(mid[i][0], mid[i][1], mid[i][2], mid[i][3]));
+                        sts128(o + 2 * L::VT_TERM, make_uint4(low[i][0], low[i][1], low[i][2], low[i][3]));
+                    }
+                    if (half && tc::named_bar_any(1, 128, (top & 0xFFFFu) >= 0x7F80u || (top >> 16) >= 0x7F80u)) {
+                        // Values that are not finite: 0 * inf in the product of P and v would
+                        // reach the chunk's earlier rows.  There they become zero, and the
+                        // outputs of their columns NaN from their row on.
+                        int* rows = bad_row + (g & 1) * DV;
+                        if (t < DV) rows[t] = C;
+                        tc::named_bar_sync(1, 128);
+#pragma unroll 1
+                        for (int i = 0; i < 8; ++i) {
+                            const uint4 r4 = lds128(vs + 2048 * i);
+                            uint32_t u[4] = {r4.x, r4.y, r4.z, r4.w};
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                if ((u[j] & 0x7F80u) == 0x7F80u) {
+                                    atomicMin(&rows[8 * piece + 2 * j], r0 + 16 * i);
+                                    u[j] &= 0xFFFF0000u;
+                                }
+                                if ((u[j] & 0x7F800000u) == 0x7F800000u) {
+                                    atomicMin(&rows[8 * piece + 2 * j + 1], r0 + 16 * i);
+                                    u[j] &= 0xFFFFu;
+                                }
+                            }
+                            sts128(vs + 2048 * i, make_uint4(u[0], u[1], u[2], u[3]));
+                        }
+                        if (t == 0) bad_chunk[g & 1] = (int)g;
+                    }
+                    tc::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(vt_ready);
                 }
             }
-            tc::umma_commit(done);
         }
-        __syncwarp();
-        failed = __any_sync(0xffffffffu, failed);
-        failed |= 1u - tc::mbar_wait_warp<true>(done, 0, 0);
     }
     if (failed && lane == 0) atomicExch(p.status, SNNB_ERR_TIMEOUT);
     tc::tc_fence_before();
     __syncthreads();
-    if (warp == 13) {
+    if (warp == 17) {
         tc::tc_fence_after();
-        tc::tmem_dealloc(tmem, L::COLS);
+        tc::tmem_dealloc(tmem, T_COLS);
     }
 }
 
 // [B, N, heads, d] as a tensor map with boxes of 128 tokens x 64 columns of one head.
 int encode(CUtensorMap* m, const void* base, const int64_t* s, int64_t B, int64_t N, int64_t heads,
-           int64_t d) {
+           int64_t d, int rows = C) {
     const uint64_t dims[4] = {(uint64_t)d, (uint64_t)heads, (uint64_t)N, (uint64_t)B};
     const uint64_t st[3] = {heads > 1 ? (uint64_t)s[2] * 2 : 16, N > 1 ? (uint64_t)s[1] * 2 : 16,
                             B > 1 ? (uint64_t)s[0] * 2 : 16};
-    const uint32_t box[4] = {64, 1, C, 1};
+    const uint32_t box[4] = {64, 1, (uint32_t)rows, 1};
     return encode_tmap(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, st, box,
                        CU_TENSOR_MAP_SWIZZLE_128B);
 }
@@ -576,33 +755,76 @@ bool mappable(const void* base, const int64_t* s, int64_t B, int64_t N, int64_t 
     return aligned16(base) && ok(s[2], heads) && ok(s[1], N) && ok(s[0], B);
 }
 
-template <int DK>
-int launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const TcArgs& p,
-           cudaStream_t s) {
+// SMs of the current device.
+int sm_count() {
+    static int counts[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    if (!counts[dev] &&
+        cudaDeviceGetAttribute(&counts[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        return 148;
+    return counts[dev];
+}
+
+template <int DK, bool STATES>
+int launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& o,
+           TcArgs p, cudaStream_t s) {
     using L = Smem<DK>;
-    if (const int st = allow_smem<decay_tc_kernel<DK>>(L::DYN)) return st;
-    return launch_k(decay_tc_kernel<DK>, dim3((unsigned)(p.a.B * p.a.H * p.tiles)), dim3(THREADS),
-                    L::DYN, s, q, k, v, p);
+    if (const int st = allow_smem<decay_tc_kernel<DK, STATES>>(L::DYN)) return st;
+    p.items = (uint32_t)(p.a.B * p.a.H * p.tiles * (STATES ? p.segs - 1 : p.segs));
+    const int sms = sm_count();
+    return launch_k(decay_tc_kernel<DK, STATES>, dim3(p.items < (uint32_t)sms ? p.items : sms), dim3(THREADS),
+                    L::DYN, s, q, k, v, o, p);
+}
+template <int DK>
+int launches(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
+             const CUtensorMap& o, const TcArgs& p, cudaStream_t s) {
+    if (p.segs > 1)
+        if (const int st = launch<DK, true>(q, k, v, o, p, s)) return st;
+    return launch<DK, false>(q, k, v, o, p, s);
+}
+
+// Segments of each sequence where items do not fill the SMs.
+int segments(int64_t items, int64_t chunks) {
+    const char* e = getenv("SEGS");
+    if (e) return atoi(e);
+    return 1;
 }
 
 }  // namespace
 
 bool tc_takes(const Args& a, int dtype) {
     return dtype == SNNB_BF16 && a.N > 0 && a.N < 0x7fffff00 && a.dk <= 128 && a.dk % 8 == 0 &&
-           a.dv % 8 == 0 && a.H <= 0x7fffffff / 8 && mappable(a.q, a.qs, a.B, a.N, a.H) &&
+           a.dv % 8 == 0 && aligned16(a.out) && aligned16(a.state_in) && aligned16(a.state_out) &&
+           mappable(a.q, a.qs, a.B, a.N, a.H) &&
            mappable(a.k, a.ks, a.B, a.N, a.Hk) && mappable(a.v, a.vs, a.B, a.N, a.Hk);
 }
 
-int tc_run(const Args& a, cudaStream_t s) {
-    CUtensorMap q, k, v;
+int64_t tc_workspace(int dtype, int64_t B, int64_t N, int64_t H, int64_t dk, int64_t dv) {
+    if (dtype != SNNB_BF16 || dk > 128 || dk % 8 || dv % 8 || B == 0 || N == 0) return 0;
+    const int64_t items = B * H * ((dv + DV - 1) / DV);
+    const int segs = segments(items, (N + C - 1) / C);
+    return segs > 1 ? segs * items * (dk <= 64 ? 64 : 128) * DV * 4 : 0;
+}
+
+int tc_run(const Args& a, void* work, int64_t bytes, cudaStream_t s) {
+    CUtensorMap q, k, v, o = {};
     int rc = encode(&q, a.q, a.qs, a.B, a.N, a.H, a.dk);
     if (!rc) rc = encode(&k, a.k, a.ks, a.B, a.N, a.Hk, a.dk);
     if (!rc) rc = encode(&v, a.v, a.vs, a.B, a.N, a.Hk, a.dv);
+    const int64_t os[3] = {a.N * a.H * a.dv, a.H * a.dv, a.dv};
+    if (!rc && a.dk <= 64) rc = encode(&o, a.out, os, a.B, a.N, a.H, a.dv, 32);
     if (rc) return rc;
-    TcArgs p = {a, (a.dv + DV - 1) / DV, device_status_ptr(),
-                aligned16(a.state_in) && aligned16(a.state_out), aligned16(a.out)};
+    const int chunks = (int)((a.N + C - 1) / C), tiles = (a.dv + DV - 1) / DV;
+    int segs = segments(a.B * a.H * tiles, chunks);
+    const int cps = (chunks + segs - 1) / segs;
+    TcArgs p = {a, tiles, segs, cps, 0, static_cast<float*>(work), device_status_ptr(),
+                a.dv % 16 == 0 && reinterpret_cast<uintptr_t>(a.out) % 32 == 0};
     if (!p.status) return SNNB_ERR_CUDA;
-    return a.dk <= 64 ? launch<64>(q, k, v, p, s) : launch<128>(q, k, v, p, s);
+    if (segs > 1 && (!work || !aligned16(work) ||
+                     bytes < tc_workspace(SNNB_BF16, a.B, a.N, a.H, a.dk, a.dv)))
+        return SNNB_ERR_ARG;
+    return a.dk <= 64 ? launches<64>(q, k, v, o, p, s) : launches<128>(q, k, v, o, p, s);
 }
 
 }  // namespace decay
