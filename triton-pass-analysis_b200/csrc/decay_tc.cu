@@ -25,9 +25,9 @@ template <int DK> struct Smem {
     static constexpr int PW_OFF = O_OFF + (STAGED ? BLOCK : 0);  // 0 (31 times), decay^0 .. ^127
     static constexpr int RW_OFF = PW_OFF + 160 * 4;            // decay^31 .. decay^0
     static constexpr int WV_OFF = RW_OFF + 32 * 4;             // the factors of v's rows
-    static constexpr int BAD_OFF = WV_OFF + C * 4;             // [2][DV] rows, [2] chunk numbers
-    static constexpr int BAR_OFF = BAD_OFF + (2 * DV + 2) * 4;
-    static constexpr int NBARS = 2 * QK_STAGES + 2 * V_STAGES + 11;
+    static constexpr int BAD_OFF = WV_OFF + C * 4;             // [4][DV] rows, [4] chunk numbers
+    static constexpr int BAR_OFF = BAD_OFF + (4 * DV + 4) * 4;
+    static constexpr int NBARS = 2 * QK_STAGES + 2 * V_STAGES + 12;
     static constexpr int TMEM_OFF = BAR_OFF + NBARS * 8;
     static constexpr int DYN = TMEM_OFF + 8 + 1024;
     static_assert(DYN <= 227 * 1024, "shared memory");
@@ -38,12 +38,12 @@ template <int DK> struct Smem {
 // times the scaled v's three terms.
 constexpr int T_QK = 0, T_QS = 128, T_PV = 256, T_KV = 320, T_COLS = 512;
 
-// Warps 0-3 scores to P, 4-7 outputs, 8-11 the state, 12-15 scaled v, 16 copies, 17 MMAs, 18 and 19
-// with warps 2 and 3, whose rows have the most scores.
-constexpr int THREADS = 20 * 32;
-// Registers a thread of each group of four warps: no more than 96 on the average, the launch's.
-constexpr int REGS_P = 88, REGS_O = 80, REGS_S = 128, REGS_V = 96;      // P: warps 16-19 too
-static_assert(2 * REGS_P + REGS_O + REGS_S + REGS_V <= 5 * 96, "registers");
+// Warps 0-3 scores to P, 4 copies, 5 MMAs, 6 and 7 with warps 2 and 3, whose rows have the most
+// scores; 8-11 outputs, 12-15 the state, 16-19 and 20-23 scaled v, a half of each chunk.
+constexpr int THREADS = 24 * 32;
+// Registers a thread of each group of four warps: no more than 80 on the average, the launch's.
+constexpr int REGS_P = 80, REGS_O = 72, REGS_S = 120, REGS_V = 64;
+static_assert(2 * REGS_P + REGS_O + REGS_S + 2 * REGS_V <= 6 * 80, "registers");
 template <int N> __device__ __forceinline__ void fewer_regs() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
@@ -179,7 +179,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     float* rw = reinterpret_cast<float*>(smem + L::RW_OFF);
     float* wv = reinterpret_cast<float*>(smem + L::WV_OFF);
     int* bad_row = reinterpret_cast<int*>(smem + L::BAD_OFF);
-    volatile int* bad_chunk = bad_row + 2 * DV;
+    volatile int* bad_chunk = bad_row + 4 * DV;
     const uint32_t bar0 = sbase + L::BAR_OFF;
     auto qk_full = [&](uint32_t s) { return bar0 + 8u * s; };
     auto qk_empty = [&](uint32_t s) { return bar0 + 8u * (NQ + s); };
@@ -187,9 +187,10 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     auto v_empty = [&](uint32_t s) { return bar0 + 8u * (2 * NQ + NV + s); };
     const uint32_t misc = bar0 + 8u * (2 * NQ + 2 * NV);
     const uint32_t qk_ready = misc, p_ready = misc + 8, o_ready = misc + 16, o_free = misc + 24,
-                   vt_ready = misc + 32, kv_ready = misc + 40, kv_read = misc + 48,
+                   kv_ready = misc + 40, kv_read = misc + 48,
                    s_ready = misc + 56, qs_done = misc + 64, vt_free = misc + 72,
                    done = misc + 80;
+    auto vt_ready = [&](int half) { return misc + (half ? 88u : 32u); };
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + L::TMEM_OFF);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Args& a = p.a;
@@ -207,7 +208,8 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         tc::mbar_init(p_ready, 6);
         tc::mbar_init(o_ready, 1);
         tc::mbar_init(o_free, 4);
-        tc::mbar_init(vt_ready, 4);
+        tc::mbar_init(vt_ready(0), 4);
+        tc::mbar_init(vt_ready(1), 4);
         tc::mbar_init(kv_ready, 1);
         tc::mbar_init(kv_read, 4);
         tc::mbar_init(qs_done, 1);
@@ -218,9 +220,10 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         tc::prefetch_tmap(&tmQ);
         tc::prefetch_tmap(&tmK);
         tc::prefetch_tmap(&tmV);
-        bad_chunk[0] = bad_chunk[1] = -1;
+        for (int i = 0; i < 4; ++i) bad_chunk[i] = -1;
     }
-    if (warp == 17) {
+    if (threadIdx.x < 4 * DV) bad_row[threadIdx.x] = C;
+    if (warp == 5) {
         tc::tmem_alloc(sbase + L::TMEM_OFF, T_COLS);
         tc::tmem_relinquish();
     }
@@ -233,9 +236,8 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 
     // Every role walks the block's items and their chunks; g counts the chunks of all.
     uint32_t failed = 0, g = 0;
-    if (warp < 4 || warp >= 16) {
-        fewer_regs<REGS_P>();
-        if (warp == 16) {
+    if (warp < 8) {
+        if (warp == 4) {
             // ------------------------------------------------ copies
             uint32_t issued_qk = 0, issued_v = 0;
             for (uint32_t it = blockIdx.x; it < p.items; it += gridDim.x) {
@@ -276,7 +278,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     tc::mbar_wait_warp<true>(v_full(i % NV), (i / NV) & 1u, 0);
                 }
             }
-        } else if (warp == 17) {
+        } else if (warp == 5) {
             // ------------------------------------------------ MMAs
             if (tc::elect_one()) {
                 auto wait = [&](uint32_t bar, uint32_t parity) {
@@ -305,7 +307,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     // k^T times the three terms of the scaled v, side by side, by half chunks
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        wait(vt_ready, (uint32_t)half);
+                        wait(vt_ready(half), ph);
                         if (failed) break;
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
@@ -348,9 +350,9 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         } else {
             // ------------------------------------------------ scores to P
             // Blocks of 32 x 32: a warp has those of its rows (its lanes of TMEM) up to the
-            // diagonal one; the third and the fourth of the last two warps' rows go to warps 18
-            // and 19.
-            const int q = warp & 3, first = warp >= 18 ? 2 : 0, row = 32 * q + lane;
+            // diagonal one; the third and the fourth of the last two warps' rows go to warps 6
+            // and 7.
+            const int q = warp & 3, first = warp >= 6 ? 2 : 0, row = 32 * q + lane;
             const bool two = q == 3 || (q >= 1 && first == 0);     // of these two blocks
             const int diag = q >= 2 && first == 0 ? -1 : q - first;     // which of the two, if any
             const uint32_t tl = tmem + ((uint32_t)(32 * q) << 16) + T_QK;
@@ -365,53 +367,48 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     if (row < 31) pw[row] = 0.0f;
                 }
                 tc::named_bar_sync(2, 6 * 32);
-                float f0 = diag == 0 ? 0.0f : pw[row - 32 * first],
-                      f1 = diag == 1 || !two ? 0.0f : pw[row - 32 * first - 32];
+                const float f0 = diag == 0 ? 0.0f : pw[row - 32 * first],
+                            f1 = diag == 1 || !two ? 0.0f : pw[row - 32 * first - 32];
 #pragma unroll 1
                 for (int c = 0; c < x.n; ++c, ++g) {
                     failed |= 1u - tc::mbar_wait_warp(qk_ready, g & 1u, failed);
                     tc::tc_fence_after();
-                    float s[32], s1[32];
-                    tc::tmem_ld32(tl + first * 32, s);
-                    if (two) tc::tmem_ld32(tl + first * 32 + 32, s1);
-                    tc::tmem_wait_ld();
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(s[i]), "+f"(s1[i]));
-                    // P takes the place of scores that the other warp of these rows reads
-                    if (q >= 2) tc::named_bar_sync(3 + q, 64);
 #pragma unroll 1
                     for (int blk = 0; blk < 2; ++blk) {
                         uint32_t w[16];
-                        if (blk == 0 || two) {
-                            if (blk == diag) {
-                                // later tokens count nothing, whatever their scores
-                                const float* d = pw + 31 + lane;
+                        float s[32];
+                        if (blk == 0 || two) tc::tmem_ld32(tl + (first + blk) * 32, s);
+                        tc::tmem_wait_ld();
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) {
-                                    const float y = s[i] * d[-i];
-                                    s[i] = i <= lane ? y : 0.0f;
-                                }
-                            } else {
-                                const float f = blk ? f1 : f0;
-                                const uint64_t ff = mx::pack2(f, f);
+                        for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(s[i]));
+                        // P of the third and fourth blocks takes the place of the second one's
+                        // scores, once those have been read
+                        if (q >= 2 && first == 0 && blk == 1) tc::named_bar_sync(3 + q, 64);
+                        if (blk == diag) {
+                            // later tokens count nothing, whatever their scores
+                            const float* d = pw + 31 + lane;
 #pragma unroll
-                                for (int i = 0; i < 32; i += 4) {
-                                    const float4 r = *reinterpret_cast<const float4*>(rw + i);
-                                    mx::unpack2(mx::mul2(mx::pack2(s[i], s[i + 1]),
-                                                         mx::mul2(ff, mx::pack2(r.x, r.y))), s[i], s[i + 1]);
-                                    mx::unpack2(mx::mul2(mx::pack2(s[i + 2], s[i + 3]),
-                                                         mx::mul2(ff, mx::pack2(r.z, r.w))), s[i + 2], s[i + 3]);
-                                }
+                            for (int i = 0; i < 32; ++i) {
+                                const float y = s[i] * d[-i];
+                                s[i] = i <= lane ? y : 0.0f;
                             }
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) w[i] = bf2(s[2 * i], s[2 * i + 1]);
                         } else {
+                            const float f = blk ? f1 : f0;
+                            const uint64_t ff = mx::pack2(f, f);
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) w[i] = 0;
+                            for (int i = 0; i < 32; i += 4) {
+                                const float4 r = *reinterpret_cast<const float4*>(rw + i);
+                                mx::unpack2(mx::mul2(mx::pack2(s[i], s[i + 1]),
+                                                     mx::mul2(ff, mx::pack2(r.x, r.y))), s[i], s[i + 1]);
+                                mx::unpack2(mx::mul2(mx::pack2(s[i + 2], s[i + 3]),
+                                                     mx::mul2(ff, mx::pack2(r.z, r.w))), s[i + 2], s[i + 3]);
+                            }
                         }
-                        tmem_st16(tl + (first + blk) * 16, w);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) s[i] = s1[i];
+                        for (int i = 0; i < 16; ++i)
+                            w[i] = blk == 0 || two ? bf2(s[2 * i], s[2 * i + 1]) : 0u;
+                        if (q >= 2 && first == 2 && blk == 0) tc::named_bar_sync(3 + q, 64);
+                        tmem_st16(tl + (first + blk) * 16, w);
                     }
                     if (q < 2) {                     // blocks of later tokens
                         const uint32_t zero[16] = {};
@@ -425,7 +422,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 }
             }
         }
-    } else if (warp < 8) {
+    } else if (warp < 12) {
         // ---------------------------------------------------- outputs
         fewer_regs<REGS_O>();
         const int q = warp & 3, row = 32 * q + lane;
@@ -449,7 +446,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 }
                 failed |= 1u - tc::mbar_wait_warp(o_ready, g & 1u, failed);
                 tc::tc_fence_after();
-                const bool spoiled = bad_chunk[g & 1] == (int)g, alive = n < x.len;
+                const bool spoiled = bad_chunk[g & 3] == (int)g, alive = n < x.len;
                 const bool write = n < a.N && !failed && SNNB_IN_BOUNDS(n, a.N, p.status);
 #pragma unroll 1
                 for (int i = 0; i < DV; i += 16) {
@@ -474,7 +471,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                                     v[j + 1]);
                     }
                     if (spoiled) {
-                        const int* rows = bad_row + (g & 1) * DV + i;
+                        const int* rows = bad_row + (g & 3) * DV + i;
 #pragma unroll
                         for (int j = 0; j < 16; ++j)
                             if (row >= rows[j]) v[j] = __int_as_float(0x7fffffff);
@@ -487,6 +484,10 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     } else if (write) {
                         store16(out + i, w, cols - i, p.out32);
                     }
+                }
+                if (spoiled) {                       // for the fourth chunk from here
+                    tc::named_bar_sync(7, 128);
+                    if (row < DV) bad_row[(g & 3) * DV + row] = C;
                 }
                 if (L::STAGED) {
                     tc::fence_proxy_async_smem();
@@ -510,12 +511,12 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             }
         }
         if (lane == 0) tc::bulk_wait_group<0>();     // the copies have left shared memory
-    } else if (warp < 12) {
+    } else if (warp < 16) {
         // ---------------------------------------------------- the state
         // This thread's row and columns: DK = 64 products have 128 rows, the second 64 the
         // first's copy, so that each half of the threads takes half of the columns.
         more_regs<REGS_S>();
-        const int t = threadIdx.x - 256;
+        const int t = threadIdx.x - 384;
         constexpr int W = DK == 64 ? 32 : 64;
         const int row = t % DK, col = DK == 64 ? t / 64 * 32 : 0;
         const uint32_t tl = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + T_KV + col;
@@ -624,7 +625,9 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         }
     } else {
         // ---------------------------------------------------- v scaled, as three bf16 terms
-        const int t = threadIdx.x - 384, piece = t & 7, r0 = t >> 3;
+        fewer_regs<REGS_V>();
+        const int t = threadIdx.x - 512, half = t >> 7;        // of each chunk
+        const int piece = t & 7, r0 = (t >> 3) & 15, first = 64 * half + r0;
         const uint32_t vt = sbase + L::VT_OFF + swizzled(r0, piece);
         const uint64_t minus = mx::pack2(-1.0f, -1.0f);
         for (uint32_t it = blockIdx.x; it < p.items; it += gridDim.x) {
@@ -635,21 +638,21 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 const uint32_t s = g % NV, sq = g % NQ;
                 const int m = c + 1 == x.n ? x.last : C;
                 if (m != held) {
-                    tc::named_bar_sync(1, 128);
-                    wv[t] = t < m ? (float)power(x.lam, m - 1 - t) : 0.0f;
+                    tc::named_bar_sync(1, 256);
+                    if (t < C) wv[t] = t < m ? (float)power(x.lam, m - 1 - t) : 0.0f;
                     held = m;
-                    tc::named_bar_sync(1, 128);
+                    tc::named_bar_sync(1, 256);
                 }
                 failed |= 1u - tc::mbar_wait_warp(v_full(s), (g / NV) & 1u, failed);
-                const uint32_t vs = sbase + L::V_OFF + s * L::BLOCK + swizzled(r0, piece);
+                const uint32_t vs = sbase + L::V_OFF + s * L::BLOCK + swizzled(first, piece);
                 if (m < C) {
                     // rows behind the sequence, whatever they hold (beyond the tensor: zeros)
                     failed |= 1u - tc::mbar_wait_warp(qk_full(sq), (g / NQ) & 1u, failed);
-                    const uint32_t ks = sbase + sq * L::QK_STAGE + L::KB * L::BLOCK + swizzled(r0, piece);
+                    const uint32_t ks = sbase + sq * L::QK_STAGE + L::KB * L::BLOCK + swizzled(first, piece);
                     const uint4 zero = make_uint4(0, 0, 0, 0);
 #pragma unroll 1
-                    for (int i = 0; i < 8; ++i)
-                        if (r0 + 16 * i >= m) {
+                    for (int i = 0; i < 4; ++i)
+                        if (first + 16 * i >= m) {
                             sts128(vs + 2048 * i, zero);
 #pragma unroll
                             for (int k = 0; k < L::KB; ++k) sts128(ks + k * L::BLOCK + 2048 * i, zero);
@@ -657,17 +660,17 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 }
                 uint32_t top = 0;
 #pragma unroll 1
-                for (int half = 0; half < 2; ++half) {
-                    uint4 raw[4];
-                    float f[4];
+                for (int i0 = 0; i0 < 4; i0 += 2) {
+                    uint4 raw[2];
+                    float f[2];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        raw[i] = lds128(vs + 2048 * (4 * half + i));
-                        f[i] = wv[r0 + 16 * (4 * half + i)];
+                    for (int i = 0; i < 2; ++i) {
+                        raw[i] = lds128(vs + 2048 * (i0 + i));
+                        f[i] = wv[first + 16 * (i0 + i)];
                     }
-                    uint32_t hi[4][4], mid[4][4], low[4][4];
+                    uint32_t hi[2][4], mid[2][4], low[2][4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < 2; ++i) {
                         const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
                         const uint64_t ff = mx::pack2(f[i], f[i]);
 #pragma unroll
@@ -687,52 +690,52 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         }
                     }
                     // the products have read the half before
-                    if (half) failed |= 1u - tc::mbar_wait_warp(vt_free, g & 1u, failed);
-                    else if (g) failed |= 1u - tc::mbar_wait_warp(kv_ready, (g - 1) & 1u, failed);
+                    if (i0 == 0) {
+                        if (half) failed |= 1u - tc::mbar_wait_warp(vt_free, g & 1u, failed);
+                        else if (g) failed |= 1u - tc::mbar_wait_warp(kv_ready, (g - 1) & 1u, failed);
+                    }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t o = vt + 2048 * i;
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t o = vt + 2048 * (i0 + i);
                         sts128(o, make_uint4(hi[i][0], hi[i][1], hi[i][2], hi[i][3]));
                         sts128(o + L::VT_TERM, make_uint4(mid[i][0], mid[i][1], mid[i][2], mid[i][3]));
                         sts128(o + 2 * L::VT_TERM, make_uint4(low[i][0], low[i][1], low[i][2], low[i][3]));
                     }
-                    if (half && tc::named_bar_any(1, 128, (top & 0xFFFFu) >= 0x7F80u || (top >> 16) >= 0x7F80u)) {
-                        // Values that are not finite: 0 * inf in the product of P and v would
-                        // reach the chunk's earlier rows.  There they become zero, and the
-                        // outputs of their columns NaN from their row on.
-                        int* rows = bad_row + (g & 1) * DV;
-                        if (t < DV) rows[t] = C;
-                        tc::named_bar_sync(1, 128);
-#pragma unroll 1
-                        for (int i = 0; i < 8; ++i) {
-                            const uint4 r4 = lds128(vs + 2048 * i);
-                            uint32_t u[4] = {r4.x, r4.y, r4.z, r4.w};
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                if ((u[j] & 0x7F80u) == 0x7F80u) {
-                                    atomicMin(&rows[8 * piece + 2 * j], r0 + 16 * i);
-                                    u[j] &= 0xFFFF0000u;
-                                }
-                                if ((u[j] & 0x7F800000u) == 0x7F800000u) {
-                                    atomicMin(&rows[8 * piece + 2 * j + 1], r0 + 16 * i);
-                                    u[j] &= 0xFFFFu;
-                                }
-                            }
-                            sts128(vs + 2048 * i, make_uint4(u[0], u[1], u[2], u[3]));
-                        }
-                        if (t == 0) bad_chunk[g & 1] = (int)g;
-                    }
-                    tc::fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(vt_ready);
                 }
+                if (__any_sync(0xffffffffu, (top & 0xFFFFu) >= 0x7F80u || (top >> 16) >= 0x7F80u)) {
+                    // Values that are not finite: 0 * inf in the product of P and v would reach
+                    // the chunk's earlier rows.  There they become zero, and the outputs of their
+                    // columns NaN from their row on.
+                    if (lane == 0) bad_chunk[g & 3] = (int)g;
+                    int* rows = bad_row + (g & 3) * DV + 8 * piece;
+#pragma unroll 1
+                    for (int i = 0; i < 4; ++i) {
+                        const uint4 r4 = lds128(vs + 2048 * i);
+                        uint32_t u[4] = {r4.x, r4.y, r4.z, r4.w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if ((u[j] & 0x7F80u) == 0x7F80u) {
+                                atomicMin(&rows[2 * j], first + 16 * i);
+                                u[j] &= 0xFFFF0000u;
+                            }
+                            if ((u[j] & 0x7F800000u) == 0x7F800000u) {
+                                atomicMin(&rows[2 * j + 1], first + 16 * i);
+                                u[j] &= 0xFFFFu;
+                            }
+                        }
+                        sts128(vs + 2048 * i, make_uint4(u[0], u[1], u[2], u[3]));
+                    }
+                }
+                tc::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(vt_ready(half));
             }
         }
     }
     if (failed && lane == 0) atomicExch(p.status, SNNB_ERR_TIMEOUT);
     tc::tc_fence_before();
     __syncthreads();
-    if (warp == 17) {
+    if (warp == 5) {
         tc::tc_fence_after();
         tc::tmem_dealloc(tmem, T_COLS);
     }
