@@ -13,15 +13,16 @@ constexpr int DV = 64;             // columns of v, and of the state, that a thr
 template <int DK> struct Smem {
     static constexpr int KB = DK / 64;                         // 64-column blocks of q and k
     static constexpr int BLOCK = C * 128;                      // 128 rows of 128 bytes
-    static constexpr int QK_STAGES = DK == 64 ? 3 : 2, V_STAGES = DK == 64 ? 3 : 2;
+    static constexpr int QK_STAGES = DK == 64 ? 3 : 2, V_STAGES = 2;
     static constexpr int QK_STAGE = 2 * KB * BLOCK;            // q, then k
     static constexpr int V_OFF = QK_STAGES * QK_STAGE;
     static constexpr int S_OFF = V_OFF + V_STAGES * BLOCK;     // state: high and low terms
     static constexpr int S_TERM = DK * 128;
-    static constexpr int VT_OFF = S_OFF + 2 * S_TERM;          // scaled v: half a chunk's three terms
-    static constexpr int VT_TERM = BLOCK / 2;
+    // the scaled v's three terms: both halves of a chunk where there is room, else one at a time
+    static constexpr int VT_HALVES = DK == 64 ? 2 : 1;
+    static constexpr int VT_OFF = S_OFF + 2 * S_TERM, VT_TERM = BLOCK / 2, VT_HALF = 3 * VT_TERM;
     static constexpr bool STAGED = DK == 64;                   // outputs leave by bulk copies
-    static constexpr int O_OFF = VT_OFF + 3 * VT_TERM;         // 32 rows for each warp
+    static constexpr int O_OFF = VT_OFF + VT_HALVES * VT_HALF;         // 32 rows for each warp
     static constexpr int PW_OFF = O_OFF + (STAGED ? BLOCK : 0);  // 0 (31 times), decay^0 .. ^127
     static constexpr int RW_OFF = PW_OFF + 160 * 4;            // decay^31 .. decay^0
     static constexpr int WV_OFF = RW_OFF + 32 * 4;             // the factors of v's rows
@@ -41,8 +42,9 @@ constexpr int T_QK = 0, T_QS = 128, T_PV = 256, T_KV = 320, T_COLS = 512;
 // Warps 0-3 scores to P, 4 copies, 5 MMAs, 6 and 7 with warps 2 and 3, whose rows have the most
 // scores; 8-11 outputs, 12-15 the state, 16-19 and 20-23 scaled v, a half of each chunk.
 constexpr int THREADS = 24 * 32;
-// Registers a thread of each group of four warps: no more than 80 on the average, the launch's.
-constexpr int REGS_P = 80, REGS_O = 72, REGS_S = 120, REGS_V = 64;
+// Registers a thread of each group of four warps, each of which sets its own before its role: no
+// more than 80 on the average, the launch's, or the state's warps would wait for theirs forever.
+constexpr int REGS_P = 72, REGS_O = 72, REGS_S = 120, REGS_V = 72;
 static_assert(2 * REGS_P + REGS_O + REGS_S + 2 * REGS_V <= 6 * 80, "registers");
 template <int N> __device__ __forceinline__ void fewer_regs() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
@@ -134,6 +136,22 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
                  : "memory");
     return v;
 }
+// Tables: written between barriers that the compiler does not move these across.
+__device__ __forceinline__ float lds_f(uint32_t a) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ float4 lds_f4(uint32_t a) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(a));
+    return v;
+}
+__device__ __forceinline__ void sts_f(uint32_t a, float v) {
+    asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
+}
 // Byte offset of 16-byte piece `piece` of row `row` in a tile of 128-byte rows.
 __device__ __forceinline__ uint32_t swizzled(int row, int piece) {
     return (uint32_t)(row * 128 + ((piece ^ (row & 7)) << 4));
@@ -175,9 +193,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     uint8_t* smem = reinterpret_cast<uint8_t*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sbase = tc::smem_u32(smem);
-    float* pw = reinterpret_cast<float*>(smem + L::PW_OFF);
-    float* rw = reinterpret_cast<float*>(smem + L::RW_OFF);
-    float* wv = reinterpret_cast<float*>(smem + L::WV_OFF);
+    const uint32_t pw = sbase + L::PW_OFF, rw = sbase + L::RW_OFF, wv = sbase + L::WV_OFF;
     int* bad_row = reinterpret_cast<int*>(smem + L::BAD_OFF);
     volatile int* bad_chunk = bad_row + 4 * DV;
     const uint32_t bar0 = sbase + L::BAR_OFF;
@@ -237,6 +253,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     // Every role walks the block's items and their chunks; g counts the chunks of all.
     uint32_t failed = 0, g = 0;
     if (warp < 8) {
+        fewer_regs<REGS_P>();
         if (warp == 4) {
             // ------------------------------------------------ copies
             uint32_t issued_qk = 0, issued_v = 0;
@@ -313,7 +330,8 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         for (int i = 0; i < 4; ++i)
                             tc::umma_bf16(tmem + T_KV,
                                           sdesc_mn_sw128(k, DK == 64 ? 0 : L::BLOCK) + 128 * (4 * half + i),
-                                          sdesc_mn_sw128(sbase + L::VT_OFF, L::VT_TERM) + 128 * i,
+                                          sdesc_mn_sw128(sbase + L::VT_OFF + (L::VT_HALVES - 1) * half * L::VT_HALF,
+                                                         L::VT_TERM) + 128 * i,
                                           tc::idesc_bf16_f32(128, 192) | A_MN | B_MN, (half | i) != 0);
                         tc::umma_commit(half ? kv_ready : vt_free);
                     }
@@ -362,13 +380,13 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 tc::named_bar_sync(2, 6 * 32);       // the last item's table has been read
                 if (warp < 4) {
                     const float f = (float)power(x.lam, row);
-                    pw[31 + row] = f;
-                    if (row < 32) rw[31 - row] = f;
-                    if (row < 31) pw[row] = 0.0f;
+                    sts_f(pw + 4 * (31 + row), f);
+                    if (row < 32) sts_f(rw + 4 * (31 - row), f);
+                    if (row < 31) sts_f(pw + 4 * row, 0.0f);
                 }
                 tc::named_bar_sync(2, 6 * 32);
-                const float f0 = diag == 0 ? 0.0f : pw[row - 32 * first],
-                            f1 = diag == 1 || !two ? 0.0f : pw[row - 32 * first - 32];
+                const float f0 = diag == 0 ? 0.0f : lds_f(pw + 4 * (row - 32 * first)),
+                            f1 = diag == 1 || !two ? 0.0f : lds_f(pw + 4 * (row - 32 * first - 32));
 #pragma unroll 1
                 for (int c = 0; c < x.n; ++c, ++g) {
                     failed |= 1u - tc::mbar_wait_warp(qk_ready, g & 1u, failed);
@@ -386,10 +404,10 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         if (q >= 2 && first == 0 && blk == 1) tc::named_bar_sync(3 + q, 64);
                         if (blk == diag) {
                             // later tokens count nothing, whatever their scores
-                            const float* d = pw + 31 + lane;
+                            const uint32_t d = pw + 4 * (31 + lane);
 #pragma unroll
                             for (int i = 0; i < 32; ++i) {
-                                const float y = s[i] * d[-i];
+                                const float y = s[i] * lds_f(d - 4 * i);
                                 s[i] = i <= lane ? y : 0.0f;
                             }
                         } else {
@@ -397,7 +415,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                             const uint64_t ff = mx::pack2(f, f);
 #pragma unroll
                             for (int i = 0; i < 32; i += 4) {
-                                const float4 r = *reinterpret_cast<const float4*>(rw + i);
+                                const float4 r = lds_f4(rw + 4 * i);
                                 mx::unpack2(mx::mul2(mx::pack2(s[i], s[i + 1]),
                                                      mx::mul2(ff, mx::pack2(r.x, r.y))), s[i], s[i + 1]);
                                 mx::unpack2(mx::mul2(mx::pack2(s[i + 2], s[i + 3]),
@@ -628,7 +646,8 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         fewer_regs<REGS_V>();
         const int t = threadIdx.x - 512, half = t >> 7;        // of each chunk
         const int piece = t & 7, r0 = (t >> 3) & 15, first = 64 * half + r0;
-        const uint32_t vt = sbase + L::VT_OFF + swizzled(r0, piece);
+        const uint32_t vt = sbase + L::VT_OFF + (L::VT_HALVES == 2 ? half * L::VT_HALF : 0) +
+                            swizzled(r0, piece);
         const uint64_t minus = mx::pack2(-1.0f, -1.0f);
         for (uint32_t it = blockIdx.x; it < p.items; it += gridDim.x) {
             const Item x(p, it);
@@ -639,7 +658,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 const int m = c + 1 == x.n ? x.last : C;
                 if (m != held) {
                     tc::named_bar_sync(1, 256);
-                    if (t < C) wv[t] = t < m ? (float)power(x.lam, m - 1 - t) : 0.0f;
+                    if (t < C) sts_f(wv + 4 * t, t < m ? (float)power(x.lam, m - 1 - t) : 0.0f);
                     held = m;
                     tc::named_bar_sync(1, 256);
                 }
@@ -658,49 +677,40 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                             for (int k = 0; k < L::KB; ++k) sts128(ks + k * L::BLOCK + 2048 * i, zero);
                         }
                 }
-                uint32_t top = 0;
-#pragma unroll 1
-                for (int i0 = 0; i0 < 4; i0 += 2) {
-                    uint4 raw[2];
-                    float f[2];
+                uint32_t top = 0, hi[4][4], mid[4][4], low[4][4];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        raw[i] = lds128(vs + 2048 * (i0 + i));
-                        f[i] = wv[first + 16 * (i0 + i)];
-                    }
-                    uint32_t hi[2][4], mid[2][4], low[2][4];
+                for (int i = 0; i < 4; ++i) {
+                    const uint4 raw = lds128(vs + 2048 * i);
+                    const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+                    const float f = lds_f(wv + 4 * (first + 16 * i));
+                    const uint64_t ff = mx::pack2(f, f);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-                        const uint64_t ff = mx::pack2(f[i], f[i]);
+                    for (int j = 0; j < 4; ++j) {
+                        top = __vmaxu2(top, u[j] & 0x7FFF7FFFu);
+                        // 24 bits, cut into three times 8: exact
+                        uint64_t yz = mx::mul2(mx::pack2(lo_f(u[j]), hi_f(u[j])), ff);
+                        float y, z;
+                        mx::unpack2(yz, y, z);
+                        hi[i][j] = tops(y, z);
+                        yz = mx::fma2(mx::pack2(top_f(y), top_f(z)), minus, yz);
+                        mx::unpack2(yz, y, z);
+                        mid[i][j] = tops(y, z);
+                        yz = mx::fma2(mx::pack2(top_f(y), top_f(z)), minus, yz);
+                        mx::unpack2(yz, y, z);
+                        low[i][j] = tops(y, z);
+                    }
+                }
+                // the products have read what was there
+                if (half && L::VT_HALVES == 1)
+                    failed |= 1u - tc::mbar_wait_warp(vt_free, g & 1u, failed);
+                else if (g)
+                    failed |= 1u - tc::mbar_wait_warp(kv_ready, (g - 1) & 1u, failed);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            top = __vmaxu2(top, u[j] & 0x7FFF7FFFu);
-                            // 24 bits, cut into three times 8: exact
-                            uint64_t yz = mx::mul2(mx::pack2(lo_f(u[j]), hi_f(u[j])), ff);
-                            float y, z;
-                            mx::unpack2(yz, y, z);
-                            hi[i][j] = tops(y, z);
-                            yz = mx::fma2(mx::pack2(top_f(y), top_f(z)), minus, yz);
-                            mx::unpack2(yz, y, z);
-                            mid[i][j] = tops(y, z);
-                            yz = mx::fma2(mx::pack2(top_f(y), top_f(z)), minus, yz);
-                            mx::unpack2(yz, y, z);
-                            low[i][j] = tops(y, z);
-                        }
-                    }
-                    // the products have read the half before
-                    if (i0 == 0) {
-                        if (half) failed |= 1u - tc::mbar_wait_warp(vt_free, g & 1u, failed);
-                        else if (g) failed |= 1u - tc::mbar_wait_warp(kv_ready, (g - 1) & 1u, failed);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t o = vt + 2048 * (i0 + i);
-                        sts128(o, make_uint4(hi[i][0], hi[i][1], hi[i][2], hi[i][3]));
-                        sts128(o + L::VT_TERM, make_uint4(mid[i][0], mid[i][1], mid[i][2], mid[i][3]));
-                        sts128(o + 2 * L::VT_TERM, make_uint4(low[i][0], low[i][1], low[i][2], low[i][3]));
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t o = vt + 2048 * i;
+                    sts128(o, make_uint4(hi[i][0], hi[i][1], hi[i][2], hi[i][3]));
+                    sts128(o + L::VT_TERM, make_uint4(mid[i][0], mid[i][1], mid[i][2], mid[i][3]));
+                    sts128(o + 2 * L::VT_TERM, make_uint4(low[i][0], low[i][1], low[i][2], low[i][3]));
                 }
                 if (__any_sync(0xffffffffu, (top & 0xFFFFu) >= 0x7F80u || (top >> 16) >= 0x7F80u)) {
                     // Values that are not finite: 0 * inf in the product of P and v would reach
