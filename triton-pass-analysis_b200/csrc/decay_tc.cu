@@ -10,18 +10,20 @@ namespace {
 constexpr int C = 128;             // tokens of a chunk
 constexpr int DV = 64;             // columns of v, and of the state, that a thread block takes
 
-template <int DK> struct Smem {
+// STATES: no q, scores or outputs.
+template <int DK, bool STATES> struct Smem {
     static constexpr int KB = DK / 64;                         // 64-column blocks of q and k
     static constexpr int BLOCK = C * 128;                      // 128 rows of 128 bytes
-    static constexpr int QK_STAGES = DK == 64 ? 3 : 2, V_STAGES = 2;
-    static constexpr int QK_STAGE = 2 * KB * BLOCK;            // q, then k
+    static constexpr int QK_STAGES = DK == 64 || STATES ? 3 : 2, V_STAGES = STATES ? 3 : 2;
+    static constexpr int K_IN_STAGE = STATES ? 0 : KB * BLOCK; // q, then k
+    static constexpr int QK_STAGE = K_IN_STAGE + KB * BLOCK;
     static constexpr int V_OFF = QK_STAGES * QK_STAGE;
     static constexpr int S_OFF = V_OFF + V_STAGES * BLOCK;     // state: high and low terms
-    static constexpr int S_TERM = DK * 128;
+    static constexpr int S_TERM = STATES ? 0 : DK * 128;
     // the scaled v's three terms: both halves of a chunk where there is room, else one at a time
-    static constexpr int VT_HALVES = DK == 64 ? 2 : 1;
+    static constexpr int VT_HALVES = DK == 64 || STATES ? 2 : 1;
     static constexpr int VT_OFF = S_OFF + 2 * S_TERM, VT_TERM = BLOCK / 2, VT_HALF = 3 * VT_TERM;
-    static constexpr bool STAGED = DK == 64;                   // outputs leave by bulk copies
+    static constexpr bool STAGED = DK == 64 && !STATES;                   // outputs leave by bulk copies
     static constexpr int O_OFF = VT_OFF + VT_HALVES * VT_HALF;         // 32 rows for each warp
     static constexpr int PW_OFF = O_OFF + (STAGED ? BLOCK : 0);  // 0 (31 times), decay^0 .. ^127
     static constexpr int RW_OFF = PW_OFF + 160 * 4;            // decay^31 .. decay^0
@@ -187,7 +189,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
                 const __grid_constant__ TcArgs p) {
-    using L = Smem<DK>;
+    using L = Smem<DK, STATES>;
     constexpr int NQ = L::QK_STAGES, NV = L::V_STAGES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -264,8 +266,8 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     const int n0 = (x.c0 + c) * C;
                     failed |= 1u - tc::mbar_wait_warp(qk_empty(s), ((g / NQ) & 1u) ^ 1u, failed);
                     if (!failed && tc::elect_one()) {
-                        const uint32_t q = sbase + s * L::QK_STAGE, k = q + L::KB * L::BLOCK;
-                        tc::mbar_expect_tx(qk_full(s), (uint32_t)(L::QK_STAGE / (STATES ? 2 : 1)));
+                        const uint32_t q = sbase + s * L::QK_STAGE, k = q + L::K_IN_STAGE;
+                        tc::mbar_expect_tx(qk_full(s), (uint32_t)L::QK_STAGE);
 #pragma unroll
                         for (int i = 0; i < L::KB; ++i) {
                             if (!STATES)
@@ -305,8 +307,11 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 uint32_t chunks = 0;
                 for (uint32_t it = blockIdx.x; it < p.items; it += gridDim.x) chunks += Item(p, it).n;
                 auto issue_qk = [&](uint32_t c) {
-                    const uint32_t q = sbase + (c % NQ) * L::QK_STAGE, k = q + L::KB * L::BLOCK;
+                    const uint32_t q = sbase + (c % NQ) * L::QK_STAGE, k = q + L::K_IN_STAGE;
                     wait(qk_full(c % NQ), (c / NQ) & 1u);
+                    // products of different shapes are in no order of their own: P V of the chunk
+                    // before, whose P the scores overwrite, has to be done
+                    if (c && !STATES) wait(o_ready, (c - 1) & 1u);
                     if (failed || STATES) return;
 #pragma unroll
                     for (int i = 0; i < 4 * L::KB; ++i)
@@ -318,7 +323,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 #pragma unroll 1
                 for (g = 0; g < chunks && !failed; ++g) {
                     const uint32_t ph = g & 1u, s = g % NQ, sv = g % NV;
-                    const uint32_t q = sbase + s * L::QK_STAGE, k = q + L::KB * L::BLOCK;
+                    const uint32_t q = sbase + s * L::QK_STAGE, k = q + L::K_IN_STAGE;
                     issue_qk(g);
                     if (g) wait(kv_read, ph ^ 1u);
                     // k^T times the three terms of the scaled v, side by side, by half chunks
@@ -335,8 +340,8 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                                           tc::idesc_bf16_f32(128, 192) | A_MN | B_MN, (half | i) != 0);
                         tc::umma_commit(half ? kv_ready : vt_free);
                     }
-                    wait(s_ready, ph);
                     if (!STATES) {
+                        wait(s_ready, ph);
                         if (g) wait(o_free, ph ^ 1u);
                         if (failed) break;
                         // q times both terms of the state, side by side
@@ -502,6 +507,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     } else if (write) {
                         store16(out + i, w, cols - i, p.out32);
                     }
+                    __syncwarp();
                 }
                 if (spoiled) {                       // for the fourth chunk from here
                     tc::named_bar_sync(7, 128);
@@ -605,9 +611,9 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         sts128(o + L::S_TERM, make_uint4(lo[0], lo[1], lo[2], lo[3]));
                     }
                     tc::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(s_ready);
                 }
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(s_ready);
                 failed |= 1u - tc::mbar_wait_warp(kv_ready, g & 1u, failed);
                 tc::tc_fence_after();
                 const bool end = c + 1 == x.n;
@@ -667,7 +673,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 if (m < C) {
                     // rows behind the sequence, whatever they hold (beyond the tensor: zeros)
                     failed |= 1u - tc::mbar_wait_warp(qk_full(sq), (g / NQ) & 1u, failed);
-                    const uint32_t ks = sbase + sq * L::QK_STAGE + L::KB * L::BLOCK + swizzled(first, piece);
+                    const uint32_t ks = sbase + sq * L::QK_STAGE + L::K_IN_STAGE + swizzled(first, piece);
                     const uint4 zero = make_uint4(0, 0, 0, 0);
 #pragma unroll 1
                     for (int i = 0; i < 4; ++i)
@@ -782,7 +788,7 @@ int sm_count() {
 template <int DK, bool STATES>
 int launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& o,
            TcArgs p, cudaStream_t s) {
-    using L = Smem<DK>;
+    using L = Smem<DK, STATES>;
     if (const int st = allow_smem<decay_tc_kernel<DK, STATES>>(L::DYN)) return st;
     p.items = (uint32_t)(p.a.B * p.a.H * p.tiles * (STATES ? p.segs - 1 : p.segs));
     const int sms = sm_count();
@@ -797,11 +803,26 @@ int launches(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
     return launch<DK, false>(q, k, v, o, p, s);
 }
 
-// Segments of each sequence where items do not fill the SMs.
+// Segments of each sequence: more of them where the items leave SMs idle, for the price of a pass over
+// k and v that leaves each segment's state.  By the time that a chunk takes in either pass, measured
+// with every SM busy: in 0.1 us, 24 (1.6 to 2.6 us) and 11, and 60 for the second launch.
 int segments(int64_t items, int64_t chunks) {
     const char* e = getenv("SEGS");
     if (e) return atoi(e);
-    return 1;
+    const int64_t sms = sm_count();
+    int best = 1;
+    int64_t least = 0;
+    for (int n = 1; n <= 16 && (n == 1 || (chunks >= 2 * n && items <= sms)); ++n) {
+        const int64_t cps = (chunks + n - 1) / n;
+        if ((n - 1) * cps >= chunks) continue;
+        const int64_t rounds = (items * n + sms - 1) / sms, before = (items * (n - 1) + sms - 1) / sms;
+        const int64_t t = cps * (rounds * 24 + before * 11) + (n > 1 ? 60 : 0);
+        if (n == 1 || t < least) {
+            best = n;
+            least = t;
+        }
+    }
+    return best;
 }
 
 }  // namespace
