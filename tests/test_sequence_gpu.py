@@ -9,9 +9,9 @@ Tolerances, derived (u: half a step of the output's type relative to the value, 
            of dk terms and of the tokens round (or are cut) at most once per term onto a partial
            sum that sum |q||k||v| bounds, N / 8 + 64 times where chunks sum in between:
            (dk + N / 8 + 64) 2^-23 of that magnitude.  16-bit inputs may go through the tensor
-           cores: bfloat16 scores round to 8 bits (2^-8, once), the other operands are held as
-           two bfloat16 terms (2^-8 of 2^-8 each): 2^-8 of the magnitude for bfloat16 outputs,
-           4 * 2^-16 for float16 ones, 2 * 2^-16 for the state.
+           cores: there scores round once to the inputs' type, by half a step of it (2^-8, 2^-11),
+           and the other operands are held as two terms of at least 8 bits (2^-8 of 2^-8 each):
+           u and 3 * 2^-16 of the magnitude for the outputs, 2 * 2^-16 for the state.
   norm     sums over n values in at least 32 partial ones: (n / 32 + 32) 2^-24 relative to the
            mean magnitude, and as much of the variance's; about 16 roundings behind that; SiLU
            and GELU have slopes below 1.13: 1.2 (n / 32 + 48) 2^-24 of the oracle's magnitude
@@ -185,7 +185,7 @@ def _lam(H):
 
 def _decay_tol(o, oa, S, A, dtype, dk, N):
     sums = (dk + N / 8 + 64) * 2.0 ** -23
-    extra = {BF16: 2.0 ** -8, F16: 4 * 2.0 ** -16, F32: 0.0}[dtype]
+    extra = 0.0 if dtype == F32 else _u(dtype) + 3 * 2.0 ** -16
     state = 0.0 if dtype == F32 else 2 * 2.0 ** -16
     return ((extra + sums) * oa + _u(dtype) * o.abs() + _tiny(dtype) + 1e-37,
             (state + sums) * A + 1e-37)

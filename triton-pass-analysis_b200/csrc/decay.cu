@@ -206,7 +206,7 @@ extern "C" int snnb_decay_attention(const void* q, const int64_t* q_strides, con
         a.vs[i] = v_strides[i];
     }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (tc_takes(a, dtype)) return tc_run(a, workspace, workspace_bytes, s);
+    if (tc_takes(a, dtype)) return tc_run(a, dtype, workspace, workspace_bytes, s);
     if (dtype == SNNB_F32) return run_any<float>(a, s);
     if (dtype == SNNB_F16) return run_any<__half>(a, s);
     return run_any<__nv_bfloat16>(a, s);

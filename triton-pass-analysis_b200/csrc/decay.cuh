@@ -59,7 +59,7 @@ int allow_smem(int bytes) {
 // need for them, and its launches.
 bool tc_takes(const Args& a, int dtype);
 int64_t tc_workspace(int dtype, int64_t B, int64_t N, int64_t H, int64_t dk, int64_t dv);
-int tc_run(const Args& a, void* work, int64_t bytes, cudaStream_t s);
+int tc_run(const Args& a, int dtype, void* work, int64_t bytes, cudaStream_t s);
 
 }  // namespace decay
 }  // namespace snnb

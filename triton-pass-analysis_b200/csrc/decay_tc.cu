@@ -1,5 +1,4 @@
 // Decay attention of 16-bit inputs on the tensor cores (formulas: decay.cu).
-#include <stdlib.h>
 #include "decay.cuh"
 #include "tc_common.cuh"
 
@@ -11,7 +10,7 @@ constexpr int C = 128;             // tokens of a chunk
 constexpr int DV = 64;             // columns of v, and of the state, that a thread block takes
 
 // STATES: no q, scores or outputs.
-template <int DK, bool STATES> struct Smem {
+template <int DK, bool STATES, bool HALF> struct Smem {
     static constexpr int KB = DK / 64;                         // 64-column blocks of q and k
     static constexpr int BLOCK = C * 128;                      // 128 rows of 128 bytes
     static constexpr int QK_STAGES = DK == 64 || STATES ? 3 : 2, V_STAGES = STATES ? 3 : 2;
@@ -22,15 +21,17 @@ template <int DK, bool STATES> struct Smem {
     static constexpr int S_TERM = STATES ? 0 : DK * 128;
     // the scaled v's three terms: both halves of a chunk where there is room, else one at a time
     static constexpr int VT_HALVES = DK == 64 || STATES ? 2 : 1;
-    static constexpr int VT_OFF = S_OFF + 2 * S_TERM, VT_TERM = BLOCK / 2, VT_HALF = 3 * VT_TERM;
+    static constexpr int TERMS = HALF ? 2 : 3;
+    static constexpr int VT_OFF = S_OFF + 2 * S_TERM, VT_TERM = BLOCK / 2, VT_HALF = TERMS * VT_TERM;
     static constexpr bool STAGED = DK == 64 && !STATES;                   // outputs leave by bulk copies
     static constexpr int O_OFF = VT_OFF + VT_HALVES * VT_HALF;         // 32 rows for each warp
     static constexpr int PW_OFF = O_OFF + (STAGED ? BLOCK : 0);  // 0 (31 times), decay^0 .. ^127
     static constexpr int RW_OFF = PW_OFF + 160 * 4;            // decay^31 .. decay^0
     static constexpr int WV_OFF = RW_OFF + 32 * 4;             // the factors of v's rows
     static constexpr int BAD_OFF = WV_OFF + C * 4;             // [4][DV] rows, [4] chunk numbers
-    static constexpr int BAR_OFF = BAD_OFF + (4 * DV + 4) * 4;
-    static constexpr int NBARS = 2 * QK_STAGES + 2 * V_STAGES + 12;
+    static constexpr int TOP_OFF = BAD_OFF + (4 * DV + 4) * 4; // [8] largest q, k, v, state
+    static constexpr int BAR_OFF = TOP_OFF + 8 * 4 * 4;
+    static constexpr int NBARS = 2 * QK_STAGES + 2 * V_STAGES + 16;
     static constexpr int TMEM_OFF = BAR_OFF + NBARS * 8;
     static constexpr int DYN = TMEM_OFF + 8 + 1024;
     static_assert(DYN <= 227 * 1024, "shared memory");
@@ -38,7 +39,7 @@ template <int DK, bool STATES> struct Smem {
 };
 
 // TMEM columns: scores (and over their first half P), q times the state's two terms, P V, K^T
-// times the scaled v's three terms.
+// times the scaled v's two or three terms.
 constexpr int T_QK = 0, T_QS = 128, T_PV = 256, T_KV = 320, T_COLS = 512;
 
 // Warps 0-3 scores to P, 4 copies, 5 MMAs, 6 and 7 with warps 2 and 3, whose rows have the most
@@ -158,11 +159,25 @@ __device__ __forceinline__ void sts_f(uint32_t a, float v) {
 __device__ __forceinline__ uint32_t swizzled(int row, int piece) {
     return (uint32_t)(row * 128 + ((piece ^ (row & 7)) << 4));
 }
-__device__ __forceinline__ uint32_t bf2(float a, float b) {
-    return mx::round_pair(a, b, (const __nv_bfloat16*)nullptr);
+template <bool HALF> __device__ __forceinline__ uint32_t pair(float a, float b) {
+    if constexpr (HALF) return mx::round_pair(a, b, (const __half*)nullptr);
+    else return mx::round_pair(a, b, (const __nv_bfloat16*)nullptr);
+}
+template <bool HALF> __device__ __forceinline__ float2 floats(uint32_t u) {
+    if constexpr (HALF) return mx::pair_f32(u, (const __half*)nullptr);
+    else return mx::pair_f32(u, (const __nv_bfloat16*)nullptr);
+}
+// Exponents.  float16 operands are brought below 2^15 by powers of two, exactly: its largest value
+// is 65504, and scores, states and sums can be any.  bfloat16 has float's range and needs none.
+__device__ __forceinline__ float pow2(int n) { return __int_as_float((n + 127) << 23); }
+// b with |x| < 2^b for the largest magnitude's bits.
+__device__ __forceinline__ int above_half(uint32_t bits) { return (int)max(bits >> 10, 1u) - 14; }
+__device__ __forceinline__ int above_float(uint32_t bits) { return max((int)(bits >> 23) - 126, -100); }
+constexpr uint32_t idesc16(bool half, int M, int N) {
+    return tc::idesc_bf16_f32(M, N) & (half ? ~((1u << 7) | (1u << 10)) : ~0u);
 }
 // 16 outputs of a row, the first `cols` (a multiple of 8) inside.
-__device__ __forceinline__ void store16(__nv_bfloat16* o, const uint32_t (&w)[8], int cols, bool al32) {
+__device__ __forceinline__ void store16(uint16_t* o, const uint32_t (&w)[8], int cols, bool al32) {
     if (al32) {                                      // then cols is a multiple of 16
         if (cols > 0)
             asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(o), "r"(w[0]),
@@ -173,23 +188,35 @@ __device__ __forceinline__ void store16(__nv_bfloat16* o, const uint32_t (&w)[8]
     if (cols > 0) reinterpret_cast<uint4*>(o)[0] = make_uint4(w[0], w[1], w[2], w[3]);
     if (cols > 8) reinterpret_cast<uint4*>(o)[1] = make_uint4(w[4], w[5], w[6], w[7]);
 }
-__device__ __forceinline__ float lo_f(uint32_t u) { return __int_as_float((int)(u << 16)); }
 // The upper halves of two floats as bf16 (cut, not rounded), and a float's upper half as a float.
 __device__ __forceinline__ uint32_t tops(float a, float b) {
     return __byte_perm((uint32_t)__float_as_int(a), (uint32_t)__float_as_int(b), 0x7632);
 }
+// The largest magnitudes' bits of 16-bit values, in pairs.
+__device__ __forceinline__ uint32_t largest(uint32_t top, uint4 r) {
+    const uint32_t m = 0x7FFF7FFFu;
+    return __vmaxu2(__vmaxu2(top, __vmaxu2(r.x & m, r.y & m)), __vmaxu2(r.z & m, r.w & m));
+}
+// The same without infinities and NaN, of float16.
+__device__ __forceinline__ uint32_t largest_finite(uint32_t top, uint4 r) {
+    const uint32_t u[4] = {r.x, r.y, r.z, r.w};
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t x = u[i >> 1] >> (16 * (i & 1)) & 0x7FFFu;
+        if (x < 0x7C00u) top = max(top, x);
+    }
+    return top;
+}
 __device__ __forceinline__ float top_f(float a) {
     return __int_as_float(__float_as_int(a) & (int)0xFFFF0000u);
 }
-__device__ __forceinline__ float hi_f(uint32_t u) { return __int_as_float((int)(u & 0xFFFF0000u)); }
 
 // STATES: only the states that the segments leave, each from zero (the first: from state_in).
-template <int DK, bool STATES>
+template <int DK, bool STATES, bool HALF>
 __global__ void __launch_bounds__(THREADS, 1)
 decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
                 const __grid_constant__ TcArgs p) {
-    using L = Smem<DK, STATES>;
+    using L = Smem<DK, STATES, HALF>;
     constexpr int NQ = L::QK_STAGES, NV = L::V_STAGES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -209,6 +236,8 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                    s_ready = misc + 56, qs_done = misc + 64, vt_free = misc + 72,
                    done = misc + 80;
     auto vt_ready = [&](int half) { return misc + (half ? 88u : 32u); };
+    auto top_ready = [&](uint32_t i) { return misc + 96u + 8u * i; };       // float16: four in turn
+    uint32_t* tops8 = reinterpret_cast<uint32_t*>(smem + L::TOP_OFF);       // of chunk g: 4 (g & 7)
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + L::TMEM_OFF);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Args& a = p.a;
@@ -232,6 +261,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         tc::mbar_init(kv_read, 4);
         tc::mbar_init(qs_done, 1);
         tc::mbar_init(vt_free, 1);
+        for (int i = 0; i < 4; ++i) tc::mbar_init(top_ready(i), 1);
         tc::mbar_init(s_ready, 4);
         tc::mbar_init(done, 1);
         tc::fence_mbar_init();
@@ -241,6 +271,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         for (int i = 0; i < 4; ++i) bad_chunk[i] = -1;
     }
     if (threadIdx.x < 4 * DV) bad_row[threadIdx.x] = C;
+    else if (threadIdx.x < 4 * DV + 32) tops8[threadIdx.x - 4 * DV] = 0;
     if (warp == 5) {
         tc::tmem_alloc(sbase + L::TMEM_OFF, T_COLS);
         tc::tmem_relinquish();
@@ -317,7 +348,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     for (int i = 0; i < 4 * L::KB; ++i)
                         tc::umma_bf16(tmem + T_QK, tc::sdesc_k_sw128(q + i / 4 * L::BLOCK) + 2 * (i % 4),
                                       tc::sdesc_k_sw128(k + i / 4 * L::BLOCK) + 2 * (i % 4),
-                                      tc::idesc_bf16_f32(128, 128), i != 0);
+                                      idesc16(HALF, 128, 128), i != 0);
                     tc::umma_commit(qk_ready);
                 };
 #pragma unroll 1
@@ -337,7 +368,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                                           sdesc_mn_sw128(k, DK == 64 ? 0 : L::BLOCK) + 128 * (4 * half + i),
                                           sdesc_mn_sw128(sbase + L::VT_OFF + (L::VT_HALVES - 1) * half * L::VT_HALF,
                                                          L::VT_TERM) + 128 * i,
-                                          tc::idesc_bf16_f32(128, 192) | A_MN | B_MN, (half | i) != 0);
+                                          idesc16(HALF, 128, 64 * L::TERMS) | A_MN | B_MN, (half | i) != 0);
                         tc::umma_commit(half ? kv_ready : vt_free);
                     }
                     if (!STATES) {
@@ -349,7 +380,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         for (int i = 0; i < DK / 16; ++i)
                             tc::umma_bf16(tmem + T_QS, tc::sdesc_k_sw128(q + i / 4 * L::BLOCK) + 2 * (i % 4),
                                           sdesc_mn_sw128(sbase + L::S_OFF, L::S_TERM) + 128 * i,
-                                          tc::idesc_bf16_f32(128, 128) | B_MN, i != 0);
+                                          idesc16(HALF, 128, 128) | B_MN, i != 0);
                         tc::umma_commit(qs_done);
                     }
                     tc::umma_commit(qk_empty(s));
@@ -360,7 +391,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         for (int i = 0; i < 8; ++i)
                             umma_ts(tmem + T_PV, tmem + T_QK + 8 * i,
                                     sdesc_mn_sw128(sbase + L::V_OFF + sv * L::BLOCK, 0) + 128 * i,
-                                    tc::idesc_bf16_f32(128, 64) | B_MN, i != 0);
+                                    idesc16(HALF, 128, 64) | B_MN, i != 0);
                         tc::umma_commit(o_ready);
                     }
                     tc::umma_commit(v_empty(sv));
@@ -396,6 +427,12 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 for (int c = 0; c < x.n; ++c, ++g) {
                     failed |= 1u - tc::mbar_wait_warp(qk_ready, g & 1u, failed);
                     tc::tc_fence_after();
+                    float down = 1.0f;
+                    if constexpr (HALF) {            // |q . k| < 128 * 2^(bounds of q and k)
+                        failed |= 1u - tc::mbar_wait_warp(top_ready(g & 3), (g >> 2) & 1u, failed);
+                        const uint32_t* top = tops8 + 4 * (g & 7);
+                        down = pow2(8 - above_half(top[0]) - above_half(top[1]));
+                    }
 #pragma unroll 1
                     for (int blk = 0; blk < 2; ++blk) {
                         uint32_t w[16];
@@ -412,11 +449,11 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                             const uint32_t d = pw + 4 * (31 + lane);
 #pragma unroll
                             for (int i = 0; i < 32; ++i) {
-                                const float y = s[i] * lds_f(d - 4 * i);
+                                const float y = s[i] * (HALF ? lds_f(d - 4 * i) * down : lds_f(d - 4 * i));
                                 s[i] = i <= lane ? y : 0.0f;
                             }
                         } else {
-                            const float f = blk ? f1 : f0;
+                            const float f = HALF ? (blk ? f1 : f0) * down : blk ? f1 : f0;
                             const uint64_t ff = mx::pack2(f, f);
 #pragma unroll
                             for (int i = 0; i < 32; i += 4) {
@@ -429,7 +466,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         }
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
-                            w[i] = blk == 0 || two ? bf2(s[2 * i], s[2 * i + 1]) : 0u;
+                            w[i] = blk == 0 || two ? pair<HALF>(s[2 * i], s[2 * i + 1]) : 0u;
                         if (q >= 2 && first == 2 && blk == 0) tc::named_bar_sync(3 + q, 64);
                         tmem_st16(tl + (first + blk) * 16, w);
                     }
@@ -454,10 +491,10 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         for (uint32_t it = blockIdx.x; !STATES && it < p.items; it += gridDim.x) {
             const Item x(p, it);
             const float fq = (float)power(x.lam, row + 1) * a.scale;
-            const uint64_t fq2 = mx::pack2(fq, fq), sc2 = mx::pack2(a.scale, a.scale);
+            uint64_t fq2 = mx::pack2(fq, fq), sc2 = mx::pack2(a.scale, a.scale);
             const int cols = min(DV, a.dv - x.tile * DV);
             const int64_t ld = a.H * a.dv;
-            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) +
+            uint16_t* out = static_cast<uint16_t*>(a.out) +
                                  ((int64_t)x.b * a.N * a.H + x.h) * a.dv + x.tile * DV +
                                  ((int64_t)x.c0 * C + row) * ld;
 #pragma unroll 1
@@ -469,6 +506,13 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 }
                 failed |= 1u - tc::mbar_wait_warp(o_ready, g & 1u, failed);
                 tc::tc_fence_after();
+                if constexpr (HALF) {                // the powers of two of q S and of P
+                    const uint32_t* top = tops8 + 4 * (g & 7);
+                    const float fs = fq * pow2(above_float(top[3]) - 15);
+                    const float fp = a.scale * pow2(above_half(top[0]) + above_half(top[1]) - 8);
+                    fq2 = mx::pack2(fs, fs);
+                    sc2 = mx::pack2(fp, fp);
+                }
                 const bool spoiled = bad_chunk[g & 3] == (int)g, alive = n < x.len;
                 const bool write = n < a.N && !failed && SNNB_IN_BOUNDS(n, a.N, p.status);
 #pragma unroll 1
@@ -500,7 +544,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                             if (row >= rows[j]) v[j] = __int_as_float(0x7fffffff);
                     }
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) w[j] = alive ? bf2(v[2 * j], v[2 * j + 1]) : 0u;
+                    for (int j = 0; j < 8; ++j) w[j] = alive ? pair<HALF>(v[2 * j], v[2 * j + 1]) : 0u;
                     if (L::STAGED) {
                         sts128(stage + swizzled(lane, i / 8), make_uint4(w[0], w[1], w[2], w[3]));
                         sts128(stage + swizzled(lane, i / 8 + 1), make_uint4(w[4], w[5], w[6], w[7]));
@@ -597,14 +641,39 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 if (!STATES) {
                     // the state before this chunk, once q times the last one is done
                     if (g) failed |= 1u - tc::mbar_wait_warp(qs_done, (g - 1) & 1u, failed);
+                    float up = 1.0f;
+                    if constexpr (HALF) {
+                        volatile uint32_t* top = tops8 + 4 * (g & 7) + 3;
+                        float m = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < W; ++i) m = fmaxf(m, fabsf(S[i]));
+                        uint32_t bits = __reduce_max_sync(0xffffffffu, (uint32_t)__float_as_int(m));
+                        if (lane == 0) atomicMax(&tops8[4 * (g & 7) + 3], bits);
+                        if (t == 0) tops8[4 * ((g + 1) & 7) + 3] = 0;
+                        tc::named_bar_sync(8, 128);
+                        if (*top >= 0x7F800000u) {   // of the finite ones
+                            tc::named_bar_sync(8, 128);
+                            if (t == 0) *top = 0;
+                            m = 0.0f;
+#pragma unroll
+                            for (int i = 0; i < W; ++i)
+                                if (fabsf(S[i]) <= 3.4028235e38f) m = fmaxf(m, fabsf(S[i]));
+                            bits = __reduce_max_sync(0xffffffffu, (uint32_t)__float_as_int(m));
+                            tc::named_bar_sync(8, 128);
+                            if (lane == 0) atomicMax(&tops8[4 * (g & 7) + 3], bits);
+                            tc::named_bar_sync(8, 128);
+                        }
+                        up = pow2(15 - above_float(*top));
+                    }
 #pragma unroll
                     for (int i = 0; i < W; i += 8) {
                         uint32_t hi[4], lo[4];
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const float y = S[i + 2 * j], z = S[i + 2 * j + 1];
-                            hi[j] = bf2(y, z);
-                            lo[j] = bf2(y - lo_f(hi[j]), z - hi_f(hi[j]));
+                            const float y = S[i + 2 * j] * up, z = S[i + 2 * j + 1] * up;
+                            hi[j] = pair<HALF>(y, z);
+                            const float2 h = floats<HALF>(hi[j]);
+                            lo[j] = pair<HALF>(y - h.x, z - h.y);
                         }
                         const uint32_t o = sbase + L::S_OFF + swizzled(row, (col + i) / 8);
                         sts128(o, make_uint4(hi[0], hi[1], hi[2], hi[3]));
@@ -619,16 +688,21 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 const bool end = c + 1 == x.n;
                 const float fh = end ? lh : ch, fl = end ? ll : cl;
                 const uint64_t fh2 = mx::pack2(fh, fh), fl2 = mx::pack2(fl, fl);
+                uint64_t back = 0;
+                if constexpr (HALF) {
+                    const float f = pow2(above_half(tops8[4 * (g & 7) + 2]) - 15);
+                    back = mx::pack2(f, f);
+                }
 #pragma unroll
                 for (int i = 0; i < W; i += 16) {
                     float y[16], z[16], u[16];
                     tc::tmem_ld16(tl + i, y);
                     tc::tmem_ld16(tl + 64 + i, z);
-                    tc::tmem_ld16(tl + 128 + i, u);
+                    if constexpr (!HALF) tc::tmem_ld16(tl + 128 + i, u);
                     tc::tmem_wait_ld();
                     tc::reg_fence16(y);
                     tc::reg_fence16(z);
-                    tc::reg_fence16(u);
+                    if constexpr (!HALF) tc::reg_fence16(u);
                     if (i + 16 == W) {
                         tc::tc_fence_before();
                         if (lane == 0) tc::mbar_arrive(kv_read);
@@ -636,11 +710,12 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     }
 #pragma unroll
                     for (int j = 0; j < 16; j += 2) {
-                        const uint64_t sum = mx::add2(mx::pack2(y[j], y[j + 1]),
-                                                      mx::add2(mx::pack2(z[j], z[j + 1]),
-                                                               mx::pack2(u[j], u[j + 1])));
                         const uint64_t old = mx::pack2(S[i + j], S[i + j + 1]);
-                        mx::unpack2(mx::fma2(old, fh2, mx::fma2(old, fl2, sum)), S[i + j], S[i + j + 1]);
+                        uint64_t sum = mx::pack2(z[j], z[j + 1]);
+                        if constexpr (!HALF) sum = mx::add2(sum, mx::pack2(u[j], u[j + 1]));
+                        sum = mx::add2(mx::pack2(y[j], y[j + 1]), sum);
+                        sum = HALF ? mx::fma2(sum, back, mx::mul2(old, fl2)) : mx::fma2(old, fl2, sum);
+                        mx::unpack2(mx::fma2(old, fh2, sum), S[i + j], S[i + j + 1]);
                     }
                 }
             }
@@ -680,30 +755,85 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         if (first + 16 * i >= m) {
                             sts128(vs + 2048 * i, zero);
 #pragma unroll
-                            for (int k = 0; k < L::KB; ++k) sts128(ks + k * L::BLOCK + 2048 * i, zero);
+                            for (int k = 0; k < L::KB; ++k) {
+                                sts128(ks + k * L::BLOCK + 2048 * i, zero);
+                                if (HALF && !STATES) sts128(ks - L::K_IN_STAGE + k * L::BLOCK + 2048 * i, zero);
+                            }
                         }
                 }
+                constexpr uint32_t INF = HALF ? 0x7C00u : 0x7F80u;
                 uint32_t top = 0, hi[4][4], mid[4][4], low[4][4];
+                uint4 raw[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint4 raw = lds128(vs + 2048 * i);
-                    const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
-                    const float f = lds_f(wv + 4 * (first + 16 * i));
+                    raw[i] = lds128(vs + 2048 * i);
+                    top = largest(top, raw[i]);
+                }
+                float up = 1.0f;
+                if constexpr (HALF) {
+                    // the largest magnitudes of the chunk's q, k and v
+                    uint32_t* tops = tops8 + 4 * (g & 7);
+                    if constexpr (!STATES) {
+                        failed |= 1u - tc::mbar_wait_warp(qk_full(sq), (g / NQ) & 1u, failed);
+                        const uint32_t qs = sbase + sq * L::QK_STAGE + swizzled(first, piece);
+#pragma unroll 1
+                        for (int x = 0; x < 2; ++x) {          // q, then k
+                            uint32_t tx = 0;
+#pragma unroll
+                            for (int i = 0; i < 4 * L::KB; ++i)
+                                tx = largest(tx, lds128(qs + x * L::K_IN_STAGE + i / 4 * L::BLOCK + i % 4 * 2048));
+                            tx = max(tx & 0xFFFFu, tx >> 16);
+                            if (tx >= INF) {
+                                tx = 0;
+#pragma unroll 1
+                                for (int i = 0; i < 4 * L::KB; ++i)
+                                    tx = largest_finite(tx, lds128(qs + x * L::K_IN_STAGE + i / 4 * L::BLOCK +
+                                                                   i % 4 * 2048));
+                            }
+                            tx = __reduce_max_sync(0xffffffffu, tx);
+                            if (lane == 0) atomicMax(&tops[x], tx);
+                        }
+                    }
+                    uint32_t tv = max(top & 0xFFFFu, top >> 16);
+                    if (tv >= INF) {
+                        tv = 0;
+#pragma unroll 1
+                        for (int i = 0; i < 4; ++i) tv = largest_finite(tv, lds128(vs + 2048 * i));
+                    }
+                    tv = __reduce_max_sync(0xffffffffu, tv);
+                    if (lane == 0) atomicMax(&tops[2], tv);
+                    if (t < 3) tops8[4 * ((g + 1) & 7) + t] = 0;
+                    tc::named_bar_sync(1, 256);
+                    if (t == 0 && !STATES) tc::mbar_arrive(top_ready(g & 3));
+                    up = pow2(15 - above_half(tops[2]));
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                    const float f = HALF ? lds_f(wv + 4 * (first + 16 * i)) * up : lds_f(wv + 4 * (first + 16 * i));
                     const uint64_t ff = mx::pack2(f, f);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        top = __vmaxu2(top, u[j] & 0x7FFF7FFFu);
-                        // 24 bits, cut into three times 8: exact
-                        uint64_t yz = mx::mul2(mx::pack2(lo_f(u[j]), hi_f(u[j])), ff);
+                        const float2 v = floats<HALF>(u[j]);
+                        uint64_t yz = mx::mul2(mx::pack2(v.x, v.y), ff);
                         float y, z;
                         mx::unpack2(yz, y, z);
-                        hi[i][j] = tops(y, z);
-                        yz = mx::fma2(mx::pack2(top_f(y), top_f(z)), minus, yz);
-                        mx::unpack2(yz, y, z);
-                        mid[i][j] = tops(y, z);
-                        yz = mx::fma2(mx::pack2(top_f(y), top_f(z)), minus, yz);
-                        mx::unpack2(yz, y, z);
-                        low[i][j] = tops(y, z);
+                        if constexpr (HALF) {
+                            // 22 of 24 bits, in two terms
+                            hi[i][j] = pair<HALF>(y, z);
+                            const float2 h = floats<HALF>(hi[i][j]);
+                            mx::unpack2(mx::fma2(mx::pack2(h.x, h.y), minus, yz), y, z);
+                            mid[i][j] = pair<HALF>(y, z);
+                        } else {
+                            // 24 bits, cut into three times 8: exact
+                            hi[i][j] = tops(y, z);
+                            yz = mx::fma2(mx::pack2(top_f(y), top_f(z)), minus, yz);
+                            mx::unpack2(yz, y, z);
+                            mid[i][j] = tops(y, z);
+                            yz = mx::fma2(mx::pack2(top_f(y), top_f(z)), minus, yz);
+                            mx::unpack2(yz, y, z);
+                            low[i][j] = tops(y, z);
+                        }
                     }
                 }
                 // the products have read what was there
@@ -716,9 +846,10 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     const uint32_t o = vt + 2048 * i;
                     sts128(o, make_uint4(hi[i][0], hi[i][1], hi[i][2], hi[i][3]));
                     sts128(o + L::VT_TERM, make_uint4(mid[i][0], mid[i][1], mid[i][2], mid[i][3]));
-                    sts128(o + 2 * L::VT_TERM, make_uint4(low[i][0], low[i][1], low[i][2], low[i][3]));
+                    if constexpr (!HALF)
+                        sts128(o + 2 * L::VT_TERM, make_uint4(low[i][0], low[i][1], low[i][2], low[i][3]));
                 }
-                if (__any_sync(0xffffffffu, (top & 0xFFFFu) >= 0x7F80u || (top >> 16) >= 0x7F80u)) {
+                if (__any_sync(0xffffffffu, (top & 0xFFFFu) >= INF || (top >> 16) >= INF)) {
                     // Values that are not finite: 0 * inf in the product of P and v would reach
                     // the chunk's earlier rows.  There they become zero, and the outputs of their
                     // columns NaN from their row on.
@@ -730,11 +861,11 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         uint32_t u[4] = {r4.x, r4.y, r4.z, r4.w};
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            if ((u[j] & 0x7F80u) == 0x7F80u) {
+                            if ((u[j] & INF) == INF) {
                                 atomicMin(&rows[2 * j], first + 16 * i);
                                 u[j] &= 0xFFFF0000u;
                             }
-                            if ((u[j] & 0x7F800000u) == 0x7F800000u) {
+                            if ((u[j] & (INF << 16)) == INF << 16) {
                                 atomicMin(&rows[2 * j + 1], first + 16 * i);
                                 u[j] &= 0xFFFFu;
                             }
@@ -759,12 +890,12 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 
 // [B, N, heads, d] as a tensor map with boxes of 128 tokens x 64 columns of one head.
 int encode(CUtensorMap* m, const void* base, const int64_t* s, int64_t B, int64_t N, int64_t heads,
-           int64_t d, int rows = C) {
+           int64_t d, bool half, int rows = C) {
     const uint64_t dims[4] = {(uint64_t)d, (uint64_t)heads, (uint64_t)N, (uint64_t)B};
     const uint64_t st[3] = {heads > 1 ? (uint64_t)s[2] * 2 : 16, N > 1 ? (uint64_t)s[1] * 2 : 16,
                             B > 1 ? (uint64_t)s[0] * 2 : 16};
     const uint32_t box[4] = {64, 1, (uint32_t)rows, 1};
-    return encode_tmap(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, st, box,
+    return encode_tmap(m, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, st, box,
                        CU_TENSOR_MAP_SWIZZLE_128B);
 }
 bool mappable(const void* base, const int64_t* s, int64_t B, int64_t N, int64_t heads) {
@@ -785,30 +916,28 @@ int sm_count() {
     return counts[dev];
 }
 
-template <int DK, bool STATES>
+template <int DK, bool STATES, bool HALF>
 int launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& o,
            TcArgs p, cudaStream_t s) {
-    using L = Smem<DK, STATES>;
-    if (const int st = allow_smem<decay_tc_kernel<DK, STATES>>(L::DYN)) return st;
+    using L = Smem<DK, STATES, HALF>;
+    if (const int st = allow_smem<decay_tc_kernel<DK, STATES, HALF>>(L::DYN)) return st;
     p.items = (uint32_t)(p.a.B * p.a.H * p.tiles * (STATES ? p.segs - 1 : p.segs));
     const int sms = sm_count();
-    return launch_k(decay_tc_kernel<DK, STATES>, dim3(p.items < (uint32_t)sms ? p.items : sms), dim3(THREADS),
+    return launch_k(decay_tc_kernel<DK, STATES, HALF>, dim3(p.items < (uint32_t)sms ? p.items : sms), dim3(THREADS),
                     L::DYN, s, q, k, v, o, p);
 }
-template <int DK>
+template <int DK, bool HALF>
 int launches(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
              const CUtensorMap& o, const TcArgs& p, cudaStream_t s) {
     if (p.segs > 1)
-        if (const int st = launch<DK, true>(q, k, v, o, p, s)) return st;
-    return launch<DK, false>(q, k, v, o, p, s);
+        if (const int st = launch<DK, true, HALF>(q, k, v, o, p, s)) return st;
+    return launch<DK, false, HALF>(q, k, v, o, p, s);
 }
 
 // Segments of each sequence: more of them where the items leave SMs idle, for the price of a pass over
-// k and v that leaves each segment's state.  By the time that a chunk takes in either pass, measured
-// with every SM busy: in 0.1 us, 24 (1.6 to 2.6 us) and 11, and 60 for the second launch.
+// k and v that leaves each segment's state.  In 0.1 us, measured with every SM busy: 24 for a chunk
+// (16 to 26), 13 for one of the pass before, 30 for an item's start, 60 for the second launch.
 int segments(int64_t items, int64_t chunks) {
-    const char* e = getenv("SEGS");
-    if (e) return atoi(e);
     const int64_t sms = sm_count();
     int best = 1;
     int64_t least = 0;
@@ -816,7 +945,7 @@ int segments(int64_t items, int64_t chunks) {
         const int64_t cps = (chunks + n - 1) / n;
         if ((n - 1) * cps >= chunks) continue;
         const int64_t rounds = (items * n + sms - 1) / sms, before = (items * (n - 1) + sms - 1) / sms;
-        const int64_t t = cps * (rounds * 24 + before * 11) + (n > 1 ? 60 : 0);
+        const int64_t t = rounds * (cps * 24 + 30) + before * (cps * 13 + 30) + (n > 1 ? 60 : 0);
         if (n == 1 || t < least) {
             best = n;
             least = t;
@@ -828,26 +957,27 @@ int segments(int64_t items, int64_t chunks) {
 }  // namespace
 
 bool tc_takes(const Args& a, int dtype) {
-    return dtype == SNNB_BF16 && a.N > 0 && a.N < 0x7fffff00 && a.dk <= 128 && a.dk % 8 == 0 &&
+    return (dtype == SNNB_BF16 || dtype == SNNB_F16) && a.N > 0 && a.N < 0x7fffff00 && a.dk <= 128 && a.dk % 8 == 0 &&
            a.dv % 8 == 0 && aligned16(a.out) && aligned16(a.state_in) && aligned16(a.state_out) &&
            mappable(a.q, a.qs, a.B, a.N, a.H) &&
            mappable(a.k, a.ks, a.B, a.N, a.Hk) && mappable(a.v, a.vs, a.B, a.N, a.Hk);
 }
 
 int64_t tc_workspace(int dtype, int64_t B, int64_t N, int64_t H, int64_t dk, int64_t dv) {
-    if (dtype != SNNB_BF16 || dk > 128 || dk % 8 || dv % 8 || B == 0 || N == 0) return 0;
+    if ((dtype != SNNB_BF16 && dtype != SNNB_F16) || dk > 128 || dk % 8 || dv % 8 || B == 0 || N == 0) return 0;
     const int64_t items = B * H * ((dv + DV - 1) / DV);
     const int segs = segments(items, (N + C - 1) / C);
     return segs > 1 ? segs * items * (dk <= 64 ? 64 : 128) * DV * 4 : 0;
 }
 
-int tc_run(const Args& a, void* work, int64_t bytes, cudaStream_t s) {
+int tc_run(const Args& a, int dtype, void* work, int64_t bytes, cudaStream_t s) {
+    const bool half = dtype == SNNB_F16;
     CUtensorMap q, k, v, o = {};
-    int rc = encode(&q, a.q, a.qs, a.B, a.N, a.H, a.dk);
-    if (!rc) rc = encode(&k, a.k, a.ks, a.B, a.N, a.Hk, a.dk);
-    if (!rc) rc = encode(&v, a.v, a.vs, a.B, a.N, a.Hk, a.dv);
+    int rc = encode(&q, a.q, a.qs, a.B, a.N, a.H, a.dk, half);
+    if (!rc) rc = encode(&k, a.k, a.ks, a.B, a.N, a.Hk, a.dk, half);
+    if (!rc) rc = encode(&v, a.v, a.vs, a.B, a.N, a.Hk, a.dv, half);
     const int64_t os[3] = {a.N * a.H * a.dv, a.H * a.dv, a.dv};
-    if (!rc && a.dk <= 64) rc = encode(&o, a.out, os, a.B, a.N, a.H, a.dv, 32);
+    if (!rc && a.dk <= 64) rc = encode(&o, a.out, os, a.B, a.N, a.H, a.dv, half, 32);
     if (rc) return rc;
     const int chunks = (int)((a.N + C - 1) / C), tiles = (a.dv + DV - 1) / DV;
     int segs = segments(a.B * a.H * tiles, chunks);
@@ -856,9 +986,10 @@ int tc_run(const Args& a, void* work, int64_t bytes, cudaStream_t s) {
                 a.dv % 16 == 0 && reinterpret_cast<uintptr_t>(a.out) % 32 == 0};
     if (!p.status) return SNNB_ERR_CUDA;
     if (segs > 1 && (!work || !aligned16(work) ||
-                     bytes < tc_workspace(SNNB_BF16, a.B, a.N, a.H, a.dk, a.dv)))
+                     bytes < tc_workspace(dtype, a.B, a.N, a.H, a.dk, a.dv)))
         return SNNB_ERR_ARG;
-    return a.dk <= 64 ? launches<64>(q, k, v, o, p, s) : launches<128>(q, k, v, o, p, s);
+    if (half) return a.dk <= 64 ? launches<64, true>(q, k, v, o, p, s) : launches<128, true>(q, k, v, o, p, s);
+    return a.dk <= 64 ? launches<64, false>(q, k, v, o, p, s) : launches<128, false>(q, k, v, o, p, s);
 }
 
 }  // namespace decay
