@@ -151,8 +151,85 @@ __global__ void __launch_bounds__(ST_THREADS) decay_step_kernel(Args a, uint32_t
     }
 }
 
+// The same in float4s: LANES of them along a row of the state, as many rows at a time as the block
+// has threads for, eight of a thread's in flight before q and k are there.
+template <typename T, int LANES>
+__global__ void __launch_bounds__(ST_THREADS) decay_step_vec_kernel(Args a, uint32_t tiles) {
+    constexpr int ROWS = ST_THREADS / LANES, AHEAD = 8;
+    __shared__ float q[MAX_DIM], k[MAX_DIM];
+    __shared__ float4 part[ROWS][LANES];
+    pdl_wait();
+    pdl_trigger();
+    const uint32_t bh = blockIdx.x / tiles, tile = blockIdx.x - bh * tiles;
+    const uint32_t b = bh / (uint32_t)a.H, h = bh - b * (uint32_t)a.H, hk = h / (uint32_t)(a.H / a.Hk);
+    const int t = threadIdx.x, c = (tile * LANES + t % LANES) * 4, r0 = t / LANES;
+    const bool in = c < a.dv;
+    const int64_t base = (int64_t)bh * a.dk * a.dv + c;
+    const float* from = a.state_in + base;
+    float* to = a.state_out + base;
+    float4 x[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+        if (in && r0 + i * ROWS < a.dk)
+            x[i] = *reinterpret_cast<const float4*>(from + (int64_t)(r0 + i * ROWS) * a.dv);
+    const T* qg = static_cast<const T*>(a.q) + b * a.qs[0] + h * a.qs[2];
+    const T* kg = static_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[2];
+    if (t < a.dk) {
+        q[t] = to_f32(qg[t]) * a.scale;
+        k[t] = to_f32(kg[t]);
+    }
+    float v[4] = {};
+    if (in) {
+        const T* vg = static_cast<const T*>(a.v) + b * a.vs[0] + hk * a.vs[2] + c;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = to_f32(vg[j]);
+    }
+    const float l = a.decay[h];
+    __syncthreads();
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int r = r0; r < a.dk; r += AHEAD * ROWS) {
+        if (r != r0) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i)
+                if (in && r + i * ROWS < a.dk)
+                    x[i] = *reinterpret_cast<const float4*>(from + (int64_t)(r + i * ROWS) * a.dv);
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int n = r + i * ROWS;
+            if (!in || n >= a.dk) continue;
+            const float kn = k[n], qn = q[n];
+            x[i] = make_float4(l * x[i].x + kn * v[0], l * x[i].y + kn * v[1], l * x[i].z + kn * v[2],
+                               l * x[i].w + kn * v[3]);
+            *reinterpret_cast<float4*>(to + (int64_t)n * a.dv) = x[i];
+            s.x += qn * x[i].x; s.y += qn * x[i].y; s.z += qn * x[i].z; s.w += qn * x[i].w;
+        }
+    }
+    part[r0][t % LANES] = s;
+    __syncthreads();
+    if (t < 4 * LANES) {                             // a column a thread
+        const int col = tile * LANES * 4 + t;
+        float y = 0.0f;
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) y += reinterpret_cast<const float*>(part[i])[t];
+        if (col < a.dv) mx::round_to(y, static_cast<T*>(a.out) + (int64_t)bh * a.dv + col);
+    }
+}
+
 template <typename T>
 int run_step(const Args& a, cudaStream_t s) {
+    if (a.dv % 4 == 0 && aligned16(a.state_in) && aligned16(a.state_out)) {
+        // rows as wide as the state's, up to 128 columns; narrower where that leaves SMs idle
+        int lanes = 32;
+        while (lanes > 8 && lanes * 2 >= a.dv) lanes /= 2;
+        auto blocks = [&](int n) { return a.B * a.H * ((a.dv + 4 * n - 1) / (4 * n)); };
+        while (lanes > 8 && blocks(lanes) < 148) lanes /= 2;
+        const uint32_t tiles = (a.dv + 4 * lanes - 1) / (4 * lanes);
+        auto k = lanes == 32   ? decay_step_vec_kernel<T, 32>
+                 : lanes == 16 ? decay_step_vec_kernel<T, 16>
+                               : decay_step_vec_kernel<T, 8>;
+        return launch_k(k, dim3((unsigned)blocks(lanes)), dim3(ST_THREADS), 0, s, a, tiles);
+    }
     const uint32_t tiles = (a.dv + ST_V - 1) / ST_V;
     return launch_k(decay_step_kernel<T>, dim3((unsigned)(a.B * a.H * tiles)), dim3(ST_THREADS), 0,
                     s, a, tiles);

@@ -7,6 +7,11 @@
 // product's whole turns are dropped there, so a far position loses nothing (in float32 a position
 // of 2^20 would be off by 0.06 rad); what remains of it, in [-1/2, 1/2], is exact enough in
 // float32 for the sine and the cosine.
+//
+// Bound: HBM (every value is read and written once).  A thread holds the sines and cosines of the
+// pairs of one piece of 16 bytes (two pieces R columns apart, or one of neighbouring pairs) and takes
+// that piece through a token's heads of queries and keys, four heads' loads in flight: they cost
+// about as much as turning six heads.
 #include "common.cuh"
 #include "mx.cuh"
 
@@ -40,6 +45,94 @@ struct Positions {
     }
 };
 
+// Rounded alike in every form.
+__device__ __forceinline__ float turned0(float a, float b, float cs, float sn) {
+    return fmaf(a, cs, -__fmul_rn(b, sn));
+}
+__device__ __forceinline__ float turned1(float a, float b, float cs, float sn) {
+    return fmaf(a, sn, __fmul_rn(b, cs));
+}
+
+template <int BYTES> struct Piece;
+template <> struct Piece<16> { typedef uint4 type; };
+template <> struct Piece<8> { typedef uint2 type; };
+template <> struct Piece<4> { typedef uint32_t type; };
+
+// The angle of a pair.
+__device__ __forceinline__ void sine(const Positions& pos, const Ladder& ladder, int64_t b, int64_t n,
+                                     uint32_t pair, int inverse, int& axis, double& place, float& cs,
+                                     float& sn) {
+    if (ladder.axis[pair] != axis) {
+        axis = ladder.axis[pair];
+        place = pos.at(b, n, axis);
+    }
+    const double t = place * ladder.turns[pair];
+    sincospif(2.0f * (float)(t - rint(t)), &sn, &cs);
+    if (inverse) sn = -sn;
+}
+
+// Pieces of VEC columns of one token, taken through `per` heads.  Units of a token: the pairs'
+// pieces, then those that are copied.  The thread's index: unit, token, group of heads.
+template <typename T, int VEC, bool INTERLEAVED>
+__global__ void __launch_bounds__(R_THREADS)
+rotary_vec_kernel(Heads q, Heads k, uint32_t hq, uint32_t hk, uint32_t per, uint32_t N, uint32_t turned,
+                  uint32_t units, uint32_t tokens_units, int64_t total, uint32_t pairs, int inverse,
+                  Positions pos, const __grid_constant__ Ladder ladder) {
+    using P = typename Piece<VEC * (int)sizeof(T)>::type;
+    constexpr int NP = INTERLEAVED ? VEC / 2 : VEC;            // pairs of a thread
+    constexpr int U = 4;                                       // heads in flight
+    pdl_wait();
+    pdl_trigger();
+    const int64_t at = (int64_t)blockIdx.x * R_THREADS + threadIdx.x;
+    if (at >= total) return;
+    const uint32_t group = (uint32_t)(at / tokens_units), rest = (uint32_t)(at - (int64_t)group * tokens_units);
+    const uint32_t token = rest / units, u = rest - token * units;
+    const int64_t b = token / N, n = token - (uint32_t)b * N;
+    const bool turn = u < turned;
+    const uint32_t c0 = turn ? u * VEC : 2 * pairs + (u - turned) * VEC;
+    float cs[NP], sn[NP];
+    if (turn) {
+        int axis = -1;
+        double place = 0.0;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) sine(pos, ladder, b, n, u * NP + i, inverse, axis, place, cs[i], sn[i]);
+    }
+    const uint32_t end = min(hq + hk, (group + 1) * per);
+    for (uint32_t h0 = group * per; h0 < end; h0 += U) {
+        P x[U], y[U];
+        T* out[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const uint32_t h = h0 + i;
+            if (h >= end) continue;
+            const Heads& t = h < hq ? q : k;
+            const uint32_t hh = h < hq ? h : h - hq;
+            const T* in = static_cast<const T*>(t.in) + b * t.ib + n * t.in_ + hh * t.ih + c0;
+            out[i] = static_cast<T*>(t.out) + b * t.ob + n * t.on + hh * t.oh + c0;
+            x[i] = *reinterpret_cast<const P*>(in);
+            if (!INTERLEAVED && turn) y[i] = *reinterpret_cast<const P*>(in + pairs);
+        }
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            if (h0 + i >= end) continue;
+            if (turn) {
+                T* a = reinterpret_cast<T*>(&x[i]);
+                T* c = reinterpret_cast<T*>(&y[i]);
+#pragma unroll
+                for (int j = 0; j < NP; ++j) {
+                    T* p0 = INTERLEAVED ? a + 2 * j : a + j;
+                    T* p1 = INTERLEAVED ? a + 2 * j + 1 : c + j;
+                    const float v0 = to_f32(*p0), v1 = to_f32(*p1);
+                    mx::round_to(turned0(v0, v1, cs[j], sn[j]), p0);
+                    mx::round_to(turned1(v0, v1, cs[j], sn[j]), p1);
+                }
+            }
+            *reinterpret_cast<P*>(out[i]) = x[i];
+            if (!INTERLEAVED && turn) *reinterpret_cast<P*>(out[i] + pairs) = y[i];
+        }
+    }
+}
+
 // One thread per token and pair (or column that is not turned); it goes through the heads.
 template <typename T>
 __global__ void __launch_bounds__(R_THREADS)
@@ -69,12 +162,52 @@ rotary_kernel(Heads q, Heads k, uint32_t hq, uint32_t hk, uint32_t N, uint32_t u
         T* out = static_cast<T*>(x.out) + b * x.ob + n * x.on + hh * x.oh;
         const float a0 = to_f32(in[c0]), a1 = to_f32(in[c1]);
         if (turn) {
-            mx::round_to(a0 * cs - a1 * sn, out + c0);
-            mx::round_to(a0 * sn + a1 * cs, out + c1);
+            mx::round_to(turned0(a0, a1, cs, sn), out + c0);
+            mx::round_to(turned1(a0, a1, cs, sn), out + c1);
         } else {
             out[c0] = in[c0];
         }
     }
+}
+
+// The widest piece that every row and both halves are made of, in elements; 1: none.
+int piece(int size, int64_t d, int64_t pairs, int interleaved, const Heads& q, int64_t hq,
+          const Heads& k, int64_t hk, int64_t B, int64_t N) {
+    for (int v = 16 / size; v > 1; v /= 2) {
+        if (d % v || (interleaved ? 2 * pairs : pairs) % v) continue;
+        auto fits = [&](const Heads& x, int64_t heads) {
+            if (!heads) return true;
+            const uintptr_t ends = reinterpret_cast<uintptr_t>(x.in) | reinterpret_cast<uintptr_t>(x.out);
+            return ends % (v * size) == 0 && (B == 1 || (x.ib | x.ob) % v == 0) &&
+                   (N == 1 || (x.in_ | x.on) % v == 0) && (heads == 1 || (x.ih | x.oh) % v == 0);
+        };
+        if (fits(q, hq) && fits(k, hk)) return v;
+    }
+    return 1;
+}
+
+struct VecArgs {
+    Heads q, k;
+    uint32_t hq, hk, per, N, turned, units, tokens_units;
+    int64_t total;
+    uint32_t pairs;
+    int inverse;
+    Positions pos;
+};
+template <typename T, int VEC>
+int run_vec(const VecArgs& a, int interleaved, const Ladder& ladder, cudaStream_t s) {
+    auto kernel = interleaved ? rotary_vec_kernel<T, VEC, true> : rotary_vec_kernel<T, VEC, false>;
+    return launch_k(kernel, dim3((unsigned)((a.total + R_THREADS - 1) / R_THREADS)), dim3(R_THREADS), 0,
+                    s, a.q, a.k, a.hq, a.hk, a.per, a.N, a.turned, a.units, a.tokens_units, a.total,
+                    a.pairs, a.inverse, a.pos, ladder);
+}
+template <typename T>
+int run_vec(const VecArgs& a, int vec, int interleaved, const Ladder& ladder, cudaStream_t s) {
+    constexpr int MOST = 16 / (int)sizeof(T);
+    if (vec == MOST) return run_vec<T, MOST>(a, interleaved, ladder, s);
+    if constexpr (MOST == 8)
+        if (vec == 4) return run_vec<T, 4>(a, interleaved, ladder, s);
+    return run_vec<T, 2>(a, interleaved, ladder, s);
 }
 
 }  // namespace
@@ -119,6 +252,21 @@ extern "C" int snnb_rotary_axes(const void* q, void* q_out, int64_t q_heads,
     const Heads hk = heads(k, k_out, k_heads ? k_strides : nullptr);
     const Positions pos{positions, positions_strides[0], positions_strides[1],
                         positions_strides[2], positions_dtype};
+    const int vec = piece(size, d, pairs, interleaved, hq, q_heads, hk, k_heads, B, N);
+    const int64_t turned = (interleaved ? 2 * pairs : pairs) / vec, pieces = turned + (d - 2 * pairs) / vec;
+    if (vec > 1 && B * N * pieces <= 0x7fffffff) {
+        // as many heads a thread as leave the machine full: 4 blocks of 256 threads an SM
+        const int64_t heads = q_heads + k_heads, tokens_units = B * N * pieces;
+        int64_t per = 16;
+        while (per > 1 && tokens_units * ((heads + per - 1) / per) < 148 * 4 * R_THREADS) per /= 2;
+        const VecArgs a = {hq, hk, (uint32_t)q_heads, (uint32_t)k_heads, (uint32_t)per, (uint32_t)N,
+                           (uint32_t)turned, (uint32_t)pieces, (uint32_t)tokens_units,
+                           tokens_units * ((heads + per - 1) / per), (uint32_t)pairs, inverse, pos};
+        cudaStream_t st = static_cast<cudaStream_t>(stream);
+        if (dtype == SNNB_F32) return run_vec<float>(a, vec, interleaved, ladder, st);
+        if (dtype == SNNB_F16) return run_vec<__half>(a, vec, interleaved, ladder, st);
+        return run_vec<__nv_bfloat16>(a, vec, interleaved, ladder, st);
+    }
     const int64_t total = B * N * units;
     auto kernel = dtype == SNNB_F32   ? rotary_kernel<float>
                   : dtype == SNNB_F16 ? rotary_kernel<__half>

@@ -13,6 +13,8 @@ Inference only: outputs carry no gradient.
 from __future__ import annotations
 
 
+import functools
+
 import torch
 
 from .. import _lib
@@ -24,13 +26,11 @@ MAX_DIM = 256
 
 def _check(q, k, v, decay, lead, what):
     """Argument checks shared by the two forms -> (dtype code, device index, H, Hkv, dk, dv)."""
-    dt = _dtype(q.dtype)
-    n = len(lead)
-    assert q.dim() == k.dim() == v.dim() == n + 2, (tuple(q.shape), tuple(k.shape), tuple(v.shape))
-    H, dk = q.shape[n:]
-    Hkv, dv = v.shape[n:]
-    assert k.shape[:n] == v.shape[:n] == lead and tuple(k.shape[n:]) == (Hkv, dk), \
-        (tuple(q.shape), tuple(k.shape), tuple(v.shape))
+    dt, n, qs, ks, vs = _dtype(q.dtype), len(lead), q.shape, k.shape, v.shape
+    assert len(qs) == len(ks) == len(vs) == n + 2, (tuple(qs), tuple(ks), tuple(vs))
+    H, dk, Hkv, dv = qs[n], qs[n + 1], vs[n], vs[n + 1]
+    assert ks[:n] == vs[:n] == lead and ks[n] == Hkv and ks[n + 1] == dk, \
+        (tuple(qs), tuple(ks), tuple(vs))
     assert k.dtype == v.dtype == q.dtype, (q.dtype, k.dtype, v.dtype)
     if H < 1 or Hkv < 1 or H % Hkv:
         raise ValueError(f"{what}: {H} query heads do not share {Hkv} key heads")
@@ -39,13 +39,13 @@ def _check(q, k, v, decay, lead, what):
     index = _index(q)
     assert k.get_device() == v.get_device() == decay.get_device() == index, \
         (q.device, k.device, v.device, decay.device)
-    assert decay.dtype == torch.float32 and tuple(decay.shape) == (H,) and \
+    assert decay.dtype == torch.float32 and decay.shape == (H,) and \
         decay.is_contiguous(), (tuple(decay.shape), decay.dtype)
     return dt, index, H, Hkv, dk, dv
 
 
 def _state(state, shape, index, what):
-    assert state.dtype == torch.float32 and tuple(state.shape) == shape and \
+    assert state.dtype == torch.float32 and state.shape == shape and \
         state.is_contiguous() and state.get_device() == index, \
         f"{what}: a contiguous float32 {shape} is needed, got {tuple(state.shape)} {state.dtype}"
     return state
@@ -54,9 +54,16 @@ def _state(state, shape, index, what):
 def _out(out, shape, q, what):
     if out is None:
         return q.new_empty(shape)
-    assert tuple(out.shape) == shape and out.dtype == q.dtype and out.is_contiguous() and \
-        out.device == q.device, f"{what}: out {tuple(out.shape)} {out.dtype}"
+    assert out.shape == shape and out.dtype == q.dtype and out.is_contiguous() and \
+        out.get_device() == q.get_device(), f"{what}: out {tuple(out.shape)} {out.dtype}"
     return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace(dt, B, N, H, dk, dv, index):
+    """Bytes of workspace; they follow from the sizes and the device's number of SMs."""
+    with torch.cuda.device(index):
+        return _lib.lib().snnb_decay_attention_workspace_bytes(dt, B, N, H, dk, dv)
 
 
 def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor, *,
@@ -89,7 +96,7 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: to
             (tuple(lengths.shape), lengths.dtype)
         ltype = 1 if lengths.dtype == torch.int64 else 0
     out = _out(out, (B, N, H, dv), q, "decay_attention")
-    need = _lib.lib().snnb_decay_attention_workspace_bytes(dt, B, N, H, dk, dv)
+    need = _workspace(dt, B, N, H, dk, dv, index)
     work = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
     q, k, v = _unit_columns(q), _unit_columns(k), _unit_columns(v)
     _launch("snnb_decay_attention", index, q.data_ptr(), _strides(q), k.data_ptr(), _strides(k),

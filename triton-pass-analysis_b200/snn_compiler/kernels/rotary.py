@@ -39,9 +39,17 @@ def _unit_columns(x: torch.Tensor) -> torch.Tensor:
     return x if x.stride(-1) == 1 or x.shape[-1] <= 1 else x.contiguous()
 
 
+@functools.lru_cache(maxsize=4096)
+def _host_array(*values):
+    return (ctypes.c_int64 * len(values))(*values)
+
+
 def _strides(*tensors):
-    s = [v for t in tensors for v in t.stride()[:-1]]
-    return (ctypes.c_int64 * len(s))(*s)
+    """The strides of all axes but the last, of one tensor after the other, as a host array."""
+    values = ()
+    for t in tensors:
+        values += t.stride()[:-1]
+    return _host_array(*values)
 
 
 def _output(out, x, what):
@@ -66,39 +74,39 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor
     columns (i, i + R), or (2i, 2i + 1) when interleaved.  Its frequency is base^(-i / R)
     (ladder="shared"), or base^(-j / sections[a]) for the j-th pair of axis a (ladder="axis").
     Angles lose nothing at far positions: they are held in float64 turns."""
-    sections = tuple(int(s) for s in sections)
+    sections = tuple(sections)
     if ladder not in ("shared", "axis"):
         raise ValueError(f"rotary_axes: unknown ladder {ladder!r} (shared or axis)")
-    if not base > 0.0 or math.isinf(base):
+    if not 0.0 < base < math.inf:
         raise ValueError(f"rotary_axes: base is {base}")
-    dt = _dtype(q.dtype)
-    assert q.dim() == 4, tuple(q.shape)
-    B, N, H, d = q.shape
-    pairs = sum(sections)
+    dt, shape = _dtype(q.dtype), q.shape
+    assert len(shape) == 4, tuple(shape)
+    B, N, H, d = shape
+    axes, pairs = len(sections), sum(sections)
     if not sections or min(sections) < 0 or pairs < 1 or 2 * pairs > d or pairs > MAX_PAIRS:
         raise ValueError(f"rotary_axes: sections {sections} do not fit a head of {d} columns")
     index = _index(q)
-    if k is not None:
-        assert k.dim() == 4 and k.shape[:2] == (B, N) and k.shape[3] == d and \
-            k.dtype == q.dtype and k.get_device() == index, (tuple(k.shape), k.dtype)
-    ptype = _POSITIONS.get(positions.dtype)
+    ptype, place = _POSITIONS.get(positions.dtype), positions.stride()
     assert ptype is not None, f"positions are int32, int64 or float32, got {positions.dtype}"
-    assert positions.get_device() == index and \
-        tuple(positions.shape) in ((N, len(sections)), (B, N, len(sections))), \
-        (tuple(positions.shape), (B, N, len(sections)))
-    if positions.dim() == 2:
-        positions = positions[None].expand(B, N, len(sections))
+    if len(place) == 2:
+        place = (0,) + place
+        assert positions.shape == (N, axes), (tuple(positions.shape), (N, axes))
+    else:
+        assert positions.shape == (B, N, axes), (tuple(positions.shape), (B, N, axes))
+    assert positions.get_device() == index, (positions.device, q.device)
     turns, axis = _ladder(sections, float(base), ladder)
     q = _unit_columns(q)
     qo = _output(q_out, q, "q_out")
     ko, k_args = None, (None, None, 0, None)
     if k is not None:
+        ks = k.shape
+        assert len(ks) == 4 and ks[0] == B and ks[1] == N and ks[3] == d and \
+            k.dtype == q.dtype and k.get_device() == index, (tuple(ks), k.dtype)
         k = _unit_columns(k)
         ko = _output(k_out, k, "k_out")
-        k_args = (k.data_ptr(), ko.data_ptr(), k.shape[2], _strides(k, ko))
-    pos_strides = (ctypes.c_int64 * 3)(*positions.stride())
+        k_args = (k.data_ptr(), ko.data_ptr(), ks[2], _strides(k, ko))
     _launch("snnb_rotary_axes", index, q.data_ptr(), qo.data_ptr(), H, _strides(q, qo), *k_args, dt,
-            B, N, d, positions.data_ptr(), ptype, pos_strides, turns, axis, pairs,
+            B, N, d, positions.data_ptr(), ptype, _host_array(*place), turns, axis, pairs,
             int(interleaved), int(inverse))
     return qo, ko
 
