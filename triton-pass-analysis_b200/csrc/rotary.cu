@@ -10,8 +10,10 @@
 //
 // Bound: HBM (every value is read and written once).  A thread holds the sines and cosines of the
 // pairs of one piece of 16 bytes (two pieces R columns apart, or one of neighbouring pairs) and takes
-// that piece through a token's heads of queries and keys, four heads' loads in flight: they cost
-// about as much as turning six heads.
+// that piece through about 20 heads (the sines and cosines cost as much as turning six), two heads at a
+// time, the next two's loads in flight.  32768 tokens x 40 heads of 128, bf16: 117 us, 5.8 TB/s (a
+// copy of the same bytes takes 109); 8 heads a thread and four at a time with no loads ahead took
+// 164, 20 heads so 141.
 #include "common.cuh"
 #include "mx.cuh"
 
@@ -74,13 +76,13 @@ __device__ __forceinline__ void sine(const Positions& pos, const Ladder& ladder,
 // Pieces of VEC columns of one token, taken through `per` heads.  Units of a token: the pairs'
 // pieces, then those that are copied.  The thread's index: unit, token, group of heads.
 template <typename T, int VEC, bool INTERLEAVED>
-__global__ void __launch_bounds__(R_THREADS)
+__global__ void __launch_bounds__(R_THREADS, 4)
 rotary_vec_kernel(Heads q, Heads k, uint32_t hq, uint32_t hk, uint32_t per, uint32_t N, uint32_t turned,
                   uint32_t units, uint32_t tokens_units, int64_t total, uint32_t pairs, int inverse,
                   Positions pos, const __grid_constant__ Ladder ladder) {
     using P = typename Piece<VEC * (int)sizeof(T)>::type;
     constexpr int NP = INTERLEAVED ? VEC / 2 : VEC;            // pairs of a thread
-    constexpr int U = 4;                                       // heads in flight
+    constexpr int U = 2;                                       // heads at a time, as many ahead
     pdl_wait();
     pdl_trigger();
     const int64_t at = (int64_t)blockIdx.x * R_THREADS + threadIdx.x;
@@ -98,26 +100,37 @@ rotary_vec_kernel(Heads q, Heads k, uint32_t hq, uint32_t hk, uint32_t per, uint
         for (int i = 0; i < NP; ++i) sine(pos, ladder, b, n, u * NP + i, inverse, axis, place, cs[i], sn[i]);
     }
     const uint32_t end = min(hq + hk, (group + 1) * per);
-    for (uint32_t h0 = group * per; h0 < end; h0 += U) {
-        P x[U], y[U];
-        T* out[U];
+    auto at_head = [&](uint32_t h, bool out) {
+        const Heads& t = h < hq ? q : k;
+        const int64_t hh = h < hq ? h : h - hq;
+        return out ? (T*)t.out + b * t.ob + n * t.on + hh * t.oh + c0
+                   : (T*)t.in + b * t.ib + n * t.in_ + hh * t.ih + c0;
+    };
+    P x[U], y[U];
+    auto load = [&](uint32_t h0) {
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            const uint32_t h = h0 + i;
-            if (h >= end) continue;
-            const Heads& t = h < hq ? q : k;
-            const uint32_t hh = h < hq ? h : h - hq;
-            const T* in = static_cast<const T*>(t.in) + b * t.ib + n * t.in_ + hh * t.ih + c0;
-            out[i] = static_cast<T*>(t.out) + b * t.ob + n * t.on + hh * t.oh + c0;
+            if (h0 + i >= end) continue;
+            const T* in = at_head(h0 + i, false);
             x[i] = *reinterpret_cast<const P*>(in);
             if (!INTERLEAVED && turn) y[i] = *reinterpret_cast<const P*>(in + pairs);
         }
+    };
+    load(group * per);
+    for (uint32_t h0 = group * per; h0 < end; h0 += U) {
+        P x0[U], y0[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            x0[i] = x[i];
+            y0[i] = y[i];
+        }
+        load(h0 + U);                                // a head is read before its piece is written
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             if (h0 + i >= end) continue;
             if (turn) {
-                T* a = reinterpret_cast<T*>(&x[i]);
-                T* c = reinterpret_cast<T*>(&y[i]);
+                T* a = reinterpret_cast<T*>(&x0[i]);
+                T* c = reinterpret_cast<T*>(&y0[i]);
 #pragma unroll
                 for (int j = 0; j < NP; ++j) {
                     T* p0 = INTERLEAVED ? a + 2 * j : a + j;
@@ -127,8 +140,9 @@ rotary_vec_kernel(Heads q, Heads k, uint32_t hq, uint32_t hk, uint32_t per, uint
                     mx::round_to(turned1(v0, v1, cs[j], sn[j]), p1);
                 }
             }
-            *reinterpret_cast<P*>(out[i]) = x[i];
-            if (!INTERLEAVED && turn) *reinterpret_cast<P*>(out[i] + pairs) = y[i];
+            T* out = at_head(h0 + i, true);
+            *reinterpret_cast<P*>(out) = x0[i];
+            if (!INTERLEAVED && turn) *reinterpret_cast<P*>(out + pairs) = y0[i];
         }
     }
 }
@@ -255,10 +269,10 @@ extern "C" int snnb_rotary_axes(const void* q, void* q_out, int64_t q_heads,
     const int vec = piece(size, d, pairs, interleaved, hq, q_heads, hk, k_heads, B, N);
     const int64_t turned = (interleaved ? 2 * pairs : pairs) / vec, pieces = turned + (d - 2 * pairs) / vec;
     if (vec > 1 && B * N * pieces <= 0x7fffffff) {
-        // as many heads a thread as leave the machine full: 4 blocks of 256 threads an SM
-        const int64_t heads = q_heads + k_heads, tokens_units = B * N * pieces;
-        int64_t per = 16;
-        while (per > 1 && tokens_units * ((heads + per - 1) / per) < 148 * 4 * R_THREADS) per /= 2;
+        // about 20 heads a thread, fewer where that leaves less than 4 blocks an SM
+        const int64_t heads = q_heads + k_heads, tokens_units = B * N * pieces, groups = (heads + 19) / 20;
+        int64_t per = (heads + groups - 1) / groups;
+        while (per > 1 && tokens_units * ((heads + per - 1) / per) < 148 * 4 * R_THREADS) per = (per + 1) / 2;
         const VecArgs a = {hq, hk, (uint32_t)q_heads, (uint32_t)k_heads, (uint32_t)per, (uint32_t)N,
                            (uint32_t)turned, (uint32_t)pieces, (uint32_t)tokens_units,
                            tokens_units * ((heads + per - 1) / per), (uint32_t)pairs, inverse, pos};

@@ -19,7 +19,7 @@ import torch
 
 from .. import _lib
 from .mx import _dtype, _index, _launch
-from .rotary import _strides, _unit_columns
+from .rotary import _host_array, _rows
 
 MAX_DIM = 256
 
@@ -86,7 +86,7 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: to
     if state is not None:
         _state(state, sshape, index, "decay_attention: state")
     if state_out is None:
-        state_out = torch.empty(sshape, dtype=torch.float32, device=q.device)
+        state_out = decay.new_empty(sshape)
     else:
         _state(state_out, sshape, index, "decay_attention: state_out")
     ltype = 0
@@ -98,9 +98,9 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: to
     out = _out(out, (B, N, H, dv), q, "decay_attention")
     need = _workspace(dt, B, N, H, dk, dv, index)
     work = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
-    q, k, v = _unit_columns(q), _unit_columns(k), _unit_columns(v)
-    _launch("snnb_decay_attention", index, q.data_ptr(), _strides(q), k.data_ptr(), _strides(k),
-            v.data_ptr(), _strides(v), dt, B, N, H, Hkv, dk, dv, decay.data_ptr(), scale,
+    (q, qs), (k, ks), (v, vs) = _rows(q), _rows(k), _rows(v)
+    (qs, _held_q), (ks, _held_k), (vs, _held_v) = _host_array(qs), _host_array(ks), _host_array(vs)
+    _launch("snnb_decay_attention", index, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, dt, B, N, H, Hkv, dk, dv, decay.data_ptr(), scale,
             None if state is None else state.data_ptr(),
             None if lengths is None else lengths.data_ptr(), ltype, out.data_ptr(),
             state_out.data_ptr(), None if work is None else work.data_ptr(), max(need, 0))
@@ -121,8 +121,8 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, deca
     state_out = state if state_out is None else \
         _state(state_out, sshape, index, "decay_attention_step: state_out")
     out = _out(out, (B, H, dv), q, "decay_attention_step")
-    q, k, v = _unit_columns(q), _unit_columns(k), _unit_columns(v)
-    _launch("snnb_decay_attention_step", index, q.data_ptr(), _strides(q), k.data_ptr(), _strides(k),
-            v.data_ptr(), _strides(v), dt, B, H, Hkv, dk, dv, decay.data_ptr(), scale,
+    (q, qs), (k, ks), (v, vs) = _rows(q), _rows(k), _rows(v)
+    (qs, _held_q), (ks, _held_k), (vs, _held_v) = _host_array(qs), _host_array(ks), _host_array(vs)
+    _launch("snnb_decay_attention_step", index, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, dt, B, H, Hkv, dk, dv, decay.data_ptr(), scale,
             state.data_ptr(), out.data_ptr(), state_out.data_ptr())
     return out, state_out

@@ -25,40 +25,44 @@ _POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 
 @functools.lru_cache(maxsize=64)
 def _ladder(sections: tuple, base: float, ladder: str):
-    """(frequency / 2 pi, axis) of every pair, as host arrays."""
+    """Addresses of (frequency / 2 pi, axis) of every pair, and the arrays, which a caller holds on
+    to while it uses the addresses."""
     total, turns, axis = sum(sections), [], []
     for a, count in enumerate(sections):
         for j in range(count):
             power = len(turns) / total if ladder == "shared" else j / count
             turns.append(base ** -power / (2.0 * math.pi))
             axis.append(a)
-    return (ctypes.c_double * total)(*turns), (ctypes.c_uint8 * total)(*axis)
-
-
-def _unit_columns(x: torch.Tensor) -> torch.Tensor:
-    return x if x.stride(-1) == 1 or x.shape[-1] <= 1 else x.contiguous()
+    turns, axis = (ctypes.c_double * total)(*turns), (ctypes.c_uint8 * total)(*axis)
+    return ctypes.addressof(turns), ctypes.addressof(axis), (turns, axis)
 
 
 @functools.lru_cache(maxsize=4096)
-def _host_array(*values):
-    return (ctypes.c_int64 * len(values))(*values)
+def _host_array(values: tuple):
+    """(address, array) of 64-bit integers; a caller holds the array while it uses the address."""
+    array = (ctypes.c_int64 * len(values))(*values)
+    return ctypes.addressof(array), array
 
 
-def _strides(*tensors):
-    """The strides of all axes but the last, of one tensor after the other, as a host array."""
-    values = ()
-    for t in tensors:
-        values += t.stride()[:-1]
-    return _host_array(*values)
+def _rows(x: torch.Tensor):
+    """(x with unit column stride: itself where it has one, the strides of its other axes)."""
+    strides = x.stride()
+    if strides[-1] != 1 and x.shape[-1] > 1:
+        x = x.contiguous()
+        strides = x.stride()
+    return x, strides[:-1]
 
 
-def _output(out, x, what):
+def _output(out, x, shape, what):
+    """(out or a new tensor for it, the strides of all its axes but the last)."""
     if out is None:
-        return x.new_empty(x.shape)
-    assert out.shape == x.shape and out.dtype == x.dtype and out.device == x.device and \
-        (out.stride(-1) == 1 or out.shape[-1] <= 1), \
-        f"rotary_axes: {what} {tuple(out.shape)} {out.dtype} does not fit {tuple(x.shape)} {x.dtype}"
-    return out
+        out = x.new_empty(shape)
+        return out, out.stride()[:-1]
+    strides = out.stride()
+    assert out.shape == shape and out.dtype == x.dtype and out.get_device() == x.get_device() and \
+        (strides[-1] == 1 or shape[-1] <= 1), \
+        f"rotary_axes: {what} {tuple(out.shape)} {out.dtype} does not fit {tuple(shape)} {x.dtype}"
+    return out, strides[:-1]
 
 
 def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, *, sections,
@@ -94,20 +98,23 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor
     else:
         assert positions.shape == (B, N, axes), (tuple(positions.shape), (B, N, axes))
     assert positions.get_device() == index, (positions.device, q.device)
-    turns, axis = _ladder(sections, float(base), ladder)
-    q = _unit_columns(q)
-    qo = _output(q_out, q, "q_out")
-    ko, k_args = None, (None, None, 0, None)
+    turns, axis, _held = _ladder(sections, float(base), ladder)
+    q, strides = _rows(q)
+    qo, out_strides = _output(q_out, q, shape, "q_out")
+    q_strides, _held_q = _host_array(strides + out_strides)
+    ko, kp, kop, Hk, k_strides = None, None, None, 0, None
     if k is not None:
         ks = k.shape
         assert len(ks) == 4 and ks[0] == B and ks[1] == N and ks[3] == d and \
             k.dtype == q.dtype and k.get_device() == index, (tuple(ks), k.dtype)
-        k = _unit_columns(k)
-        ko = _output(k_out, k, "k_out")
-        k_args = (k.data_ptr(), ko.data_ptr(), ks[2], _strides(k, ko))
-    _launch("snnb_rotary_axes", index, q.data_ptr(), qo.data_ptr(), H, _strides(q, qo), *k_args, dt,
-            B, N, d, positions.data_ptr(), ptype, _host_array(*place), turns, axis, pairs,
-            int(interleaved), int(inverse))
+        k, strides = _rows(k)
+        ko, out_strides = _output(k_out, k, ks, "k_out")
+        kp, kop, Hk = k.data_ptr(), ko.data_ptr(), ks[2]
+        k_strides, _held_k = _host_array(strides + out_strides)
+    place, _held_p = _host_array(place)
+    _launch("snnb_rotary_axes", index, q.data_ptr(), qo.data_ptr(), H, q_strides, kp, kop, Hk,
+            k_strides, dt, B, N, d, positions.data_ptr(), ptype, place, turns, axis, pairs,
+            1 if interleaved else 0, 1 if inverse else 0)
     return qo, ko
 
 
