@@ -620,7 +620,7 @@ int snnb_decay_attention_step(const void* q, const int64_t* q_strides, const voi
  * out = act((x - mean) / sqrt(var + eps) * weight + bias) of channels-last x [B, S, C], mean and
  * biased variance over the S * C / groups values of each group of channels of a sample.  weight
  * and bias [C] of weight_dtype (x's or F32), either may be NULL; out [B, S, C] contiguous, of x's
- * type.
+ * type, may be x where that is contiguous.  C up to 16384.
  */
 int snnb_group_norm_act(const void* x, int64_t x_batch_stride, int64_t x_row_stride, int dtype,
                         int64_t B, int64_t S, int64_t C, int64_t groups, const void* weight,

@@ -11,6 +11,7 @@ import torch
 
 from .mx import _DTYPES, _dtype, _index, _launch
 
+MAX_CHANNELS = 16384
 ACTIVATIONS = {"none": 0, "silu": 1, "relu": 2, "gelu": 3}
 
 
@@ -30,8 +31,8 @@ def group_norm_act(x: torch.Tensor, groups: int, weight: torch.Tensor | None = N
         raise ValueError(f"group_norm_act: eps is {eps}")
     assert len(shape) >= 2, f"group_norm_act: x is [B, ..., C], got {tuple(shape)}"
     B, C = shape[0], shape[-1]
-    if groups < 1 or C < 1 or C % groups:
-        raise ValueError(f"group_norm_act: {C} channels in {groups} groups")
+    if groups < 1 or C < 1 or C % groups or C > MAX_CHANNELS:
+        raise ValueError(f"group_norm_act: {C} channels in {groups} groups (up to {MAX_CHANNELS})")
     index = _index(x)
     wd = None
     for name, t in (("weight", weight), ("bias", bias)):
