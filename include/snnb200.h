@@ -620,12 +620,14 @@ int snnb_decay_attention_step(const void* q, const int64_t* q_strides, const voi
  * out = act((x - mean) / sqrt(var + eps) * weight + bias) of channels-last x [B, S, C], mean and
  * biased variance over the S * C / groups values of each group of channels of a sample.  weight
  * and bias [C] of weight_dtype (x's or F32), either may be NULL; out [B, S, C] contiguous, of x's
- * type, may be x where that is contiguous.  C up to 16384.
+ * type, may be x where that is contiguous.  C up to 16384.  workspace: 8-byte aligned, of
+ * snnb_group_norm_act_workspace_bytes (negative: bad sizes; 0: none), for this call alone.
  */
+int64_t snnb_group_norm_act_workspace_bytes(int dtype, int64_t B, int64_t S, int64_t C, int64_t groups);
 int snnb_group_norm_act(const void* x, int64_t x_batch_stride, int64_t x_row_stride, int dtype,
                         int64_t B, int64_t S, int64_t C, int64_t groups, const void* weight,
                         const void* bias, int weight_dtype, float eps, int act, void* out,
-                        snnb_stream_t stream);
+                        void* workspace, int64_t workspace_bytes, snnb_stream_t stream);
 
 /*
  * Reads and clears the device status word that kernels with bounded waits write

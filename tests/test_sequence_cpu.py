@@ -195,7 +195,7 @@ def test_c_entries_reject_bad_arguments_without_a_device():
 
     def norm(**kw):
         a = dict(x=p, xb=96, xs=12, dt=2, B=2, S=8, C=12, G=4, w=p, b=p, wd=0, eps=1e-5, act=0,
-                 out=p, st=None)
+                 out=p, ws=None, wsb=0, st=None)
         a.update(kw)
         return L.snnb_group_norm_act(*a.values())
     for bad in (dict(dt=3), dict(wd=1), dict(act=4), dict(act=-1), dict(eps=-1.0),
@@ -204,3 +204,9 @@ def test_c_entries_reject_bad_arguments_without_a_device():
                 dict(B=1 << 31), dict(S=1 << 31), dict(C=1 << 30, G=1)):
         assert norm(**bad) == -1, bad
     assert norm(B=0) == 0 and norm(S=0) == 0
+    need = L.snnb_group_norm_act_workspace_bytes(2, 64, 3136, 256, 32)
+    assert need > 0 and L.snnb_group_norm_act_workspace_bytes(2, 2, 8, 12, 4) == 0
+    assert L.snnb_group_norm_act_workspace_bytes(2, 2, 8, 12, 5) < 0
+    large = dict(B=64, S=3136, C=256, G=32, xb=3136 * 256, xs=256)
+    assert norm(**large) == -1 and norm(ws=p, wsb=need - 1, **large) == -1
+    assert norm(ws=ctypes.c_void_p((1 << 20) + 4), wsb=need, **large) == -1

@@ -414,6 +414,24 @@ def test_group_norm_against_oracle(shape, groups, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape,groups,pad", [((9, 37, 41, 330), 33, 0), ((3, 9000, 257), 257, 0),
+                                              ((40, 200, 1030), 2, 3), ((2, 20000, 130), 26, 6),
+                                              ((33, 4, 40000), 8, 0), ((1, 70000, 64), 1, 0),
+                                              ((5, 300, 6, 512), 4, 16), ((1100, 4096), 1, 0)])
+def test_group_norm_of_large_tensors(shape, groups, pad, dtype):
+    g = _gen(groups)
+    C = min(shape[-1], 16384)
+    x = torch.randn(*shape[:-1], C + pad, generator=g) * 2
+    x = (x + torch.randn(C + pad, generator=g) * 3).to(dtype)
+    w, b = (torch.randn(C, generator=g).to(dtype) for _ in range(2))
+    view = x.to(DEV)[..., :C]
+    _norm_check(x[..., :C].contiguous(), groups, w, b, act="silu", view=view)
+    if not pad:                                                 # in place
+        y = _k().group_norm_act(view, groups, act="gelu")
+        assert torch.equal(_k().group_norm_act(view, groups, act="gelu", out=view), y)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("cols,at,C,groups", [(48, 0, 40, 5), (48, 8, 40, 5), (47, 3, 40, 5), (391, 7, 384, 8),
                                               (90, 1, 66, 22)])
 def test_group_norm_slices_of_a_wider_tensor(cols, at, C, groups, dtype):

@@ -75,7 +75,8 @@ SIGNATURES = {
     "snnb_decay_attention": [P, P, P, P, P, P, I32, I64, I64, I64, I64, I64, I64, P, F, P, P, I32, P,
                              P, P, I64, P],
     "snnb_decay_attention_step": [P, P, P, P, P, P, I32, I64, I64, I64, I64, I64, P, F, P, P, P, P],
-    "snnb_group_norm_act": [P, I64, I64, I32, I64, I64, I64, I64, P, P, I32, F, I32, P, P],
+    "snnb_group_norm_act_workspace_bytes": [I32, I64, I64, I64, I64],
+    "snnb_group_norm_act": [P, I64, I64, I32, I64, I64, I64, I64, P, P, I32, F, I32, P, P, I64, P],
     "snnb_conv3x3_lif_static_scratch": [P, I64, I64, I64, I64, I64, P, P, I64, F, F, F, F, I32,
                                         I32, I32, I32, P, P],
 }
@@ -110,6 +111,7 @@ def lib():
             fn.argtypes = args
             fn.restype = ctypes.c_int
         L.snnb_decay_attention_workspace_bytes.restype = ctypes.c_int64
+        L.snnb_group_norm_act_workspace_bytes.restype = ctypes.c_int64
         _lib = L
     return _lib
 

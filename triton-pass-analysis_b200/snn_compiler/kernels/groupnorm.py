@@ -7,12 +7,20 @@ Inference only: outputs carry no gradient.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
+from .. import _lib
 from .mx import _DTYPES, _dtype, _index, _launch
 
 MAX_CHANNELS = 16384
 ACTIVATIONS = {"none": 0, "silu": 1, "relu": 2, "gelu": 3}
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace(dt, B, S, C, groups):
+    return _lib.lib().snnb_group_norm_act_workspace_bytes(dt, B, S, C, groups)
 
 
 def group_norm_act(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None,
@@ -53,8 +61,10 @@ def group_norm_act(x: torch.Tensor, groups: int, weight: torch.Tensor | None = N
     x3 = x.view(B, 1, C) if x.dim() == 2 else x.flatten(1, -2)
     if x3.stride(2) != 1 and C > 1:
         x3 = x3.contiguous()
+    need = _workspace(dt, B, x3.shape[1], C, groups)
+    work = x.new_empty(need, dtype=torch.uint8) if need > 0 else None
     _launch("snnb_group_norm_act", index, x3.data_ptr(), x3.stride(0), x3.stride(1), dt, B,
             x3.shape[1], C, groups, None if weight is None else weight.data_ptr(),
             None if bias is None else bias.data_ptr(), _DTYPES[wd or torch.float32], eps, code,
-            out.data_ptr())
+            out.data_ptr(), None if work is None else work.data_ptr(), max(need, 0))
     return out
