@@ -90,15 +90,19 @@ __device__ __forceinline__ void params(const void* p, int f32, uint32_t c, float
         for (int i = 0; i < VEC; ++i) v[i] = to_f32(static_cast<const T*>(p)[c + i]);
     }
 }
-// (x - mean) * scale + shift, activated and rounded.
-template <typename T, int VEC, int ACT>
+// (x - mean) * scale + shift, activated and rounded.  FOLDED: shift holds - mean * scale too.
+template <typename T, int VEC, int ACT, bool FOLDED = false>
 __device__ __forceinline__ Bits<VEC * sizeof(T)> finish(const float (&x)[VEC], const float (&mean)[VEC],
-                                                                       const float (&scale)[VEC],
-                                                                       const float (&shift)[VEC]) {
+                                                        const float (&scale)[VEC], const float (&shift)[VEC]) {
     Bits<VEC * sizeof(T)> r;
     float f[VEC];
     if constexpr (VEC == 1) {
-        f[0] = fmaf(x[0] - mean[0], scale[0], shift[0]);
+        f[0] = FOLDED ? fmaf(x[0], scale[0], shift[0]) : fmaf(x[0] - mean[0], scale[0], shift[0]);
+    } else if constexpr (FOLDED) {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 2)
+            mx::unpack2(mx::fma2(mx::pack2(x[i], x[i + 1]), mx::pack2(scale[i], scale[i + 1]),
+                                 mx::pack2(shift[i], shift[i + 1])), f[i], f[i + 1]);
     } else {
 #pragma unroll
         for (int i = 0; i < VEC; i += 2) {
@@ -457,7 +461,7 @@ struct PassArgs {
 template <typename T, int VEC>
 __global__ void __launch_bounds__(GN_THREADS, 4) gn_stats_kernel(const __grid_constant__ PassArgs s) {
     using V = Bits<VEC * (int)sizeof(T)>;
-    constexpr int U = 8;                       // rows in flight
+    constexpr int U = 4;                       // rows at a time, as many ahead
     extern __shared__ float part[];            // [rows][width], then [groups] means
     const GnArgs& a = s.a;
     pdl_wait();
@@ -489,21 +493,31 @@ __global__ void __launch_bounds__(GN_THREADS, 4) gn_stats_kernel(const __grid_co
             }
         }
     };
+    V raw[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+        if (i < left) raw[i] = *reinterpret_cast<const V*>(x + i * step);
     if (left) {                                // minus the first row: near enough to the mean that the
-        unpack<T, VEC>(*reinterpret_cast<const V*>(x), base);  // squares do not cancel
+        unpack<T, VEC>(raw[0], base);          // squares do not cancel
         if constexpr (VEC > 1) {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) base[j] = -base[j];
         }
     }
-    for (; left >= U; left -= U, x += U * step) {
-        V raw[U];
+    for (; left >= 2 * U; left -= U) {         // the next rows in flight
+        V now[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) now[i] = raw[i];
+        x += U * step;
 #pragma unroll
         for (int i = 0; i < U; ++i) raw[i] = *reinterpret_cast<const V*>(x + i * step);
 #pragma unroll
-        for (int i = 0; i < U; ++i) add(raw[i]);
+        for (int i = 0; i < U; ++i) add(now[i]);
     }
-    for (; left; --left, x += step) add(*reinterpret_cast<const V*>(x));
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+        if (i < left) add(raw[i]);
+    for (uint32_t i = U; i < left; ++i) add(*reinterpret_cast<const V*>(x + i * step));
     // the thread's own means and squares around them
     const float over = count > 0.0f ? 1.0f / count : 0.0f;
     float acc[VEC];
@@ -556,6 +570,7 @@ template <typename T, int VEC, int ACT>
 __global__ void __launch_bounds__(GN_THREADS, 4) gn_apply_kernel(const __grid_constant__ PassArgs s) {
     using V = Bits<VEC * (int)sizeof(T)>;
     constexpr int U = 4;
+    constexpr bool FOLDED = sizeof(T) == 2;
     extern __shared__ float groups_of[];       // [groups] mean, [groups] 1 / deviation
     const GnArgs& a = s.a;
     pdl_wait();
@@ -606,11 +621,13 @@ __global__ void __launch_bounds__(GN_THREADS, 4) gn_apply_kernel(const __grid_co
         const uint32_t g = s.per_group.div(vc * VEC + j);
         mean[j] = groups_of[g];
         w[j] *= groups_of[groups + g];
+        // 16-bit values: a mean that is 2^k deviations leaves them 11 - k bits or fewer, and this 24 - k
+        if (FOLDED) shift[j] = fmaf(-mean[j], w[j], shift[j]);
     }
     auto put = [&](const V& bits, T* to) {
         float f[VEC];
         unpack<T, VEC>(bits, f);
-        *reinterpret_cast<V*>(to) = finish<T, VEC, ACT>(f, mean, w, shift);
+        *reinterpret_cast<V*>(to) = finish<T, VEC, ACT, FOLDED>(f, mean, w, shift);
     };
     for (; left >= 2 * U; left -= U) {         // the next rows in flight
         V now[U];
@@ -652,8 +669,9 @@ bool plan_passes(const GnArgs& a, uint32_t vec, PassArgs& p) {
     p.chunks = (a.S + p.chunk - 1) / p.chunk;
     return (int64_t)a.B * p.chunks * p.slabs <= 0x7fffffff;
 }
-// From here on the two passes are faster (64 x 784 x 256 bf16, 26 MB: 20 us in one pass).
-constexpr int64_t TWO_PASSES = int64_t(8) << 20;
+// Bytes from which the two passes are faster (bf16: 64 x 784 x 256, 26 MB, 28 us and 19 in one pass;
+// 64 x 3136 x 256, 103 MB, 72 and 81).
+constexpr int64_t TWO_PASSES = int64_t(64) << 20;
 
 template <typename T, int VEC, int ACT>
 int run_passes(PassArgs p, cudaStream_t s) {
