@@ -16,100 +16,248 @@ namespace {
 
 using namespace decay;
 
-constexpr int GC = 32;             // tokens of a chunk
-constexpr int GV = 32;             // columns of the state that a thread block holds
+constexpr int GC = 64;             // tokens of a chunk
+constexpr int GV = 64;             // columns of the state that a thread block holds
+constexpr int GP = GC + 4;         // floats of a row of a tile: 16-byte aligned, four banks on a row
 constexpr int G_THREADS = 256;
 
-// Every type, size and stride: products in float32 on the CUDA cores, a thread block per
-// sequence, head and GV columns of its state.
-template <typename T>
-__global__ void __launch_bounds__(G_THREADS) decay_any_kernel(Args a, uint32_t tiles) {
-    extern __shared__ float sm[];
-    const int dk = a.dk;
-    float* S = sm;                                 // [dk][GV]
-    float* q = S + dk * GV;                        // [GC][dk + 1]
-    float* k = q + GC * (dk + 1);
-    float* v = k + GC * (dk + 1);                  // [GC][GV]
-    float* p = v + GC * GV;                        // [GC][GC + 1]
-    float* pw = p + GC * (GC + 1);                 // [GC + 1]
+struct AnyArgs {
+    Args a;
+    uint32_t tiles, items;         // of GV columns; of this launch
+    int segs, cps;                 // segments of each sequence, chunks of a segment
+    float* work;                   // [segs][B H tiles][dk][GV] states (slot segs - 1: the start)
+};
+
+__device__ __forceinline__ void fma44(float (&c)[4][4], const float4& a, const float4& b) {
+    const float x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c[i][j] = fmaf(x[i], y[j], c[i][j]);
+}
+
+// Every type, size and stride: products in float32 on the CUDA cores, 4 x 4 results a thread, from
+// tiles in shared memory.  A thread block takes a segment of a sequence, a head and GV columns.
+// STATES: only the states that the segments leave, each from zero (the first: from state_in).
+template <typename T, bool STATES>
+__global__ void __launch_bounds__(G_THREADS, 2) decay_any_kernel(const __grid_constant__ AnyArgs p) {
+    extern __shared__ float4 sm4[];
+    const Args& a = p.a;
+    const int dk = a.dk, dkp = (dk + 3) / 4 * 4, t = threadIdx.x, warp = t >> 5, lane = t & 31;
+    float* S = reinterpret_cast<float*>(sm4);      // [dkp][GP]
+    float* k = S + dkp * GP;                       // [dkp][GP]: column-major, tokens along a row
+    float* v = k + dkp * GP;                       // [GC][GP]
+    float* q = v + GC * GP;                        // [dkp][GP], as k; then the scores, [GC][GP]
+    float* pt = q;
+    float* pw = q + (STATES ? 0 : max(dkp, GC) * GP);          // decay^0 .. decay^GC
     pdl_wait();
     pdl_trigger();
-    const uint32_t tile = blockIdx.x % tiles, bh = blockIdx.x / tiles;
-    const int64_t b = bh / a.H, h = bh - b * a.H, hk = h / (a.H / a.Hk);
-    const int c0 = tile * GV, nv = min(GV, a.dv - c0), t = threadIdx.x;
-    const int64_t len = a.length(b);
-    if (t <= GC) pw[t] = (float)power(a.decay[h], t);
-    const float* s_in = a.state_in ? a.state_in + (b * a.H + h) * dk * a.dv + c0 : nullptr;
-    for (int i = t; i < dk * GV; i += G_THREADS)
-        S[i] = s_in && i % GV < nv ? s_in[(int64_t)(i / GV) * a.dv + i % GV] : 0.0f;
+    const uint32_t rest = blockIdx.x / p.tiles, tile = blockIdx.x - rest * p.tiles;
+    const uint32_t sb = rest / (uint32_t)a.H, h = rest - sb * (uint32_t)a.H;
+    const uint32_t seg = sb / (uint32_t)a.B, b = sb - seg * (uint32_t)a.B, hk = h / (uint32_t)(a.H / a.Hk);
+    const int c0 = tile * GV, nv = min(GV, a.dv - c0);
+    const int64_t len = a.length(b), chunks = (len + GC - 1) / GC;
+    const int64_t first = min((int64_t)seg * p.cps, chunks), count = min((int64_t)p.cps, chunks - first);
+    const bool end = first + count == chunks && (count > 0 || seg == 0);
+    const float lam = a.decay[h];
+    const int last = count > 0 && first + count == chunks ? (int)(len - (chunks - 1) * GC) : GC;
+    if (t <= GC) pw[t] = (float)power(lam, t);
+    const int64_t bht = ((int64_t)b * a.H + h) * p.tiles + tile, slot = a.B * a.H * p.tiles * (int64_t)(dk * GV);
+    float* work = p.work + bht * (dk * GV);
+    const int64_t state = ((int64_t)b * a.H + h) * dk * a.dv + c0;
+    // what there is before the first chunk
+    {
+        const double d = power(lam, p.cps * GC);
+        const float fh = (float)d, fl = (float)(d - (double)fh);
+        for (int i = t; i < dkp * GV; i += G_THREADS) {
+            const int r = i / GV, c = i % GV;
+            float x = 0.0f;
+            if (r < dk && c < nv) {
+                if (seg == 0) {
+                    if (a.state_in)
+                        x = !STATES && p.segs > 1 ? work[(p.segs - 1) * slot + r * GV + c]
+                                                  : a.state_in[state + (int64_t)r * a.dv + c];
+                } else if (!STATES) {
+                    x = work[r * GV + c];
+                    for (uint32_t s = 1; s < seg; ++s)
+                        x = fmaf(x, fh, fmaf(x, fl, work[s * slot + r * GV + c]));
+                }
+                // state_out may be state_in
+                if (STATES && seg == 0 && a.state_in) work[(p.segs - 1) * slot + r * GV + c] = x;
+            }
+            S[r * GP + c] = x;
+        }
+    }
+    const double dc = power(lam, GC), dl = power(lam, last);
+    const float ch = (float)dc, cl = (float)(dc - (double)ch), lh = (float)dl, ll = (float)(dl - (double)lh);
     const T* qg = static_cast<const T*>(a.q) + b * a.qs[0] + h * a.qs[2];
     const T* kg = static_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[2];
     const T* vg = static_cast<const T*>(a.v) + b * a.vs[0] + hk * a.vs[2] + c0;
-    T* og = static_cast<T*>(a.out) + (b * a.N * a.H + h) * a.dv + c0;
-    for (int64_t n0 = 0; n0 < a.N; n0 += GC) {
-        const int m = (int)max((int64_t)0, min((int64_t)GC, len - n0));
-        if (m == 0) {                              // rows behind the sequence
-            const int left = (int)min((int64_t)GC, a.N - n0);
-            for (int i = t; i < left * GV; i += G_THREADS)
-                if (i % GV < nv) mx::round_to(0.0f, og + (n0 + i / GV) * a.H * a.dv + i % GV);
-            continue;
-        }
+    T* og = static_cast<T*>(a.out) + ((int64_t)b * a.N * a.H + h) * a.dv + c0;
+    const int64_t ld = a.H * a.dv;
+    const int i0 = t / 16 * 4, j0 = t % 16 * 4;    // this thread's rows and columns
+    for (int64_t n = 0; n < count; ++n) {
+        const int64_t n0 = (first + n) * GC;
+        const int m = n + 1 == count ? last : GC;
         __syncthreads();
-        for (int i = t; i < GC * dk; i += G_THREADS) {
-            const int r = i / dk, c = i - r * dk;
-            q[r * (dk + 1) + c] = r < m ? to_f32(qg[(n0 + r) * a.qs[1] + c]) * a.scale : 0.0f;
-            k[r * (dk + 1) + c] = r < m ? to_f32(kg[(n0 + r) * a.ks[1] + c]) : 0.0f;
-        }
-        for (int i = t; i < GC * GV; i += G_THREADS) {
-            const int r = i / GV, c = i % GV;
-            v[i] = r < m && c < nv ? to_f32(vg[(n0 + r) * a.vs[1] + c]) : 0.0f;
-        }
-        __syncthreads();
-        for (int i = t; i < GC * GC; i += G_THREADS) {
-            const int r = i / GC, c = i % GC;
-            float s = 0.0f;
-            if (c <= r) {
-                for (int x = 0; x < dk; ++x) s += q[r * (dk + 1) + x] * k[c * (dk + 1) + x];
-                s *= pw[r - c];
+        bool bad = false;
+        for (int r = warp; r < GC; r += G_THREADS / 32) {      // a warp: a token's row
+            const T* kr = kg + (n0 + r) * a.ks[1];
+            const T* qr = qg + (n0 + r) * a.qs[1];
+            const T* vr = vg + (n0 + r) * a.vs[1];
+            for (int c = lane; c < dkp; c += 32) {
+                const bool in = r < m && c < dk;
+                k[c * GP + r] = in ? to_f32(kr[c]) : 0.0f;
+                if (!STATES) q[c * GP + r] = in ? to_f32(qr[c]) * a.scale : 0.0f;
             }
-            p[r * (GC + 1) + c] = s;
+            for (int c = lane; c < GV; c += 32) {
+                const float x = r < m && c < nv ? to_f32(vr[c]) : 0.0f;
+                bad |= !(fabsf(x) <= 3.4028235e38f);
+                v[r * GP + c] = x;
+            }
         }
-        __syncthreads();
+        bad = __syncthreads_or(bad);
+        if (!STATES) {
+            float s[4][4] = {};
+            if (j0 <= i0 + 3) {
+#pragma unroll 4
+                for (int x = 0; x < dkp; ++x)
+                    fma44(s, *reinterpret_cast<const float4*>(q + x * GP + i0),
+                          *reinterpret_cast<const float4*>(k + x * GP + j0));
+            }
+            float o[4][4] = {};
+#pragma unroll 4
+            for (int x = 0; x < dkp; ++x)
+                fma44(o, *reinterpret_cast<const float4*>(q + x * GP + i0),
+                      *reinterpret_cast<const float4*>(S + x * GP + j0));
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[i][j] *= pw[i0 + i + 1];
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {          // later tokens count nothing, whatever their scores
+                float y[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] = j0 + j <= i0 + i ? s[i][j] * pw[i0 + i - j0 - j] : 0.0f;
+                *reinterpret_cast<float4*>(pt + (j0 + j) * GP + i0) = make_float4(y[0], y[1], y[2], y[3]);
+            }
+            __syncthreads();
+            if (!bad) {
+#pragma unroll 4
+                for (int x = 0; x < i0 + 4; ++x)
+                    fma44(o, *reinterpret_cast<const float4*>(pt + x * GP + i0),
+                          *reinterpret_cast<const float4*>(v + x * GP + j0));
+            } else {                               // 0 * inf would reach rows before the infinity
+                for (int x = 0; x < i0 + 4; ++x)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (x <= i0 + i)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                o[i][j] = fmaf(pt[x * GP + i0 + i], v[x * GP + j0 + j], o[i][j]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (n0 + i0 + i < a.N && j0 + j < nv)
+                        mx::round_to(i0 + i < m ? o[i][j] : 0.0f, og + (n0 + i0 + i) * ld + j0 + j);
+            __syncthreads();
+        }
+        // the rows of v by what is left of them at the chunk's end
         for (int i = t; i < GC * GV; i += G_THREADS) {
-            const int r = i / GV, c = i % GV;
-            float s = 0.0f;
-            for (int x = 0; x < dk; ++x) s += q[r * (dk + 1) + x] * S[x * GV + c];
-            s *= pw[r + 1];
-            for (int x = 0; x <= r; ++x) s += p[r * (GC + 1) + x] * v[x * GV + c];
-            if (n0 + r < a.N && c < nv)
-                mx::round_to(r < m ? s : 0.0f, og + (n0 + r) * a.H * a.dv + c);
+            const int r = i / GV;
+            if (r < m) v[r * GP + i % GV] *= pw[m - 1 - r];
         }
         __syncthreads();
-        for (int i = t; i < dk * GV; i += G_THREADS) {
-            const int r = i / GV, c = i % GV;
-            float s = pw[m] * S[i];
-            for (int x = 0; x < m; ++x) s += pw[m - 1 - x] * k[x * (dk + 1) + r] * v[x * GV + c];
-            S[i] = s;
+        const float fh = m == GC ? ch : lh, fl = m == GC ? cl : ll;
+        for (int r = i0; r < dkp; r += 64) {
+            float s[4][4] = {};
+#pragma unroll 4
+            for (int x = 0; x < GC; x += 4) {
+                float4 kk[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) kk[i] = *reinterpret_cast<const float4*>(k + (r + i) * GP + x);
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const float4 vv = *reinterpret_cast<const float4*>(v + (x + y) * GP + j0);
+                    const float* k0 = reinterpret_cast<const float*>(&kk[0]);
+                    fma44(s, make_float4(k0[y], k0[4 + y], k0[8 + y], k0[12 + y]), vv);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float& x = S[(r + i) * GP + j0 + j];
+                    x = fmaf(x, fh, fmaf(x, fl, s[i][j]));
+                }
         }
     }
-    if (a.state_out) {
-        float* s_out = a.state_out + (b * a.H + h) * dk * a.dv + c0;
-        __syncthreads();
-        for (int i = t; i < dk * GV; i += G_THREADS)
-            if (i % GV < nv) s_out[(int64_t)(i / GV) * a.dv + i % GV] = S[i];
+    if (!STATES && end) {                          // rows behind the last chunk
+        for (int64_t n = chunks * GC + warp; n < a.N; n += G_THREADS / 32)
+            for (int c = lane; c < nv; c += 32) mx::round_to(0.0f, og + n * ld + c);
+    }
+    __syncthreads();
+    if (STATES || (end && a.state_out)) {
+        for (int i = t; i < dk * GV; i += G_THREADS) {
+            const int r = i / GV, c = i % GV;
+            if (c >= nv) continue;
+            if (STATES) work[seg * slot + r * GV + c] = S[r * GP + c];
+            else a.state_out[state + (int64_t)r * a.dv + c] = S[r * GP + c];
+        }
     }
 }
 
-template <typename T>
-int run_any(const Args& a, cudaStream_t s) {
-    const uint32_t tiles = (a.dv + GV - 1) / GV;
-    const size_t smem = (size_t)(a.dk * GV + 2 * GC * (a.dk + 1) + GC * GV + GC * (GC + 1) + GC + 1) * 4;
-    auto k = decay_any_kernel<T>;
+// As for the tensor cores' form; a chunk of 64 tokens at 64 columns of k takes about 6 us (1.5 in the
+// pass before), both in proportion to dk.
+int any_segments(int64_t items, int64_t chunks, int64_t dk) {
+    const int64_t slots = dk <= 64 ? 296 : 148;
+    int best = 1;
+    int64_t least = 0;
+    for (int n = 1; n <= 16 && (n == 1 || (chunks >= 2 * n && items <= slots)); ++n) {
+        const int64_t cps = (chunks + n - 1) / n;
+        if ((n - 1) * cps >= chunks) continue;
+        const int64_t rounds = (items * n + slots - 1) / slots, before = (items * (n - 1) + slots - 1) / slots;
+        const int64_t t = rounds * (cps * dk + 40) + before * (cps * dk / 4 + 40) + (n > 1 ? 60 : 0);
+        if (n == 1 || t < least) {
+            best = n;
+            least = t;
+        }
+    }
+    return best;
+}
+int64_t any_workspace(int64_t B, int64_t N, int64_t H, int64_t dk, int64_t dv) {
+    const int64_t items = B * H * ((dv + GV - 1) / GV);
+    const int segs = any_segments(items, (N + GC - 1) / GC, dk);
+    return segs > 1 ? segs * items * dk * GV * 4 : 0;
+}
+
+constexpr int any_smem(int dk, bool states) {
+    const int dkp = (dk + 3) / 4 * 4;
+    return ((2 * dkp + (states ? 0 : dkp > GC ? dkp : GC) + GC) * GP + GC + 4) * 4;
+}
+static_assert(any_smem(MAX_DIM, false) <= 227 * 1024, "shared memory");
+template <typename T, bool STATES>
+int launch_any(AnyArgs p, cudaStream_t s) {
     // once per device, at the most that any call asks for
-    if (const int st = allow_smem<decay_any_kernel<T>>(
-            (MAX_DIM * GV + 2 * GC * (MAX_DIM + 1) + GC * GV + GC * (GC + 1) + GC + 1) * 4))
-        return st;
-    return launch_k(k, dim3((unsigned)(a.B * a.H * tiles)), dim3(G_THREADS), smem, s, a, tiles);
+    if (const int st = allow_smem<decay_any_kernel<T, STATES>>(any_smem(MAX_DIM, STATES))) return st;
+    p.items = (uint32_t)(p.a.B * p.a.H * p.tiles * (STATES ? p.segs - 1 : p.segs));
+    return launch_k(decay_any_kernel<T, STATES>, dim3(p.items), dim3(G_THREADS), any_smem(p.a.dk, STATES), s, p);
+}
+template <typename T>
+int run_any(const Args& a, void* work, int64_t bytes, cudaStream_t s) {
+    const uint32_t tiles = (a.dv + GV - 1) / GV;
+    const int64_t chunks = (a.N + GC - 1) / GC;
+    const int segs = any_segments(a.B * a.H * tiles, chunks, a.dk);
+    if (segs > 1 && (!work || !aligned16(work) || bytes < any_workspace(a.B, a.N, a.H, a.dk, a.dv)))
+        return SNNB_ERR_ARG;
+    if (chunks / segs > 0x7ffffff) return SNNB_ERR_ARG;
+    const AnyArgs p = {a, tiles, 0, segs, (int)((chunks + segs - 1) / segs), static_cast<float*>(work)};
+    if (segs > 1)
+        if (const int st = launch_any<T, true>(p, s)) return st;
+    return launch_any<T, false>(p, s);
 }
 
 // One token of each sequence: a thread block per sequence, head and ST_V columns of its state,
@@ -252,7 +400,10 @@ using namespace snnb;
 extern "C" int64_t snnb_decay_attention_workspace_bytes(int dtype, int64_t B, int64_t N, int64_t H,
                                                         int64_t dk, int64_t dv) {
     if (!heads_ok(dtype, B, H, H, dk, dv) || N < 0) return -1;
-    return decay::tc_workspace(dtype, B, N, H, dk, dv);
+    if (B == 0 || N == 0) return 0;
+    // strides and alignment decide between the forms
+    const int64_t tc = decay::tc_workspace(dtype, B, N, H, dk, dv), any = any_workspace(B, N, H, dk, dv);
+    return tc > any ? tc : any;
 }
 
 extern "C" int snnb_decay_attention(const void* q, const int64_t* q_strides, const void* k,
@@ -284,9 +435,9 @@ extern "C" int snnb_decay_attention(const void* q, const int64_t* q_strides, con
     }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (tc_takes(a, dtype)) return tc_run(a, dtype, workspace, workspace_bytes, s);
-    if (dtype == SNNB_F32) return run_any<float>(a, s);
-    if (dtype == SNNB_F16) return run_any<__half>(a, s);
-    return run_any<__nv_bfloat16>(a, s);
+    if (dtype == SNNB_F32) return run_any<float>(a, workspace, workspace_bytes, s);
+    if (dtype == SNNB_F16) return run_any<__half>(a, workspace, workspace_bytes, s);
+    return run_any<__nv_bfloat16>(a, workspace, workspace_bytes, s);
 }
 
 extern "C" int snnb_decay_attention_step(const void* q, const int64_t* q_strides, const void* k,
