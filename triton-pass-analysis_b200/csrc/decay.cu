@@ -101,25 +101,45 @@ __global__ void __launch_bounds__(G_THREADS, 2) decay_any_kernel(const __grid_co
         const int m = n + 1 == count ? last : GC;
         __syncthreads();
         bool bad = false;
-        for (int r = warp; r < GC; r += G_THREADS / 32) {      // a warp: a token's row
-            const T* kr = kg + (n0 + r) * a.ks[1];
-            const T* qr = qg + (n0 + r) * a.qs[1];
-            const T* vr = vg + (n0 + r) * a.vs[1];
-            for (int c = lane; c < dkp; c += 32) {
+        // a warp: every eighth token's row, a column a lane, a column's rows in flight together
+        const int mp = (m + 3) / 4 * 4;            // rows that are used
+        constexpr int R = GC / (G_THREADS / 32);
+        const T* kr = kg + n0 * a.ks[1];
+        const T* qr = qg + n0 * a.qs[1];
+        const T* vr = vg + n0 * a.vs[1];
+        for (int c = lane; c < dkp; c += 32) {
+            float x[R], y[R];
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const int r = warp + i * (G_THREADS / 32);
                 const bool in = r < m && c < dk;
-                k[c * GP + r] = in ? to_f32(kr[c]) : 0.0f;
-                if (!STATES) q[c * GP + r] = in ? to_f32(qr[c]) * a.scale : 0.0f;
+                x[i] = in ? to_f32(kr[r * a.ks[1] + c]) : 0.0f;
+                if (!STATES) y[i] = in ? to_f32(qr[r * a.qs[1] + c]) * a.scale : 0.0f;
             }
-            for (int c = lane; c < GV; c += 32) {
-                const float x = r < m && c < nv ? to_f32(vr[c]) : 0.0f;
-                bad |= !(fabsf(x) <= 3.4028235e38f);
-                v[r * GP + c] = x;
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const int r = warp + i * (G_THREADS / 32);
+                k[c * GP + r] = x[i];
+                if (!STATES) q[c * GP + r] = y[i];
+            }
+        }
+        for (int c = lane; c < GV; c += 32) {
+            float x[R];
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const int r = warp + i * (G_THREADS / 32);
+                x[i] = r < m && c < nv ? to_f32(vr[r * a.vs[1] + c]) : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                bad |= !(fabsf(x[i]) <= 3.4028235e38f);
+                v[(warp + i * (G_THREADS / 32)) * GP + c] = x[i];
             }
         }
         bad = __syncthreads_or(bad);
         if (!STATES) {
             float s[4][4] = {};
-            if (j0 <= i0 + 3) {
+            if (j0 <= i0 + 3 && i0 < m) {
 #pragma unroll 4
                 for (int x = 0; x < dkp; ++x)
                     fma44(s, *reinterpret_cast<const float4*>(q + x * GP + i0),
@@ -127,7 +147,7 @@ __global__ void __launch_bounds__(G_THREADS, 2) decay_any_kernel(const __grid_co
             }
             float o[4][4] = {};
 #pragma unroll 4
-            for (int x = 0; x < dkp; ++x)
+            for (int x = 0; x < (i0 < m ? dkp : 0); ++x)
                 fma44(o, *reinterpret_cast<const float4*>(q + x * GP + i0),
                       *reinterpret_cast<const float4*>(S + x * GP + j0));
 #pragma unroll
@@ -145,7 +165,7 @@ __global__ void __launch_bounds__(G_THREADS, 2) decay_any_kernel(const __grid_co
             __syncthreads();
             if (!bad) {
 #pragma unroll 4
-                for (int x = 0; x < i0 + 4; ++x)
+                for (int x = 0; x < (i0 < m ? i0 + 4 : 0); ++x)
                     fma44(o, *reinterpret_cast<const float4*>(pt + x * GP + i0),
                           *reinterpret_cast<const float4*>(v + x * GP + j0));
             } else {                               // 0 * inf would reach rows before the infinity
@@ -166,16 +186,13 @@ __global__ void __launch_bounds__(G_THREADS, 2) decay_any_kernel(const __grid_co
             __syncthreads();
         }
         // the rows of v by what is left of them at the chunk's end
-        for (int i = t; i < GC * GV; i += G_THREADS) {
-            const int r = i / GV;
-            if (r < m) v[r * GP + i % GV] *= pw[m - 1 - r];
-        }
+        for (int i = t; i < m * GV; i += G_THREADS) v[i / GV * GP + i % GV] *= pw[m - 1 - i / GV];
         __syncthreads();
         const float fh = m == GC ? ch : lh, fl = m == GC ? cl : ll;
         for (int r = i0; r < dkp; r += 64) {
             float s[4][4] = {};
 #pragma unroll 4
-            for (int x = 0; x < GC; x += 4) {
+            for (int x = 0; x < mp; x += 4) {
                 float4 kk[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) kk[i] = *reinterpret_cast<const float4*>(k + (r + i) * GP + x);
@@ -286,8 +303,9 @@ __global__ void __launch_bounds__(ST_THREADS) decay_step_kernel(Args a, uint32_t
         const float l = a.decay[h];
         const int64_t base = (b * a.H + h) * a.dk * a.dv + c;
         for (int r = r0; r < a.dk; r += ST_THREADS / ST_V) {
-            const float x = l * a.state_in[base + (int64_t)r * a.dv] + k[r] * v;
-            a.state_out[base + (int64_t)r * a.dv] = x;
+            const float old = a.state_in ? a.state_in[base + (int64_t)r * a.dv] : 0.0f;
+            const float x = l * old + k[r] * v;
+            if (a.state_out) a.state_out[base + (int64_t)r * a.dv] = x;
             s += q[r] * x;
         }
     }
@@ -317,9 +335,11 @@ __global__ void __launch_bounds__(ST_THREADS) decay_step_vec_kernel(Args a, uint
     float* to = a.state_out + base;
     float4 x[AHEAD];
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i)
-        if (in && r0 + i * ROWS < a.dk)
+    for (int i = 0; i < AHEAD; ++i) {
+        x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (in && a.state_in && r0 + i * ROWS < a.dk)
             x[i] = *reinterpret_cast<const float4*>(from + (int64_t)(r0 + i * ROWS) * a.dv);
+    }
     const T* qg = static_cast<const T*>(a.q) + b * a.qs[0] + h * a.qs[2];
     const T* kg = static_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[2];
     if (t < a.dk) {
@@ -339,7 +359,7 @@ __global__ void __launch_bounds__(ST_THREADS) decay_step_vec_kernel(Args a, uint
         if (r != r0) {
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i)
-                if (in && r + i * ROWS < a.dk)
+                if (in && a.state_in && r + i * ROWS < a.dk)
                     x[i] = *reinterpret_cast<const float4*>(from + (int64_t)(r + i * ROWS) * a.dv);
         }
 #pragma unroll
@@ -349,7 +369,7 @@ __global__ void __launch_bounds__(ST_THREADS) decay_step_vec_kernel(Args a, uint
             const float kn = k[n], qn = q[n];
             x[i] = make_float4(l * x[i].x + kn * v[0], l * x[i].y + kn * v[1], l * x[i].z + kn * v[2],
                                l * x[i].w + kn * v[3]);
-            *reinterpret_cast<float4*>(to + (int64_t)n * a.dv) = x[i];
+            if (a.state_out) *reinterpret_cast<float4*>(to + (int64_t)n * a.dv) = x[i];
             s.x += qn * x[i].x; s.y += qn * x[i].y; s.z += qn * x[i].z; s.w += qn * x[i].w;
         }
     }
@@ -382,6 +402,11 @@ int run_step(const Args& a, cudaStream_t s) {
     return launch_k(decay_step_kernel<T>, dim3((unsigned)(a.B * a.H * tiles)), dim3(ST_THREADS), 0,
                     s, a, tiles);
 }
+
+// Short sequences of few heads go to the CUDA cores whatever their type: there the rounding of the
+// tensor cores' scores, which more tokens average out, shows in the outputs (1.4 times a float32
+// result's own rounding), and both take less than the call's host time (8 heads of 64: 11 us, 6.5).
+constexpr int64_t FEW_TOKENS = 8;
 
 bool heads_ok(int dtype, int64_t B, int64_t H, int64_t Hk, int64_t dk, int64_t dv) {
     return (dtype == SNNB_F32 || dtype == SNNB_F16 || dtype == SNNB_BF16) && B >= 0 && H >= 1 &&
@@ -434,7 +459,12 @@ extern "C" int snnb_decay_attention(const void* q, const int64_t* q_strides, con
         a.vs[i] = v_strides[i];
     }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (tc_takes(a, dtype)) return tc_run(a, dtype, workspace, workspace_bytes, s);
+    if (N == 1 && !lengths) {                      // one token: no chunk
+        if (dtype == SNNB_F32) return run_step<float>(a, s);
+        if (dtype == SNNB_F16) return run_step<__half>(a, s);
+        return run_step<__nv_bfloat16>(a, s);
+    }
+    if ((N > FEW_TOKENS || B * H * ((dv + GV - 1) / GV) > 148) && tc_takes(a, dtype)) return tc_run(a, dtype, workspace, workspace_bytes, s);
     if (dtype == SNNB_F32) return run_any<float>(a, workspace, workspace_bytes, s);
     if (dtype == SNNB_F16) return run_any<__half>(a, workspace, workspace_bytes, s);
     return run_any<__nv_bfloat16>(a, workspace, workspace_bytes, s);
