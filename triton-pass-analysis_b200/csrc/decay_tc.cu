@@ -223,8 +223,9 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sbase = tc::smem_u32(smem);
     const uint32_t pw = sbase + L::PW_OFF, rw = sbase + L::RW_OFF, wv = sbase + L::WV_OFF;
-    int* bad_row = reinterpret_cast<int*>(smem + L::BAD_OFF);
-    volatile int* bad_chunk = bad_row + 4 * DV;
+    // of a chunk's columns, the first row that is not finite: 256 times the chunk's number + 255 - row
+    uint32_t* bad_row = reinterpret_cast<uint32_t*>(smem + L::BAD_OFF);
+    volatile int* bad_chunk = reinterpret_cast<int*>(bad_row + 4 * DV);
     const uint32_t bar0 = sbase + L::BAR_OFF;
     auto qk_full = [&](uint32_t s) { return bar0 + 8u * s; };
     auto qk_empty = [&](uint32_t s) { return bar0 + 8u * (NQ + s); };
@@ -270,7 +271,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         tc::prefetch_tmap(&tmV);
         for (int i = 0; i < 4; ++i) bad_chunk[i] = -1;
     }
-    if (threadIdx.x < 4 * DV) bad_row[threadIdx.x] = C;
+    if (threadIdx.x < 4 * DV) bad_row[threadIdx.x] = 0;
     else if (threadIdx.x < 4 * DV + 32) tops8[threadIdx.x - 4 * DV] = 0;
     if (warp == 5) {
         tc::tmem_alloc(sbase + L::TMEM_OFF, T_COLS);
@@ -318,15 +319,14 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     if (!failed) ++issued_v;
                 }
             }
-            if (failed) {                            // copies in flight land before the block ends
-                for (uint32_t k = 0; k < issued_qk && k < (uint32_t)NQ; ++k) {
-                    const uint32_t i = issued_qk - 1 - k;
-                    tc::mbar_wait_warp<true>(qk_full(i % NQ), (i / NQ) & 1u, 0);
-                }
-                for (uint32_t k = 0; k < issued_v && k < (uint32_t)NV; ++k) {
-                    const uint32_t i = issued_v - 1 - k;
-                    tc::mbar_wait_warp<true>(v_full(i % NV), (i / NV) & 1u, 0);
-                }
+            // copies in flight land before the block ends, whoever has given up waiting for them
+            for (uint32_t k = 0; k < issued_qk && k < (uint32_t)NQ; ++k) {
+                const uint32_t i = issued_qk - 1 - k;
+                tc::mbar_wait_warp<true>(qk_full(i % NQ), (i / NQ) & 1u, 0);
+            }
+            for (uint32_t k = 0; k < issued_v && k < (uint32_t)NV; ++k) {
+                const uint32_t i = issued_v - 1 - k;
+                tc::mbar_wait_warp<true>(v_full(i % NV), (i / NV) & 1u, 0);
             }
         } else if (warp == 5) {
             // ------------------------------------------------ MMAs
@@ -371,6 +371,10 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                                           idesc16(HALF, 128, 64 * L::TERMS) | A_MN | B_MN, (half | i) != 0);
                         tc::umma_commit(half ? kv_ready : vt_free);
                     }
+                    // No stage is handed back before its copies have landed, which those that scale v
+                    // may have given up waiting for: its barrier's phase would still be open.
+                    wait(v_full(sv), (g / NV) & 1u);
+                    if (failed) break;
                     if (!STATES) {
                         wait(s_ready, ph);
                         if (g) wait(o_free, ph ^ 1u);
@@ -538,10 +542,10 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                                     v[j + 1]);
                     }
                     if (spoiled) {
-                        const int* rows = bad_row + (g & 3) * DV + i;
+                        const uint32_t* rows = bad_row + (g & 3) * DV + i;
 #pragma unroll
                         for (int j = 0; j < 16; ++j)
-                            if (row >= rows[j]) v[j] = __int_as_float(0x7fffffff);
+                            if (rows[j] >= (g << 8 | (255u - row))) v[j] = __int_as_float(0x7fffffff);
                     }
 #pragma unroll
                     for (int j = 0; j < 8; ++j) w[j] = alive ? pair<HALF>(v[2 * j], v[2 * j + 1]) : 0u;
@@ -552,10 +556,6 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         store16(out + i, w, cols - i, p.out32);
                     }
                     __syncwarp();
-                }
-                if (spoiled) {                       // for the fourth chunk from here
-                    tc::named_bar_sync(7, 128);
-                    if (row < DV) bad_row[(g & 3) * DV + row] = C;
                 }
                 if (L::STAGED) {
                     tc::fence_proxy_async_smem();
@@ -854,7 +854,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     // the chunk's earlier rows.  There they become zero, and the outputs of their
                     // columns NaN from their row on.
                     if (lane == 0) bad_chunk[g & 3] = (int)g;
-                    int* rows = bad_row + (g & 3) * DV + 8 * piece;
+                    uint32_t* rows = bad_row + (g & 3) * DV + 8 * piece;
 #pragma unroll 1
                     for (int i = 0; i < 4; ++i) {
                         const uint4 r4 = lds128(vs + 2048 * i);
@@ -862,11 +862,11 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             if ((u[j] & INF) == INF) {
-                                atomicMin(&rows[2 * j], first + 16 * i);
+                                atomicMax(&rows[2 * j], g << 8 | (255u - (first + 16 * i)));
                                 u[j] &= 0xFFFF0000u;
                             }
                             if ((u[j] & (INF << 16)) == INF << 16) {
-                                atomicMin(&rows[2 * j + 1], first + 16 * i);
+                                atomicMax(&rows[2 * j + 1], g << 8 | (255u - (first + 16 * i)));
                                 u[j] &= 0xFFFFu;
                             }
                         }

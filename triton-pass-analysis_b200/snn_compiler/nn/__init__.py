@@ -7,10 +7,11 @@ from .fused_layers import (FusedConvNeuron, FusedLinearNeuron, FusedConvBNNeuron
 from .attention import (FusedSpikeAttention, SpikeAttentionBlock, is_spiking_self_attention,
                         is_ms_attention, is_spiking_attention)
 from .mx import MXLinear, RMSNormMX, SpikingMLP
+from .decay import DecayAttention, GroupNormAct
 
 __all__ = ["IFNode", "LIFNode", "PLIFNode", "CubaLIFNode", "EIFNode", "ChunkedForward",
            "run_chunked", "FusedAddNeuron", "FusedConvNeuron",
            "FusedLinearNeuron", "FusedConvBNNeuron", "FusedConvBNAddNeuron", "FusedConvBN", "tune_convs", "RateCodedIFNode",
            "RateCodedLIFNode", "StatefulLIFNode", "FusedSpikeAttention", "SpikeAttentionBlock",
            "is_spiking_self_attention", "is_ms_attention", "is_spiking_attention",
-           "MXLinear", "RMSNormMX", "SpikingMLP"]
+           "MXLinear", "RMSNormMX", "SpikingMLP", "DecayAttention", "GroupNormAct"]
