@@ -27,6 +27,11 @@ template <int BYTES> struct alignas(BYTES) Bits {
 };
 template <> struct Bits<2> { uint16_t w[1]; };
 
+// Rows that a thread has in flight: 64 bytes, or as many as registers allow of narrow pieces.
+template <typename T, int VEC> constexpr int rows_ahead() {
+    return VEC * (int)sizeof(T) >= 16 ? 4 : VEC * (int)sizeof(T) == 8 ? 8 : 16;
+}
+
 struct GnArgs {
     const void* x;
     int64_t xb, xs;                // strides of sample and row
@@ -233,7 +238,7 @@ struct SlabArgs {
 template <typename T, int VEC, int ACT, bool KEEP>
 __global__ void __launch_bounds__(GN_THREADS, 4) gn_slab_kernel(const __grid_constant__ SlabArgs s) {
     using V = Bits<VEC * (int)sizeof(T)>;
-    constexpr int U = 4;                       // rows in flight
+    constexpr int U = rows_ahead<T, VEC>();
     extern __shared__ uint8_t smem[];
     const GnArgs& a = s.a;
     V* tile = reinterpret_cast<V*>(smem);
@@ -450,25 +455,27 @@ int run_slab(const GnArgs& a, cudaStream_t s) {
 
 
 // ---- two passes over large tensors -----------------------------------------------------------
-// Of every block of `chunk` rows of a sample, each group's mean and sum of squares around it, then the
-// outputs from those of the sample's blocks.  Slabs hold whole groups, at most one piece a thread.
+// Of every block of `chunk` rows of a sample, each part of a group's mean and sum of squares around it,
+// then the outputs from those of the sample's blocks.  Slabs hold whole parts (a group is one, or
+// several where it has more pieces than a block has threads), at most one piece a thread.
 struct PassArgs {
     GnArgs a;
     uint32_t slabs, width, chunk, chunks;      // channels of a slab; rows of a block; blocks of a sample
-    mx::FastDiv per_group;
-    float2* stats;                             // [B][chunks][G]
+    uint32_t parts, pc;                        // of a group; channels of one
+    mx::FastDiv per_group, per_part;
+    float2* stats;                             // [B][chunks][G parts]
 };
 template <typename T, int VEC>
 __global__ void __launch_bounds__(GN_THREADS, 4) gn_stats_kernel(const __grid_constant__ PassArgs s) {
     using V = Bits<VEC * (int)sizeof(T)>;
-    constexpr int U = 4;                       // rows at a time, as many ahead
+    constexpr int U = rows_ahead<T, VEC>();    // at a time, as many ahead
     extern __shared__ float part[];            // [rows][width], then [groups] means
     const GnArgs& a = s.a;
     pdl_wait();
     pdl_trigger();
     const uint32_t slab = blockIdx.x % s.slabs, rest = blockIdx.x / s.slabs;
     const uint32_t b = rest / s.chunks, chunk = rest - b * s.chunks, c0 = slab * s.width;
-    const uint32_t width = min(s.width, a.C - c0), groups = width / a.cg, nv = width / VEC, t = threadIdx.x;
+    const uint32_t width = min(s.width, a.C - c0), groups = width / s.pc, nv = width / VEC, t = threadIdx.x;
     const uint32_t r0 = chunk * s.chunk, rows = min(s.chunk, a.S - r0);
     const uint32_t nc = s.width / VEC, rp = GN_THREADS / nc, vc = t % nc, rr = t / nc;
     const bool in = t < rp * nc && vc < nv && rr < rows;
@@ -546,30 +553,30 @@ __global__ void __launch_bounds__(GN_THREADS, 4) gn_stats_kernel(const __grid_co
     auto each_group = [&](auto f) {
         for (uint32_t g = t >> 5; g < groups; g += GN_THREADS / 32) {
             float v = 0.0f;
-            for (uint32_t c = t & 31; c < a.cg; c += 32) v += part[g * a.cg + c];
+            for (uint32_t c = t & 31; c < s.pc; c += 32) v += part[g * s.pc + c];
 #pragma unroll
             for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
             if ((t & 31) == 0) f(g, v);
         }
     };
     to_part();
-    const float all = 1.0f / ((float)rows * (float)a.cg);
+    const float all = 1.0f / ((float)rows * (float)s.pc);
     each_group([&](uint32_t g, float v) { mean[g] = v * all; });
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-        const float d = vc < nv ? s1[j] - mean[s.per_group.div(vc * VEC + j)] : 0.0f;
+        const float d = vc < nv ? s1[j] - mean[s.per_part.div(vc * VEC + j)] : 0.0f;
         acc[j] = count > 0.0f ? fmaf(count * d, d, s2[j]) : 0.0f;
     }
     to_part();
-    float2* out = s.stats + ((int64_t)b * s.chunks + chunk) * a.G + c0 / a.cg;
+    float2* out = s.stats + ((int64_t)b * s.chunks + chunk) * (a.G * s.parts) + c0 / s.pc;
     each_group([&](uint32_t g, float v) { out[g] = make_float2(mean[g], v); });
 }
 
 template <typename T, int VEC, int ACT>
 __global__ void __launch_bounds__(GN_THREADS, 4) gn_apply_kernel(const __grid_constant__ PassArgs s) {
     using V = Bits<VEC * (int)sizeof(T)>;
-    constexpr int U = 4;
+    constexpr int U = rows_ahead<T, VEC>();
     constexpr bool FOLDED = sizeof(T) == 2;
     extern __shared__ float groups_of[];       // [groups] mean, [groups] 1 / deviation
     const GnArgs& a = s.a;
@@ -578,7 +585,8 @@ __global__ void __launch_bounds__(GN_THREADS, 4) gn_apply_kernel(const __grid_co
     // the last blocks first: their rows are the likeliest to be in L2 still
     const uint32_t at = gridDim.x - 1 - blockIdx.x, slab = at % s.slabs, rest = at / s.slabs;
     const uint32_t b = rest / s.chunks, chunk = rest - b * s.chunks, c0 = slab * s.width;
-    const uint32_t width = min(s.width, a.C - c0), groups = width / a.cg, nv = width / VEC, t = threadIdx.x;
+    const uint32_t width = min(s.width, a.C - c0), nv = width / VEC, t = threadIdx.x;
+    const uint32_t g0 = c0 / a.cg, groups = (c0 + width - 1) / a.cg - g0 + 1;      // that the slab touches
     const uint32_t r0 = chunk * s.chunk, rows = min(s.chunk, a.S - r0);
     const uint32_t nc = s.width / VEC, rp = GN_THREADS / nc, vc = t % nc, rr = t / nc;
     const bool in = t < rp * nc && vc < nv && rr < rows;
@@ -590,19 +598,24 @@ __global__ void __launch_bounds__(GN_THREADS, 4) gn_apply_kernel(const __grid_co
 #pragma unroll
     for (int i = 0; i < U; ++i)
         if (i < left) raw[i] = *reinterpret_cast<const V*>(x + i * step);
-    const float2* stats = s.stats + (int64_t)b * s.chunks * a.G + c0 / a.cg;
-    const float over_n = 1.0f / ((float)a.S * (float)a.cg), last = (float)(a.S - (s.chunks - 1) * s.chunk);
+    const uint32_t of = a.G * s.parts, all = s.chunks * s.parts;
+    const float2* stats = s.stats + (int64_t)b * s.chunks * of + g0 * s.parts;
+    const float over_n = 1.0f / ((float)a.S * (float)a.cg), pc = (float)s.pc;
+    const float whole = (float)s.chunk * pc, last = (float)(a.S - (s.chunks - 1) * s.chunk) * pc;
     for (uint32_t g = t >> 5; g < groups; g += GN_THREADS / 32) {
         float sum = 0.0f, sq = 0.0f;
-        for (uint32_t c = t & 31; c < s.chunks; c += 32)
-            sum += stats[(int64_t)c * a.G + g].x * (c + 1 == s.chunks ? last : (float)s.chunk) * (float)a.cg;
+        for (uint32_t i = t & 31; i < all; i += 32) {
+            const uint32_t c = i / s.parts;
+            sum += stats[(int64_t)c * of + g * s.parts + i - c * s.parts].x * (c + 1 == s.chunks ? last : whole);
+        }
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         const float mean = sum * over_n;
-        for (uint32_t c = t & 31; c < s.chunks; c += 32) {
-            const float2 v = stats[(int64_t)c * a.G + g];
+        for (uint32_t i = t & 31; i < all; i += 32) {
+            const uint32_t c = i / s.parts;
+            const float2 v = stats[(int64_t)c * of + g * s.parts + i - c * s.parts];
             const float d = v.x - mean;
-            sq += fmaf((c + 1 == s.chunks ? last : (float)s.chunk) * (float)a.cg * d, d, v.y);
+            sq += fmaf((c + 1 == s.chunks ? last : whole) * d, d, v.y);
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
@@ -618,7 +631,7 @@ __global__ void __launch_bounds__(GN_THREADS, 4) gn_apply_kernel(const __grid_co
     params<T, VEC>(a.bias, a.wf32, c0 + vc * VEC, 0.0f, shift);
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-        const uint32_t g = s.per_group.div(vc * VEC + j);
+        const uint32_t g = s.per_group.div(c0 + vc * VEC + j) - g0;
         mean[j] = groups_of[g];
         w[j] *= groups_of[groups + g];
         // 16-bit values: a mean that is 2^k deviations leaves them 11 - k bits or fewer, and this 24 - k
@@ -649,16 +662,26 @@ __global__ void __launch_bounds__(GN_THREADS, 4) gn_apply_kernel(const __grid_co
 // Slabs and blocks of the two passes for pieces of `vec` values; false: no slab of whole
 // groups has at most a piece a thread.
 bool plan_passes(const GnArgs& a, uint32_t vec, PassArgs& p) {
-    uint32_t unit = a.cg;
+    const uint32_t most = GN_THREADS * vec;
+    // a group's parts, alike: whole pieces where it has several, and then whole parts a slab
+    uint32_t parts = 1, unit = a.cg;
     while (unit % vec) unit += a.cg;
-    if (unit > GN_THREADS * vec) return false;
+    if (unit > most) {
+        for (parts = 2; parts < a.cg; ++parts)
+            if (a.cg % parts == 0 && a.cg / parts <= most && a.cg / parts % vec == 0) break;
+        unit = a.cg / parts;
+        if (a.cg % parts || unit > most || unit % vec) return false;
+    }
     p.a = a;
-    p.width = GN_THREADS * vec / unit * unit;
+    p.parts = parts;
+    p.pc = a.cg / parts;
+    p.width = most / unit * unit;
     if (p.width > a.C) p.width = a.C;
     p.slabs = (a.C + p.width - 1) / p.width;
     p.width = (a.C / unit + p.slabs - 1) / p.slabs * unit;     // alike in width
     p.slabs = (a.C + p.width - 1) / p.width;
     p.per_group = mx::FastDiv(a.cg);
+    p.per_part = mx::FastDiv(p.pc);
     const uint32_t rp = GN_THREADS / (p.width / vec);
     // one round of four blocks an SM where samples are few, 8 rows a thread or more: a thread's start
     // and end cost as much as some 10 rows (64 KB a block: 136 us for 64 x 3136 x 256, so 70)
@@ -676,12 +699,12 @@ constexpr int64_t TWO_PASSES = int64_t(64) << 20;
 template <typename T, int VEC, int ACT>
 int run_passes(PassArgs p, cudaStream_t s) {
     const uint32_t nc = p.width / VEC, rp = GN_THREADS / nc, rows = 32 % nc == 0 ? GN_THREADS / 32 : rp;
-    const uint32_t groups = p.width / p.a.cg;
+    const uint32_t groups = p.width / p.pc;            // or more of either kind
     const dim3 grid(p.a.B * p.chunks * p.slabs);
     if (const int st = launch_k(gn_stats_kernel<T, VEC>, grid, dim3(GN_THREADS),
                                 (rows * p.width + groups) * sizeof(float), s, p))
         return st;
-    return launch_k(gn_apply_kernel<T, VEC, ACT>, grid, dim3(GN_THREADS), 2 * groups * sizeof(float), s, p);
+    return launch_k(gn_apply_kernel<T, VEC, ACT>, grid, dim3(GN_THREADS), 2 * (groups + 2) * sizeof(float), s, p);
 }
 
 template <typename T, int VEC, int ACT>
@@ -756,7 +779,7 @@ extern "C" int64_t snnb_group_norm_act_workspace_bytes(int dtype, int64_t B, int
     for (int v = 16 / size; v >= 1; v /= 2) {
         PassArgs p;
         if (C % v == 0 && plan_passes(a, v, p)) {
-            const int64_t n = B * p.chunks * groups * (int64_t)sizeof(float2);
+            const int64_t n = B * p.chunks * groups * p.parts * (int64_t)sizeof(float2);
             most = n > most ? n : most;
         }
     }
