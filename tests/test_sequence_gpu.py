@@ -396,7 +396,7 @@ def _norm_check(x, groups, weight=None, bias=None, eps=1e-5, act="none", view=No
 NORM = [((1, 1), 1), ((3, 8), 2), ((2, 5, 12), 4), ((1, 7, 3, 90), 30), ((2, 16, 16, 64), 32),
         ((700, 384), 8), ((1, 33, 31, 96), 6), ((3, 1, 1, 2048), 64), ((2, 1000, 24), 24),
         ((1, 3000, 7), 1), ((5, 14, 14, 320), 32), ((2, 56, 56, 64), 32), ((1, 9, 2050), 2),
-        ((9000, 40), 5), ((1, 4096, 8), 1), ((2, 50, 1003), 17)]
+        ((9000, 40), 5), ((300, 2048), 1), ((300, 1005), 3), ((257, 1023), 1), ((130, 1500), 1), ((1, 4096, 8), 1), ((2, 50, 1003), 17)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -133,28 +133,27 @@ __device__ __forceinline__ Bits<VEC * sizeof(T)> finish(const float (&x)[VEC], c
 // A team of P lanes holds one group of one sample: R pieces of VEC values a lane, a row's pieces
 // next to one another.
 template <typename T, int VEC, int P, int R, int ACT>
-__global__ void __launch_bounds__(GN_THREADS) gn_team_kernel(GnArgs a, uint32_t per_row, uint32_t items) {
+__global__ void __launch_bounds__(GN_THREADS) gn_team_kernel(GnArgs a, mx::FastDiv per_row, uint32_t items) {
     using V = Bits<VEC * (int)sizeof(T)>;
     pdl_wait();
     pdl_trigger();
     const uint32_t item = (blockIdx.x * GN_THREADS + threadIdx.x) / P, l = threadIdx.x % P;
     const bool in = item < items;
-    const uint32_t b = item / a.G, g = item - b * a.G, pieces = a.S * per_row;
+    const uint32_t b = item / a.G, g = item - b * a.G, pieces = a.S * per_row.d;
     const T* x = static_cast<const T*>(a.x) + b * a.xb + g * a.cg;
     float v[R][VEC];
-    uint32_t row[R], c[R];
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        const uint32_t p = l + i * P;
-        row[i] = p / per_row;
-        c[i] = (p - row[i] * per_row) * VEC;
-        if (in && p < pieces) {
-            unpack<T, VEC>(*reinterpret_cast<const V*>(x + row[i] * a.xs + c[i]), v[i]);
+        const uint32_t p = l + i * P, row = per_row.div(p), c = (p - row * per_row.d) * VEC;
+        if (in && p < pieces) unpack<T, VEC>(*reinterpret_cast<const V*>(x + row * a.xs + c), v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+        if (in && l + i * P < pieces) {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) sum += v[i][j];
         }
-    }
 #pragma unroll
     for (int o = P / 2; o; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const float n = (float)(a.S * a.cg), mean = sum / n;
@@ -171,16 +170,17 @@ __global__ void __launch_bounds__(GN_THREADS) gn_team_kernel(GnArgs a, uint32_t 
     T* y = static_cast<T*>(a.y) + (int64_t)b * a.S * a.C + g * a.cg;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        if (!in || l + i * P >= pieces) continue;
+        const uint32_t p = l + i * P, row = per_row.div(p), c = (p - row * per_row.d) * VEC;
+        if (!in || p >= pieces) continue;
         float m[VEC], w[VEC], s[VEC];
-        params<T, VEC>(a.weight, a.wf32, g * a.cg + c[i], 1.0f, w);
-        params<T, VEC>(a.bias, a.wf32, g * a.cg + c[i], 0.0f, s);
+        params<T, VEC>(a.weight, a.wf32, g * a.cg + c, 1.0f, w);
+        params<T, VEC>(a.bias, a.wf32, g * a.cg + c, 0.0f, s);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
             m[j] = mean;
             w[j] *= r;
         }
-        *reinterpret_cast<V*>(y + (int64_t)row[i] * a.C + c[i]) = finish<T, VEC, ACT>(v[i], m, w, s);
+        *reinterpret_cast<V*>(y + (int64_t)row * a.C + c) = finish<T, VEC, ACT>(v[i], m, w, s);
     }
 }
 
@@ -387,11 +387,14 @@ __global__ void __launch_bounds__(GN_THREADS, 4) gn_slab_kernel(const __grid_con
     if (s.blocks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
 
+// Values of a group that a warp can hold.
+constexpr uint32_t TEAM_VALUES = 2048;
+
 template <typename T, int VEC, int P, int R, int ACT>
 int launch_team(const GnArgs& a, cudaStream_t s) {
     const int64_t items = (int64_t)a.B * a.G;
     return launch_k(gn_team_kernel<T, VEC, P, R, ACT>, dim3((unsigned)((items * P + GN_THREADS - 1) / GN_THREADS)),
-                    dim3(GN_THREADS), 0, s, a, a.cg / VEC, (uint32_t)items);
+                    dim3(GN_THREADS), 0, s, a, mx::FastDiv(a.cg / VEC), (uint32_t)items);
 }
 template <typename T, int VEC, int ACT>
 int run_team(const GnArgs& a, cudaStream_t s) {
@@ -400,7 +403,12 @@ int run_team(const GnArgs& a, cudaStream_t s) {
     if (pieces <= 8) return launch_team<T, VEC, 8, 1, ACT>(a, s);
     if (pieces <= 16) return launch_team<T, VEC, 16, 1, ACT>(a, s);
     if (pieces <= 32) return launch_team<T, VEC, 32, 1, ACT>(a, s);
-    return launch_team<T, VEC, 32, 4, ACT>(a, s);
+    if (pieces <= 128) return launch_team<T, VEC, 32, 4, ACT>(a, s);
+    if constexpr (VEC <= 4)
+        if (pieces <= 512) return launch_team<T, VEC, 32, 16, ACT>(a, s);
+    if constexpr (VEC == 1)
+        if (pieces <= 1024) return launch_team<T, VEC, 32, 32, ACT>(a, s);
+    return launch_team<T, VEC, 32, TEAM_VALUES / 32 / VEC, ACT>(a, s);
 }
 
 // Shared memory of a block: four an SM, or one, for groups of many channels.
@@ -729,7 +737,7 @@ int widest(const GnArgs& a, int size, bool team) {
 }
 // Few values a group, in pieces of 32 bytes or of single rows: a row's pieces are then neighbours'.
 bool team_takes(const GnArgs& a, int size, int v) {
-    return (int64_t)a.S * (a.cg / v) <= 128 && (a.S == 1 || a.cg * size >= 32);
+    return (int64_t)a.S * (a.cg / v) <= (a.S == 1 ? TEAM_VALUES / v : 128) && (a.S == 1 || a.cg * size >= 32);
 }
 template <typename T, int ACT>
 int run(const GnArgs& a, float2* work, cudaStream_t s) {
@@ -783,7 +791,7 @@ extern "C" int64_t snnb_group_norm_act_workspace_bytes(int dtype, int64_t B, int
             most = n > most ? n : most;
         }
     }
-    return S == 1 && a.cg <= 128 ? 0 : most;
+    return S == 1 && a.cg <= TEAM_VALUES ? 0 : most;
 }
 
 extern "C" int snnb_group_norm_act(const void* x, int64_t x_batch_stride, int64_t x_row_stride,
