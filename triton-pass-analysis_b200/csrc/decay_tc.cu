@@ -1,4 +1,31 @@
 // Decay attention of 16-bit inputs on the tensor cores (formulas: decay.cu).
+//
+// A chunk of 128 tokens, a head's dk <= 128 columns of q and k and 64 of v are four products:
+//
+//   scores  Q K^T            128 x 128 x dk    -> P = scores . L, rounded once to the inputs' type
+//   P V                      128 x 64 x 128    P from tensor memory, over the scores' first half
+//   Q S                      128 x 64 x dk     S as two terms, side by side in N
+//   K^T (w V)                dk x 64 x 128     w_j = decay^(C-1-j); w V as terms, side by side in N
+//
+// The state S stays in registers, float32, and takes the last product as S <- decay^C S + it (the power
+// as two floats: it compounds over the chunks).  The factors w have 24 bits, so bfloat16's w V is cut
+// into three terms of 8 bits, exactly; float16's is rounded to two of 11, which leaves 22, and so
+// is S, of either type, to two for its product.  (Two bfloat16 terms of w V would leave errors of
+// 2.5e-6 in the state; these leave 3e-7.)  Only P is rounded to 8 or 11 bits, as often as the output.
+//
+// Tensor memory holds 512 columns: scores 128, Q S 2 x 64, P V 64, K^T (w V) 3 x 64.  Terms lie side by
+// side because such narrow products are bound by shared memory: 128 x 64 x 16 reads 6 KB of operands,
+// 48 cycles, where the tensor pipe needs 16; the other operand is read once for all terms.
+//
+// Warps have one role each, and each walks the block's items (a segment of a sequence, a head, 64 columns
+// of v) and their chunks; what bounds a chunk is the chain scores -> P -> P V -> the next scores, which
+// share their columns, and beside it instruction issue (53% of the slots taken, the tensor pipe
+// 39%; DRAM 35%).  The code is kept short on purpose: with every loop unrolled it had 150 KB and
+// ran at half the speed, waiting for instructions.  16 x 2048 tokens x 16 heads of 64, bf16: 78 us,
+// 3.4 TB/s of 6.5; 64 x 2048 x 8 of 128: 338 us, 3.2 TB/s; one sequence of 16384 x 32 of 128: 250 us,
+// of which a third is the pass before, over k and v, that leaves the state of its first half.
+//
+// Waits are bounded as elsewhere (tc_common.cuh).
 #include "decay.cuh"
 #include "tc_common.cuh"
 

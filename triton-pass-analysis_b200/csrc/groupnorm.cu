@@ -12,6 +12,10 @@
 //           their sums through it
 //   passes  large tensors: statistics of blocks of whole rows, then the outputs; what the second
 //           pass finds in L2 is not read from memory again
+//
+// bf16, us (floor): 12544 x 384 in 8 groups 9.5 (2.9); 64 x 28 x 28 x 256 in 32 18.5 (7.8); 64 x 56 x 56 x 256
+// 68 (31, or 47 when the second pass reads memory too, which it does: 27 for the statistics and 41,
+// issue slots 45% taken in both).
 #include "common.cuh"
 #include "mx.cuh"
 #include "tc_common.cuh"
