@@ -113,6 +113,77 @@ def test_module_refusals():
         DecayAttention.from_linears(*_linears(96, 6, 3, 32), torch.ones(6), heads=6, kv_heads=4)
 
 
+def test_block_after_a_cast():
+    from snn_compiler import kernels as K
+    m = _block()
+    x, r = _inputs((2, 40, 96), 8)
+    pos = K.grid_positions(2, 4, 5)
+    y, _, S = m(x, pos, r)
+    decay = m.decay.clone()
+    y2, _, S2 = m.to(torch.bfloat16)(x, pos, r)                # norms rounded, decays as they were
+    assert m.decay.dtype == torch.float32 and torch.equal(m.decay, decay)
+    with pytest.raises(ValueError, match="positions"):
+        m(x)
+    with pytest.raises(ValueError, match="positions"):
+        m.step(x[:, 0], S)
+    assert y2.isfinite().all() and (S2 - S).norm() < 0.1 * S.norm()
+
+
+def test_two_captured_graphs_hold_their_own_workspaces():
+    """Sequences in segments: each captured call has a workspace of its own; replays on two streams at
+    once give what the eager calls gave."""
+    from snn_compiler import kernels as K
+    g = torch.Generator(device=DEV).manual_seed(11)
+    lam = torch.tensor([0.9, 0.999], device=DEV)
+    sets = [[torch.randn(1, 6000, 2, 64, generator=g, device=DEV).to(torch.bfloat16) for _ in range(3)]
+            for _ in range(2)]
+    state = torch.randn(1, 2, 64, 64, generator=g, device=DEV)
+    want = [K.decay_attention(*s, lam, state=state) for s in sets]
+    again = state.clone()                                      # in place, through the segments
+    o, S = K.decay_attention(*sets[0], lam, state=again, state_out=again)
+    assert S is again and torch.equal(S, want[0][1]) and torch.equal(o, want[0][0])
+    graphs = []
+    for s in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            graphs.append((graph, K.decay_attention(*s, lam, state=state)))
+        graphs[-1] = (graph, graphs[-1][1])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(5):
+        for stream, (graph, _) in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for (_, got), ref in zip(graphs, want):
+        assert all(torch.equal(a, b) for a, b in zip(got, ref))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_offsets_past_32_bits(dtype):
+    """Sequences, samples and states whose starts lie more than 2^32 bytes apart."""
+    from snn_compiler import kernels as K
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    far = (1 << 32) // (2 if dtype == torch.float32 else 1)
+    big = torch.empty(far + (1 << 20), dtype=dtype, device=DEV)
+    g = torch.Generator().manual_seed(12)
+    x = torch.randn(2, 40, 192, generator=g).to(dtype).to(DEV)
+    row = big.as_strided((2, 40, 192), (far, 192, 1))
+    row.copy_(x)
+    lam = torch.tensor([0.9, 1.0], device=DEV)
+
+    def parts(r):
+        return [t.unflatten(-1, (2, 32)) for t in r.split(64, -1)]
+    for a, b in zip(K.decay_attention(*parts(row), lam), K.decay_attention(*parts(x), lam)):
+        assert torch.equal(a, b)
+    old = torch.randn(2, 2, 32, 32, generator=g).to(DEV)
+    a = K.decay_attention_step(*[t[:, 3] for t in parts(row)], lam, old.clone())
+    b = K.decay_attention_step(*[t[:, 3] for t in parts(x)], lam, old.clone())
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    assert torch.equal(K.group_norm_act(row, 4, act="silu"), K.group_norm_act(x, 4, act="silu"))
+
+
 def test_captured_block_replays():
     from snn_compiler import kernels as K
     m = _block()

@@ -78,7 +78,8 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: to
     behind the last and may be `state` itself.  lengths [B] int32 or int64: tokens of each sequence,
     clamped to [0, N]; what lies behind them is not used, o is zero there, and the state is that
     after the last token (`state` for a length of zero).  dk, dv: 1 to 256.  Powers, sums and the
-    state are held in float32."""
+    state are held in float32.  out and state_out overlap no other argument (but for state_out, state
+    as a whole).  A token that is not finite shows in itself and those behind it only."""
     assert q.dim() == 4, tuple(q.shape)
     B, N = q.shape[:2]
     dt, index, H, Hkv, dk, dv = _check(q, k, v, decay, q.shape[:2], "decay_attention")
@@ -112,7 +113,7 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, deca
                          out: torch.Tensor | None = None, state_out: torch.Tensor | None = None):
     """One token of each sequence: q [B, H, dk], k [B, Hkv, dk], v [B, Hkv, dv], state [B, H, dk, dv]
     float32 -> (o [B, H, dv], the new state), the state updated in place unless state_out is
-    given."""
+    given.  out and state_out overlap no other argument (but for state_out, state as a whole)."""
     assert q.dim() == 3, tuple(q.shape)
     B = q.shape[0]
     dt, index, H, Hkv, dk, dv = _check(q, k, v, decay, q.shape[:1], "decay_attention_step")

@@ -30,7 +30,8 @@ def group_norm_act(x: torch.Tensor, groups: int, weight: torch.Tensor | None = N
     the biased variance of a group are over its channels and all axes between the first and the
     last, in float32.  weight and bias [C], of x's type or float32 (the same for both); act "none",
     "silu", "relu" or "gelu" (the exact form).  Rows may be strided (a slice of a wider tensor)
-    without a copy; the output is contiguous, of x's type."""
+    without a copy; the output is contiguous, of x's type; `out` may be x where that is contiguous, and
+    otherwise does not overlap it."""
     dt, shape = _dtype(x.dtype), x.shape
     code = ACTIVATIONS.get(act)
     if code is None:

@@ -101,6 +101,21 @@ class DecayAttention(nn.Module):
                    torch.as_tensor(decay), heads=heads, kv_heads=kv_heads, dk=dk, dv=dv, neuron=neuron,
                    **kw)
 
+    def _apply(self, fn, recurse=True):
+        decay = self.decay
+        super()._apply(fn, recurse)
+        if self.decay.dtype != torch.float32:      # .half() and the like: 0.999 in bfloat16 is one
+            self.decay = decay.to(self.decay.device)
+        return self
+
+    def _turn(self, q, k, positions):
+        if self.sections is None:
+            return
+        if positions is None:
+            raise ValueError(f"DecayAttention: sections {self.sections} need positions")
+        rotary_axes(q, k, positions, sections=self.sections, base=self.base, ladder=self.ladder,
+                    q_out=q, k_out=k)
+
     def _heads(self, row, lead):
         H, Hk, dk, dv = self.heads, self.kv_heads, self.dk, self.dv
         q, k, v = row.view(*lead, -1).split([H * dk, Hk * dk, Hk * dv], -1)
@@ -120,9 +135,7 @@ class DecayAttention(nn.Module):
         codes, h = self.norm(x, residual)
         N = x.shape[-2]
         q, k, v = self._heads(self.qkv(codes), (x.shape[:-2].numel(), N))
-        if self.sections is not None:
-            rotary_axes(q, k, positions, sections=self.sections, base=self.base, ladder=self.ladder,
-                        q_out=q, k_out=k)
+        self._turn(q, k, positions)
         o, state = decay_attention(q, k, v, self.decay, scale=self.scale, state=state, lengths=lengths)
         return self._finish(o, x.shape), h, state
 
@@ -131,10 +144,8 @@ class DecayAttention(nn.Module):
         (y [..., D], h, state), the state updated in place."""
         codes, h = self.norm(x, residual)
         q, k, v = self._heads(self.qkv(codes), (x.shape[:-1].numel(),))
-        if self.sections is not None:
-            at = positions[None] if positions.dim() == 1 else positions[:, None]
-            q4, k4 = q[:, None], k[:, None]
-            rotary_axes(q4, k4, at, sections=self.sections, base=self.base, ladder=self.ladder,
-                        q_out=q4, k_out=k4)
+        if positions is not None:
+            positions = positions[None] if positions.dim() == 1 else positions[:, None]
+        self._turn(q[:, None], k[:, None], positions)
         o, state = decay_attention_step(q, k, v, self.decay, state, scale=self.scale)
         return self._finish(o, x.shape), h, state
