@@ -41,8 +41,9 @@ __device__ __forceinline__ void fma44(float (&c)[4][4], const float4& a, const f
 // Every type, size and stride: products in float32 on the CUDA cores, 4 x 4 results a thread, from
 // tiles in shared memory (two 16-byte loads for 16 products: bound by issue and shared memory, and by
 // latency, at two blocks an SM).  A thread block takes a segment of a sequence, a head and GV
-// columns.  3 x 1003 tokens x 6 heads of 64 and 96, float32: 71 us (with one result a thread at a time
-// from chunks of 32 tokens 438; floor 1.9).
+// columns.  3 x 1003 tokens x 6 heads of 64 and 96, float32: 56 us (with one result a thread at a time
+// from chunks of 32 tokens 438; with fewer loads in flight, of the segments' states above all, 71; floor
+// 1.9).  8 x 2048 x 16 of 64: 390 us, issue slots 61% busy, two thirds of them multiply-adds.
 // STATES: only the states that the segments leave, each from zero (the first: from state_in).
 template <typename T, bool STATES>
 __global__ void __launch_bounds__(G_THREADS, 2) decay_any_kernel(const __grid_constant__ AnyArgs p) {
@@ -74,23 +75,36 @@ __global__ void __launch_bounds__(G_THREADS, 2) decay_any_kernel(const __grid_co
     {
         const double d = power(lam, p.cps * GC);
         const float fh = (float)d, fl = (float)(d - (double)fh);
-        for (int i = t; i < dkp * GV; i += G_THREADS) {
-            const int r = i / GV, c = i % GV;
-            float x = 0.0f;
-            if (r < dk && c < nv) {
-                if (seg == 0) {
-                    if (a.state_in)
-                        x = !STATES && p.segs > 1 ? work[(p.segs - 1) * slot + r * GV + c]
-                                                  : a.state_in[state + (int64_t)r * a.dv + c];
-                } else if (!STATES) {
-                    x = work[r * GV + c];
-                    for (uint32_t s = 1; s < seg; ++s)
-                        x = fmaf(x, fh, fmaf(x, fl, work[s * slot + r * GV + c]));
+        // AHEAD rows of a thread's column at a time, their loads in flight together
+        constexpr int STEP = G_THREADS / GV, AHEAD = 16;
+        const int c = t % GV;
+        const bool own = seg == 0 && a.state_in;
+        const float* from = !own ? work : !STATES && p.segs > 1 ? work + (p.segs - 1) * slot : a.state_in + state;
+        const int64_t width = own && from == a.state_in + state ? a.dv : GV;
+        for (int r0 = t / GV; r0 < dkp; r0 += AHEAD * STEP) {
+            float x[AHEAD];
+            auto get = [&](const float* at, int64_t width, float (&y)[AHEAD], bool any) {
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) {
+                    const int r = r0 + i * STEP;
+                    y[i] = any && r < dk && c < nv ? at[r * width + c] : 0.0f;
                 }
-                // state_out may be state_in
-                if (STATES && seg == 0 && a.state_in) work[(p.segs - 1) * slot + r * GV + c] = x;
+            };
+            get(from, width, x, own || (!STATES && seg > 0));
+            for (uint32_t s = 1; !STATES && s < seg; ++s) {
+                float y[AHEAD];
+                get(work + s * slot, GV, y, true);
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) x[i] = fmaf(x[i], fh, fmaf(x[i], fl, y[i]));
             }
-            S[r * GP + c] = x;
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const int r = r0 + i * STEP;
+                if (r >= dkp) continue;
+                // state_out may be state_in
+                if (STATES && own && r < dk && c < nv) work[(p.segs - 1) * slot + r * GV + c] = x[i];
+                S[r * GP + c] = x[i];
+            }
         }
     }
     const double dc = power(lam, GC), dl = power(lam, last);
@@ -101,60 +115,67 @@ __global__ void __launch_bounds__(G_THREADS, 2) decay_any_kernel(const __grid_co
     T* og = static_cast<T*>(a.out) + ((int64_t)b * a.N * a.H + h) * a.dv + c0;
     const int64_t ld = a.H * a.dv;
     const int i0 = t / 16 * 4, j0 = t % 16 * 4;    // this thread's rows and columns
+    const bool wide = a.dv % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % (4 * sizeof(T)) == 0;
     for (int64_t n = 0; n < count; ++n) {
         const int64_t n0 = (first + n) * GC;
         const int m = n + 1 == count ? last : GC;
         __syncthreads();
         bool bad = false;
-        // a warp: every eighth token's row, a column a lane, a column's rows in flight together
+        // a warp: eight tokens' rows, a column a lane, two columns of k and q in flight together with v's;
+        // four tokens a store (single ones met four to a bank)
         const int mp = (m + 3) / 4 * 4;            // rows that are used
         constexpr int R = GC / (G_THREADS / 32);
         const T* kr = kg + n0 * a.ks[1];
         const T* qr = qg + n0 * a.qs[1];
         const T* vr = vg + n0 * a.vs[1];
-        for (int c = lane; c < dkp; c += 32) {
-            float x[R], y[R];
+        float z[GV / 32][R];
+#pragma unroll
+        for (int j = 0; j < GV / 32; ++j)
 #pragma unroll
             for (int i = 0; i < R; ++i) {
-                const int r = warp + i * (G_THREADS / 32);
-                const bool in = r < m && c < dk;
-                x[i] = in ? to_f32(kr[r * a.ks[1] + c]) : 0.0f;
-                if (!STATES) y[i] = in ? to_f32(qr[r * a.qs[1] + c]) * a.scale : 0.0f;
+                const int r = warp * R + i, c = lane + 32 * j;
+                z[j][i] = r < m && c < nv ? to_f32(vr[r * a.vs[1] + c]) : 0.0f;
             }
+        for (int l = lane; l < dkp; l += 64) {
+            float x[2][R], y[2][R];
 #pragma unroll
-            for (int i = 0; i < R; ++i) {
-                const int r = warp + i * (G_THREADS / 32);
-                k[c * GP + r] = x[i];
-                if (!STATES) q[c * GP + r] = y[i];
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    const int r = warp * R + i, c = l + 32 * j;
+                    const bool in = r < m && c < dk;
+                    x[j][i] = in ? to_f32(kr[r * a.ks[1] + c]) : 0.0f;
+                    if (!STATES) y[j][i] = in ? to_f32(qr[r * a.qs[1] + c]) * a.scale : 0.0f;
+                }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int c = l + 32 * j;
+                if (c >= dkp) continue;
+#pragma unroll
+                for (int i = 0; i < R; i += 4) {
+                    const int at = c * GP + warp * R + i;
+                    *reinterpret_cast<float4*>(k + at) = make_float4(x[j][i], x[j][i + 1], x[j][i + 2], x[j][i + 3]);
+                    if (!STATES)
+                        *reinterpret_cast<float4*>(q + at) = make_float4(y[j][i], y[j][i + 1], y[j][i + 2], y[j][i + 3]);
+                }
             }
         }
-        for (int c = lane; c < GV; c += 32) {
-            float x[R];
+#pragma unroll
+        for (int j = 0; j < GV / 32; ++j)
 #pragma unroll
             for (int i = 0; i < R; ++i) {
-                const int r = warp + i * (G_THREADS / 32);
-                x[i] = r < m && c < nv ? to_f32(vr[r * a.vs[1] + c]) : 0.0f;
+                bad |= !(fabsf(z[j][i]) <= 3.4028235e38f);
+                v[(warp * R + i) * GP + lane + 32 * j] = z[j][i];
             }
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                bad |= !(fabsf(x[i]) <= 3.4028235e38f);
-                v[(warp + i * (G_THREADS / 32)) * GP + c] = x[i];
-            }
-        }
         bad = __syncthreads_or(bad);
         if (!STATES) {
-            float s[4][4] = {};
-            if (j0 <= i0 + 3 && i0 < m) {
+            float s[4][4] = {}, o[4][4] = {};
 #pragma unroll 4
-                for (int x = 0; x < dkp; ++x)
-                    fma44(s, *reinterpret_cast<const float4*>(q + x * GP + i0),
-                          *reinterpret_cast<const float4*>(k + x * GP + j0));
+            for (int x = 0; x < (i0 < m ? dkp : 0); ++x) {
+                const float4 qx = *reinterpret_cast<const float4*>(q + x * GP + i0);
+                fma44(s, qx, *reinterpret_cast<const float4*>(k + x * GP + j0));
+                fma44(o, qx, *reinterpret_cast<const float4*>(S + x * GP + j0));
             }
-            float o[4][4] = {};
-#pragma unroll 4
-            for (int x = 0; x < (i0 < m ? dkp : 0); ++x)
-                fma44(o, *reinterpret_cast<const float4*>(q + x * GP + i0),
-                      *reinterpret_cast<const float4*>(S + x * GP + j0));
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -183,11 +204,21 @@ __global__ void __launch_bounds__(G_THREADS, 2) decay_any_kernel(const __grid_co
                                 o[i][j] = fmaf(pt[x * GP + i0 + i], v[x * GP + j0 + j], o[i][j]);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 4; ++i) {
+                T y[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (n0 + i0 + i < a.N && j0 + j < nv)
-                        mx::round_to(i0 + i < m ? o[i][j] : 0.0f, og + (n0 + i0 + i) * ld + j0 + j);
+                for (int j = 0; j < 4; ++j) mx::round_to(i0 + i < m ? o[i][j] : 0.0f, y + j);
+                T* to = og + (n0 + i0 + i) * ld + j0;
+                if (n0 + i0 + i >= a.N || j0 >= nv) continue;
+                if (wide) {
+                    struct alignas(4 * sizeof(T)) Four { T x[4]; };
+                    *reinterpret_cast<Four*>(to) = {{y[0], y[1], y[2], y[3]}};
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (j0 + j < nv) to[j] = y[j];
+                }
+            }
             __syncthreads();
         }
         // the rows of v by what is left of them at the chunk's end
@@ -232,8 +263,8 @@ __global__ void __launch_bounds__(G_THREADS, 2) decay_any_kernel(const __grid_co
     }
 }
 
-// As for the tensor cores' form; a chunk of 64 tokens at 64 columns of k takes about 6 us (1.5 in the
-// pass before), both in proportion to dk.
+// As for the tensor cores' form; a chunk of 64 tokens at 64 columns of k takes 19 us for the two blocks of
+// an SM (5 for one in the pass before), both in proportion to dk.
 int any_segments(int64_t items, int64_t chunks, int64_t dk) {
     const int64_t slots = dk <= 64 ? 296 : 148;
     int best = 1;
@@ -412,7 +443,7 @@ int run_step(const Args& a, cudaStream_t s) {
 // Short sequences of few heads go to the CUDA cores whatever their type: there the rounding of the
 // tensor cores' scores, which more results average out, shows in the outputs (1.4 times a float32
 // result's own rounding on the mean; of 9 to 64 tokens of one head up to 1.7 times, of 64 tokens of
-// four 1.5).  8 heads of 64: 11 us for 9 tokens, on the tensor cores 6; one head of 64 tokens: 16, 6.
+// four 1.5).  8 heads of 64: 9 us for 9 tokens, on the tensor cores 6; two of 64 tokens: 14, 6.
 constexpr int64_t FEW_TOKENS = 8, SHORT = 64, FEW_ROWS = 128;
 
 bool heads_ok(int dtype, int64_t B, int64_t H, int64_t Hk, int64_t dk, int64_t dv) {
