@@ -2,20 +2,21 @@
 //
 // A chunk of 128 tokens, a head's dk <= 128 columns of q and k and 64 of v are four products:
 //
-//   scores  Q K^T            128 x 128 x dk    -> P = scores . L, rounded once to the inputs' type
-//   P V                      128 x 64 x 128    P from tensor memory, over the scores' first half
+//   scores  Q K^T            128 x 128 x dk    -> P = scores . L, rounded once (bfloat16) or as two terms
+//   P V                      128 x 64 x 128    P from tensor memory, where its scores were
 //   Q S                      128 x 64 x dk     S as two terms, side by side in N
 //   K^T (w V)                dk x 64 x 128     w_j = decay^(C-1-j); w V as terms, side by side in N
 //
 // The state S stays in registers, float32, and takes the last product as S <- decay^C S + it (the power
 // as two floats: it compounds over the chunks).  The factors w have 24 bits, so bfloat16's w V is cut
-// into three terms of 8 bits, exactly; float16's is rounded to two of 11, which leaves 22, and so
-// is S, of either type, to two for its product.  (Two bfloat16 terms of w V would leave errors of
-// 2.5e-6 in the state; these leave 3e-7.)  Only P is rounded to 8 or 11 bits, as often as the output.
+// into three terms of 8 bits, exactly; float16's is rounded to two of 11, which leaves 22.  (Two
+// bfloat16 terms of w V would leave errors of 2.5e-6 in the state; these leave 3e-7.)  S is rounded to
+// two terms for its product: 16 bits of bfloat16, 22 of float16; and P to 8 bits, once, or to two terms
+// of 11.  float16's range is far below what scores and states take: see its exponents below.
 //
-// Tensor memory holds 512 columns: scores 128, Q S 2 x 64, P V 64, K^T (w V) 3 x 64.  Terms lie side by
-// side because such narrow products are bound by shared memory: 128 x 64 x 16 reads 6 KB of operands,
-// 48 cycles, where the tensor pipe needs 16; the other operand is read once for all terms.
+// Tensor memory holds 512 columns: scores 128, Q S 2 x 64, P V 64 (float16: 2 x 64), K^T (w V) 3 x 64 (2 x 64).
+// Terms lie side by side because such narrow products are bound by shared memory: 128 x 64 x 16 reads 6 KB of
+// operands, 48 cycles, where the tensor pipe needs 16; the other operand is read once for all terms.
 //
 // Warps have one role each, and each walks the block's items (a segment of a sequence, a head, 64 columns
 // of v) and their chunks; what bounds a chunk is the chain scores -> P -> P V -> the next scores, which
@@ -56,18 +57,23 @@ template <int DK, bool STATES, bool HALF> struct Smem {
     static constexpr int RW_OFF = PW_OFF + 160 * 4;            // decay^31 .. decay^0
     static constexpr int WV_OFF = RW_OFF + 32 * 4;             // the factors of v's rows
     static constexpr int BAD_OFF = WV_OFF + C * 4;             // [4][DV] rows, [4] chunk numbers
-    static constexpr int TOP_OFF = BAD_OFF + (4 * DV + 4) * 4; // [8] largest q, k, v, state
-    static constexpr int BAR_OFF = TOP_OFF + 8 * 4 * 4;
+    static constexpr int TOP_OFF = BAD_OFF + (4 * DV + 4) * 4; // [8][2] largest v, state
+    // float16: the powers of two of P's rows [4 chunks][C], and what they come from: each row's largest
+    // q and k [2][C]
+    static constexpr int PROW_OFF = TOP_OFF + 8 * 2 * 4;
+    static constexpr int TOP_ROW_OFF = PROW_OFF + (HALF ? 4 * C * 4 : 0);
+    static constexpr int BAR_OFF = TOP_ROW_OFF + (HALF ? 2 * C * 4 : 0);
     static constexpr int NBARS = 2 * QK_STAGES + 2 * V_STAGES + 16;
     static constexpr int TMEM_OFF = BAR_OFF + NBARS * 8;
     static constexpr int DYN = TMEM_OFF + 8 + 1024;
     static_assert(DYN <= 227 * 1024, "shared memory");
-    static_assert(BAR_OFF % 8 == 0 && RW_OFF % 16 == 0, "alignment");
+    static_assert(BAR_OFF % 8 == 0 && RW_OFF % 16 == 0 && PROW_OFF % 16 == 0, "alignment");
 };
 
 // TMEM columns: scores (and over their first half P), q times the state's two terms, P V, K^T
 // times the scaled v's two or three terms.
 constexpr int T_QK = 0, T_QS = 128, T_PV = 256, T_KV = 320, T_COLS = 512;
+constexpr int T_PV_LOW = 448;      // float16's second term of P times v, behind its two of the scaled v
 
 // Warps 0-3 scores to P, 4 copies, 5 MMAs, 6 and 7 with warps 2 and 3, whose rows have the most
 // scores; 8-11 outputs, 12-15 the state, 16-19 and 20-23 scaled v, a half of each chunk.
@@ -196,10 +202,21 @@ template <bool HALF> __device__ __forceinline__ float2 floats(uint32_t u) {
 }
 // Exponents.  float16 operands are brought below 2^15 by powers of two, exactly: its largest value
 // is 65504, and scores, states and sums can be any.  bfloat16 has float's range and needs none.
+//   P    each row by itself: |P_ij| < 2^7 |q_i| |k_j| with the largest |k| of j <= i, so that no later token
+//        costs an earlier row its bits (one power for the chunk left scores of small rows beside large
+//        ones few bits or none)
+//   w V  by the largest of the chunk's 64 columns of v; S by the largest of the state's
+// What a first term leaves, 2^-25 of the scaled range at most for values that are float16's
+// subnormals there, is multiplied by LOW before it is rounded to the second, whose products are summed
+// by themselves: a value is held to 2^-22 of itself or 2^-50 of the largest in that range, whichever is more.
+// Rows' largest values and second terms of P: 8 x 2048 x 16 of 64 57 us (48 with one power for all).
 __device__ __forceinline__ float pow2(int n) { return __int_as_float((n + 127) << 23); }
 // b with |x| < 2^b for the largest magnitude's bits.
 __device__ __forceinline__ int above_half(uint32_t bits) { return (int)max(bits >> 10, 1u) - 14; }
 __device__ __forceinline__ int above_float(uint32_t bits) { return max((int)(bits >> 23) - 126, -100); }
+constexpr float LOW = 2048.0f;
+// 1 / x of a power of two.
+__device__ __forceinline__ float over_pow2(float x) { return __int_as_float(0x7F000000 - __float_as_int(x)); }
 constexpr uint32_t idesc16(bool half, int M, int N) {
     return tc::idesc_bf16_f32(M, N) & (half ? ~((1u << 7) | (1u << 10)) : ~0u);
 }
@@ -250,6 +267,8 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sbase = tc::smem_u32(smem);
     const uint32_t pw = sbase + L::PW_OFF, rw = sbase + L::RW_OFF, wv = sbase + L::WV_OFF;
+    const uint32_t prow = sbase + L::PROW_OFF;
+    uint32_t* tops8 = reinterpret_cast<uint32_t*>(smem + L::TOP_OFF);       // of chunk g: 2 (g & 7)
     // of a chunk's columns, the first row that is not finite: 256 times the chunk's number + 255 - row
     uint32_t* bad_row = reinterpret_cast<uint32_t*>(smem + L::BAD_OFF);
     volatile int* bad_chunk = reinterpret_cast<int*>(bad_row + 4 * DV);
@@ -265,7 +284,6 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                    done = misc + 80;
     auto vt_ready = [&](int half) { return misc + (half ? 88u : 32u); };
     auto top_ready = [&](uint32_t i) { return misc + 96u + 8u * i; };       // float16: four in turn
-    uint32_t* tops8 = reinterpret_cast<uint32_t*>(smem + L::TOP_OFF);       // of chunk g: 4 (g & 7)
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + L::TMEM_OFF);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Args& a = p.a;
@@ -289,7 +307,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         tc::mbar_init(kv_read, 4);
         tc::mbar_init(qs_done, 1);
         tc::mbar_init(vt_free, 1);
-        for (int i = 0; i < 4; ++i) tc::mbar_init(top_ready(i), 1);
+        for (int i = 0; i < 4; ++i) tc::mbar_init(top_ready(i), 4);
         tc::mbar_init(s_ready, 4);
         tc::mbar_init(done, 1);
         tc::fence_mbar_init();
@@ -299,7 +317,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         for (int i = 0; i < 4; ++i) bad_chunk[i] = -1;
     }
     if (threadIdx.x < 4 * DV) bad_row[threadIdx.x] = 0;
-    else if (threadIdx.x < 4 * DV + 32) tops8[threadIdx.x - 4 * DV] = 0;
+    else if (threadIdx.x < 4 * DV + 16) tops8[threadIdx.x - 4 * DV] = 0;
     if (warp == 5) {
         tc::tmem_alloc(sbase + L::TMEM_OFF, T_COLS);
         tc::tmem_relinquish();
@@ -419,10 +437,12 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         wait(p_ready, ph);
                         if (failed) break;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            umma_ts(tmem + T_PV, tmem + T_QK + 8 * i,
-                                    sdesc_mn_sw128(sbase + L::V_OFF + sv * L::BLOCK, 0) + 128 * i,
-                                    idesc16(HALF, 128, 64) | B_MN, i != 0);
+                        for (int i = 0; i < 16; ++i)   // first terms, then second ones
+                            if (HALF || i < 8)
+                                umma_ts(tmem + (i < 8 ? T_PV : T_PV_LOW),
+                                        tmem + T_QK + 32 * (i % 8 / 2) + 8 * (i % 2) + i / 8 * 16,
+                                        sdesc_mn_sw128(sbase + L::V_OFF + sv * L::BLOCK, 0) + 128 * (i % 8),
+                                        idesc16(HALF, 128, 64) | B_MN, i % 8 != 0);
                         tc::umma_commit(o_ready);
                     }
                     tc::umma_commit(v_empty(sv));
@@ -436,11 +456,17 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             // ------------------------------------------------ scores to P
             // Blocks of 32 x 32: a warp has those of its rows (its lanes of TMEM) up to the
             // diagonal one; the third and the fourth of the last two warps' rows go to warps 6
-            // and 7.
+            // and 7.  A block's P lies over its scores: 16 columns, and 16 of float16's second terms.
             const int q = warp & 3, first = warp >= 6 ? 2 : 0, row = 32 * q + lane;
             const bool two = q == 3 || (q >= 1 && first == 0);     // of these two blocks
             const int diag = q >= 2 && first == 0 ? -1 : q - first;     // which of the two, if any
             const uint32_t tl = tmem + ((uint32_t)(32 * q) << 16) + T_QK;
+            const uint64_t minus = mx::pack2(-1.0f, -1.0f), low2 = mx::pack2(LOW, LOW);
+            auto clear = [&](uint32_t at) {
+                const uint32_t zero[16] = {};
+                tmem_st16(at, zero);
+                if (HALF) tmem_st16(at + 16, zero);
+            };
             for (uint32_t it = blockIdx.x; !STATES && it < p.items; it += gridDim.x) {
                 const Item x(p, it);
                 if (x.n == 0) continue;
@@ -459,22 +485,23 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     failed |= 1u - tc::mbar_wait_warp(qk_ready, g & 1u, failed);
                     tc::tc_fence_after();
                     float down = 1.0f;
-                    if constexpr (HALF) {            // |q . k| < 128 * 2^(bounds of q and k)
+                    if constexpr (HALF) {
                         failed |= 1u - tc::mbar_wait_warp(top_ready(g & 3), (g >> 2) & 1u, failed);
-                        const uint32_t* top = tops8 + 4 * (g & 7);
-                        down = pow2(8 - above_half(top[0]) - above_half(top[1]));
+                        down = lds_f(prow + 4 * ((g & 3) * C + row));
                     }
 #pragma unroll 1
                     for (int blk = 0; blk < 2; ++blk) {
+                        const uint32_t at = tl + (first + blk) * 32;      // P takes its scores' place
                         uint32_t w[16];
+                        if (blk && !two) {           // blocks of later tokens
+                            clear(at);
+                            continue;
+                        }
                         float s[32];
-                        if (blk == 0 || two) tc::tmem_ld32(tl + (first + blk) * 32, s);
+                        tc::tmem_ld32(at, s);
                         tc::tmem_wait_ld();
 #pragma unroll
                         for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(s[i]));
-                        // P of the third and fourth blocks takes the place of the second one's
-                        // scores, once those have been read
-                        if (q >= 2 && first == 0 && blk == 1) tc::named_bar_sync(3 + q, 64);
                         if (blk == diag) {
                             // later tokens count nothing, whatever their scores
                             const uint32_t d = pw + 4 * (31 + lane);
@@ -496,15 +523,25 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                             }
                         }
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            w[i] = blk == 0 || two ? pair<HALF>(s[2 * i], s[2 * i + 1]) : 0u;
-                        if (q >= 2 && first == 2 && blk == 0) tc::named_bar_sync(3 + q, 64);
-                        tmem_st16(tl + (first + blk) * 16, w);
+                        for (int i = 0; i < 16; ++i) {
+                            w[i] = pair<HALF>(s[2 * i], s[2 * i + 1]);
+                            if constexpr (HALF) {    // what that leaves
+                                const float2 h = floats<HALF>(w[i]);
+                                mx::unpack2(mx::mul2(low2, mx::fma2(mx::pack2(h.x, h.y), minus,
+                                                                    mx::pack2(s[2 * i], s[2 * i + 1]))),
+                                            s[2 * i], s[2 * i + 1]);
+                            }
+                        }
+                        tmem_st16(at, w);
+                        if constexpr (HALF) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) w[i] = pair<HALF>(s[2 * i], s[2 * i + 1]);
+                            tmem_st16(at + 16, w);
+                        }
                     }
-                    if (q < 2) {                     // blocks of later tokens
-                        const uint32_t zero[16] = {};
-                        tmem_st16(tl + 32, zero);
-                        tmem_st16(tl + 48, zero);
+                    if (q < 2) {
+                        clear(tl + 64);
+                        clear(tl + 96);
                     }
                     tmem_wait_st();
                     tc::tc_fence_before();
@@ -521,8 +558,10 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         const uint32_t stage = sbase + L::O_OFF + q * 32 * 128;
         for (uint32_t it = blockIdx.x; !STATES && it < p.items; it += gridDim.x) {
             const Item x(p, it);
-            const float fq = (float)power(x.lam, row + 1) * a.scale;
-            uint64_t fq2 = mx::pack2(fq, fq), sc2 = mx::pack2(a.scale, a.scale);
+            // a small scale and a power of the decay apart: their product may be less than float holds
+            const float fq = HALF ? (float)power(x.lam, row + 1) : (float)power(x.lam, row + 1) * a.scale;
+            uint64_t fq2 = mx::pack2(fq, fq);
+            const uint64_t sc2 = mx::pack2(a.scale, a.scale), up2 = mx::pack2(1.0f / LOW, 1.0f / LOW);
             const int cols = min(DV, a.dv - x.tile * DV);
             const int64_t ld = a.H * a.dv;
             uint16_t* out = static_cast<uint16_t*>(a.out) +
@@ -537,12 +576,12 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 }
                 failed |= 1u - tc::mbar_wait_warp(o_ready, g & 1u, failed);
                 tc::tc_fence_after();
-                if constexpr (HALF) {                // the powers of two of q S and of P
-                    const uint32_t* top = tops8 + 4 * (g & 7);
-                    const float fs = fq * pow2(above_float(top[3]) - 15);
-                    const float fp = a.scale * pow2(above_half(top[0]) + above_half(top[1]) - 8);
+                uint64_t row2 = 0;
+                if constexpr (HALF) {                // the powers of two of q S and of P's row undone
+                    const float fs = fq * pow2(above_float(tops8[2 * (g & 7) + 1]) - 15);
+                    const float f = over_pow2(lds_f(prow + 4 * ((g & 3) * C + row)));
                     fq2 = mx::pack2(fs, fs);
-                    sc2 = mx::pack2(fp, fp);
+                    row2 = mx::pack2(f, f);
                 }
                 const bool spoiled = bad_chunk[g & 3] == (int)g, alive = n < x.len;
                 const bool write = n < a.N && !failed && SNNB_IN_BOUNDS(n, a.N, p.status);
@@ -551,9 +590,19 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     float s[16], l[16], v[16];
                     tc::tmem_ld16(tl + T_QS + i, s);
                     tc::tmem_ld16(tl + T_QS + 64 + i, l);
+                    if constexpr (HALF) {            // registers for two of the four
+                        tc::tmem_wait_ld();
+                        tc::reg_fence16(s);
+                        tc::reg_fence16(l);
+#pragma unroll
+                        for (int j = 0; j < 16; j += 2)
+                            mx::unpack2(mx::mul2(fq2, mx::fma2(mx::pack2(l[j], l[j + 1]), up2,
+                                                               mx::pack2(s[j], s[j + 1]))), s[j], s[j + 1]);
+                        tc::tmem_ld16(tl + T_PV_LOW + i, l);
+                    }
                     tc::tmem_ld16(tl + T_PV + i, v);
                     tc::tmem_wait_ld();
-                    tc::reg_fence16(s);
+                    if constexpr (!HALF) tc::reg_fence16(s);
                     tc::reg_fence16(l);
                     tc::reg_fence16(v);
                     if (i + 16 == DV) {
@@ -564,9 +613,14 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     uint32_t w[8];
 #pragma unroll
                     for (int j = 0; j < 16; j += 2) {
-                        const uint64_t y = mx::add2(mx::pack2(s[j], s[j + 1]), mx::pack2(l[j], l[j + 1]));
-                        mx::unpack2(mx::fma2(fq2, y, mx::mul2(sc2, mx::pack2(v[j], v[j + 1]))), v[j],
-                                    v[j + 1]);
+                        if constexpr (HALF) {
+                            const uint64_t y = mx::fma2(mx::pack2(l[j], l[j + 1]), up2, mx::pack2(v[j], v[j + 1]));
+                            mx::unpack2(mx::mul2(sc2, mx::fma2(row2, y, mx::pack2(s[j], s[j + 1]))), v[j], v[j + 1]);
+                        } else {
+                            const uint64_t y = mx::add2(mx::pack2(s[j], s[j + 1]), mx::pack2(l[j], l[j + 1]));
+                            mx::unpack2(mx::fma2(fq2, y, mx::mul2(sc2, mx::pack2(v[j], v[j + 1]))), v[j],
+                                        v[j + 1]);
+                        }
                     }
                     if (spoiled) {
                         const uint32_t* rows = bad_row + (g & 3) * DV + i;
@@ -670,13 +724,13 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     if (g) failed |= 1u - tc::mbar_wait_warp(qs_done, (g - 1) & 1u, failed);
                     float up = 1.0f;
                     if constexpr (HALF) {
-                        volatile uint32_t* top = tops8 + 4 * (g & 7) + 3;
+                        volatile uint32_t* top = tops8 + 2 * (g & 7) + 1;
                         float m = 0.0f;
 #pragma unroll
                         for (int i = 0; i < W; ++i) m = fmaxf(m, fabsf(S[i]));
                         uint32_t bits = __reduce_max_sync(0xffffffffu, (uint32_t)__float_as_int(m));
-                        if (lane == 0) atomicMax(&tops8[4 * (g & 7) + 3], bits);
-                        if (t == 0) tops8[4 * ((g + 1) & 7) + 3] = 0;
+                        if (lane == 0) atomicMax(&tops8[2 * (g & 7) + 1], bits);
+                        if (t == 0) tops8[2 * ((g + 1) & 7) + 1] = 0;
                         tc::named_bar_sync(8, 128);
                         if (*top >= 0x7F800000u) {   // of the finite ones
                             tc::named_bar_sync(8, 128);
@@ -687,7 +741,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                                 if (fabsf(S[i]) <= 3.4028235e38f) m = fmaxf(m, fabsf(S[i]));
                             bits = __reduce_max_sync(0xffffffffu, (uint32_t)__float_as_int(m));
                             tc::named_bar_sync(8, 128);
-                            if (lane == 0) atomicMax(&tops8[4 * (g & 7) + 3], bits);
+                            if (lane == 0) atomicMax(&tops8[2 * (g & 7) + 1], bits);
                             tc::named_bar_sync(8, 128);
                         }
                         up = pow2(15 - above_float(*top));
@@ -700,7 +754,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                             const float y = S[i + 2 * j] * up, z = S[i + 2 * j + 1] * up;
                             hi[j] = pair<HALF>(y, z);
                             const float2 h = floats<HALF>(hi[j]);
-                            lo[j] = pair<HALF>(y - h.x, z - h.y);
+                            lo[j] = HALF ? pair<HALF>((y - h.x) * LOW, (z - h.y) * LOW) : pair<HALF>(y - h.x, z - h.y);
                         }
                         const uint32_t o = sbase + L::S_OFF + swizzled(row, (col + i) / 8);
                         sts128(o, make_uint4(hi[0], hi[1], hi[2], hi[3]));
@@ -715,9 +769,10 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 const bool end = c + 1 == x.n;
                 const float fh = end ? lh : ch, fl = end ? ll : cl;
                 const uint64_t fh2 = mx::pack2(fh, fh), fl2 = mx::pack2(fl, fl);
+                const uint64_t up2 = mx::pack2(1.0f / LOW, 1.0f / LOW);
                 uint64_t back = 0;
                 if constexpr (HALF) {
-                    const float f = pow2(above_half(tops8[4 * (g & 7) + 2]) - 15);
+                    const float f = pow2(above_half(tops8[2 * (g & 7)]) - 15);
                     back = mx::pack2(f, f);
                 }
 #pragma unroll
@@ -739,9 +794,14 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     for (int j = 0; j < 16; j += 2) {
                         const uint64_t old = mx::pack2(S[i + j], S[i + j + 1]);
                         uint64_t sum = mx::pack2(z[j], z[j + 1]);
-                        if constexpr (!HALF) sum = mx::add2(sum, mx::pack2(u[j], u[j + 1]));
-                        sum = mx::add2(mx::pack2(y[j], y[j + 1]), sum);
-                        sum = HALF ? mx::fma2(sum, back, mx::mul2(old, fl2)) : mx::fma2(old, fl2, sum);
+                        if constexpr (HALF) {
+                            sum = mx::fma2(sum, up2, mx::pack2(y[j], y[j + 1]));
+                            sum = mx::fma2(sum, back, mx::mul2(old, fl2));
+                        } else {
+                            sum = mx::add2(sum, mx::pack2(u[j], u[j + 1]));
+                            sum = mx::add2(mx::pack2(y[j], y[j + 1]), sum);
+                            sum = mx::fma2(old, fl2, sum);
+                        }
                         mx::unpack2(mx::fma2(old, fh2, sum), S[i + j], S[i + j + 1]);
                     }
                 }
@@ -756,7 +816,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         const int piece = t & 7, r0 = (t >> 3) & 15, first = 64 * half + r0;
         const uint32_t vt = sbase + L::VT_OFF + (L::VT_HALVES == 2 ? half * L::VT_HALF : 0) +
                             swizzled(r0, piece);
-        const uint64_t minus = mx::pack2(-1.0f, -1.0f);
+        const uint64_t minus = mx::pack2(-1.0f, -1.0f), low2 = mx::pack2(LOW, LOW);
         for (uint32_t it = blockIdx.x; it < p.items; it += gridDim.x) {
             const Item x(p, it);
             int held = -1;                           // tokens that the factors are for
@@ -788,6 +848,30 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                             }
                         }
                 }
+                if constexpr (HALF && !STATES) {
+                    // of each row the largest magnitudes of q (upper half) and of k
+                    uint32_t* rows = reinterpret_cast<uint32_t*>(smem + L::TOP_ROW_OFF) + (g & 1) * C;
+                    failed |= 1u - tc::mbar_wait_warp(qk_full(sq), (g / NQ) & 1u, failed);
+                    const uint32_t qs = sbase + sq * L::QK_STAGE + swizzled(first, piece);
+                    uint32_t y[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t tq = 0, tk = 0;
+#pragma unroll
+                        for (int k = 0; k < L::KB; ++k) {
+                            tq = largest(tq, lds128(qs + k * L::BLOCK + 2048 * i));
+                            tk = largest(tk, lds128(qs + L::K_IN_STAGE + k * L::BLOCK + 2048 * i));
+                        }
+                        y[i] = __vmaxu2(__byte_perm(tq, tk, 0x1054), __byte_perm(tq, tk, 0x3276));
+                    }
+#pragma unroll
+                    for (int o = 1; o < 8; o *= 2)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) y[i] = __vmaxu2(y[i], __shfl_xor_sync(0xffffffffu, y[i], o));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (piece == 0) rows[first + 16 * i] = y[i];
+                }
                 constexpr uint32_t INF = HALF ? 0x7C00u : 0x7F80u;
                 uint32_t top = 0, hi[4][4], mid[4][4], low[4][4];
                 uint4 raw[4];
@@ -798,29 +882,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 }
                 float up = 1.0f;
                 if constexpr (HALF) {
-                    // the largest magnitudes of the chunk's q, k and v
-                    uint32_t* tops = tops8 + 4 * (g & 7);
-                    if constexpr (!STATES) {
-                        failed |= 1u - tc::mbar_wait_warp(qk_full(sq), (g / NQ) & 1u, failed);
-                        const uint32_t qs = sbase + sq * L::QK_STAGE + swizzled(first, piece);
-#pragma unroll 1
-                        for (int x = 0; x < 2; ++x) {          // q, then k
-                            uint32_t tx = 0;
-#pragma unroll
-                            for (int i = 0; i < 4 * L::KB; ++i)
-                                tx = largest(tx, lds128(qs + x * L::K_IN_STAGE + i / 4 * L::BLOCK + i % 4 * 2048));
-                            tx = max(tx & 0xFFFFu, tx >> 16);
-                            if (tx >= INF) {
-                                tx = 0;
-#pragma unroll 1
-                                for (int i = 0; i < 4 * L::KB; ++i)
-                                    tx = largest_finite(tx, lds128(qs + x * L::K_IN_STAGE + i / 4 * L::BLOCK +
-                                                                   i % 4 * 2048));
-                            }
-                            tx = __reduce_max_sync(0xffffffffu, tx);
-                            if (lane == 0) atomicMax(&tops[x], tx);
-                        }
-                    }
+                    uint32_t* tops = tops8 + 2 * (g & 7);
                     uint32_t tv = max(top & 0xFFFFu, top >> 16);
                     if (tv >= INF) {
                         tv = 0;
@@ -828,11 +890,26 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         for (int i = 0; i < 4; ++i) tv = largest_finite(tv, lds128(vs + 2048 * i));
                     }
                     tv = __reduce_max_sync(0xffffffffu, tv);
-                    if (lane == 0) atomicMax(&tops[2], tv);
-                    if (t < 3) tops8[4 * ((g + 1) & 7) + t] = 0;
+                    if (lane == 0) atomicMax(&tops[0], tv);
+                    if (t == 0) tops8[2 * ((g + 1) & 7)] = 0;
                     tc::named_bar_sync(1, 256);
-                    if (t == 0 && !STATES) tc::mbar_arrive(top_ready(g & 3));
-                    up = pow2(15 - above_half(tops[2]));
+                    up = pow2(15 - above_half(tops[0]));
+                    if (!STATES && half == 1) {
+                        // P of row i is below 2^7 |q_i| |k_j|, j <= i: the rows' largest |k| so far
+                        const uint32_t* rows = reinterpret_cast<uint32_t*>(smem + L::TOP_ROW_OFF) + (g & 1) * C;
+                        const int r = t - 128;
+                        const uint32_t own = rows[r];
+                        uint32_t before = 0, most = own & 0xFFFFu;
+#pragma unroll
+                        for (int i = 0; i < 3; ++i)
+                            if (i < r >> 5) before = max(before, rows[32 * i + lane] & 0xFFFFu);
+#pragma unroll
+                        for (int o = 1; o < 32; o *= 2) most = max(most, __shfl_up_sync(0xffffffffu, most, o));
+                        most = max(most, __reduce_max_sync(0xffffffffu, before));
+                        sts_f(prow + 4 * ((g & 3) * C + r), pow2(8 - above_half(own >> 16) - above_half(most)));
+                        __syncwarp();
+                        if (lane == 0) tc::mbar_arrive(top_ready(g & 3));
+                    }
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -849,7 +926,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                             // 22 of 24 bits, in two terms
                             hi[i][j] = pair<HALF>(y, z);
                             const float2 h = floats<HALF>(hi[i][j]);
-                            mx::unpack2(mx::fma2(mx::pack2(h.x, h.y), minus, yz), y, z);
+                            mx::unpack2(mx::mul2(low2, mx::fma2(mx::pack2(h.x, h.y), minus, yz)), y, z);
                             mid[i][j] = pair<HALF>(y, z);
                         } else {
                             // 24 bits, cut into three times 8: exact
