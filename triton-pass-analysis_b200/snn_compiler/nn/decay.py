@@ -89,12 +89,15 @@ class DecayAttention(nn.Module):
         """Quantises four float layers; the head dimensions follow from their sizes."""
         kv_heads = heads if kv_heads is None else kv_heads
         dk, dv = q.out_features // heads, v.out_features // kv_heads
-        joint = nn.Linear(q.in_features, q.out_features + k.out_features + v.out_features,
-                          bias=q.bias is not None, device=q.weight.device, dtype=q.weight.dtype)
+        parts = (q, k, v)
+        joint = nn.Linear(q.in_features, sum(m.out_features for m in parts),
+                          bias=any(m.bias is not None for m in parts), device=q.weight.device,
+                          dtype=q.weight.dtype)
         with torch.no_grad():
-            joint.weight.copy_(torch.cat([q.weight, k.weight, v.weight]))
-            if q.bias is not None:
-                joint.bias.copy_(torch.cat([q.bias, k.bias, v.bias]))
+            joint.weight.copy_(torch.cat([m.weight for m in parts]))
+            if joint.bias is not None:             # zeros for those without one
+                joint.bias.copy_(torch.cat([m.weight.new_zeros(m.out_features) if m.bias is None
+                                            else m.bias for m in parts]))
         return cls(RMSNormMX(q.in_features, eps=eps, weight=norm_weight, device=q.weight.device),
                    MXLinear.from_linear(joint, act="mxfp8", dtype=dtype),
                    MXLinear.from_linear(out, act="mxfp8" if neuron is None else "mxfp4", dtype=dtype),
