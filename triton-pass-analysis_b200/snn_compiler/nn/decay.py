@@ -88,6 +88,10 @@ class DecayAttention(nn.Module):
                      dtype=torch.bfloat16, neuron: nn.Module | None = None, **kw):
         """Quantises four float layers; the head dimensions follow from their sizes."""
         kv_heads = heads if kv_heads is None else kv_heads
+        if heads < 1 or kv_heads < 1 or q.out_features % heads or v.out_features % kv_heads or \
+                k.out_features * heads != q.out_features * kv_heads:
+            raise ValueError(f"DecayAttention: layers of {q.out_features}, {k.out_features} and {v.out_features} "
+                             f"features do not divide into {heads} and {kv_heads} heads")
         dk, dv = q.out_features // heads, v.out_features // kv_heads
         parts = (q, k, v)
         joint = nn.Linear(q.in_features, sum(m.out_features for m in parts),
