@@ -134,3 +134,14 @@ def test_float16_values_that_are_not_finite(pad):
         others = [c for c in range(64) if c != 7]
         assert torch.equal(o[..., others], ref[..., others]) and torch.equal(o[:, :, 0], ref[:, :, 0])
         assert torch.equal(S[..., others], rS[..., others])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("pad", [0, 1])
+@pytest.mark.parametrize("size", [1e-30, 1e30])
+def test_scale_that_undoes_the_state(size, pad, dtype):
+    """A scale of 1e-30 beside a state of 1e30: what a decayed state leaves is a number of ordinary size
+    or far below it, never one that the scale pushed out of float32's range on the way."""
+    q, k, v = _tokens(1, 260, 4, 4, 64, 64, dtype, 46)
+    state = torch.randn(1, 4, 64, 64, generator=_gen(6)) * size
+    _check(q, k, v, LAM, min(1.0, 1.0 / size), state, pad=pad)

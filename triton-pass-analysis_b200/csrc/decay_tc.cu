@@ -559,7 +559,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         for (uint32_t it = blockIdx.x; !STATES && it < p.items; it += gridDim.x) {
             const Item x(p, it);
             // a small scale and a power of the decay apart: their product may be less than float holds
-            const float fq = HALF ? (float)power(x.lam, row + 1) : (float)power(x.lam, row + 1) * a.scale;
+            const float fq = (float)power(x.lam, row + 1);
             uint64_t fq2 = mx::pack2(fq, fq);
             const uint64_t sc2 = mx::pack2(a.scale, a.scale), up2 = mx::pack2(1.0f / LOW, 1.0f / LOW);
             const int cols = min(DV, a.dv - x.tile * DV);
@@ -618,7 +618,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                             mx::unpack2(mx::mul2(sc2, mx::fma2(row2, y, mx::pack2(s[j], s[j + 1]))), v[j], v[j + 1]);
                         } else {
                             const uint64_t y = mx::add2(mx::pack2(s[j], s[j + 1]), mx::pack2(l[j], l[j + 1]));
-                            mx::unpack2(mx::fma2(fq2, y, mx::mul2(sc2, mx::pack2(v[j], v[j + 1]))), v[j],
+                            mx::unpack2(mx::mul2(sc2, mx::fma2(fq2, y, mx::pack2(v[j], v[j + 1]))), v[j],
                                         v[j + 1]);
                         }
                     }
