@@ -585,7 +585,7 @@ int snnb_rotary_axes(const void* q, void* q_out, int64_t q_heads, const int64_t*
 
 /*
  * Linear attention with a decay for each head, q [B, N, H, dk], k [B, N, Hkv, dk],
- * v [B, N, Hkv, dv] (query head h reads key head h / (H / Hkv)), dk and dv up to 256:
+ * v [B, N, Hkv, dv] (query head h reads key head h / (H / Hkv)), dk and dv up to 256, N up to 2^31 - 256:
  *   S_t = decay[h] S_{t-1} + k_t v_t^T,   out_t = scale q_t S_t
  * decay [H] float32; state_in (NULL: zero) and state_out (NULL: not wanted) [B, H, dk, dv]
  * float32, which may be the same; lengths [B] int32 (0) or int64 (1) or NULL: tokens of each

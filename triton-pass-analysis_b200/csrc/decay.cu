@@ -306,7 +306,6 @@ int run_any(const Args& a, void* work, int64_t bytes, cudaStream_t s) {
     const int segs = any_segments(a.B * a.H * tiles, chunks, a.dk);
     if (segs > 1 && (!work || !aligned16(work) || bytes < any_workspace(a.B, a.N, a.H, a.dk, a.dv)))
         return SNNB_ERR_ARG;
-    if (chunks / segs > 0x7ffffff) return SNNB_ERR_ARG;
     const AnyArgs p = {a, tiles, 0, segs, (int)((chunks + segs - 1) / segs), static_cast<float*>(work)};
     if (segs > 1)
         if (const int st = launch_any<T, true>(p, s)) return st;
@@ -462,7 +461,7 @@ using namespace snnb;
 
 extern "C" int64_t snnb_decay_attention_workspace_bytes(int dtype, int64_t B, int64_t N, int64_t H,
                                                         int64_t dk, int64_t dv) {
-    if (!heads_ok(dtype, B, H, H, dk, dv) || N < 0) return -1;
+    if (!heads_ok(dtype, B, H, H, dk, dv) || N < 0 || N > MOST_TOKENS) return -1;
     if (B == 0 || N == 0) return 0;
     // strides and alignment decide between the forms
     const int64_t tc = decay::tc_workspace(dtype, B, N, H, dk, dv), any = any_workspace(B, N, H, dk, dv);
@@ -478,7 +477,7 @@ extern "C" int snnb_decay_attention(const void* q, const int64_t* q_strides, con
                                     float* state_out, void* workspace, int64_t workspace_bytes,
                                     snnb_stream_t stream) {
     if (const int inj = take_injected_status()) return inj;
-    if (!heads_ok(dtype, B, H, Hkv, dk, dv) || N < 0) return SNNB_ERR_ARG;
+    if (!heads_ok(dtype, B, H, Hkv, dk, dv) || N < 0 || N > MOST_TOKENS) return SNNB_ERR_ARG;
     if (N > (int64_t(1) << 40) / (H * dv) / (B ? B : 1)) return SNNB_ERR_ARG;
     if (lengths && lengths_dtype != 0 && lengths_dtype != 1) return SNNB_ERR_ARG;
     if (B == 0) return SNNB_OK;

@@ -8,6 +8,9 @@ namespace snnb {
 namespace decay {
 
 constexpr int MAX_DIM = 256;       // of a head's keys and of its values
+// Tokens of a sequence: the exponents below, whole chunks of them, are 32 bits (a negative one would
+// not end).
+constexpr int64_t MOST_TOKENS = 0x7fffff00;
 
 struct Args {
     const void *q, *k, *v;         // [B, N, H or Hk, dk or dv], unit column stride

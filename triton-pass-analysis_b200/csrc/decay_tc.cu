@@ -1061,7 +1061,7 @@ int segments(int64_t items, int64_t chunks) {
 }  // namespace
 
 bool tc_takes(const Args& a, int dtype) {
-    return (dtype == SNNB_BF16 || dtype == SNNB_F16) && a.N > 0 && a.N < 0x7fffff00 && a.dk <= 128 && a.dk % 8 == 0 &&
+    return (dtype == SNNB_BF16 || dtype == SNNB_F16) && a.N > 0 && a.dk <= 128 && a.dk % 8 == 0 &&
            a.dv % 8 == 0 && aligned16(a.out) && aligned16(a.state_in) && aligned16(a.state_out) &&
            mappable(a.q, a.qs, a.B, a.N, a.H) &&
            mappable(a.k, a.ks, a.B, a.N, a.Hk) && mappable(a.v, a.vs, a.B, a.N, a.Hk);

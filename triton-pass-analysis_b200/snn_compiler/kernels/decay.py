@@ -77,7 +77,7 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: to
     state: the state before the first token (zero without one); state_out receives the state
     behind the last and may be `state` itself.  lengths [B] int32 or int64: tokens of each sequence,
     clamped to [0, N]; what lies behind them is not used, o is zero there, and the state is that
-    after the last token (`state` for a length of zero).  dk, dv: 1 to 256.  Powers, sums and the
+    after the last token (`state` for a length of zero).  dk, dv: 1 to 256, N below 2^31 - 255.  Powers, sums and the
     state are held in float32.  out and state_out overlap no other argument (but for state_out, state
     as a whole).  A token that is not finite shows in itself and those behind it only."""
     assert q.dim() == 4, tuple(q.shape)
