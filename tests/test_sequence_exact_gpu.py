@@ -1,0 +1,44 @@
+"""Decay attention of 16-bit inputs is a float32 sum, rounded once, at every length, number of heads and
+alignment, against the float64 oracle.
+
+Tolerances, derived: on the tensor cores P and the state are held as two terms of at least 8 bits (2^-16
+each of what they hold), sums as in test_sequence_gpu.py, (dk + N / 8 + 64) 2^-23 of the magnitude; the
+output's one rounding is half a step of its type.  The state's operands have 22 bits or more: 2^-22
+(float16's two terms of 11) and the sums.
+"""
+import pytest
+import torch
+
+from oracle import sequence as OS
+from test_sequence_gpu import BF16, DEV, DTYPES, F16, F32, _gen, _k, _lam, _near, _tiny, _tokens, _u
+from test_sequence_ranges_gpu import _views
+
+pytestmark = pytest.mark.gpu
+
+
+def _check(q, k, v, lam, scale=1.0, state=None, lengths=None, pad=0, in_place=False):
+    old = None if state is None else state.to(DEV)
+    o, S = _k().decay_attention(*_views((q, k, v), pad), lam.to(DEV), scale=scale, state=old,
+                                lengths=None if lengths is None else lengths.to(DEV),
+                                state_out=old if in_place else None)
+    ro, rS, oa, A = OS.decay(q, k, v, lam, scale, state, lengths)
+    sums = (q.shape[-1] + q.shape[1] / 8 + 64) * 2.0 ** -23
+    terms = 0.0 if q.dtype == F32 else 2.0 ** -15
+    _near(o, ro, (terms + sums) * oa + _u(q.dtype) * ro.abs() + _tiny(q.dtype) + 1e-37)
+    _near(S, rS, (2.0 ** -22 + sums) * A + 1e-37)
+    return o, S, ro
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("pad", [0, 1])
+@pytest.mark.parametrize("B,N,H,d", [(1, 2, 1, 64), (1, 8, 2, 64), (1, 9, 1, 128), (2, 33, 1, 48), (1, 64, 1, 64),
+                                     (1, 64, 2, 64), (1, 65, 1, 64), (2, 64, 4, 128), (1, 128, 1, 64), (1, 200, 2, 128)])
+def test_outputs_are_rounded_once(B, N, H, d, pad, dtype):
+    """Of every size alike: no output is off by more than its own rounding and float32's sums, and all
+    together by no more than a tenth above the rounding's."""
+    q, k, v = _tokens(B, N, H, H, d, d, dtype, 50 + N)
+    state = torch.randn(B, H, d, d, generator=_gen(7))
+    lam = 1 - torch.exp2(-5.0 - torch.arange(H))
+    o, _, ro = _check(q, k, v, lam, d ** -0.5, state, None, pad)
+    if dtype != F32 and B * N * H * d >= 512:                 # enough values for a mean
+        assert (o.cpu().double() - ro).norm() <= 1.1 * (ro.to(dtype).double() - ro).norm()

@@ -2,7 +2,7 @@
 //
 // A chunk of 128 tokens, a head's dk <= 128 columns of q and k and 64 of v are four products:
 //
-//   scores  Q K^T            128 x 128 x dk    -> P = scores . L, rounded once (bfloat16) or as two terms
+//   scores  Q K^T            128 x 128 x dk    -> P = scores . L, as two terms
 //   P V                      128 x 64 x 128    P from tensor memory, where its scores were
 //   Q S                      128 x 64 x dk     S as two terms, side by side in N
 //   K^T (w V)                dk x 64 x 128     w_j = decay^(C-1-j); w V as terms, side by side in N
@@ -10,9 +10,11 @@
 // The state S stays in registers, float32, and takes the last product as S <- decay^C S + it (the power
 // as two floats: it compounds over the chunks).  The factors w have 24 bits, so bfloat16's w V is cut
 // into three terms of 8 bits, exactly; float16's is rounded to two of 11, which leaves 22.  (Two
-// bfloat16 terms of w V would leave errors of 2.5e-6 in the state; these leave 3e-7.)  S is rounded to
-// two terms for its product: 16 bits of bfloat16, 22 of float16; and P to 8 bits, once, or to two terms
-// of 11.  float16's range is far below what scores and states take: see its exponents below.
+// bfloat16 terms of w V would leave errors of 2.5e-6 in the state; these leave 3e-7.)  P and S are rounded to
+// two terms for their products: 16 bits of bfloat16, 22 of float16, so that an output is as good as a
+// float32 sum that is rounded once.  (P as one term: the error of bfloat16 outputs was 1.25 times that, of
+// one head's 64 tokens 1.7 times; 16 x 2048 x 16 heads of 64 took 69 us, and takes 81.)  float16's range is far
+// below what scores and states take: see its exponents below.
 //
 // Tensor memory holds 512 columns: scores 128, Q S 2 x 64, P V 64 (float16: 2 x 64), K^T (w V) 3 x 64 (2 x 64).
 // Terms lie side by side because such narrow products are bound by shared memory: 128 x 64 x 16 reads 6 KB of
@@ -438,11 +440,10 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         if (failed) break;
 #pragma unroll
                         for (int i = 0; i < 16; ++i)   // first terms, then second ones
-                            if (HALF || i < 8)
-                                umma_ts(tmem + (i < 8 ? T_PV : T_PV_LOW),
-                                        tmem + T_QK + 32 * (i % 8 / 2) + 8 * (i % 2) + i / 8 * 16,
-                                        sdesc_mn_sw128(sbase + L::V_OFF + sv * L::BLOCK, 0) + 128 * (i % 8),
-                                        idesc16(HALF, 128, 64) | B_MN, i % 8 != 0);
+                            umma_ts(tmem + (HALF && i >= 8 ? T_PV_LOW : T_PV),
+                                    tmem + T_QK + 32 * (i % 8 / 2) + 8 * (i % 2) + i / 8 * 16,
+                                    sdesc_mn_sw128(sbase + L::V_OFF + sv * L::BLOCK, 0) + 128 * (i % 8),
+                                    idesc16(HALF, 128, 64) | B_MN, HALF ? i % 8 != 0 : i != 0);
                         tc::umma_commit(o_ready);
                     }
                     tc::umma_commit(v_empty(sv));
@@ -456,7 +457,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             // ------------------------------------------------ scores to P
             // Blocks of 32 x 32: a warp has those of its rows (its lanes of TMEM) up to the
             // diagonal one; the third and the fourth of the last two warps' rows go to warps 6
-            // and 7.  A block's P lies over its scores: 16 columns, and 16 of float16's second terms.
+            // and 7.  A block's P lies over its scores: 16 columns of first terms, 16 of second ones.
             const int q = warp & 3, first = warp >= 6 ? 2 : 0, row = 32 * q + lane;
             const bool two = q == 3 || (q >= 1 && first == 0);     // of these two blocks
             const int diag = q >= 2 && first == 0 ? -1 : q - first;     // which of the two, if any
@@ -465,7 +466,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             auto clear = [&](uint32_t at) {
                 const uint32_t zero[16] = {};
                 tmem_st16(at, zero);
-                if (HALF) tmem_st16(at + 16, zero);
+                tmem_st16(at + 16, zero);
             };
             for (uint32_t it = blockIdx.x; !STATES && it < p.items; it += gridDim.x) {
                 const Item x(p, it);
@@ -492,7 +493,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 #pragma unroll 1
                     for (int blk = 0; blk < 2; ++blk) {
                         const uint32_t at = tl + (first + blk) * 32;      // P takes its scores' place
-                        uint32_t w[16];
+                        uint32_t w[16], low[16];
                         if (blk && !two) {           // blocks of later tokens
                             clear(at);
                             continue;
@@ -523,21 +524,17 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                             }
                         }
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
+                        for (int i = 0; i < 16; ++i) {         // the first terms, and what they leave
                             w[i] = pair<HALF>(s[2 * i], s[2 * i + 1]);
-                            if constexpr (HALF) {    // what that leaves
-                                const float2 h = floats<HALF>(w[i]);
-                                mx::unpack2(mx::mul2(low2, mx::fma2(mx::pack2(h.x, h.y), minus,
-                                                                    mx::pack2(s[2 * i], s[2 * i + 1]))),
-                                            s[2 * i], s[2 * i + 1]);
-                            }
+                            const float2 h = floats<HALF>(w[i]);
+                            uint64_t yz = mx::fma2(mx::pack2(h.x, h.y), minus, mx::pack2(s[2 * i], s[2 * i + 1]));
+                            if constexpr (HALF) yz = mx::mul2(low2, yz);
+                            float y, z;
+                            mx::unpack2(yz, y, z);
+                            low[i] = pair<HALF>(y, z);
                         }
                         tmem_st16(at, w);
-                        if constexpr (HALF) {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) w[i] = pair<HALF>(s[2 * i], s[2 * i + 1]);
-                            tmem_st16(at + 16, w);
-                        }
+                        tmem_st16(at + 16, low);
                     }
                     if (q < 2) {
                         clear(tl + 64);
