@@ -42,3 +42,15 @@ def test_outputs_are_rounded_once(B, N, H, d, pad, dtype):
     o, _, ro = _check(q, k, v, lam, d ** -0.5, state, None, pad)
     if dtype != F32 and B * N * H * d >= 512:                 # enough values for a mean
         assert (o.cpu().double() - ro).norm() <= 1.1 * (ro.to(dtype).double() - ro).norm()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("N,H,d", [(2, 1, 64), (8, 8, 32), (9, 2, 64), (40, 1, 128), (64, 2, 64)])
+def test_a_sequence_alone_is_the_one_in_a_batch(N, H, d, dtype):
+    """One form takes the same sequence, however many stand beside it: the same bits."""
+    q, k, v = (x.to(DEV) for x in _tokens(200, N, H, H, d, d, dtype, 51))
+    lam = _lam(H).to(DEV)
+    o, S = _k().decay_attention(q, k, v, lam)
+    for b in (1, 3):
+        a, s = _k().decay_attention(q[:b], k[:b], v[:b], lam)
+        assert torch.equal(a, o[:b]) and torch.equal(s, S[:b])

@@ -439,12 +439,6 @@ int run_step(const Args& a, cudaStream_t s) {
                     s, a, tiles);
 }
 
-// Short sequences of few heads go to the CUDA cores whatever their type: there the rounding of the
-// tensor cores' scores, which more results average out, shows in the outputs (1.4 times a float32
-// result's own rounding on the mean; of 9 to 64 tokens of one head up to 1.7 times, of 64 tokens of
-// four 1.5).  8 heads of 64: 9 us for 9 tokens, on the tensor cores 6; two of 64 tokens: 14, 6.
-constexpr int64_t FEW_TOKENS = 8, SHORT = 64, FEW_ROWS = 128;
-
 bool heads_ok(int dtype, int64_t B, int64_t H, int64_t Hk, int64_t dk, int64_t dv) {
     return (dtype == SNNB_F32 || dtype == SNNB_F16 || dtype == SNNB_BF16) && B >= 0 && H >= 1 &&
            Hk >= 1 && H % Hk == 0 && dk >= 1 && dk <= MAX_DIM && dv >= 1 && dv <= MAX_DIM &&
@@ -501,8 +495,9 @@ extern "C" int snnb_decay_attention(const void* q, const int64_t* q_strides, con
         if (dtype == SNNB_F16) return run_step<__half>(a, s);
         return run_step<__nv_bfloat16>(a, s);
     }
-    const bool few = N <= FEW_TOKENS ? B * H * ((dv + GV - 1) / GV) <= 148 : N <= SHORT && B * H * N <= FEW_ROWS;
-    if (!few && tc_takes(a, dtype)) return tc_run(a, dtype, workspace, workspace_bytes, s);
+    // The tensor cores, where they take the arguments, whatever the length: bf16, 8 heads of 64, 2 tokens 6.0 us (on
+    // the CUDA cores 8.7), 64 6.1 (14.2), 128 6.2 (25.5); 256 heads of 64, 2 tokens 12.0 (10.8), 9 12.1 (13.0).
+    if (tc_takes(a, dtype)) return tc_run(a, dtype, workspace, workspace_bytes, s);
     if (dtype == SNNB_F32) return run_any<float>(a, workspace, workspace_bytes, s);
     if (dtype == SNNB_F16) return run_any<__half>(a, workspace, workspace_bytes, s);
     return run_any<__nv_bfloat16>(a, workspace, workspace_bytes, s);
