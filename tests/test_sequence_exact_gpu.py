@@ -54,3 +54,27 @@ def test_a_sequence_alone_is_the_one_in_a_batch(N, H, d, dtype):
     for b in (1, 3):
         a, s = _k().decay_attention(q[:b], k[:b], v[:b], lam)
         assert torch.equal(a, o[:b]) and torch.equal(s, S[:b])
+
+
+# 9 to 19 chunks of 128 tokens (18 to 38 of 64 on the CUDA cores) of few heads: 3 to 7 segments (9 to 13), each of
+# which starts from what those before it leave
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("pad", [0, 1])
+@pytest.mark.parametrize("H,Hk,dk,dv,N", [(2, 1, 64, 64, 2390), (1, 1, 128, 128, 1100), (2, 2, 40, 72, 1500)])
+def test_long_sequences_in_segments(H, Hk, dk, dv, N, pad, dtype):
+    """Lengths that end in the first, a middle and the last segment, at a chunk's border, at none; from no
+    state, from one, and in place."""
+    B = 6
+    q, k, v = _tokens(B, N, H, Hk, dk, dv, dtype, 52)
+    lam = torch.tensor([0.999, 0.9])[:H]
+    state = torch.randn(B, H, dk, dv, generator=_gen(8)) * 4
+    lengths = torch.tensor([0, 1, N // 2, 1024, N - 1, N], dtype=torch.int64)
+    o, S, _ = _check(q, k, v, lam, dk ** -0.5, state, lengths, pad)
+    for b, n in enumerate(lengths.tolist()):
+        assert not o[b, n:].any()
+    assert torch.equal(S[0].cpu(), state[0])
+    o2, S2, _ = _check(q, k, v, lam, dk ** -0.5, state, lengths, pad, in_place=True)
+    assert torch.equal(o2, o) and torch.equal(S2, S)
+    _check(q[:1], k[:1], v[:1], lam, dk ** -0.5, None, None, pad)
+    o3, S3, _ = _check(q[-1:], k[-1:], v[-1:], lam, dk ** -0.5, state[-1:], None, pad)
+    assert torch.equal(o3, o[-1:]) and torch.equal(S3, S[-1:])       # in as many segments
