@@ -3,9 +3,9 @@
 //   pair i of a head, columns (i, i + R) or (2i, 2i + 1) of its first 2R, turns by the angle
 //   t = positions[axis(i)] * f(i):   (a, b) -> (a cos t - b sin t, a sin t + b cos t)
 //
-// The angle is held in turns: positions are exact in float64, f / 2 pi comes in float64 and the
-// product's whole turns are dropped there, so a far position loses nothing (in float32 a position
-// of 2^20 would be off by 0.06 rad); what remains of it, in [-1/2, 1/2], is exact enough in
+// The angle is held in turns: positions are exact in float64 (up to 2^53), f / 2 pi comes in float64 and
+// the product's whole turns are dropped there, so that an angle is good to 2^-50 of itself (in float32 a
+// position of 2^20 would be off by 0.06 rad); what remains of it, in [-1/2, 1/2], is exact enough in
 // float32 for the sine and the cosine.
 //
 // Bound: HBM (every value is read and written once).  A thread holds the sines and cosines of the

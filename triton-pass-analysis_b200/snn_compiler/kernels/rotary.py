@@ -77,7 +77,8 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor
     axis, sum(sections) = R <= d / 2 (and <= 256); columns from 2 R on are copied.  Pair i is
     columns (i, i + R), or (2i, 2i + 1) when interleaved.  Its frequency is base^(-i / R)
     (ladder="shared"), or base^(-j / sections[a]) for the j-th pair of axis a (ladder="axis").
-    Angles lose nothing at far positions: they are held in float64 turns."""
+    Angles are formed in float64 turns: good to 2^-50 of themselves, however far the position (whole
+    positions are exact up to 2^53)."""
     sections = tuple(sections)
     if ladder not in ("shared", "axis"):
         raise ValueError(f"rotary_axes: unknown ladder {ladder!r} (shared or axis)")
