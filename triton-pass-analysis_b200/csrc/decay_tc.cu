@@ -13,7 +13,7 @@
 // bfloat16 terms of w V would leave errors of 2.5e-6 in the state; these leave 3e-7.)  P and S are rounded to
 // two terms for their products: 16 bits of bfloat16, 22 of float16, so that an output is as good as a
 // float32 sum that is rounded once.  (P as one term: the error of bfloat16 outputs was 1.25 times that, of
-// one head's 64 tokens 1.7 times; 16 x 2048 x 16 heads of 64 took 69 us, and takes 81.)  float16's range is far
+// one head's 64 tokens 1.7 times; 16 x 2048 x 16 heads of 64 took 69 us, and takes 79.)  float16's range is far
 // below what scores and states take: see its exponents below.
 //
 // Tensor memory holds 512 columns: scores 128, Q S 2 x 64, P V 64 (float16: 2 x 64), K^T (w V) 3 x 64 (2 x 64).
@@ -22,11 +22,11 @@
 //
 // Warps have one role each, and each walks the block's items (a segment of a sequence, a head, 64 columns
 // of v) and their chunks; what bounds a chunk is the chain scores -> P -> P V -> the next scores, which
-// share their columns, and beside it instruction issue (53% of the slots taken, the tensor pipe
-// 39%; DRAM 35%).  The code is kept short on purpose: with every loop unrolled it had 150 KB and
-// ran at half the speed, waiting for instructions.  16 x 2048 tokens x 16 heads of 64, bf16: 78 us,
-// 3.4 TB/s of 6.5; 64 x 2048 x 8 of 128: 338 us, 3.2 TB/s; one sequence of 16384 x 32 of 128: 250 us,
-// of which a third is the pass before, over k and v, that leaves the state of its first half.
+// share their columns, and beside it instruction issue (49% of the slots taken, the tensor pipe
+// 42%; DRAM 34%).  The code is kept short on purpose: with every loop unrolled it had 150 KB and
+// ran at half the speed, waiting for instructions.  16 x 2048 tokens x 16 heads of 64, bf16: 79 us,
+// 3.4 TB/s of 6.5 (float16: 110); 64 x 2048 x 8 of 128: 352 us, 3.1 TB/s; one sequence of 16384 x 32 of 128:
+// 262 us (346), of which a third is the pass before, over k and v, that leaves the state of its first half.
 //
 // Waits are bounded as elsewhere (tc_common.cuh).
 #include "decay.cuh"
