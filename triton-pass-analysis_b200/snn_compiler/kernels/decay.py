@@ -80,9 +80,9 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: to
     after the last token (`state` for a length of zero).  dk, dv: 1 to 256, N below 2^31 - 255.  Powers, sums and the
     state are held in float32.  16-bit operands of the tensor cores are held to 2^-16 of themselves or better: an
     output is off by half a step of its type and about 2^-15 of the sum of its terms' magnitudes, and a state by a
-    float32 sum's error and 2^-22 of that sum.  float16 there holds scores to 2^-50 of 128 |q_i| times the largest
-    |k_j| so far too, values to 2^-50 of their chunk's largest and the state in front of q to 2^-50 of its largest
-    (64 columns of v at a time).  out and state_out overlap no other argument (but for state_out, state
+    float32 sum's error and 2^-22 of that sum.  float16 has less range than that: beside it, scores are held there
+    to 2^-49 of 128 |q_i| times the largest |k_j| so far, values to 2^-50 of their chunk's largest and the state
+    that q reads to 2^-50 of its largest (64 columns of v at a time).  out and state_out overlap no other argument (but for state_out, state
     as a whole).  A token that is not finite shows in itself and those behind it only."""
     assert q.dim() == 4, tuple(q.shape)
     B, N = q.shape[:2]
